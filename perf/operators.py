@@ -1,0 +1,393 @@
+"""The channel half of a sparse transformer-style block on voxel features, as cases that can be timed
+and checked.
+
+A sparse convolution mixes voxels; the operators here do the rest of such a block on the ``[rows,
+channels]`` features it returns: the residual's addition with a root-mean-square norm, a gated
+feed-forward block, and activations kept in 8 bits for the backward pass.  Kinds:
+
+* ``norm``: summed = x + residual, y = summed / rms(summed) * weight; with ``train`` the gradients of
+  x, the residual and the weight, with ``int8`` a copy of y in 8 bits, returned as the values that it
+  stands for;
+* ``keep``: rows to 8 bits (one scale for each 128 channels of a row) and back;
+* ``ffn``: (act(x Wg') * (x Wu')) Wd' (+ residual); with ``train`` the gradients of x and the three
+  weights; with ``int8`` the backward pass takes x from its 8-bit copy;
+* ``block``: the three together, training step: norm of x + residual with an 8-bit copy, then the
+  feed-forward block, which adds the sum again and whose backward pass takes that copy.
+
+``own`` false computes the same with elementary torch operations in fp32, each operator's results
+rounded once to the rows' type.  Widths are those of the sparse networks here (16 to 512 channels) with hidden
+widths of 2, 8/3 and 4 times as many; row counts go from one voxel to a batch of large scenes.  With
+``wide`` rows are the first channels of a wider tensor (the half of a concatenation), so that their
+stride is not their width.
+"""
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+SIZE = {"f16": 2, "bf16": 2, "f32": 4}
+EPS = 1e-6
+GROUP = 128  # channels that share a scale
+
+
+def listed():
+    return [
+        # one voxel: what a call costs at least
+        {"name": "norm_f16_1x64", "kind": "norm", "rows": 1, "c": 64, "dtype": "f16",
+         "train": False, "int8": False, "wide": False},
+        # a full-resolution stage's inference norm that also emits the 8-bit copy
+        {"name": "norm_int8_f16_200k_x64", "kind": "norm", "rows": 200000, "c": 64,
+         "dtype": "f16", "train": False, "int8": True, "wide": False},
+        # training on a batch of two street scenes
+        {"name": "norm_train_bf16_240k_x128", "kind": "norm", "rows": 240000, "c": 128,
+         "dtype": "bf16", "train": True, "int8": False, "wide": False},
+        # fp32 training with a width that 16 bytes do not divide, on half of a concatenation
+        {"name": "norm_train_f32_50001_x99", "kind": "norm", "rows": 50001, "c": 99,
+         "dtype": "f32", "train": True, "int8": False, "wide": True},
+        # activations of a large scene to 8 bits and back
+        {"name": "keep_f16_400k_x64", "kind": "keep", "rows": 400000, "c": 64, "dtype": "f16",
+         "wide": False},
+        # a wide stage with an odd row count: two scales a row, on half of a concatenation
+        {"name": "keep_bf16_77777_x256", "kind": "keep", "rows": 77777, "c": 256,
+         "dtype": "bf16", "wide": True},
+        # one voxel through the feed-forward block
+        {"name": "ffn_f16_1x64_172", "kind": "ffn", "rows": 1, "c": 64, "hidden": 172,
+         "act": "silu", "dtype": "f16", "train": False, "int8": False, "wide": False},
+        # a full-resolution stage's inference pass
+        {"name": "ffn_f16_200k_x64_256", "kind": "ffn", "rows": 200000, "c": 64, "hidden": 256,
+         "act": "silu", "dtype": "f16", "train": False, "int8": False, "wide": False},
+        # a wide decoder stage's training step
+        {"name": "ffn_train_bf16_75001_x256_688", "kind": "ffn", "rows": 75001, "c": 256,
+         "hidden": 688, "act": "gelu", "dtype": "bf16", "train": True, "int8": False,
+         "wide": False},
+        # fp32 training of a middle stage, x kept in 8 bits
+        {"name": "ffn_train_f32_30001_x96_256", "kind": "ffn", "rows": 30001, "c": 96,
+         "hidden": 256, "act": "silu", "dtype": "f32", "train": True, "int8": True,
+         "wide": False},
+        # the largest: the widest stage's training step
+        {"name": "ffn_train_bf16_50k_x512_1376", "kind": "ffn", "rows": 50000, "c": 512,
+         "hidden": 1376, "act": "silu", "dtype": "bf16", "train": True, "int8": False,
+         "wide": False},
+        # the operators together: a full-resolution stage's training step, batch 2 x 120k voxels
+        {"name": "block_train_f16_240k_x64_256", "kind": "block", "rows": 240000, "c": 64,
+         "hidden": 256, "act": "silu", "dtype": "f16", "wide": False},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+WIDTHS = [16, 20, 24, 32, 40, 48, 64, 64, 96, 99, 128, 128, 160, 192, 256, 320, 384, 512]
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "norm", "keep", "ffn", "ffn", "ffn", "block"])
+    dtype = rng.choice(["f16", "f16", "bf16", "bf16", "f32"])
+    c = rng.choice(WIDTHS)
+    case = {"kind": kind, "c": c, "dtype": dtype, "wide": rng.random() < 0.25}
+    if kind in ("norm", "keep"):
+        case["rows"] = min(_log(rng, 1, 400000), 400000 * 128 // c)
+        if kind == "norm":
+            case["train"] = rng.random() < 0.6
+            case["int8"] = not case["train"] and dtype != "f32" and rng.random() < 0.6
+        return case
+    case["hidden"] = rng.choice([2 * c, 4 * c, (8 * c // 3 + 7) // 8 * 8, 8 * c // 3])
+    case["act"] = rng.choice(["silu", "silu", "gelu", "relu"])
+    # the largest listed work; fp32 products cost some sixteen times the 16-bit ones
+    most = 50000 * 512 * 1376 // (16 if dtype == "f32" else 1)
+    case["rows"] = min(_log(rng, 1, 400000), most // (c * case["hidden"]))
+    if kind == "ffn":
+        case["train"] = rng.random() < 0.6
+        case["int8"] = case["train"] and rng.random() < 0.5
+    elif dtype == "f32":
+        case["dtype"] = "f16"  # the block under mixed precision
+    return case
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+
+def prepare(case, seed):
+    dev = torch.device("cuda:0" if torch.cuda.is_available() else "cpu")
+    dtype = DTYPES[case["dtype"]]
+    n, c = case["rows"], case["c"]
+    g = torch.Generator(device=dev)
+    g.manual_seed(int(seed) * 7919 + 29)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=dev)
+
+    def rows():
+        # rows of their own magnitude and a few strong channels, as trained networks have them
+        t = normal(n, c) * torch.exp(0.5 * normal(n, 1)) * (1 + 3 * (normal(c) > 1.5))
+        if case["wide"]:
+            t = torch.cat([t, normal(n, c + 8 - c % 8)], 1)
+        t = t.to(dtype)
+        return t[:, :c] if case["wide"] else t
+
+    def weight(out, inner):
+        return (normal(out, inner) / math.sqrt(inner)).to(dtype)
+
+    s = {"case": dict(case), "x": rows()}
+    train = case["kind"] == "block" or case.get("train", False)
+    if case["kind"] in ("norm", "block"):
+        s["residual"] = rows()
+        s["scale"] = (1 + 0.1 * normal(c)).to(dtype)
+    if case["kind"] in ("ffn", "block"):
+        s["wg"], s["wu"] = weight(case["hidden"], c), weight(case["hidden"], c)
+        s["wd"] = weight(c, case["hidden"])
+        if case["kind"] == "ffn":
+            # its input is normalised, as after a norm
+            x = s["x"].float()
+            s["x"].copy_(x * torch.rsqrt((x * x).mean(1, keepdim=True) + EPS))
+    if train:
+        s["dy"] = (0.01 * normal(n, c)).to(dtype)
+        if case["kind"] == "norm":
+            s["dsum"] = (0.01 * normal(n, c)).to(dtype)
+        for k in ("x", "residual", "scale", "wg", "wu", "wd"):
+            if k in s:
+                s[k] = s[k].detach().requires_grad_(True)
+    return s
+
+
+# ---------------------------------------------------------------------------
+# the framework's own
+# ---------------------------------------------------------------------------
+
+def _run_own(s):
+    pkg = os.path.join(ROOT, "spconv-triton_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from spconv_triton.pytorch import functional as Fsp
+
+    case = s["case"]
+    kind = case["kind"]
+    if kind == "keep":
+        return Fsp.restore_rows(Fsp.quantize_rows(s["x"]))
+    if kind == "norm":
+        if not case["train"]:
+            with torch.no_grad():
+                out = Fsp.rms_norm(s["x"], s["scale"], EPS, residual=s["residual"],
+                                   int8=case["int8"])
+                if case["int8"]:
+                    return [out[0], out[1], Fsp.restore_rows(out[2])]
+                return list(out)
+        y, total = Fsp.rms_norm(s["x"], s["scale"], EPS, residual=s["residual"])
+        grads = torch.autograd.grad([y, total], [s["x"], s["residual"], s["scale"]],
+                                    [s["dy"], s["dsum"]])
+        return [y.detach(), total.detach(), *grads]
+    if kind == "ffn":
+        if not case["train"]:
+            with torch.no_grad():
+                return Fsp.gated_ffn(s["x"], s["wg"], s["wu"], s["wd"], act=case["act"])
+        y = Fsp.gated_ffn(s["x"], s["wg"], s["wu"], s["wd"], act=case["act"],
+                          saved="int8" if case["int8"] else None)
+        grads = torch.autograd.grad(y, [s["x"], s["wg"], s["wu"], s["wd"]], s["dy"])
+        return [y.detach(), *grads]
+    y, total, kept = Fsp.rms_norm(s["x"], s["scale"], EPS, residual=s["residual"], int8=True)
+    out = Fsp.gated_ffn(y, s["wg"], s["wu"], s["wd"], act=case["act"], residual=total, saved=kept)
+    grads = torch.autograd.grad(out, [s[k] for k in ("x", "residual", "scale", "wg", "wu", "wd")],
+                                s["dy"])
+    return [out.detach(), *grads]
+
+
+# ---------------------------------------------------------------------------
+# plain forms: fp32 operations, each operator's results rounded once
+# ---------------------------------------------------------------------------
+
+def _plain_norm(x, residual, scale):
+    total = x.float() + residual.float()
+    inv = torch.rsqrt((total * total).mean(1, keepdim=True) + EPS)
+    return total * inv * scale.float(), total, inv
+
+
+def _plain_norm_grads(dy, dsum, total, inv, scale):
+    t = dy * scale.float()
+    dx = dsum + inv * t - total * (inv * inv * inv) * (t * total).mean(1, keepdim=True)
+    return dx, (dy * total * inv).sum(0)
+
+
+def _groups(x):
+    """[rows, groups, 128], the last group filled up with zeros."""
+    n, c = x.shape
+    pad = -c % GROUP
+    if pad:
+        x = torch.cat([x, x.new_zeros(n, pad)], 1)
+    return x.reshape(n, -1, GROUP)
+
+
+def _plain_codes(x):
+    """Whole numbers of -127..127 and the factor of each group of 128 channels."""
+    g = _groups(x.float())
+    top = g.abs().amax(2, keepdim=True)
+    some = top > 0
+    up = torch.where(some, 127.0 / top, torch.zeros_like(top))
+    return torch.round(g * up).to(torch.int8), top / 127.0
+
+
+def _plain_restored(x):
+    codes, step = _plain_codes(x)
+    return (codes.float() * step).reshape(x.shape[0], -1)[:, :x.shape[1]].to(x.dtype)
+
+
+def _plain_act(z, act):
+    """(value, derivative) of the gate's activation."""
+    if act == "silu":
+        sig = 1 / (1 + torch.exp(-z))
+        return z * sig, sig * (1 + z * (1 - sig))
+    if act == "gelu":
+        cdf = 0.5 * (1 + torch.erf(z * math.sqrt(0.5)))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) * (1 / math.sqrt(2 * math.pi))
+    return z.clamp(min=0), (z > 0).float()
+
+
+def _plain_ffn(x, s, act):
+    x = x.float()
+    value, _ = _plain_act(x @ s["wg"].float().t(), act)
+    return (value * (x @ s["wu"].float().t())) @ s["wd"].float().t()
+
+
+def _plain_ffn_grads(dy, x, s, act):
+    x, dy = x.float(), dy.float()
+    wg, wu, wd = s["wg"].float(), s["wu"].float(), s["wd"].float()
+    u = x @ wu.t()
+    value, slope = _plain_act(x @ wg.t(), act)
+    dh = dy @ wd
+    dg, du = dh * u * slope, dh * value
+    return dg @ wg + du @ wu, dg.t() @ x, du.t() @ x, dy.t() @ (value * u)
+
+
+@torch.no_grad()
+def _run_plain(s):
+    case = s["case"]
+    kind, dtype = case["kind"], DTYPES[case["dtype"]]
+    if kind == "keep":
+        return _plain_restored(s["x"])
+    if kind == "norm":
+        y, total, inv = _plain_norm(s["x"], s["residual"], s["scale"])
+        y = y.to(dtype)
+        if case["int8"]:
+            return [y, total.to(dtype), _plain_restored(y)]
+        if not case["train"]:
+            return [y, total.to(dtype)]
+        dx, dscale = _plain_norm_grads(s["dy"].float(), s["dsum"].float(), total, inv, s["scale"])
+        dx = dx.to(dtype)
+        return [y, total.to(dtype), dx, dx, dscale.to(dtype)]
+    if kind == "ffn":
+        y = _plain_ffn(s["x"], s, case["act"]).to(dtype)
+        if not case["train"]:
+            return y
+        x = _plain_restored(s["x"]) if case["int8"] else s["x"]
+        return [y, *(t.to(dtype) for t in _plain_ffn_grads(s["dy"], x, s, case["act"]))]
+    y, total, inv = _plain_norm(s["x"], s["residual"], s["scale"])
+    y, total = y.to(dtype), total.to(dtype).float()
+    out = _plain_ffn(y, s, case["act"]) + total
+    grads = _plain_ffn_grads(s["dy"], _plain_restored(y), s, case["act"])
+    dyn = grads[0].to(dtype).float()
+    dx, dscale = _plain_norm_grads(dyn, s["dy"].float(), total, inv, s["scale"])
+    dx = dx.to(dtype)
+    return [t.to(dtype) for t in (out, dx, dx, dscale, *grads[1:])]
+
+
+def run(s):
+    return _run_own(s) if own else _run_plain(s)
+
+
+# ---------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------
+
+def _exact_kept(v):
+    """v with every value on its group's grid of 127 steps up and down."""
+    parts = []
+    for lo in range(0, v.shape[1], GROUP):
+        part = v[:, lo:lo + GROUP]
+        step = part.abs().max(1, keepdim=True).values / 127
+        parts.append(torch.where(step > 0, (part / step).round() * step, torch.zeros_like(part)))
+    return torch.cat(parts, 1)
+
+
+def _exact_gate(z, act):
+    if act == "silu":
+        return torch.nn.functional.silu(z)
+    return torch.nn.functional.gelu(z) if act == "gelu" else torch.relu(z)
+
+
+def _exact_slope(z, act):
+    with torch.enable_grad():
+        z = z.detach().requires_grad_(True)
+        return torch.autograd.grad(_exact_gate(z, act).sum(), z)[0]
+
+
+def _exact_step(d, kept, up, act):
+    """The feed-forward block's gradients at x = kept, from the gradient `up` of its result."""
+    z, u = torch.mm(kept, d["wg"].T), torch.mm(kept, d["wu"].T)
+    dh, h = torch.mm(up, d["wd"]), _exact_gate(z, act)
+    dz, du = dh * u * _exact_slope(z, act), dh * h
+    return (torch.mm(dz, d["wg"]) + torch.mm(du, d["wu"]), torch.mm(dz.T, kept),
+            torch.mm(du.T, kept), torch.mm(up.T, h * u))
+
+
+@torch.no_grad()
+def exact(case, seed):
+    d = {k: v.detach().double() for k, v in prepare(case, seed).items() if k != "case"}
+    kind, act = case["kind"], case.get("act")
+    if kind == "keep":
+        return _exact_kept(d["x"])
+    if kind == "ffn":
+        y = torch.mm(_exact_gate(torch.mm(d["x"], d["wg"].T), act) * torch.mm(d["x"], d["wu"].T),
+                     d["wd"].T)
+        if not case["train"]:
+            return y
+        kept = _exact_kept(d["x"]) if case["int8"] else d["x"]
+        return [y, *_exact_step(d, kept, d["dy"], act)]
+    total = d["x"] + d["residual"]
+    rms = (total.square().mean(1, keepdim=True) + EPS).sqrt()
+    unit = total / rms
+    y = unit * d["scale"]
+    if kind == "norm" and not case["train"]:
+        return [y, total, _exact_kept(y)] if case["int8"] else [y, total]
+    if kind == "norm":
+        up, straight, rest = d["dy"], d["dsum"], None
+        head = [y, total]
+    else:
+        value = _exact_gate(torch.mm(y, d["wg"].T), act) * torch.mm(y, d["wu"].T)
+        up, *rest = _exact_step(d, _exact_kept(y), d["dy"], act)
+        straight, head = d["dy"], [torch.mm(value, d["wd"].T) + total]
+    t = up * d["scale"]
+    dx = straight + (t - unit * (t * unit).mean(1, keepdim=True)) / rms
+    return [*head, dx, dx, (up * unit).sum(0), *(rest or [])]
+
+
+# ---------------------------------------------------------------------------
+# what a pass cannot do without
+# ---------------------------------------------------------------------------
+
+def work(case):
+    n, c, size = case["rows"], case["c"], SIZE[case["dtype"]]
+    row = n * c * size
+    kept = n * (c + 4 * -(-c // GROUP))  # 8-bit values and their scales
+    if case["kind"] == "keep":
+        return {"bytes": 2 * row + 2 * kept, "flops": 4 * n * c}
+    if case["kind"] == "norm":
+        # x, residual, y, sum; the two gradients that come and the one that goes
+        b = 4 * row + c * size
+        if case["int8"]:
+            b += 2 * kept + row
+        if case["train"]:
+            b += 3 * row + c * size
+        return {"bytes": b, "flops": (16 if case["train"] else 6) * n * c}
+    weights = 3 * c * case["hidden"]
+    train = case["kind"] == "block" or case["train"]
+    b = (4 if train else 2) * row + (2 if train else 1) * weights * size
+    if case["kind"] == "block":
+        b += row  # the residual
+    return {"bytes": b, "flops": (6 if train else 2) * n * weights}
