@@ -228,9 +228,9 @@ def _plain_codes(x):
     """Whole numbers of -127..127 and the factor of each group of 128 channels."""
     g = _groups(x.float())
     top = g.abs().amax(2, keepdim=True)
-    some = top > 0
-    up = torch.where(some, 127.0 / top, torch.zeros_like(top))
-    return torch.round(g * up).to(torch.int8), top / 127.0
+    most = torch.full_like(top, 127.0)  # (a division by a plain number multiplies by its inverse)
+    up = torch.where(top > 0, most / top, torch.zeros_like(top))
+    return torch.round(g * up).to(torch.int8), top / most
 
 
 def _plain_restored(x):
