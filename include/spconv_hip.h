@@ -440,6 +440,58 @@ int sp_point2voxel(const void* points, int32_t dtype, int64_t n_points, int64_t 
                    int64_t* pc_voxel_id, int64_t* num_voxels, void* ws, size_t ws_bytes,
                    void* stream);
 
+/* ---- whole rows: norm and 8-bit copies --------------------------------- */
+/* Operators of this library's own (the reference has none of this kind) on
+ * feature rows of f16, bf16 or f32.  ld*: elements from row to row (>= C); rows without
+ * one are contiguous.  Sums and statistics are fp32.
+ *
+ * s = x + residual (residual null: s = x), y = s / sqrt(mean(s^2) + eps) *
+ * weight, each rounded once to the rows' type; weight [C] of type param_dtype
+ * (the rows' or SP_F32; null: ones).  sum (nullable) receives s.  codes
+ * [rows, C] and scales [rows, ceil(C / 128)] (both or none) receive y as sp_quantize_rows
+ * would make them of the stored y. */
+int sp_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int32_t dtype,
+                int64_t rows, int64_t C, const void* weight, int32_t param_dtype, float eps,
+                void* y, void* sum, int8_t* codes, float* scales, void* stream);
+/* Gradients of sp_rms_norm from those of y (dy) and of s (dsum, nullable), with s as stored:
+ * ds [rows, C] (of x and of the residual alike) and dweight [C] of type
+ * param_dtype (nullable; its sums over rows have a fixed order).  The workspace, 16-byte
+ * aligned, is read only with dweight. */
+size_t sp_rms_norm_bwd_workspace(int64_t rows, int64_t C);
+int sp_rms_norm_bwd(const void* dy, int64_t lddy, const void* dsum, int64_t ldds, const void* s,
+                    int64_t lds, int32_t dtype, int64_t rows, int64_t C, const void* weight,
+                    int32_t param_dtype, float eps, void* ds, void* dweight, void* ws,
+                    size_t ws_bytes, void* stream);
+/* Rows in 8 bits: for each row and 128 channels, scale = max|x| / 127 and code =
+ * rint(x * (127 / max|x|)) in -127..127, both in fp32.  A group whose largest magnitude is below
+ * 2^-100 has scale 0; one with an infinity or a NaN has scale NaN (and codes 0), so that it is
+ * NaN when restored. */
+int sp_quantize_rows(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
+                     int8_t* codes, float* scales, void* stream);
+/* out [rows, C] = code * scale in fp32, rounded to dtype. */
+int sp_restore_rows(const int8_t* codes, const float* scales, int64_t rows, int64_t C,
+                    int32_t dtype, void* out, void* stream);
+
+/* ---- gated feed-forward block ------------------------------------------- */
+/* g = x w_gate', u = x w_up', y = (act(g) * u) w_down' (+ residual, nullable),
+ * for rows x [rows, C] and weights w_gate, w_up [F, C], w_down [Co, F] of one
+ * type (f16, bf16 or f32), contiguous; y [rows, Co].  act: 0 silu, 1 gelu (the exact one), 2 relu.  Sums are
+ * fp32; act(g) * u is rounded to the type between the products.  Workspaces are 16-byte
+ * aligned. */
+size_t sp_gated_ffn_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
+int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
+                 const void* w_gate, const void* w_up, int64_t F, const void* w_down, int64_t Co,
+                 int32_t act, const void* residual, int64_t ldr, void* y, void* ws,
+                 size_t ws_bytes, void* stream);
+/* Its gradients from dy [rows, Co]: dx [rows, C], dw_gate, dw_up, dw_down (each nullable).  g, u and
+ * the gradient of the hidden rows are formed again; the latter's parts are rounded to the type
+ * between the products.  Sums over rows have a fixed order. */
+size_t sp_gated_ffn_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
+int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                     int64_t rows, int64_t C, const void* w_gate, const void* w_up, int64_t F,
+                     const void* w_down, int64_t Co, int32_t act, void* dx, void* dw_gate,
+                     void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- hash table (spconv_triton/pytorch/hash.py:15-110) ----------------- */
 /* A table of `capacity` (a power of two) slots lives in one caller-owned
  * device buffer of sp_hash_table_bytes(capacity).  Keys are int32 (key64 = 0)

@@ -6,6 +6,7 @@
 """Public PyTorch API, a drop-in for ``spconv.pytorch`` / ``spconv_triton.pytorch``."""
 
 from spconv_triton.pytorch import functional, ops
+from spconv_triton.pytorch.blocks import GatedFFN, RMSNorm, SparseFFNBlock
 from spconv_triton.pytorch.conv import (
     SparseConv1d,
     SparseConv2d,

@@ -19,6 +19,8 @@ from torch.autograd.function import once_differentiable
 
 from spconv_triton.compat import tv
 from spconv_triton.pytorch import ops
+from spconv_triton.pytorch._impl import rows as _rows
+from spconv_triton.pytorch._impl.rows import Int8Rows
 from spconv_triton.pytorch.hash import HashTable
 from spconv_triton.tools import CUDAKernelTimer
 
@@ -210,6 +212,110 @@ indice_subm_conv = SubMConvFunction.apply
 indice_maxpool = SparseMaxPoolFunction.apply
 indice_maxpool_implicit_gemm = SparseMaxPoolImplicitGemmFunction.apply
 indice_avgpool_implicit_gemm = SparseAvgPoolImplicitGemmFunction.apply
+
+
+# ---------------------------------------------------------------------------
+# the channel half of a block: norm, gated feed-forward, rows in 8 bits
+# ---------------------------------------------------------------------------
+
+class RMSNormFunction(Function):
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, x, weight, eps, residual, int8):
+        y, total, kept = ops.rms_norm(x, weight, eps, residual, int8)
+        ctx.save_for_backward(x if residual is None else total, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return y, total, kept
+
+    @staticmethod
+    @once_differentiable
+    @_BWD
+    def backward(ctx, dy, dsum, _):
+        total, weight = ctx.saved_tensors
+        need_x, need_w, _, need_res, _ = ctx.needs_input_grad
+        if dy is None:  # the sum alone was used
+            ds, dw = dsum, torch.zeros_like(weight) if need_w else None
+        else:
+            ds, dw = ops.rms_norm_backward(dy, dsum, total, weight, ctx.eps, need_w)
+        return ds if need_x else None, dw, None, ds if need_res else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+             residual: torch.Tensor | None = None, int8: bool = False):
+    """Root-mean-square norm of feature rows, with the residual's addition before it:
+    ``s = x + residual``, ``y = s / sqrt(mean(s * s) + eps) * weight``.
+
+    Returns ``y``; with ``residual`` also ``s``; with ``int8`` also y's :class:`Int8Rows` (which
+    carries no gradient).  ``weight`` has the rows' type or float32; statistics are float32.
+    """
+    y, total, kept = RMSNormFunction.apply(x, weight, eps, residual, int8)
+    out = (y,) if residual is None else (y, total)
+    if int8:
+        out += (kept,)
+    return out[0] if len(out) == 1 else out
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """Feature rows in 8 bits, one scale for each row and 128 channels: ``scale = max|x| / 127``,
+    ``code = rint(x * (127 / max|x|))``.  A group with an infinity or a NaN is NaN when restored.
+    No gradient passes."""
+    return ops.quantize_rows(x.detach())
+
+
+def restore_rows(rows: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The values that 8-bit rows stand for, in ``dtype`` (default: the type they came from)."""
+    return ops.restore_rows(rows, dtype)
+
+
+class GatedFFNFunction(Function):
+    @staticmethod
+    @_FWD
+    def forward(ctx, x, w_gate, w_up, w_down, act, residual, saved):
+        y = ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
+        ctx.act = act
+        ctx.kept_type = None
+        if any(ctx.needs_input_grad[:4]):
+            if saved == "int8":
+                saved = ops.quantize_rows(x)
+            if saved is None:
+                ctx.save_for_backward(w_gate, w_up, w_down, x)
+            else:
+                ctx.kept_type = x.dtype
+                ctx.save_for_backward(w_gate, w_up, w_down, saved.codes, saved.scales)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    @_BWD
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        grads = [None] * 4
+        if any(need[:4]):
+            w_gate, w_up, w_down, *x = ctx.saved_tensors
+            x = x[0] if ctx.kept_type is None else Int8Rows(*x, ctx.kept_type)
+            grads = ops.gated_ffn_backward(dy, x, w_gate, w_up, w_down, ctx.act, need[:4])
+        return (*grads, None, dy if need[5] else None, None)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              act: str = "silu", residual: torch.Tensor | None = None, saved=None):
+    """Gated feed-forward block on feature rows: ``(act(x w_gate') * (x w_up')) w_down'``, plus
+    ``residual`` where one is given.  Weights are ``[out, in]`` like ``nn.Linear``'s; ``act`` is
+    ``"silu"``, ``"gelu"`` (exact) or ``"relu"``.
+
+    Of the activations only x is kept for the backward pass: as it is (``saved=None``), as an 8-bit
+    copy made here (``saved="int8"``), or as a copy that the caller has (``saved`` an
+    :class:`Int8Rows`, as ``rms_norm`` returns).  With a copy the gradients are those at the
+    values that it stands for.
+    """
+    if isinstance(saved, Int8Rows):
+        if saved.shape != x.shape or saved.device != x.device:
+            raise ValueError(f"gated_ffn: saved has shape {tuple(saved.shape)} on {saved.device}, "
+                             f"x {tuple(x.shape)} on {x.device}")
+    elif saved not in (None, "int8"):
+        raise ValueError(f"gated_ffn: saved is None, 'int8' or Int8Rows, got {saved!r}")
+    return GatedFFNFunction.apply(x, w_gate, w_up, w_down, act, residual, saved)
 
 
 _MAX_INT32 = 2 ** 31 - 1

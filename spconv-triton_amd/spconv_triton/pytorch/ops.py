@@ -28,6 +28,15 @@ from spconv_triton.pytorch._impl import gemm as _gemm
 from spconv_triton.pytorch._impl import pairs as _pairs
 from spconv_triton.pytorch._impl import pool as _pool
 from spconv_triton.pytorch._impl.pairs import get_conv_output_size, get_deconv_output_size
+from spconv_triton.pytorch._impl.rows import (
+    Int8Rows,
+    gated_ffn,
+    gated_ffn_backward,
+    quantize_rows,
+    restore_rows,
+    rms_norm,
+    rms_norm_backward,
+)
 from spconv_triton.pytorch.core import ThrustSortAllocator
 from spconv_triton.pytorch.cppcore import get_current_stream  # noqa: F401
 from spconv_triton.tools import CPU_ONLY_BUILD, CUDAKernelTimer  # noqa: F401
@@ -39,6 +48,9 @@ DEBUG_INT64_HASH_K = False
 
 __all__ = [
     "ConvAlgo",
+    "Int8Rows",
+    "gated_ffn",
+    "gated_ffn_backward",
     "get_conv_output_size",
     "get_deconv_output_size",
     "get_indice_pairs",
@@ -55,6 +67,10 @@ __all__ = [
     "indice_maxpool_implicit_gemm",
     "indice_maxpool_implicit_gemm_backward",
     "maximum_value_int_",
+    "quantize_rows",
+    "restore_rows",
+    "rms_norm",
+    "rms_norm_backward",
 ]
 
 
