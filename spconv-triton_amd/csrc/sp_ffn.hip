@@ -301,77 +301,177 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_transpose(const T* __restrict
   }
 }
 
-// Partials of a' b over a share of the rows: a [rows, P], b [rows, Q], 64 x 64 of the result a
-// workgroup.  Rows are the reduction: 32 of them a stage, read from LDS one value at a time.
+// ---- weight gradients ------------------------------------------------------------
+// Partials of a' b over a share of the rows: a [rows, P] is of the hidden width, b [rows, Q] of x's
+// or dy's, 128 x TQ of the result a workgroup.  Rows are the MFMA's reduction: 64 of them
+// (fp32: 32) a stage lie in LDS as in memory, 16-bit operands come out of it
+// transposed (ds_read_b64_tr_b16: sixteen lanes take a 4 x 16 block and get a column of it each),
+// fp32 ones value by value.
 template <typename T>
 struct Gram {
   const T *a, *b;
   int64_t lda, ldb;
   int P, Q;
-  int tiles_q, tiles;   // 64 x 64 tiles along Q, and all
-  float* part;          // [shares][P][Q]
+  int tiles_q, tiles;  // tiles along Q, and all
+  int vec_a, vec_b;
+  float* part;  // [shares][P][Q]
 };
 
-constexpr int kGramTile = 64;
-constexpr int kGramRows = 32;
+constexpr int kGramP = 128;
+constexpr int kGramStage = 16384;  // bytes of 128 columns in a stage
 
 template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
-                                                        int64_t share) {
+constexpr int gram_rows() { return kGramStage / (kGramP * int(sizeof(T))); }
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// COLS columns of a stage in LDS.  16-bit rows hold their 16-byte pieces permuted: the four rows that
+// sixteen lanes read at once, 32 bytes of each, fall on different banks, and so do the 64 bytes of
+// each that 32 lanes read.
+template <typename T, int COLS>
+struct GramStage {
   using frag = typename Mfma<T>::frag;
-  constexpr int V = Mfma<T>::V;
-  __shared__ T sa[kGramRows][kGramTile + 2], sb[kGramRows][kGramTile + 2];
+  static constexpr int V = Mfma<T>::V, PER = COLS / V, ROWS = gram_rows<T>();
+  static constexpr int N = ROWS * PER / kFfnThreads;
+  frag r[N];
+
+  __device__ __forceinline__ static int slot(int row, int piece) {
+    if constexpr (sizeof(T) == 4) return piece;
+    if constexpr (COLS == 128) return piece ^ ((row & 1) * 4 + ((row >> 1) & 1) * 10);
+    return piece ^ ((row & 3) << 1);
+  }
+  __device__ __forceinline__ void load(const T* p, int64_t ld, int vec, int64_t m, int64_t hi,
+                                       int c0, int n) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = int(threadIdx.x) + j * kFfnThreads, row = i / PER;
+      const int c = c0 + (i - row * PER) * V;
+      r[j] = frag{};
+      if (m + row >= hi || c >= n) continue;
+      const T* q = p + (m + row) * ld + c;
+      if (vec && c + V <= n) {
+        r[j] = *reinterpret_cast<const frag*>(q);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (c + k < n) r[j][k] = q[k];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = int(threadIdx.x) + j * kFfnThreads, row = i / PER;
+      *reinterpret_cast<frag*>(lds + (row * PER + slot(row, i - row * PER)) * 16) = r[j];
+    }
+  }
+  // columns c0 .. c0 + 31, rows k .. k + 2 V - 1, as the MFMA wants them (rows in one order for
+  // both of its operands)
+  __device__ __forceinline__ static frag read(const char* lds, int k, int c0) {
+    const int lane = int(threadIdx.x) & 63, half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      frag f;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        f[i] = *reinterpret_cast<const T*>(lds + ((k + half * V + i) * COLS + c0 + (lane & 31)) * 4);
+      return f;
+    } else {
+      const int t = lane & 15, c = c0 + (lane & 16) + (t & 3) * 4;
+      union {
+        short4v q[2];
+        frag f;
+      } u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = k + 8 * half + 4 * j + (t >> 2);
+        const char* at = lds + (row * PER + slot(row, c >> 3)) * 16 + (c & 7) * 2;
+        u.q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4v*)(at));
+      }
+      return u.f;
+    }
+  }
+};
+
+template <typename T, int TQ>
+__global__ __launch_bounds__(kFfnThreads, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
+                                                           int64_t share) {
+  using frag = typename Mfma<T>::frag;
+  constexpr int ROWS = gram_rows<T>(), NQ = TQ / 64;
+  constexpr int STAGE = kGramStage + kGramStage / kGramP * TQ;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   int tile = int(blockIdx.x);
   const bool second = tile >= g0.tiles;
-  const Gram<T>& g = second ? g1 : g0;
   if (second) tile -= g0.tiles;
-  const int p0 = tile / g.tiles_q * kGramTile, q0 = tile % g.tiles_q * kGramTile;
+  const Gram<T> g = second ? g1 : g0;
+  const int p0 = tile / g.tiles_q * kGramP, q0 = tile % g.tiles_q * TQ;
   const int64_t lo = int64_t(blockIdx.y) * share;
   const int64_t hi = lo + share < rows ? lo + share : rows;
-  const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 32, wq = (wave & 1) * 32;
-  const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
-  floatx16 acc;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int64_t m = lo; m < hi; m += kGramRows) {
-    for (int i = int(threadIdx.x); i < kGramRows * kGramTile; i += kFfnThreads) {
-      const int r = i / kGramTile, c = i % kGramTile;
-      sa[r][c] = m + r < hi && p0 + c < g.P ? g.a[(m + r) * g.lda + p0 + c] : T(0.f);
-      sb[r][c] = m + r < hi && q0 + c < g.Q ? g.b[(m + r) * g.ldb + q0 + c] : T(0.f);
-    }
+  const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 64, wq = (wave & 1) * (TQ / 2);
+  floatx16 acc[2][NQ];
+  clear(acc);
+  GramStage<T, kGramP> sa;
+  GramStage<T, TQ> sb;
+  auto fetch = [&](int64_t m) {
+    sa.load(g.a, g.lda, g.vec_a, m, hi, p0, g.P);
+    sb.load(g.b, g.ldb, g.vec_b, m, hi, q0, g.Q);
+  };
+  fetch(lo);
+  int s = 0;
+  for (int64_t m = lo; m < hi; m += ROWS, s ^= 1) {
+    char* la = lds + s * STAGE;
+    char* lb = la + kGramStage;
+    sa.store(la);
+    sb.store(lb);
     __syncthreads();
+    if (m + ROWS < hi) fetch(m + ROWS);
 #pragma unroll
-    for (int k = 0; k < kGramRows; k += 2 * V) {
-      frag fa, fb;
+    for (int k = 0; k < ROWS; k += 2 * Mfma<T>::V) {
+      frag fa[2], fb[NQ];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        fa[i] = sa[k + half * V + i][wp + lane];
-        fb[i] = sb[k + half * V + i][wq + lane];
-      }
-      Mfma<T>::mma(fa, fb, acc);
+      for (int i = 0; i < 2; ++i) fa[i] = GramStage<T, kGramP>::read(la, k, wp + 32 * i);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) fb[i] = GramStage<T, TQ>::read(lb, k, wq + 32 * i);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) Mfma<T>::mma(fa[i], fb[j], acc[i][j]);
     }
-    __syncthreads();
   }
   float* part = g.part + int64_t(blockIdx.y) * g.P * g.Q;
+  const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int p = p0 + wp + (i & 3) + 8 * (i >> 2) + 4 * half, q = q0 + wq + lane;
-    if (p < g.P && q < g.Q) part[int64_t(p) * g.Q + q] = acc[i];
-  }
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int p = p0 + wp + 32 * i + (k & 3) + 8 * (k >> 2) + 4 * half;
+        const int q = q0 + wq + 32 * j + lane;
+        if (p < g.P && q < g.Q) part[int64_t(p) * g.Q + q] = acc[i][j][k];
+      }
 }
 
-// dst = the partials of every value in ascending share.  Rows of the partial from `skip_at` on
-// lie `skip` rows further (the second of two padded blocks).
+// The three weight gradients from their partials, in ascending share: dWg and dWu [F][C] from rows
+// 0 and Fp on of the first product, dWd [Co][F] from the second, [F][Co].
 template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part,
-                                                          int64_t stride, int shares, int64_t n,
-                                                          T* __restrict__ dst) {
+__global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part0,
+                                                          const float* __restrict__ part1,
+                                                          int shares, int C, int F, int Fp, int Co,
+                                                          T* __restrict__ dwg, T* __restrict__ dwu,
+                                                          T* __restrict__ dwd) {
   const int64_t i = int64_t(blockIdx.x) * kFfnThreads + threadIdx.x;
-  if (i >= n) return;
+  const int64_t n0 = int64_t(F) * C, n1 = int64_t(F) * Co;
+  const int which = int(blockIdx.y);
+  T* dst = which == 0 ? dwg : which == 1 ? dwu : dwd;
+  if (!dst || i >= (which == 2 ? n1 : n0)) return;
+  const float* p = which == 2 ? part1 + i : part0 + (which ? int64_t(Fp) * C : 0) + i;
+  const int64_t stride = which == 2 ? n1 : 2 * int64_t(Fp) * C;
   float v = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < shares; ++s) v += part[int64_t(s) * stride + i];
-  dst[i] = from_f32<T>(v);
+  for (int s = 0; s < shares; ++s) v += p[int64_t(s) * stride];
+  const int64_t f = i / Co;
+  dst[which == 2 ? (i - f * Co) * F + f : i] = from_f32<T>(v);
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -394,14 +494,16 @@ struct FfnCall {
   hipStream_t stream;
 };
 
-// Shares of the rows in the weight gradients: enough workgroups for the chip, each with 256 rows.
-static int64_t gram_shares(int64_t rows, int64_t tiles) {
-  const int64_t want = cdiv(2048, tiles), most = cdiv(rows, 256);
-  return want < most ? want : most;
-}
+// Columns of a weight gradient's tile: 128, or 64 where both widths fit (half of a 128-wide tile would be
+// idle).
+static int gram_tile_q(int64_t C, int64_t Co) { return C <= 64 && Co <= 64 ? 64 : 128; }
 
-static int64_t gram_tiles(int64_t P, int64_t Q) {
-  return cdiv(P, kGramTile) * cdiv(Q, kGramTile);
+static int64_t gram_tiles(int64_t P, int64_t Q, int tq) { return cdiv(P, kGramP) * cdiv(Q, tq); }
+
+// Shares of the rows in the weight gradients: two workgroups a CU, each with at least 256 rows.
+static int64_t gram_shares(int64_t rows, int64_t tiles) {
+  const int64_t want = cdiv(512, tiles), most = cdiv(rows, 256);
+  return want < most ? want : most;
 }
 
 struct FfnLayout {
@@ -416,7 +518,8 @@ static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t
   const size_t z = size_of(dtype);
   l.Fp = int(cdiv(F, V) * V);
   l.Cop = int(cdiv(Co, V) * V);
-  l.shares = gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C) + gram_tiles(Co, F));
+  const int tq = gram_tile_q(C, Co);
+  l.shares = gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C, tq) + gram_tiles(F, Co, tq));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -466,15 +569,6 @@ static int transpose(const void* src, int rows, int cols, int rows_out, int64_t 
 }
 
 template <typename T>
-static int reduce(const float* part, int64_t stride, int64_t shares, int64_t n, void* dst,
-                  hipStream_t s) {
-  ffn_reduce<T><<<unsigned(cdiv(n, kFfnThreads)), kFfnThreads, 0, s>>>(
-      part, stride, int(shares), n, static_cast<T*>(dst));
-  SP_LAUNCHED();
-  return SP_OK;
-}
-
-template <typename T>
 static int backward(const FfnCall& a, const FfnLayout& l) {
   char* ws = static_cast<char*>(a.ws);
   T* hid = reinterpret_cast<T*>(ws + l.h);
@@ -498,32 +592,37 @@ static int backward(const FfnCall& a, const FfnLayout& l) {
   }
   Gram<T> g0{}, g1{};
   const int64_t ld = 3 * int64_t(l.Fp);
-  if (a.dwg || a.dwu) {
-    g0 = Gram<T>{hid, static_cast<const T*>(a.x), ld, a.ldx, 2 * l.Fp, a.C,
-                 int(cdiv(a.C, kGramTile)), int(gram_tiles(2 * int64_t(l.Fp), a.C)),
-                 reinterpret_cast<float*>(ws + l.part0)};
-  }
-  if (a.dwd) {
-    g1 = Gram<T>{static_cast<const T*>(a.dy), hid + 2 * int64_t(l.Fp), a.lddy, ld, a.Co, a.F,
-                 int(cdiv(a.F, kGramTile)), int(gram_tiles(a.Co, a.F)),
-                 reinterpret_cast<float*>(ws + l.part1)};
-  }
+  const int tq = gram_tile_q(a.C, a.Co);
+  auto gram = [&](const T* h, int P, const void* b, int64_t ldb, int Q, size_t part) {
+    return Gram<T>{h,
+                   static_cast<const T*>(b),
+                   ld,
+                   ldb,
+                   P,
+                   Q,
+                   int(cdiv(Q, tq)),
+                   int(gram_tiles(P, Q, tq)),
+                   1,
+                   aligned(b) && ldb % Mfma<T>::V == 0,
+                   reinterpret_cast<float*>(ws + part)};
+  };
+  if (a.dwg || a.dwu) g0 = gram(hid, 2 * l.Fp, a.x, a.ldx, a.C, l.part0);
+  if (a.dwd) g1 = gram(hid + 2 * int64_t(l.Fp), a.F, a.dy, a.lddy, a.Co, l.part1);
   if (g0.tiles + g1.tiles == 0) return SP_OK;
-  const int64_t share = cdiv(cdiv(a.rows, l.shares), kGramRows) * kGramRows;
+  constexpr int stage = gram_rows<T>();
+  const int64_t share = cdiv(cdiv(a.rows, l.shares), stage) * stage;
   const int64_t shares = cdiv(a.rows, share);
-  ffn_gram<T><<<dim3(unsigned(g0.tiles + g1.tiles), unsigned(shares)), kFfnThreads, 0,
-                a.stream>>>(g0, g1, a.rows, share);
+  const dim3 grid2(unsigned(g0.tiles + g1.tiles), unsigned(shares));
+  if (tq == 64)
+    ffn_gram<T, 64><<<grid2, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
+  else
+    ffn_gram<T, 128><<<grid2, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
   SP_LAUNCHED();
-  const int64_t s0 = 2 * int64_t(l.Fp) * a.C, n0 = int64_t(a.F) * a.C;
-  if (a.dwg)
-    if (int rc = reduce<T>(g0.part, s0, shares, n0, a.dwg, a.stream)) return rc;
-  if (a.dwu)
-    if (int rc = reduce<T>(g0.part + int64_t(l.Fp) * a.C, s0, shares, n0, a.dwu, a.stream))
-      return rc;
-  if (a.dwd)
-    if (int rc = reduce<T>(g1.part, int64_t(a.Co) * a.F, shares, int64_t(a.Co) * a.F, a.dwd,
-                           a.stream))
-      return rc;
+  const int64_t most = int64_t(a.F) * (a.C > a.Co ? a.C : a.Co);
+  ffn_reduce<T><<<dim3(unsigned(cdiv(most, kFfnThreads)), 3), kFfnThreads, 0, a.stream>>>(
+      g0.part, g1.part, int(shares), a.C, a.F, l.Fp, a.Co, static_cast<T*>(a.dwg),
+      static_cast<T*>(a.dwu), static_cast<T*>(a.dwd));
+  SP_LAUNCHED();
   return SP_OK;
 }
 
