@@ -1,0 +1,85 @@
+// What the kernels of the gated feed-forward block share.
+#pragma once
+
+#include "sp_common.h"
+#include "sp_mfma.h"
+
+namespace sp {
+
+constexpr int kFfnThreads = 256;
+constexpr int kTileRows = 128;  // rows of an operand in a stage
+constexpr int kStagePieces = 8;  // 16-byte pieces of a row in a stage: 64 16-bit values
+constexpr int kStageBytes = kTileRows * kStagePieces * 16;
+constexpr int kHiddenTile = 64;  // hidden units of a workgroup where it forms gate and up
+
+enum { kActSilu = 0, kActGelu = 1, kActRelu = 2 };
+
+// 1 / (1 + exp(-z)) from the hardware's exponential and reciprocal, each of about one ulp: for
+// values that are rounded to 16 bits (a fp32 row takes expf and a division).
+__device__ __forceinline__ float sigmoid_fast(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+}
+
+// The gate's activation and its derivative, FAST for 16-bit rows.
+template <bool FAST, int ACT>
+__device__ __forceinline__ void gate(float z, float& value, float& slope) {
+  if constexpr (ACT == kActSilu) {
+    const float sig = FAST ? sigmoid_fast(z) : 1.f / (1.f + expf(-z));
+    value = z * sig;
+    slope = __builtin_fmaf(value, 1.f - sig, sig);
+  } else if constexpr (ACT == kActGelu && FAST) {
+    // Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erfc(x) =
+    // (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0, to 1.5e-7; the exponential is
+    // the derivative's too.
+    const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    const float e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f) * t;
+    const float tail = 0.5f * p * e, cdf = z < 0.f ? tail : 1.f - tail;
+    value = z * cdf;
+    slope = __builtin_fmaf(z * 0.39894228040143268f, e, cdf);
+  } else if constexpr (ACT == kActGelu) {
+    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    value = z * cdf;
+    slope = cdf + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  } else {
+    value = z < 0.f ? 0.f : z;  // (a NaN stays)
+    slope = z > 0.f ? 1.f : 0.f;
+  }
+}
+
+// f(z, value, slope) for the call's activation: one branch around the whole of `loop`.
+template <bool FAST, typename Loop>
+__device__ __forceinline__ void with_gate(int act, Loop&& loop) {
+  if (act == kActSilu)
+    loop([](float z, float& v, float& s) { gate<FAST, kActSilu>(z, v, s); });
+  else if (act == kActGelu)
+    loop([](float z, float& v, float& s) { gate<FAST, kActGelu>(z, v, s); });
+  else
+    loop([](float z, float& v, float& s) { gate<FAST, kActRelu>(z, v, s); });
+}
+
+inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+inline int vec_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 8; }
+inline size_t size_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 2; }
+
+struct FfnCall {
+  const void *x, *wg, *wu, *wd, *residual, *dy;
+  int64_t ldx, ldr, lddy, rows;
+  int C, F, Co, act;
+  void *y, *dx, *dwg, *dwu, *dwd;
+  void* ws;
+  hipStream_t stream;
+};
+
+// The one-kernel forward pass (sp_ffn_fused.hip), for 16-bit rows of at most kFusedWidth channels on either side.
+constexpr int kFusedWidth = 256;
+bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
+size_t fused_forward_workspace(int64_t C, int64_t F, int64_t Co);
+int fused_forward(int32_t dtype, const FfnCall& a);
+
+}  // namespace sp

@@ -9,34 +9,9 @@
 // never leave the registers.  The backward pass forms g, u and dh again in one
 // kernel whose epilogue writes h, dg and du; nothing of the hidden width is kept
 // between the passes.
-#include "sp_common.h"
-#include "sp_mfma.h"
+#include "sp_ffn.h"
 
 namespace sp {
-
-constexpr int kFfnThreads = 256;
-constexpr int kTileRows = 128;  // rows of an operand in a stage
-constexpr int kStagePieces = 8;  // 16-byte pieces of a row in a stage: 64 16-bit values
-constexpr int kStageBytes = kTileRows * kStagePieces * 16;
-constexpr int kHiddenTile = 64;  // hidden units of a workgroup where it forms gate and up
-
-enum { kActSilu = 0, kActGelu = 1, kActRelu = 2 };
-
-// The gate's activation and its derivative.
-__device__ __forceinline__ void gate(int act, float z, float& value, float& slope) {
-  if (act == kActSilu) {
-    const float sig = 1.f / (1.f + expf(-z));
-    value = z * sig;
-    slope = sig * (1.f + z * (1.f - sig));
-  } else if (act == kActGelu) {
-    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    value = z * cdf;
-    slope = cdf + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-  } else {
-    value = z < 0.f ? 0.f : z;  // (a NaN stays)
-    slope = z > 0.f ? 1.f : 0.f;
-  }
-}
 
 // A row-major operand: rows of K values; vec: rows start at multiples of 16 bytes.
 template <typename T>
@@ -194,13 +169,15 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_up(Rows<T> x, Rows<T> wg, Row
   const int wrow[2] = {wn * 32, kHiddenTile + wn * 32};
   products<T, 2>(x, x0, wg, &wu, f0, wrow, wm * 64, lds, acc);
   constexpr int pitch = kHiddenTile * int(sizeof(T)) + 16;
+  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    put_tile<T>(lds, pitch, wm * 64 + 32 * j, wn * 32, [&](int i) {
-      float value, slope;
-      gate(act, acc[j][0][i], value, slope);
-      return value * acc[j][1][i];
-    });
+    for (int j = 0; j < 2; ++j)
+      put_tile<T>(lds, pitch, wm * 64 + 32 * j, wn * 32, [&](int i) {
+        float value, slope;
+        gate(acc[j][0][i], value, slope);
+        return value * acc[j][1][i];
+      });
+  });
   __syncthreads();
   write_rows<T, kHiddenTile>(lds, pitch, h, Fp, x0, x.n, f0, Fp);
 }
@@ -221,17 +198,19 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_grad_hidden(Rows<T> x, Rows<T
   products<T, 2>(x, x0, wg, &wu, f0, wrow, wm * 64, lds, acc);
   products<T, 1>(dy, x0, wdt, nullptr, f0, drow, wm * 64, lds, dh);
   constexpr int pitch = kHiddenTile * int(sizeof(T)) + 16;
+  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float value, slope;
-      gate(act, acc[j][0][i], value, slope);
-      const float u = acc[j][1][i], d = dh[j][0][i];
-      acc[j][0][i] = d * u * slope;
-      acc[j][1][i] = d * value;
-      dh[j][0][i] = value * u;
-    }
+      for (int i = 0; i < 16; ++i) {
+        float value, slope;
+        gate(acc[j][0][i], value, slope);
+        const float u = acc[j][1][i], d = dh[j][0][i];
+        acc[j][0][i] = d * u * slope;
+        acc[j][1][i] = d * value;
+        dh[j][0][i] = value * u;
+      }
+  });
 #pragma unroll
   for (int part = 0; part < 3; ++part) {
     if (part) __syncthreads();
@@ -475,24 +454,10 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restric
 }
 
 // ---- host ------------------------------------------------------------------------
-static bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 template <typename T>
 static Rows<T> operand(const void* p, int64_t ld, int64_t n, int64_t K) {
   return Rows<T>{static_cast<const T*>(p), ld, n, int(K), aligned(p) && ld % Mfma<T>::V == 0};
 }
-
-static int vec_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 8; }
-static size_t size_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 2; }
-
-struct FfnCall {
-  const void *x, *wg, *wu, *wd, *residual, *dy;
-  int64_t ldx, ldr, lddy, rows;
-  int C, F, Co, act;
-  void *y, *dx, *dwg, *dwu, *dwd;
-  void* ws;
-  hipStream_t stream;
-};
 
 // Columns of a weight gradient's tile: 128, or 64 where both widths fit (half of a 128-wide tile would be
 // idle).
@@ -647,6 +612,7 @@ using namespace sp;
 extern "C" size_t sp_gated_ffn_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F,
                                          int64_t Co) {
   if (check_ffn("gated_ffn", dtype, rows, C, F, Co, 0) != SP_OK || rows == 0) return 0;
+  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_forward_workspace(C, F, Co);
   return size_t(rows) * (cdiv(F, vec_of(dtype)) * vec_of(dtype)) * size_of(dtype);
 }
 
@@ -668,6 +634,7 @@ extern "C" int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t r
   a.ldx = ldx, a.ldr = ldr, a.rows = rows;
   a.C = int(C), a.F = int(F), a.Co = int(Co), a.act = act;
   a.y = y, a.ws = ws, a.stream = as_stream(stream);
+  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_forward(dtype, a);
   return dtype == SP_F16 ? forward<_Float16>(a)
                          : dtype == SP_BF16 ? forward<__bf16>(a) : forward<float>(a);
 }
