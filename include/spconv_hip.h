@@ -483,12 +483,16 @@ int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_
                  const void* w_gate, const void* w_up, int64_t F, const void* w_down, int64_t Co,
                  int32_t act, const void* residual, int64_t ldr, void* y, void* ws,
                  size_t ws_bytes, void* stream);
-/* Its gradients from dy [rows, Co]: dx [rows, C], dw_gate, dw_up, dw_down (each nullable).  g, u and
- * the gradient of the hidden rows are formed again; the latter's parts are rounded to the type
- * between the products.  Sums over rows have a fixed order. */
-size_t sp_gated_ffn_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
-int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
-                     int64_t rows, int64_t C, const void* w_gate, const void* w_up, int64_t F,
+/* Its gradients from dy [rows, Co]: dx [rows, C], dw_gate, dw_up, dw_down (each nullable).  Either x, or
+ * codes and scales as sp_quantize_rows makes them (ldx is not read), whose values then stand for
+ * x throughout; `int8` of the workspace query says which.  g, u and the gradient of the
+ * hidden rows are formed again; the latter's parts are rounded to the type between the products.
+ * Sums over rows have a fixed order. */
+size_t sp_gated_ffn_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co,
+                                  int32_t int8);
+int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                     const int8_t* codes, const float* scales, int32_t dtype, int64_t rows,
+                     int64_t C, const void* w_gate, const void* w_up, int64_t F,
                      const void* w_down, int64_t Co, int32_t act, void* dx, void* dw_gate,
                      void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream);
 

@@ -64,6 +64,21 @@ __device__ __forceinline__ void with_gate(int act, Loop&& loop) {
 
 inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// A row-major operand: rows of K values; vec: rows start at multiples of 16 bytes.
+template <typename T>
+struct Rows {
+  const T* p;
+  int64_t ld;
+  int64_t n;  // rows; what lies past them reads as zero
+  int K;
+  int vec;
+};
+
+template <typename T>
+Rows<T> operand(const void* p, int64_t ld, int64_t n, int64_t K) {
+  return Rows<T>{static_cast<const T*>(p), ld, n, int(K), aligned(p) && ld % Mfma<T>::V == 0};
+}
+
 inline int vec_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 8; }
 inline size_t size_of(int32_t dtype) { return dtype == SP_F32 ? 4 : 2; }
 
@@ -71,15 +86,34 @@ struct FfnCall {
   const void *x, *wg, *wu, *wd, *residual, *dy;
   int64_t ldx, ldr, lddy, rows;
   int C, F, Co, act;
+  const int8_t* codes;  // of x, with scales, instead of x itself (backward)
+  const float* scales;
   void *y, *dx, *dwg, *dwu, *dwd;
   void* ws;
   hipStream_t stream;
 };
 
-// The one-kernel forward pass (sp_ffn_fused.hip), for 16-bit rows of at most kFusedWidth channels on either side.
+// The one-kernel passes, for 16-bit rows of at most kFusedWidth channels on either side
+// (sp_ffn_fused.hip, sp_ffn_grad.hip).  `weights`: what copies of weights may take whose rows do not
+// start at multiples of 16 bytes.
 constexpr int kFusedWidth = 256;
+constexpr int kFusedGramWidth = 128;  // the weight gradients' own kernel
+size_t fused_weights_bytes(int64_t C, int64_t F, int64_t Co);
 bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
-size_t fused_forward_workspace(int64_t C, int64_t F, int64_t Co);
 int fused_forward(int32_t dtype, const FfnCall& a);
+
+// The backward pass: dx, and either the weight gradients' partials or the hidden rows for a
+// kernel that makes them (wider than kFusedGramWidth).
+struct FusedGrad {
+  void *weights, *hid;
+  float *part0, *part1;
+  int64_t shares;
+  int Fp;
+};
+bool fused_backward_takes(int32_t dtype, int64_t C, int64_t Co);
+bool fused_weights_take(int32_t dtype, int64_t C, int64_t Co);
+int64_t fused_weights_shares(int64_t rows, int64_t C, int64_t F, int64_t Co);
+// *shares: how many partials there are (at most o.shares)
+int fused_backward(int32_t dtype, const FfnCall& a, const FusedGrad& o, int64_t* shares);
 
 }  // namespace sp

@@ -13,16 +13,6 @@
 
 namespace sp {
 
-// A row-major operand: rows of K values; vec: rows start at multiples of 16 bytes.
-template <typename T>
-struct Rows {
-  const T* p;
-  int64_t ld;
-  int64_t n;  // rows; what lies past them reads as zero
-  int K;
-  int vec;
-};
-
 // Pieces [128 rows][8] of an operand on their way from memory to LDS; thread t holds piece
 // t % 8 of rows t / 8 + 32 j.  In LDS piece c of row r lies at r * 8 + (c ^ (r & 7)),
 // so that the eight lanes that write a row and the rows that an MFMA operand
@@ -431,34 +421,40 @@ __global__ __launch_bounds__(kFfnThreads, 2) void ffn_gram(Gram<T> g0, Gram<T> g
       }
 }
 
-// The three weight gradients from their partials, in ascending share: dWg and dWu [F][C] from rows
-// 0 and Fp on of the first product, dWd [Co][F] from the second, [F][Co].
+// The three weight gradients from their partials: dWg and dWu [F][C] from rows 0 and Fp on of the
+// first product, dWd [Co][F] from the second, [F][Co].  64 values a workgroup, four runs of the shares
+// summed apart and then in order.
 template <typename T>
 __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part0,
                                                           const float* __restrict__ part1,
                                                           int shares, int C, int F, int Fp, int Co,
                                                           T* __restrict__ dwg, T* __restrict__ dwu,
                                                           T* __restrict__ dwd) {
-  const int64_t i = int64_t(blockIdx.x) * kFfnThreads + threadIdx.x;
+  __shared__ float lds[4][64];
+  const int lane = int(threadIdx.x) & 63, run = int(threadIdx.x) >> 6;
+  const int64_t i = int64_t(blockIdx.x) * 64 + lane;
   const int64_t n0 = int64_t(F) * C, n1 = int64_t(F) * Co;
   const int which = int(blockIdx.y);
   T* dst = which == 0 ? dwg : which == 1 ? dwu : dwd;
-  if (!dst || i >= (which == 2 ? n1 : n0)) return;
+  if (!dst) return;
+  const bool in = i < (which == 2 ? n1 : n0);
   const float* p = which == 2 ? part1 + i : part0 + (which ? int64_t(Fp) * C : 0) + i;
   const int64_t stride = which == 2 ? n1 : 2 * int64_t(Fp) * C;
   float v = 0.f;
+  if (in) {
+    const int per = (shares + 3) / 4, end = (run + 1) * per < shares ? (run + 1) * per : shares;
 #pragma unroll 8
-  for (int s = 0; s < shares; ++s) v += p[int64_t(s) * stride];
+    for (int s = run * per; s < end; ++s) v += p[int64_t(s) * stride];
+  }
+  lds[run][lane] = v;
+  __syncthreads();
+  if (run != 0 || !in) return;
+  v = ((lds[0][lane] + lds[1][lane]) + lds[2][lane]) + lds[3][lane];
   const int64_t f = i / Co;
   dst[which == 2 ? (i - f * Co) * F + f : i] = from_f32<T>(v);
 }
 
 // ---- host ------------------------------------------------------------------------
-template <typename T>
-static Rows<T> operand(const void* p, int64_t ld, int64_t n, int64_t K) {
-  return Rows<T>{static_cast<const T*>(p), ld, n, int(K), aligned(p) && ld % Mfma<T>::V == 0};
-}
-
 // Columns of a weight gradient's tile: 128, or 64 where both widths fit (half of a 128-wide tile would be
 // idle).
 static int gram_tile_q(int64_t C, int64_t Co) { return C <= 64 && Co <= 64 ? 64 : 128; }
@@ -471,29 +467,43 @@ static int64_t gram_shares(int64_t rows, int64_t tiles) {
   return want < most ? want : most;
 }
 
+// The backward pass's workspace, and which kernels it takes: for 16-bit rows of up to 128 channels two
+// that form everything again (fused, fused_weights), up to 256 one that also writes the hidden
+// rows, from which ffn_gram makes the weight gradients (fused); else ffn_grad_hidden,
+// ffn_rows and ffn_gram.
 struct FfnLayout {
-  size_t h, wdt, wt, part0, part1, total;
+  bool fused, fused_weights;
+  size_t x, weights, hid, wdt, wt, part0, part1, total;
   int Fp, Cop;
   int64_t shares;
 };
 
-static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co) {
+static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co,
+                                 bool codes) {
   FfnLayout l{};
   const int V = vec_of(dtype);
   const size_t z = size_of(dtype);
+  l.fused = fused_backward_takes(dtype, C, Co);
+  l.fused_weights = fused_weights_take(dtype, C, Co);
   l.Fp = int(cdiv(F, V) * V);
   l.Cop = int(cdiv(Co, V) * V);
   const int tq = gram_tile_q(C, Co);
-  l.shares = gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C, tq) + gram_tiles(F, Co, tq));
+  l.shares = l.fused_weights
+                 ? fused_weights_shares(rows, C, F, Co)
+                 : gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C, tq) + gram_tiles(F, Co, tq));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = align_up(off + bytes, 256);
     return at;
   };
-  l.h = take(size_t(rows) * 3 * l.Fp * z);
-  l.wdt = take(size_t(F) * l.Cop * z);
-  l.wt = take(size_t(C) * 2 * l.Fp * z);
+  if (codes && !l.fused_weights) l.x = take(size_t(rows) * C * z);
+  if (l.fused) l.weights = take(fused_weights_bytes(C, F, Co));
+  if (!l.fused_weights) l.hid = take(size_t(rows) * 3 * l.Fp * z);
+  if (!l.fused) {
+    l.wdt = take(size_t(F) * l.Cop * z);
+    l.wt = take(size_t(C) * 2 * l.Fp * z);
+  }
   l.part0 = take(size_t(l.shares) * 2 * l.Fp * C * sizeof(float));
   l.part1 = take(size_t(l.shares) * Co * F * sizeof(float));
   l.total = off;
@@ -533,59 +543,88 @@ static int transpose(const void* src, int rows, int cols, int rows_out, int64_t 
   return SP_OK;
 }
 
+// dg, du and h of all rows, and dx, by the kernels of their own.
 template <typename T>
-static int backward(const FfnCall& a, const FfnLayout& l) {
+static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
   char* ws = static_cast<char*>(a.ws);
-  T* hid = reinterpret_cast<T*>(ws + l.h);
   T* wdt = reinterpret_cast<T*>(ws + l.wdt);
   T* wt = reinterpret_cast<T*>(ws + l.wt);
   if (int rc = transpose<T>(a.wd, a.Co, a.F, l.Cop, l.Cop, wdt, a.stream)) return rc;
-  if (int rc = transpose<T>(a.wg, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt, a.stream)) return rc;
-  if (int rc = transpose<T>(a.wu, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt + l.Fp, a.stream))
-    return rc;
   const dim3 grid(unsigned(cdiv(a.F, kHiddenTile)), unsigned(cdiv(a.rows, kTileRows)));
   ffn_grad_hidden<T><<<grid, kFfnThreads, 0, a.stream>>>(
       operand<T>(a.x, a.ldx, a.rows, a.C), operand<T>(a.wg, a.C, a.F, a.C),
       operand<T>(a.wu, a.C, a.F, a.C), operand<T>(a.dy, a.lddy, a.rows, a.Co),
       operand<T>(wdt, l.Cop, a.F, a.Co), a.act, hid, l.Fp);
   SP_LAUNCHED();
-  if (a.dx) {
-    if (int rc = launch_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
-                                operand<T>(wt, 2 * int64_t(l.Fp), a.C, 2 * int64_t(l.Fp)),
-                                nullptr, 0, a.dx, a.C, a.stream))
-      return rc;
-  }
+  if (!a.dx) return SP_OK;
+  if (int rc = transpose<T>(a.wg, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt, a.stream)) return rc;
+  if (int rc = transpose<T>(a.wu, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt + l.Fp, a.stream))
+    return rc;
+  return launch_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
+                        operand<T>(wt, 2 * int64_t(l.Fp), a.C, 2 * int64_t(l.Fp)), nullptr, 0,
+                        a.dx, a.C, a.stream);
+}
+
+// The weight gradients' partials from the hidden rows.
+template <typename T>
+static int weight_products(const FfnCall& a, const FfnLayout& l, const T* hid, float* part0,
+                           float* part1, int64_t* shares) {
   Gram<T> g0{}, g1{};
-  const int64_t ld = 3 * int64_t(l.Fp);
   const int tq = gram_tile_q(a.C, a.Co);
-  auto gram = [&](const T* h, int P, const void* b, int64_t ldb, int Q, size_t part) {
-    return Gram<T>{h,
-                   static_cast<const T*>(b),
-                   ld,
-                   ldb,
-                   P,
-                   Q,
-                   int(cdiv(Q, tq)),
-                   int(gram_tiles(P, Q, tq)),
-                   1,
-                   aligned(b) && ldb % Mfma<T>::V == 0,
-                   reinterpret_cast<float*>(ws + part)};
+  auto gram = [&](const T* h, int P, const void* b, int64_t ldb, int Q, float* part) {
+    return Gram<T>{h, static_cast<const T*>(b), 3 * int64_t(l.Fp), ldb, P, Q, int(cdiv(Q, tq)),
+                   int(gram_tiles(P, Q, tq)), 1, aligned(b) && ldb % Mfma<T>::V == 0, part};
   };
-  if (a.dwg || a.dwu) g0 = gram(hid, 2 * l.Fp, a.x, a.ldx, a.C, l.part0);
-  if (a.dwd) g1 = gram(hid + 2 * int64_t(l.Fp), a.F, a.dy, a.lddy, a.Co, l.part1);
-  if (g0.tiles + g1.tiles == 0) return SP_OK;
+  if (a.dwg || a.dwu) g0 = gram(hid, 2 * l.Fp, a.x, a.ldx, a.C, part0);
+  if (a.dwd) g1 = gram(hid + 2 * int64_t(l.Fp), a.F, a.dy, a.lddy, a.Co, part1);
   constexpr int stage = gram_rows<T>();
   const int64_t share = cdiv(cdiv(a.rows, l.shares), stage) * stage;
-  const int64_t shares = cdiv(a.rows, share);
-  const dim3 grid2(unsigned(g0.tiles + g1.tiles), unsigned(shares));
+  *shares = cdiv(a.rows, share);
+  const dim3 grid(unsigned(g0.tiles + g1.tiles), unsigned(*shares));
   if (tq == 64)
-    ffn_gram<T, 64><<<grid2, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 64><<<grid, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
   else
-    ffn_gram<T, 128><<<grid2, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 128><<<grid, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
   SP_LAUNCHED();
+  return SP_OK;
+}
+
+template <typename T>
+static int backward(int32_t dtype, FfnCall a, const FfnLayout& l) {
+  char* ws = static_cast<char*>(a.ws);
+  if (a.codes && !l.fused_weights) {
+    if (int rc = sp_restore_rows(a.codes, a.scales, a.rows, a.C, dtype, ws + l.x, a.stream))
+      return rc;
+    a.x = ws + l.x;
+    a.ldx = a.C;
+    a.codes = nullptr;
+  }
+  const bool weights = a.dwg || a.dwu || a.dwd;
+  float* part0 = reinterpret_cast<float*>(ws + l.part0);
+  float* part1 = reinterpret_cast<float*>(ws + l.part1);
+  T* hid = reinterpret_cast<T*>(ws + l.hid);
+  int64_t shares = 0;
+  if (l.fused) {
+    FusedGrad o{};
+    o.weights = ws + l.weights;
+    o.Fp = l.Fp;
+    o.shares = l.shares;
+    if (!weights) {
+    } else if (l.fused_weights) {
+      o.part0 = part0, o.part1 = part1;
+    } else {
+      o.hid = hid;
+    }
+    if (int rc = fused_backward(dtype, a, o, &shares)) return rc;
+  } else {
+    if (int rc = hidden_and_dx<T>(a, l, hid)) return rc;
+  }
+  if (!weights) return SP_OK;
+  if (!l.fused_weights)
+    if (int rc = weight_products<T>(a, l, hid, part0, part1, &shares)) return rc;
   const int64_t most = int64_t(a.F) * (a.C > a.Co ? a.C : a.Co);
-  ffn_reduce<T><<<dim3(unsigned(cdiv(most, kFfnThreads)), 3), kFfnThreads, 0, a.stream>>>(
-      g0.part, g1.part, int(shares), a.C, a.F, l.Fp, a.Co, static_cast<T*>(a.dwg),
+  ffn_reduce<T><<<dim3(unsigned(cdiv(most, 64)), 3), kFfnThreads, 0, a.stream>>>(
+      part0, part1, int(shares), a.C, a.F, l.Fp, a.Co, static_cast<T*>(a.dwg),
       static_cast<T*>(a.dwu), static_cast<T*>(a.dwd));
   SP_LAUNCHED();
   return SP_OK;
@@ -612,7 +651,7 @@ using namespace sp;
 extern "C" size_t sp_gated_ffn_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F,
                                          int64_t Co) {
   if (check_ffn("gated_ffn", dtype, rows, C, F, Co, 0) != SP_OK || rows == 0) return 0;
-  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_forward_workspace(C, F, Co);
+  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_weights_bytes(C, F, Co);
   return size_t(rows) * (cdiv(F, vec_of(dtype)) * vec_of(dtype)) * size_of(dtype);
 }
 
@@ -640,31 +679,36 @@ extern "C" int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t r
 }
 
 extern "C" size_t sp_gated_ffn_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F,
-                                             int64_t Co) {
+                                             int64_t Co, int32_t int8) {
   if (check_ffn("gated_ffn_bwd", dtype, rows, C, F, Co, 0) != SP_OK || rows == 0) return 0;
-  return backward_layout(dtype, rows, C, F, Co).total;
+  return backward_layout(dtype, rows, C, F, Co, int8 != 0).total;
 }
 
 extern "C" int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
-                                int32_t dtype, int64_t rows, int64_t C, const void* w_gate,
-                                const void* w_up, int64_t F, const void* w_down, int64_t Co,
-                                int32_t act, void* dx, void* dw_gate, void* dw_up, void* dw_down,
-                                void* ws, size_t ws_bytes, void* stream) {
+                                const int8_t* codes, const float* scales, int32_t dtype,
+                                int64_t rows, int64_t C, const void* w_gate, const void* w_up,
+                                int64_t F, const void* w_down, int64_t Co, int32_t act, void* dx,
+                                void* dw_gate, void* dw_up, void* dw_down, void* ws,
+                                size_t ws_bytes, void* stream) {
   if (int rc = check_ffn("gated_ffn_bwd", dtype, rows, C, F, Co, act)) return rc;
   if (rows == 0) return SP_OK;
-  SP_CHECK_ARG(dy && x && w_gate && w_up && w_down && ws, "gated_ffn_bwd: null pointer");
-  SP_CHECK_ARG(ldx >= C && lddy >= Co, "gated_ffn_bwd: rows overlap");
+  SP_CHECK_ARG((x == nullptr) != (codes == nullptr) && (codes == nullptr) == (scales == nullptr),
+               "gated_ffn_bwd: either x or its codes and scales");
+  SP_CHECK_ARG(dy && w_gate && w_up && w_down && ws, "gated_ffn_bwd: null pointer");
+  SP_CHECK_ARG((codes || ldx >= C) && lddy >= Co, "gated_ffn_bwd: rows overlap");
   SP_CHECK_ARG(aligned(ws), "gated_ffn_bwd: the workspace must be 16-byte aligned");
-  const FfnLayout l = backward_layout(dtype, rows, C, F, Co);
+  const FfnLayout l = backward_layout(dtype, rows, C, F, Co, codes != nullptr);
   if (ws_bytes < l.total)
     return set_error(SP_ERR_WORKSPACE, "gated_ffn_bwd: workspace of %zu bytes, needs %zu",
                      ws_bytes, l.total);
   FfnCall a{};
   a.dy = dy, a.x = x, a.wg = w_gate, a.wu = w_up, a.wd = w_down;
   a.ldx = ldx, a.lddy = lddy, a.rows = rows;
+  a.codes = codes, a.scales = scales;
   a.C = int(C), a.F = int(F), a.Co = int(Co), a.act = act;
   a.dx = dx, a.dwg = dw_gate, a.dwu = dw_up, a.dwd = dw_down;
   a.ws = ws, a.stream = as_stream(stream);
-  return dtype == SP_F16 ? backward<_Float16>(a, l)
-                         : dtype == SP_BF16 ? backward<__bf16>(a, l) : backward<float>(a, l);
+  return dtype == SP_F16 ? backward<_Float16>(dtype, a, l)
+                         : dtype == SP_BF16 ? backward<__bf16>(dtype, a, l)
+                                            : backward<float>(dtype, a, l);
 }

@@ -146,9 +146,9 @@ _SIGNATURES = {
     "sp_gated_ffn_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64]),
     "sp_gated_ffn": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P,
                                     _I64, _P, _P, _SZ, _P]),
-    "sp_gated_ffn_bwd_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64]),
-    "sp_gated_ffn_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _I64, _P,
-                                        _I64, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "sp_gated_ffn_bwd_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I32]),
+    "sp_gated_ffn_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _I32, _I64, _I64, _P, _P, _I64,
+                                        _P, _I64, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
     "sp_maxpool_fwd": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P]),
     "sp_maxpool_bwd": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P]),
     "sp_avgpool_fwd": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P, _P]),

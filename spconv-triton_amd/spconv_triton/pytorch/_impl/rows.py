@@ -185,7 +185,10 @@ def restore_rows(kept: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tens
 # ---------------------------------------------------------------------------
 
 def check_ffn(x, w_gate, w_up, w_down, act, residual) -> None:
-    _check_rows("gated_ffn", "x", x)
+    if isinstance(x, Int8Rows):
+        _lib.require_gpu(x.codes)
+    else:
+        _check_rows("gated_ffn", "x", x)
     if act not in ACTIVATIONS:
         raise ValueError(f"gated_ffn: unknown activation {act!r} ({', '.join(ACTIVATIONS)})")
     if w_gate.dim() != 2 or w_gate.shape[0] == 0 or w_down.dim() != 2 or w_down.shape[0] == 0:
@@ -221,14 +224,15 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, act: str = "silu",
                        need=(True, True, True, True)):
     """Gradients of x, w_gate, w_up and w_down (None where ``need`` is false).  ``x``: the rows,
     or their ``Int8Rows``, whose values then stand for them throughout."""
-    if isinstance(x, Int8Rows):
-        x = restore_rows(x)
     check_ffn(x, w_gate, w_up, w_down, act, None)
     n, c = x.shape
     hidden, c_out = w_gate.shape[0], w_down.shape[0]
     _check_like("gated_ffn_backward", "dy", dy, (n, c_out), x)
-    x, ldx = _strided(x)
     dy, lddy = _strided(dy)
+    if isinstance(x, Int8Rows):
+        rows, ldx, codes, scales = None, 0, x.codes, x.scales
+    else:
+        (rows, ldx), codes, scales = _strided(x), None, None
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     make = torch.zeros_like if n == 0 else torch.empty_like
     dx = torch.empty((n, c), dtype=x.dtype, device=x.device) if need[0] else None
@@ -236,11 +240,12 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, act: str = "silu",
                      for w, k in zip((w_gate, w_up, w_down), need[1:]))
     if n and any(need):
         code = _lib.dtype_code(x.dtype)
-        nbytes = _lib.lib().sp_gated_ffn_bwd_workspace(code, n, c, hidden, c_out)
+        nbytes = _lib.lib().sp_gated_ffn_bwd_workspace(code, n, c, hidden, c_out,
+                                                       codes is not None)
         ws = _lib.workspace(nbytes, x.device)
         _lib.check(_lib.lib().sp_gated_ffn_bwd(
-            _lib.ptr(dy), lddy, _lib.ptr(x), ldx, code, n, c, _lib.ptr(w_gate), _lib.ptr(w_up),
-            hidden, _lib.ptr(w_down), c_out, ACTIVATIONS[act], _lib.ptr(dx), _lib.ptr(dwg),
-            _lib.ptr(dwu), _lib.ptr(dwd), _lib.ptr(ws), nbytes, _lib.stream_of(x.device)),
-            "sp_gated_ffn_bwd")
+            _lib.ptr(dy), lddy, _lib.ptr(rows), ldx, _lib.ptr(codes), _lib.ptr(scales), code, n,
+            c, _lib.ptr(w_gate), _lib.ptr(w_up), hidden, _lib.ptr(w_down), c_out,
+            ACTIVATIONS[act], _lib.ptr(dx), _lib.ptr(dwg), _lib.ptr(dwu), _lib.ptr(dwd),
+            _lib.ptr(ws), nbytes, _lib.stream_of(x.device)), "sp_gated_ffn_bwd")
     return dx, dwg, dwu, dwd

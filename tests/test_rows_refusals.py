@@ -71,14 +71,16 @@ def test_bad_sizes_and_workspaces_are_refused():
         assert ffn(**kw) == bad, kw
     if need:
         assert ffn(nbytes=need - 1) == ws_err
-    need = L.sp_gated_ffn_bwd_workspace(f16, 100, 64, 172, 64)
-    assert need > 0 and L.sp_gated_ffn_bwd_workspace(f16, 0, 64, 172, 64) == 0
+    need = L.sp_gated_ffn_bwd_workspace(f16, 100, 64, 172, 64, 0)
+    assert need > 0 and L.sp_gated_ffn_bwd_workspace(f16, 0, 64, 172, 64, 0) == 0
 
-    def back(nbytes=need, lddy=64, ws=p):
-        return L.sp_gated_ffn_bwd(p, lddy, p, 64, f16, 100, 64, p, p, 172, p, 64, 0, p, p, p, p,
-                                  ws, nbytes, None)
+    def back(nbytes=need, lddy=64, ws=p, x=p, codes=None, scales=None, ldx=64):
+        return L.sp_gated_ffn_bwd(p, lddy, x, ldx, codes, scales, f16, 100, 64, p, p, 172, p, 64,
+                                  0, p, p, p, p, ws, nbytes, None)
 
     assert back(nbytes=need - 1) == ws_err and back(lddy=63) == bad and back(ws=odd) == bad
+    assert back(ldx=63) == bad and back(x=None) == bad and back(codes=p, scales=p) == bad
+    assert back(x=None, codes=p) == bad and back(x=None, scales=p) == bad
 
 
 def test_modules_build_and_reload():
