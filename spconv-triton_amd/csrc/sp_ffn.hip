@@ -14,9 +14,7 @@
 namespace sp {
 
 // Pieces [128 rows][8] of an operand on their way from memory to LDS; thread t holds piece
-// t % 8 of rows t / 8 + 32 j.  In LDS piece c of row r lies at r * 8 + (c ^ (r & 7)),
-// so that the eight lanes that write a row and the rows that an MFMA operand
-// reads (one piece of 32 rows) spread over all banks.
+// t % 8 of rows t / 8 + 32 j.
 template <typename T>
 struct Stage {
   using frag = typename Mfma<T>::frag;
@@ -53,11 +51,11 @@ struct Stage {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = t + 32 * j;
-      *reinterpret_cast<frag*>(lds + (row * 8 + (c ^ (row & 7))) * 16) = r[j];
+      *reinterpret_cast<frag*>(lds + (row * 8 + swizzled<8>(row, c)) * 16) = r[j];
     }
   }
   __device__ __forceinline__ static frag read(const char* lds, int row, int c) {
-    return *reinterpret_cast<const frag*>(lds + (row * 8 + (c ^ (row & 7))) * 16);
+    return *reinterpret_cast<const frag*>(lds + (row * 8 + swizzled<8>(row, c)) * 16);
   }
 };
 

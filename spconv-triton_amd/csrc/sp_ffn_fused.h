@@ -14,15 +14,6 @@ __device__ __forceinline__ int unit_of(int m) {
   return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);
 }
 
-// Where piece c (16 bytes) of row r lies in LDS rows of PIECES pieces.  Rows of whole 128 bytes are
-// permuted by three bits of r, others by two, so that both kinds of reads meet different banks: one
-// piece of eight rows (16 bytes a lane), and 32 or 64 bytes of four rows (transposed).
-template <int PIECES>
-__device__ __forceinline__ int swizzled(int r, int c) {
-  if constexpr (PIECES % 8 == 0) return c ^ (((r & 3) << 1) | ((r >> 2) & 1));
-  return c ^ ((r & 2) | ((r >> 2) & 1));
-}
-
 __device__ const uint4 g_zero_piece = {0, 0, 0, 0};
 
 // 16 bytes from memory to LDS at `to` (the wave's first lane's) + 16 * lane.
@@ -32,9 +23,10 @@ __device__ __forceinline__ void copy_piece(const void* from, char* to) {
       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-__device__ __forceinline__ void copies_done() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+// At most N of the wave's loads still on their way.
+template <int N>
+__device__ __forceinline__ void loads_in_flight() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // The weights as they lie in memory: rows of ldu (g, u) and ldd (d) elements.
@@ -50,49 +42,78 @@ struct Weights {
 // bytes each.
 template <int CP>
 struct Chunk {
-  static constexpr int UP = CP / 8;         // pieces of a Wg or Wu row
-  static constexpr int MATRIX = CP * 4;     // pieces of a matrix
-  static constexpr int BYTES = 3 * MATRIX * 16;
+  static constexpr int UP = CP / 8;      // pieces of a Wg or Wu row
+  static constexpr int MATRIX = CP * 4;  // pieces of a matrix
+  static constexpr int ROUNDS = (MATRIX + kFfnThreads - 1) / kFfnThreads;
+  static constexpr int LOADS = 3 * ROUNDS;  // of every wave
+  // a matrix in LDS, with what the last round writes past it
+  static constexpr int STRIDE = ROUNDS * kFfnThreads * 16;
+  static constexpr int BYTES = 3 * STRIDE;
 
-  __device__ __forceinline__ static const char* up(const char* chunk, int m, int c) {
-    return chunk + (m * UP + swizzled<UP>(m & 31, c)) * 16;
+  __device__ __forceinline__ static const char* up(const char* chunk, int which, int m, int c) {
+    return chunk + which * STRIDE + (m * UP + swizzled<UP>(m, c)) * 16;
   }
   __device__ __forceinline__ static const char* down(const char* chunk, int m, int c) {
-    return chunk + (2 * MATRIX + m * 4 + swizzled<4>(m, c)) * 16;
+    return chunk + 2 * STRIDE + (m * 4 + swizzled<4>(m, c)) * 16;
   }
 
-  // Loads a chunk.  Whole chunks of whole matrices take addresses of one part that is the
-  // wave's and one that is the lane's for good; the others go by piece, zeros past the ends.
+  // Loads a chunk, every wave with as many loads, also past the last chunk and the matrices (zeros),
+  // so that a wave knows how many are younger than a chunk's.  Whole chunks of whole matrices take
+  // addresses of one part that is the wave's and one that is the lane's for good.
   template <typename T>
   __device__ __forceinline__ static void load(const Weights<T>& w, int f0, char* to) {
-    constexpr int THREADS = kFfnThreads, LOADS = (MATRIX + THREADS - 1) / THREADS;
     const int tid = int(threadIdx.x);
-    const bool whole = f0 + 32 <= w.Fw && w.C == CP && w.Cow == CP;
+    const bool whole = MATRIX % kFfnThreads == 0 && f0 + 32 <= w.Fw && w.C == CP && w.Cow == CP;
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int i = j * THREADS + tid;
-      if (LOADS * THREADS > MATRIX && i >= MATRIX) break;  // (whole waves)
-      const int mu = i / UP, cu = swizzled<UP>(mu, i - mu * UP) * 8, fu = unit_of(mu);
+    for (int j = 0; j < ROUNDS; ++j) {
+      const int i = j * kFfnThreads + tid;
+      const int mu = i / UP, cu = swizzled<UP>(mu, i - mu * UP) * 8, fu = unit_of(mu & 31);
       const int md = i >> 2, fd = swizzled<4>(md, i & 3) * 8, cd = (md & ~31) + unit_of(md & 31);
       const unsigned ou = unsigned(fu * w.ldu + cu), od = unsigned(cd * w.ldd + fd);
-      const T* bu = w.g + int64_t(f0) * w.ldu;
-      const T* bv = w.u + int64_t(f0) * w.ldu;
+      const T* bg = w.g + int64_t(f0) * w.ldu;
+      const T* bu = w.u + int64_t(f0) * w.ldu;
       const T* bd = w.d + f0;
       char* at = to + (i - (tid & 63)) * 16;
       if (whole) {
-        copy_piece(bu + ou, at);
-        copy_piece(bv + ou, at + MATRIX * 16);
-        copy_piece(bd + od, at + 2 * MATRIX * 16);
+        copy_piece(bg + ou, at);
+        copy_piece(bu + ou, at + STRIDE);
+        copy_piece(bd + od, at + 2 * STRIDE);
       } else {
-        const bool in = f0 + fu < w.Fw && cu < w.C;
+        const bool in = i < MATRIX && f0 + fu < w.Fw && cu < w.C;
+        const bool ind = i < MATRIX && cd < w.Cow && f0 + fd < w.Fw;
         const void* zero = &g_zero_piece;
-        copy_piece(in ? static_cast<const void*>(bu + ou) : zero, at);
-        copy_piece(in ? static_cast<const void*>(bv + ou) : zero, at + MATRIX * 16);
-        copy_piece(cd < w.Cow && f0 + fd < w.Fw ? static_cast<const void*>(bd + od) : zero,
-                   at + 2 * MATRIX * 16);
+        copy_piece(in ? static_cast<const void*>(bg + ou) : zero, at);
+        copy_piece(in ? static_cast<const void*>(bu + ou) : zero, at + STRIDE);
+        copy_piece(ind ? static_cast<const void*>(bd + od) : zero, at + 2 * STRIDE);
       }
     }
   }
+};
+
+// The chunks of a call's weights, N of them in LDS: `first` starts N - 1; `next` waits for a chunk, for all
+// waves' loads of it, and starts the one N - 1 further into the buffer that all waves have left; `done` waits for
+// the loads past the end, which may not outlive the workgroup.
+template <typename T, int CP, int N>
+struct Chunks {
+  using C = Chunk<CP>;
+  const Weights<T>& w;
+  char* lds;
+  int f, at;
+  __device__ __forceinline__ Chunks(const Weights<T>& w_, char* lds_) : w(w_), lds(lds_), f(0), at(0) {
+#pragma unroll
+    for (int i = 0; i + 1 < N; ++i) C::load(w, 32 * i, lds + i * C::BYTES);
+  }
+  __device__ __forceinline__ const char* next() {
+    loads_in_flight<(N - 2) * C::LOADS>();
+    __syncthreads();
+    const int into = at == 0 ? N - 1 : at - 1;
+    C::load(w, f + 32 * (N - 1), lds + into * C::BYTES);
+    const char* chunk = lds + at * C::BYTES;
+    at = at + 1 == N ? 0 : at + 1;
+    f += 32;
+    return chunk;
+  }
+  __device__ __forceinline__ void done() { loads_in_flight<0>(); }
 };
 
 // A lane's 8 values of a row; past n zeros.
@@ -118,6 +139,39 @@ __device__ __forceinline__ void load_rows(const Rows<T>& x, int64_t r,
   }
 }
 
+// STEPS steps of products whose operands F come from LDS, B steps' reads at a time: a batch is read while the
+// one before is in use.  Left to itself the compiler reads and waits step by step (LDS latency
+// each time; 1.6 times the time of a 256-channel call).  `start` may come early.
+template <typename F, int STEPS, int B>
+struct Batched {
+  static constexpr int BATCHES = (STEPS + B - 1) / B;
+  F f[2][B];
+  template <typename Read>
+  __device__ __forceinline__ void start(Read&& read) {
+#pragma unroll
+    for (int i = 0; i < B && i < STEPS; ++i) f[0][i] = read(i);
+  }
+  template <typename Read, typename Use>
+  __device__ __forceinline__ void run(Read&& read, Use&& use) {
+#pragma unroll
+    for (int b = 0; b < BATCHES; ++b) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if ((b + 1) * B + i < STEPS) f[(b + 1) & 1][i] = read((b + 1) * B + i);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (b * B + i < STEPS) use(b * B + i, f[b & 1][i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+};
+
+template <typename T>
+struct FragPair {
+  typename Mfma<T>::frag a, b;
+};
+
 // 32 hidden units of a wave's 32 rows: their gate and up values, ...
 template <typename T, int CP>
 __device__ __forceinline__ void fused_up(const char* chunk,
@@ -125,32 +179,19 @@ __device__ __forceinline__ void fused_up(const char* chunk,
                                          floatx16& u) {
   using frag = typename Mfma<T>::frag;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
+  auto read = [&](int k) {
+    return FragPair<T>{
+        *reinterpret_cast<const frag*>(Chunk<CP>::up(chunk, 0, lane, 2 * k + half)),
+        *reinterpret_cast<const frag*>(Chunk<CP>::up(chunk, 1, lane, 2 * k + half))};
+  };
+  Batched<FragPair<T>, CP / 16, 4> w;
+  w.start(read);
 #pragma unroll
   for (int i = 0; i < 16; ++i) g[i] = u[i] = 0.f;
-#pragma unroll
-  for (int k = 0; k < CP / 16; ++k) {
-    const frag fg = *reinterpret_cast<const frag*>(Chunk<CP>::up(chunk, lane, 2 * k + half));
-    const frag fu = *reinterpret_cast<const frag*>(Chunk<CP>::up(chunk, lane + 32, 2 * k + half));
-    Mfma<T>::mma(fg, x[k], g);
-    Mfma<T>::mma(fu, x[k], u);
-  }
-}
-
-// ... and what they add to y.
-template <typename T, int CP>
-__device__ __forceinline__ void fused_down(const char* chunk,
-                                           const typename Mfma<T>::frag (&h)[2],
-                                           floatx16 (&y)[CP / 32]) {
-  using frag = typename Mfma<T>::frag;
-  const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
-#pragma unroll
-  for (int t = 0; t < CP / 32; ++t)
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const frag fd = *reinterpret_cast<const frag*>(
-          Chunk<CP>::down(chunk, t * 32 + lane, 2 * s + half));
-      Mfma<T>::mma(fd, h[s], y[t]);
-    }
+  w.run(read, [&](int k, const FragPair<T>& f) {
+    Mfma<T>::mma(f.a, x[k], g);
+    Mfma<T>::mma(f.b, x[k], u);
+  });
 }
 
 template <int N>

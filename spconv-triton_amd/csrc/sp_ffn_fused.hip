@@ -56,34 +56,34 @@ __device__ __forceinline__ void fused_store(const FusedArgs<T>& a, int64_t r,
     }
 }
 
-// CP: channels of x and y, rounded up to 32.  The chunks pass through two buffers.
-template <typename T, int ACT, int CP, int MINW>
+// CP: channels of x and y, rounded up to 32.  N: chunks in LDS.
+template <typename T, int ACT, int CP, int N, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   using frag = typename Mfma<T>::frag;
-  __shared__ __attribute__((aligned(16))) char lds[2][Chunk<CP>::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds[N * Chunk<CP>::BYTES];
   const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 31;
+  const int half = (int(threadIdx.x) >> 5) & 1;
   const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * kFusedRows + lane;
-  Chunk<CP>::load(a.w, 0, lds[0]);
+  Chunks<T, CP, N> chunks(a.w, lds);
   frag x[CP / 16];
   load_rows<T, CP>(a.x, r, x);
   floatx16 y[CP / 32];
   clear_rows(y);
-  copies_done();
-  int buf = 0;
-  for (int f0 = 0; f0 < a.w.F; f0 += 32, buf ^= 1) {
-    if (f0 + 32 < a.w.F) Chunk<CP>::load(a.w, f0 + 32, lds[buf ^ 1]);
+  for (int f0 = 0; f0 < a.w.F; f0 += 32) {
+    const char* chunk = chunks.next();
     floatx16 g, u;
-    fused_up<T, CP>(lds[buf], x, g, u);
+    fused_up<T, CP>(chunk, x, g, u);
+    auto read = [&](int i) {  // Wd's 32 channels i / 2, its 16 hidden units i % 2
+      return *reinterpret_cast<const frag*>(
+          Chunk<CP>::down(chunk, (i >> 1) * 32 + lane, 2 * (i & 1) + half));
+    };
+    Batched<frag, CP / 16, 4> down;
+    down.start(read);
     frag h[2];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float value, slope;
-      gate<true, ACT>(g[i], value, slope);
-      h[i >> 3][i & 7] = T(value * u[i]);
-    }
-    fused_down<T, CP>(lds[buf], h, y);
-    copies_done();
+    gate16<ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
+    down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i & 1], y[i >> 1]); });
   }
+  chunks.done();
   fused_store<T, CP>(a, r, y);
 }
 
@@ -119,14 +119,14 @@ size_t fused_weights_bytes(int64_t C, int64_t F, int64_t Co) {
   return (2 * size_t(up8(F)) * up8(C) + size_t(up8(Co)) * up8(F)) * 2;
 }
 
-template <typename T, int CP, int MINW>
+template <typename T, int CP, int N, int MINW>
 static int launch_fused(const FusedArgs<T>& a, int act, hipStream_t s) {
   const int64_t tiles = cdiv(a.x.n, kFusedRows);
   SP_CHECK_ARG(tiles <= kMaxGridX, "gated_ffn: too many rows");
   using Kern = void (*)(FusedArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused<T, kActSilu, CP, MINW>)
-                    : act == kActGelu ? Kern(ffn_fused<T, kActGelu, CP, MINW>)
-                                      : Kern(ffn_fused<T, kActRelu, CP, MINW>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused<T, kActSilu, CP, N, MINW>)
+                    : act == kActGelu ? Kern(ffn_fused<T, kActGelu, CP, N, MINW>)
+                                      : Kern(ffn_fused<T, kActRelu, CP, N, MINW>);
   kern<<<unsigned(cdiv(tiles, 4)), kFfnThreads, 0, s>>>(a);
   SP_LAUNCHED();
   return SP_OK;
@@ -168,13 +168,13 @@ static int run_fused(const FfnCall& c) {
   a.vec_y = aligned(c.y) && c.Co % 8 == 0;
   if (int rc = fused_weights(c, static_cast<T*>(c.ws), a.w)) return rc;
   const int widest = c.C > c.Co ? c.C : c.Co;
-  if (widest <= 32) return launch_fused<T, 32, 4>(a, c.act, c.stream);
-  if (widest <= 64) return launch_fused<T, 64, 4>(a, c.act, c.stream);
-  if (widest <= 96) return launch_fused<T, 96, 3>(a, c.act, c.stream);
-  if (widest <= 128) return launch_fused<T, 128, 2>(a, c.act, c.stream);
-  if (widest <= 160) return launch_fused<T, 160, 2>(a, c.act, c.stream);
-  if (widest <= 192) return launch_fused<T, 192, 2>(a, c.act, c.stream);
-  return launch_fused<T, 256, 1>(a, c.act, c.stream);
+  if (widest <= 32) return launch_fused<T, 32, 2, 4>(a, c.act, c.stream);
+  if (widest <= 64) return launch_fused<T, 64, 2, 4>(a, c.act, c.stream);
+  if (widest <= 96) return launch_fused<T, 96, 2, 3>(a, c.act, c.stream);
+  if (widest <= 128) return launch_fused<T, 128, 2, 2>(a, c.act, c.stream);
+  if (widest <= 160) return launch_fused<T, 160, 2, 2>(a, c.act, c.stream);
+  if (widest <= 192) return launch_fused<T, 192, 2, 2>(a, c.act, c.stream);
+  return launch_fused<T, 256, 2, 1>(a, c.act, c.stream);
 }
 
 int fused_forward(int32_t dtype, const FfnCall& a) {

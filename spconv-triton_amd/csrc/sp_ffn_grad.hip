@@ -94,53 +94,50 @@ __device__ __forceinline__ typename Mfma<T>::frag x_piece(const GradArgs<T>& a, 
                       : row_piece<T>(a.x.p + r * a.x.ld, c, a.x.K, a.x.vec);
 }
 
-template <typename T, int ACT, int CP, bool HIDDEN, int MINW>
+template <typename T, int ACT, int CP, int N, bool HIDDEN, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a) {
   using frag = typename Mfma<T>::frag;
   using C = Chunk<CP>;
-  __shared__ __attribute__((aligned(16))) char lds[2][C::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds[N * C::BYTES];
   const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 31;
   const int half = (int(threadIdx.x) >> 5) & 1;
   const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * kFusedRows + lane;
-  C::load(a.w, 0, lds[0]);
+  Chunks<T, CP, N> chunks(a.w, lds);
   frag x[CP / 16], dy[CP / 16];
 #pragma unroll
   for (int k = 0; k < CP / 16; ++k) x[k] = x_piece(a, r, k * 16 + half * 8);
   load_rows<T, CP>(a.dy, r, dy);
   floatx16 dx[CP / 32];
   clear_rows(dx);
-  copies_done();
-  int buf = 0;
-  for (int f0 = 0; f0 < a.w.F; f0 += 32, buf ^= 1) {
-    if (f0 + 32 < a.w.F) C::load(a.w, f0 + 32, lds[buf ^ 1]);
-    const char* chunk = lds[buf];
+  for (int f0 = 0; f0 < a.w.F; f0 += 32) {
+    const char* chunk = chunks.next();
     floatx16 g, u, dh;
     fused_up<T, CP>(chunk, x, g, u);
 #pragma unroll
     for (int i = 0; i < 16; ++i) dh[i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < CP / 16; ++k)
-      Mfma<T>::mma(columns_of<T>([&](int m, int c) { return C::down(chunk, m, c); }, k, 0), dy[k],
-                   dh);
+    auto down = [&](int k) {
+      return columns_of<T>([&](int m, int c) { return C::down(chunk, m, c); }, k, 0);
+    };
+    Batched<frag, CP / 16, 4> wd;
+    wd.start(down);
+    wd.run(down, [&](int k, const frag& f) { Mfma<T>::mma(f, dy[k], dh); });
+    auto up = [&](int i) {  // Wg's and Wu's 32 channels i / 2, 16 hidden units i % 2
+      return FragPair<T>{
+          columns_of<T>([&](int m, int c) { return C::up(chunk, 0, m, c); }, i & 1, 4 * (i >> 1)),
+          columns_of<T>([&](int m, int c) { return C::up(chunk, 1, m, c); }, i & 1, 4 * (i >> 1))};
+    };
+    Batched<FragPair<T>, CP / 16, 2> wgu;
+    wgu.start(up);
     frag dg[2], du[2], h[2];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float value, slope;
-      gate<true, ACT>(g[i], value, slope);
+    gate16<ACT>(g, [&](int i, float value, float slope) {
       dg[i >> 3][i & 7] = T(dh[i] * u[i] * slope);
       du[i >> 3][i & 7] = T(dh[i] * value);
       if (HIDDEN) h[i >> 3][i & 7] = T(value * u[i]);
-    }
-#pragma unroll
-    for (int t = 0; t < CP / 32; ++t)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        Mfma<T>::mma(columns_of<T>([&](int m, int c) { return C::up(chunk, m, c); }, s, 4 * t),
-                     dg[s], dx[t]);
-        Mfma<T>::mma(columns_of<T>([&](int m, int c) { return C::up(chunk, m + 32, c); }, s,
-                                   4 * t),
-                     du[s], dx[t]);
-      }
+    });
+    wgu.run(up, [&](int i, const FragPair<T>& f) {
+      Mfma<T>::mma(f.a, dg[i & 1], dx[i >> 1]);
+      Mfma<T>::mma(f.b, du[i & 1], dx[i >> 1]);
+    });
     if (HIDDEN && a.hid && r < a.x.n) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -153,8 +150,8 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a)
         }
       }
     }
-    copies_done();
   }
+  chunks.done();
   if (!a.dx || r >= a.x.n) return;
 #pragma unroll
   for (int t = 0; t < CP / 32; ++t)
@@ -209,12 +206,12 @@ struct RowTile {
   }
 };
 
-// A workgroup: 128 hidden units (four waves of 32) and a share of the rows, HALVES tiles of 32 rows at a
-// time, each by four waves of its own.
-template <typename T, int ACT, int CP, int HALVES>
+// A workgroup: 128 hidden units (four waves of 32) and a share of the rows, HALVES * U tiles of 32 rows
+// between barriers, U of them for each four waves.
+template <typename T, int ACT, int CP, int HALVES, int U>
 __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradArgs<T> a) {
   using frag = typename Mfma<T>::frag;
-  constexpr int THREADS = kFfnThreads * HALVES, ROWS = kFusedRows * HALVES, UP = CP / 8;
+  constexpr int THREADS = kFfnThreads * HALVES, ROWS = kFusedRows * HALVES * U, UP = CP / 8;
   constexpr int K = CP / 16, TILES = CP / 32;
   using Tile = RowTile<T, CP, THREADS, ROWS>;
   constexpr int JOIN = HALVES > 1 ? 4 * TILES * 4096 : 0;  // a matrix of four waves
@@ -249,46 +246,49 @@ __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradAr
     tile.store(at);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) tile.load(a, m + ROWS, hi);
-    const char* xs = at + (wave >> 2) * (kFusedRows * UP * 16);
+    const char* xs = at + (wave >> 2) * (U * kFusedRows * UP * 16);
     const char* ds = xs + Tile::BYTES;
-    floatx16 g, u, dh;
+    floatx16 g[U], u[U], dh[U];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) g[i] = u[i] = dh[i] = 0.f;
+    for (int n = 0; n < U; ++n) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int piece = (lane * UP + swizzled<UP>(lane, 2 * k + half)) * 16;
-      const frag fx = *reinterpret_cast<const frag*>(xs + piece);
-      const frag fd = *reinterpret_cast<const frag*>(ds + piece);
-      Mfma<T>::mma(fx, wg[k], g);
-      Mfma<T>::mma(fx, wu[k], u);
-      Mfma<T>::mma(fd, wd[k], dh);
-    }
-    // register 8 s + j of lane half b holds row 16 s + 8 (j >> 2) + 4 b + (j & 3) of the tile
-    frag dg[2], du[2], h[2];
+      for (int i = 0; i < 16; ++i) g[n][i] = u[n][i] = dh[n][i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float value, slope;
-      gate<true, ACT>(g[i], value, slope);
-      dg[i >> 3][i & 7] = T(dh[i] * u[i] * slope);
-      du[i >> 3][i & 7] = T(dh[i] * value);
-      h[i >> 3][i & 7] = T(value * u[i]);
-    }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        // columns 32 t .. of those rows
-        const int l = int(threadIdx.x) & 15;
-        const int col = 4 * t + 2 * ((int(threadIdx.x) >> 4) & 1) + ((l >> 1) & 1);
-        const int row = 16 * s + 4 * half + (l >> 2);
-        const int p0 = (row * UP + swizzled<UP>(row, col)) * 16 + (l & 1) * 8;
-        const int p1 = ((row + 8) * UP + swizzled<UP>(row + 8, col)) * 16 + (l & 1) * 8;
-        const frag fx = read_transposed<T>(xs + p0, xs + p1);
-        const frag fd = read_transposed<T>(ds + p0, ds + p1);
-        Mfma<T>::mma(dg[s], fx, dwg[t]);
-        Mfma<T>::mma(du[s], fx, dwu[t]);
-        Mfma<T>::mma(h[s], fd, dwd[t]);
+      for (int k = 0; k < K; ++k) {
+        const int piece = ((n * kFusedRows + lane) * UP + swizzled<UP>(lane, 2 * k + half)) * 16;
+        const frag fx = *reinterpret_cast<const frag*>(xs + piece);
+        const frag fd = *reinterpret_cast<const frag*>(ds + piece);
+        Mfma<T>::mma(fx, wg[k], g[n]);
+        Mfma<T>::mma(fx, wu[k], u[n]);
+        Mfma<T>::mma(fd, wd[k], dh[n]);
       }
+    }
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      // register 8 s + j of lane half b holds row 16 s + 8 (j >> 2) + 4 b + (j & 3) of the tile
+      frag dg[2], du[2], h[2];
+      gate16<ACT>(g[n], [&](int i, float value, float slope) {
+        dg[i >> 3][i & 7] = T(dh[n][i] * u[n][i] * slope);
+        du[i >> 3][i & 7] = T(dh[n][i] * value);
+        h[i >> 3][i & 7] = T(value * u[n][i]);
+      });
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          // columns 32 t .. of those rows
+          const int l = int(threadIdx.x) & 15;
+          const int col = 4 * t + 2 * ((int(threadIdx.x) >> 4) & 1) + ((l >> 1) & 1);
+          const int row = n * kFusedRows + 16 * s + 4 * half + (l >> 2);
+          const int p0 = (row * UP + swizzled<UP>(row, col)) * 16 + (l & 1) * 8;
+          const int p1 = ((row + 8) * UP + swizzled<UP>(row + 8, col)) * 16 + (l & 1) * 8;
+          const frag fx = read_transposed<T>(xs + p0, xs + p1);
+          const frag fd = read_transposed<T>(ds + p0, ds + p1);
+          Mfma<T>::mma(dg[s], fx, dwg[t]);
+          Mfma<T>::mma(du[s], fx, dwu[t]);
+          Mfma<T>::mma(h[s], fd, dwd[t]);
+        }
+    }
   }
   // the second four waves' sums through LDS to the first's
   auto join = [&](floatx16(&d)[TILES]) {
@@ -350,25 +350,25 @@ int64_t fused_weights_shares(int64_t rows, int64_t C, int64_t F, int64_t Co) {
   return want < most ? want : most;
 }
 
-template <typename T, int CP, bool HIDDEN, int MINW>
+template <typename T, int CP, int N, bool HIDDEN, int MINW>
 static int launch_dx(const GradArgs<T>& a, int act, hipStream_t s) {
   const int64_t blocks = cdiv(a.x.n, 4 * kFusedRows);
   SP_CHECK_ARG(blocks <= kMaxGridX, "gated_ffn_bwd: too many rows");
   using Kern = void (*)(GradArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused_dx<T, kActSilu, CP, HIDDEN, MINW>)
-                    : act == kActGelu ? Kern(ffn_fused_dx<T, kActGelu, CP, HIDDEN, MINW>)
-                                      : Kern(ffn_fused_dx<T, kActRelu, CP, HIDDEN, MINW>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused_dx<T, kActSilu, CP, N, HIDDEN, MINW>)
+                    : act == kActGelu ? Kern(ffn_fused_dx<T, kActGelu, CP, N, HIDDEN, MINW>)
+                                      : Kern(ffn_fused_dx<T, kActRelu, CP, N, HIDDEN, MINW>);
   kern<<<unsigned(blocks), kFfnThreads, 0, s>>>(a);
   SP_LAUNCHED();
   return SP_OK;
 }
 
-template <typename T, int CP, int HALVES>
+template <typename T, int CP, int HALVES, int U>
 static int launch_weights(const GradArgs<T>& a, int act, hipStream_t s) {
   using Kern = void (*)(GradArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused_weights<T, kActSilu, CP, HALVES>)
-                    : act == kActGelu ? Kern(ffn_fused_weights<T, kActGelu, CP, HALVES>)
-                                      : Kern(ffn_fused_weights<T, kActRelu, CP, HALVES>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused_weights<T, kActSilu, CP, HALVES, U>)
+                    : act == kActGelu ? Kern(ffn_fused_weights<T, kActGelu, CP, HALVES, U>)
+                                      : Kern(ffn_fused_weights<T, kActRelu, CP, HALVES, U>);
   const dim3 grid(unsigned(cdiv(a.w.F, 128)), unsigned(cdiv(a.x.n, a.share)));
   kern<<<grid, kFfnThreads * HALVES, 0, s>>>(a);
   SP_LAUNCHED();
@@ -394,24 +394,24 @@ static int run_grad(const FfnCall& c, const FusedGrad& o, int64_t* shares) {
   if (a.dx || a.hid) {
     int rc;
     if (n > kFusedGramWidth)
-      rc = n <= 160   ? launch_dx<T, 160, true, 1>(a, c.act, c.stream)
-           : n <= 192 ? launch_dx<T, 192, true, 1>(a, c.act, c.stream)
-                      : launch_dx<T, 256, true, 1>(a, c.act, c.stream);
+      rc = n <= 160   ? launch_dx<T, 160, 2, true, 1>(a, c.act, c.stream)
+           : n <= 192 ? launch_dx<T, 192, 2, true, 1>(a, c.act, c.stream)
+                      : launch_dx<T, 256, 2, true, 1>(a, c.act, c.stream);
     else
-      rc = n <= 32   ? launch_dx<T, 32, false, 4>(a, c.act, c.stream)
-           : n <= 64 ? launch_dx<T, 64, false, 3>(a, c.act, c.stream)
-           : n <= 96 ? launch_dx<T, 96, false, 2>(a, c.act, c.stream)
-                     : launch_dx<T, 128, false, 2>(a, c.act, c.stream);
+      rc = n <= 32   ? launch_dx<T, 32, 2, false, 4>(a, c.act, c.stream)
+           : n <= 64 ? launch_dx<T, 64, 2, false, 3>(a, c.act, c.stream)
+           : n <= 96 ? launch_dx<T, 96, 2, false, 2>(a, c.act, c.stream)
+                     : launch_dx<T, 128, 2, false, 2>(a, c.act, c.stream);
     if (rc) return rc;
   }
   if (!o.part0) return SP_OK;
   const int tile = tile_rows(c.C, c.Co);
   a.share = cdiv(cdiv(c.rows, o.shares), tile) * tile;
   *shares = cdiv(c.rows, a.share);
-  return n <= 32   ? launch_weights<T, 32, 2>(a, c.act, c.stream)
-         : n <= 64 ? launch_weights<T, 64, 2>(a, c.act, c.stream)
-         : n <= 96 ? launch_weights<T, 96, 1>(a, c.act, c.stream)
-                   : launch_weights<T, 128, 1>(a, c.act, c.stream);
+  return n <= 32   ? launch_weights<T, 32, 2, 1>(a, c.act, c.stream)
+         : n <= 64 ? launch_weights<T, 64, 2, 1>(a, c.act, c.stream)
+         : n <= 96 ? launch_weights<T, 96, 1, 1>(a, c.act, c.stream)
+                   : launch_weights<T, 128, 1, 1>(a, c.act, c.stream);
 }
 
 int fused_backward(int32_t dtype, const FfnCall& a, const FusedGrad& o, int64_t* shares) {
