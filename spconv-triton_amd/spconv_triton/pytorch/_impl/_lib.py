@@ -244,8 +244,14 @@ def ptr(t: torch.Tensor | None):
     return ctypes.c_void_p(t.data_ptr())
 
 
+#: the current stream's handle without a Stream object around it (0.3 us a call for 4)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if _raw_stream is None or device.index is None:
+        return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return ctypes.c_void_p(_raw_stream(device.index))
 
 
 def dtype_code(dtype: torch.dtype) -> int:

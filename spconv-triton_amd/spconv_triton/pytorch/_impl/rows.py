@@ -58,22 +58,24 @@ def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
 
 
 def _check_like(what: str, name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape == shape and t.dtype is like.dtype and t.device == like.device:
+        return
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != like.dtype:
         raise ValueError(f"{what}: {name} is {t.dtype}, the rows are {like.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{what}: {name} is on {t.device}, the rows are on {like.device}")
+    raise ValueError(f"{what}: {name} is on {t.device}, the rows are on {like.device}")
 
 
 def _strided(t: torch.Tensor | None):
-    """(tensor, row stride) as the kernels take it."""
+    """(tensor, its address or None, row stride) as the kernels take them."""
     if t is None:
-        return None, 0
+        return None, None, 0
     n, c = t.shape
-    if (c > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < c):
-        t = t.contiguous()
-    return t, (t.stride(0) if n > 1 else c)
+    s0, s1 = t.stride()
+    if (c > 1 and s1 != 1) or (n > 1 and s0 < c):
+        t, s0 = t.contiguous(), c
+    return t, t.data_ptr(), (s0 if n > 1 else c)
 
 
 # ---------------------------------------------------------------------------
@@ -85,7 +87,7 @@ def check_norm(x, weight, eps, residual) -> None:
     if residual is not None:
         _check_like("rms_norm", "residual", residual, x.shape, x)
     if weight is not None:
-        if tuple(weight.shape) != (x.shape[1],):
+        if weight.shape != x.shape[1:]:
             raise ValueError(f"rms_norm: weight has shape {tuple(weight.shape)}, expected "
                              f"({x.shape[1]},)")
         if weight.dtype not in (x.dtype, torch.float32):
@@ -96,25 +98,26 @@ def check_norm(x, weight, eps, residual) -> None:
         raise ValueError(f"rms_norm: eps is {eps}")
 
 
-def _param_code(weight, x):
-    return _lib.dtype_code(x.dtype if weight is None else weight.dtype)
-
-
 def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, int8: bool = False):
     """(y, x + residual or None without one, the 8-bit copy of y or None)."""
     check_norm(x, weight, eps, residual)
-    x, ldx = _strided(x)
-    residual, ldr = _strided(residual)
-    weight = None if weight is None else weight.contiguous()
+    dtype, device = x.dtype, x.device
+    x, px, ldx = _strided(x)
+    residual, pr, ldr = _strided(residual)
     n, c = x.shape
-    y = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    code = pcode = _lib.dtype_code(dtype)
+    pw = None
+    if weight is not None:
+        weight = weight.contiguous()
+        pw, pcode = weight.data_ptr(), _lib.dtype_code(weight.dtype)
+    y = torch.empty((n, c), dtype=dtype, device=device)
     total = None if residual is None else torch.empty_like(y)
     kept = _empty_codes(n, c, x) if int8 else None
-    _lib.check(_lib.lib().sp_rms_norm(
-        _lib.ptr(x), ldx, _lib.ptr(residual), ldr, _lib.dtype_code(x.dtype), n, c,
-        _lib.ptr(weight), _param_code(weight, x), float(eps), _lib.ptr(y), _lib.ptr(total),
-        _lib.ptr(kept.codes) if int8 else None, _lib.ptr(kept.scales) if int8 else None,
-        _lib.stream_of(x.device)), "sp_rms_norm")
+    L = _lib.lib()
+    _lib.check(L.sp_rms_norm(
+        px, ldx, pr, ldr, code, n, c, pw, pcode, eps, y.data_ptr(),
+        None if total is None else total.data_ptr(), kept.codes.data_ptr() if int8 else None,
+        kept.scales.data_ptr() if int8 else None, _lib.stream_of(device)), "sp_rms_norm")
     return y, total, kept
 
 
@@ -122,25 +125,30 @@ def rms_norm_backward(dy, dsum, total, weight=None, eps: float = 1e-6, need_weig
     """(gradient of x and of the residual, gradient of the weight or None).  ``total`` is x
     + residual as the forward pass returned it, ``dsum`` its own gradient or None."""
     check_norm(total, weight, eps, dsum)
+    dtype, device = total.dtype, total.device
     _check_like("rms_norm_backward", "dy", dy, total.shape, total)
-    dy, lddy = _strided(dy)
-    dsum, ldds = _strided(dsum)
-    total, lds = _strided(total)
-    weight = None if weight is None else weight.contiguous()
+    dy, py, lddy = _strided(dy)
+    dsum, pd, ldds = _strided(dsum)
+    total, pt, lds = _strided(total)
     n, c = total.shape
-    ds = torch.empty((n, c), dtype=total.dtype, device=total.device)
-    dw, ws, nbytes = None, None, 0
-    if need_weight and weight is not None:
-        if n == 0:
-            return ds, torch.zeros_like(weight)
-        dw = torch.empty_like(weight)
-        nbytes = _lib.lib().sp_rms_norm_bwd_workspace(n, c)
-        ws = _lib.workspace(nbytes, total.device)
-    _lib.check(_lib.lib().sp_rms_norm_bwd(
-        _lib.ptr(dy), lddy, _lib.ptr(dsum), ldds, _lib.ptr(total), lds,
-        _lib.dtype_code(total.dtype), n, c, _lib.ptr(weight), _param_code(weight, total),
-        float(eps), _lib.ptr(ds), _lib.ptr(dw), _lib.ptr(ws), nbytes,
-        _lib.stream_of(total.device)), "sp_rms_norm_bwd")
+    code = pcode = _lib.dtype_code(dtype)
+    ds = torch.empty((n, c), dtype=dtype, device=device)
+    L = _lib.lib()
+    pw = dw = pdw = pws = None
+    nbytes = 0
+    if weight is not None:
+        weight = weight.contiguous()
+        pw, pcode = weight.data_ptr(), _lib.dtype_code(weight.dtype)
+        if need_weight:
+            if n == 0:
+                return ds, torch.zeros_like(weight)
+            dw = torch.empty_like(weight)
+            nbytes = L.sp_rms_norm_bwd_workspace(n, c)
+            ws = _lib.workspace(nbytes, device)
+            pdw, pws = dw.data_ptr(), ws.data_ptr()
+    _lib.check(L.sp_rms_norm_bwd(py, lddy, pd, ldds, pt, lds, code, n, c, pw, pcode, eps,
+                                 ds.data_ptr(), pdw, pws, nbytes, _lib.stream_of(device)),
+               "sp_rms_norm_bwd")
     return ds, dw
 
 
@@ -156,12 +164,12 @@ def _empty_codes(n: int, c: int, x: torch.Tensor) -> Int8Rows:
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     _check_rows("quantize_rows", "x", x)
-    x, ldx = _strided(x)
+    x, px, ldx = _strided(x)
     n, c = x.shape
     kept = _empty_codes(n, c, x)
     _lib.check(_lib.lib().sp_quantize_rows(
-        _lib.ptr(x), ldx, _lib.dtype_code(x.dtype), n, c, _lib.ptr(kept.codes),
-        _lib.ptr(kept.scales), _lib.stream_of(x.device)), "sp_quantize_rows")
+        px, ldx, _lib.dtype_code(x.dtype), n, c, kept.codes.data_ptr(), kept.scales.data_ptr(),
+        _lib.stream_of(x.device)), "sp_quantize_rows")
     return kept
 
 
@@ -175,8 +183,8 @@ def restore_rows(kept: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tens
     n, c = kept.shape
     out = torch.empty((n, c), dtype=dtype, device=kept.device)
     _lib.check(_lib.lib().sp_restore_rows(
-        _lib.ptr(kept.codes), _lib.ptr(kept.scales), n, c, _lib.dtype_code(dtype), _lib.ptr(out),
-        _lib.stream_of(out.device)), "sp_restore_rows")
+        kept.codes.data_ptr(), kept.scales.data_ptr(), n, c, _lib.dtype_code(dtype),
+        out.data_ptr(), _lib.stream_of(out.device)), "sp_restore_rows")
     return out
 
 
@@ -204,19 +212,21 @@ def check_ffn(x, w_gate, w_up, w_down, act, residual) -> None:
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu", residual=None) -> torch.Tensor:
     """(act(x w_gate') * (x w_up')) w_down' (+ residual)."""
     check_ffn(x, w_gate, w_up, w_down, act, residual)
-    x, ldx = _strided(x)
-    residual, ldr = _strided(residual)
+    dtype, device = x.dtype, x.device
+    x, px, ldx = _strided(x)
+    residual, pr, ldr = _strided(residual)
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     n, c = x.shape
     hidden, c_out = w_gate.shape[0], w_down.shape[0]
-    y = torch.empty((n, c_out), dtype=x.dtype, device=x.device)
-    code = _lib.dtype_code(x.dtype)
-    nbytes = _lib.lib().sp_gated_ffn_workspace(code, n, c, hidden, c_out)
-    ws = _lib.workspace(nbytes, x.device)
-    _lib.check(_lib.lib().sp_gated_ffn(
-        _lib.ptr(x), ldx, code, n, c, _lib.ptr(w_gate), _lib.ptr(w_up), hidden,
-        _lib.ptr(w_down), c_out, ACTIVATIONS[act], _lib.ptr(residual), ldr, _lib.ptr(y),
-        _lib.ptr(ws), nbytes, _lib.stream_of(x.device)), "sp_gated_ffn")
+    y = torch.empty((n, c_out), dtype=dtype, device=device)
+    L = _lib.lib()
+    code = _lib.dtype_code(dtype)
+    nbytes = L.sp_gated_ffn_workspace(code, n, c, hidden, c_out)
+    ws = _lib.workspace(nbytes, device)
+    _lib.check(L.sp_gated_ffn(
+        px, ldx, code, n, c, w_gate.data_ptr(), w_up.data_ptr(), hidden, w_down.data_ptr(), c_out,
+        ACTIVATIONS[act], pr, ldr, y.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(device)),
+        "sp_gated_ffn")
     return y
 
 
@@ -226,26 +236,28 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, act: str = "silu",
     or their ``Int8Rows``, whose values then stand for them throughout."""
     check_ffn(x, w_gate, w_up, w_down, act, None)
     n, c = x.shape
+    dtype, device = x.dtype, x.device
     hidden, c_out = w_gate.shape[0], w_down.shape[0]
     _check_like("gated_ffn_backward", "dy", dy, (n, c_out), x)
-    dy, lddy = _strided(dy)
+    dy, py, lddy = _strided(dy)
+    px = codes = scales = None
+    ldx = 0
     if isinstance(x, Int8Rows):
-        rows, ldx, codes, scales = None, 0, x.codes, x.scales
+        codes, scales = x.codes.data_ptr(), x.scales.data_ptr()
     else:
-        (rows, ldx), codes, scales = _strided(x), None, None
+        x, px, ldx = _strided(x)
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     make = torch.zeros_like if n == 0 else torch.empty_like
-    dx = torch.empty((n, c), dtype=x.dtype, device=x.device) if need[0] else None
-    dwg, dwu, dwd = (make(w) if k else None
-                     for w, k in zip((w_gate, w_up, w_down), need[1:]))
+    dx = torch.empty((n, c), dtype=dtype, device=device) if need[0] else None
+    grads = [make(w) if k else None for w, k in zip((w_gate, w_up, w_down), need[1:])]
     if n and any(need):
-        code = _lib.dtype_code(x.dtype)
-        nbytes = _lib.lib().sp_gated_ffn_bwd_workspace(code, n, c, hidden, c_out,
-                                                       codes is not None)
-        ws = _lib.workspace(nbytes, x.device)
-        _lib.check(_lib.lib().sp_gated_ffn_bwd(
-            _lib.ptr(dy), lddy, _lib.ptr(rows), ldx, _lib.ptr(codes), _lib.ptr(scales), code, n,
-            c, _lib.ptr(w_gate), _lib.ptr(w_up), hidden, _lib.ptr(w_down), c_out,
-            ACTIVATIONS[act], _lib.ptr(dx), _lib.ptr(dwg), _lib.ptr(dwu), _lib.ptr(dwd),
-            _lib.ptr(ws), nbytes, _lib.stream_of(x.device)), "sp_gated_ffn_bwd")
-    return dx, dwg, dwu, dwd
+        L = _lib.lib()
+        code = _lib.dtype_code(dtype)
+        nbytes = L.sp_gated_ffn_bwd_workspace(code, n, c, hidden, c_out, codes is not None)
+        ws = _lib.workspace(nbytes, device)
+        pdx, pdg, pdu, pdd = (None if t is None else t.data_ptr() for t in (dx, *grads))
+        _lib.check(L.sp_gated_ffn_bwd(
+            py, lddy, px, ldx, codes, scales, code, n, c, w_gate.data_ptr(), w_up.data_ptr(),
+            hidden, w_down.data_ptr(), c_out, ACTIVATIONS[act], pdx, pdg, pdu, pdd,
+            ws.data_ptr(), nbytes, _lib.stream_of(device)), "sp_gated_ffn_bwd")
+    return (dx, *grads)

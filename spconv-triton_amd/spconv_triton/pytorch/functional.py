@@ -19,7 +19,6 @@ from torch.autograd.function import once_differentiable
 
 from spconv_triton.compat import tv
 from spconv_triton.pytorch import ops
-from spconv_triton.pytorch._impl import rows as _rows
 from spconv_triton.pytorch._impl.rows import Int8Rows
 from spconv_triton.pytorch.hash import HashTable
 from spconv_triton.tools import CUDAKernelTimer
@@ -218,9 +217,9 @@ indice_avgpool_implicit_gemm = SparseAvgPoolImplicitGemmFunction.apply
 # the channel half of a block: norm, gated feed-forward, rows in 8 bits
 # ---------------------------------------------------------------------------
 
+# (the backward passes below run no operation that autocast looks at, and go without custom_bwd)
 class RMSNormFunction(Function):
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, eps, residual, int8):
         y, total, kept = ops.rms_norm(x, weight, eps, residual, int8)
         ctx.save_for_backward(x if residual is None else total, weight)
@@ -230,7 +229,6 @@ class RMSNormFunction(Function):
 
     @staticmethod
     @once_differentiable
-    @_BWD
     def backward(ctx, dy, dsum, _):
         total, weight = ctx.saved_tensors
         need_x, need_w, _, need_res, _ = ctx.needs_input_grad
@@ -287,7 +285,6 @@ class GatedFFNFunction(Function):
 
     @staticmethod
     @once_differentiable
-    @_BWD
     def backward(ctx, dy):
         need = ctx.needs_input_grad
         grads = [None] * 4
