@@ -7,10 +7,7 @@
 namespace sp {
 
 constexpr int kFfnThreads = 256;
-constexpr int kTileRows = 128;  // rows of an operand in a stage
 constexpr int kStagePieces = 8;  // 16-byte pieces of a row in a stage: 64 16-bit values
-constexpr int kStageBytes = kTileRows * kStagePieces * 16;
-constexpr int kHiddenTile = 64;  // hidden units of a workgroup where it forms gate and up
 
 enum { kActSilu = 0, kActGelu = 1, kActRelu = 2 };
 
@@ -101,6 +98,27 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   if constexpr (PIECES % 8 == 0) return c ^ (((r & 2) << 1) | ((r >> 2) & 3));
   static_assert(PIECES % 4 == 0, "pieces are permuted within four, eight or sixteen");
   return c ^ ((r >> 2) & 3);
+}
+
+// Row of a 32-row weight block that lies at operand row m: then accumulator register i of lane half b is
+// row 16 (i >> 3) + 8 b + (i & 7).
+__device__ __forceinline__ int unit_of(int m) {
+  return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);
+}
+
+__device__ const uint4 g_zero_piece = {0, 0, 0, 0};
+
+// 16 bytes from memory to LDS at `to` (the wave's first lane's) + 16 * lane.
+__device__ __forceinline__ void copy_piece(const void* from, char* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void*)from,
+      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// At most N of the wave's loads still on their way.
+template <int N>
+__device__ __forceinline__ void loads_in_flight() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -13,14 +13,41 @@
 
 namespace sp {
 
-// Pieces [128 rows][8] of an operand on their way from memory to LDS; thread t holds piece
-// t % 8 of rows t / 8 + 32 j.
+// ---- products of rows with weight rows -------------------------------------------
+// A workgroup's tile: WX x WW waves, each with XT x WT tiles of 32 rows of x and of 32 weight rows.  The
+// MFMA's rows are the weights' and its columns x's, so that a lane holds one row of x and
+// neighbouring outputs of it.  Every operand byte that the LDS gives serves 32 XT or 32 WT products:
+// with 2 x 2 tiles a wave the reads of four waves alone take the LDS as long as the MFMAs
+// take, and the L2 hands out 2.2 GB for the gate and up products of 50k rows of 512 channels
+// (64 hidden units a workgroup), 1.1 GB with 256 rows and 128 hidden units.
+template <int XT_, int WT_, int WX_, int WW_>
+struct TileShape {
+  static constexpr int XT = XT_, WT = WT_, WX = WX_, WW = WW_;
+  static constexpr int X = 32 * XT * WX, W = 32 * WT * WW;  // rows of a stage
+  static constexpr int THREADS = 64 * WX * WW;
+  static constexpr int PIECES = (X + W) * kStagePieces, BYTES = PIECES * 16;
+};
+using SmallTile = TileShape<2, 2, 2, 2>;   // 128 x 128, four waves
+using LongTile = TileShape<2, 2, 4, 2>;    // 256 x 128, eight waves
+using LargeTile = TileShape<2, 4, 4, 2>;   // 256 x 256, eight waves
+
+// Weight row of operand row m: 16-bit lanes then hold eight neighbouring outputs in eight
+// registers, fp32 ones (as it is) four in four.
 template <typename T>
+__device__ __forceinline__ int weight_row(int m) {
+  return sizeof(T) == 2 ? (m & ~31) + unit_of(m & 31) : m;
+}
+
+// A stage: 128 bytes of X rows of x and of W weight rows, from w, or the first half of them from w and
+// the other from w2.  ASYNC: straight to LDS, for operands whose rows start at multiples of 16 bytes
+// and have whole pieces; else through registers.
+template <typename T, typename S, bool ASYNC>
 struct Stage {
   using frag = typename Mfma<T>::frag;
-  static constexpr int V = Mfma<T>::V;
-  frag r[4];
+  static constexpr int V = Mfma<T>::V, N = S::PIECES / S::THREADS;
+  frag r[ASYNC ? 1 : N];
 
+  // operand row i / 8 and piece i % 8 of LDS slot i
   __device__ __forceinline__ static frag piece(const Rows<T>& a, int64_t row, int k) {
     frag f = {};
     if (row >= a.n || k >= a.K) return f;
@@ -31,27 +58,33 @@ struct Stage {
       if (k + i < a.K) f[i] = q[i];
     return f;
   }
-
-  // 128 rows from row0, or where `b` is given 64 of each
-  __device__ __forceinline__ void load(const Rows<T>& a, int64_t row0, int k0) {
-    const int c = int(threadIdx.x) & 7, t = int(threadIdx.x) >> 3;
+  __device__ __forceinline__ void start(const Rows<T>& x, int64_t x0, const Rows<T>& w,
+                                        const Rows<T>* w2, int64_t w0, int k0, char* lds) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = piece(a, row0 + t + 32 * j, k0 + c * V);
-  }
-  __device__ __forceinline__ void load(const Rows<T>& a, const Rows<T>& b, int64_t row0, int k0) {
-    const int c = int(threadIdx.x) & 7, t = int(threadIdx.x) >> 3;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      r[j] = piece(a, row0 + t + 32 * j, k0 + c * V);
-      r[j + 2] = piece(b, row0 + t + 32 * j, k0 + c * V);
+    for (int j = 0; j < N; ++j) {
+      const int i = j * S::THREADS + int(threadIdx.x), row = i >> 3;
+      const int k = k0 + swizzled<8>(row, i & 7) * V;
+      const bool second = w2 && j * S::THREADS >= (S::X + S::W / 2) * 8;  // (whole rounds)
+      const bool weights = j * S::THREADS >= S::X * 8;
+      const Rows<T>& a = second ? *w2 : weights ? w : x;
+      const int64_t at = !weights ? x0 + row
+                                  : w0 + weight_row<T>(row - S::X - (second ? S::W / 2 : 0));
+      if constexpr (ASYNC) {
+        const void* from = &g_zero_piece;
+        if (at < a.n && k < a.K) from = a.p + at * a.ld + k;
+        copy_piece(from, lds + (i - (int(threadIdx.x) & 63)) * 16);
+      } else {
+        r[j] = piece(a, at, k);
+      }
     }
   }
-  __device__ __forceinline__ void store(char* lds) const {
-    const int c = int(threadIdx.x) & 7, t = int(threadIdx.x) >> 3;
+  __device__ __forceinline__ void finish(char* lds) const {
+    if constexpr (ASYNC) {
+      loads_in_flight<0>();
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = t + 32 * j;
-      *reinterpret_cast<frag*>(lds + (row * 8 + swizzled<8>(row, c)) * 16) = r[j];
+      for (int j = 0; j < N; ++j)
+        *reinterpret_cast<frag*>(lds + (j * S::THREADS + int(threadIdx.x)) * 16) = r[j];
     }
   }
   __device__ __forceinline__ static frag read(const char* lds, int row, int c) {
@@ -59,42 +92,33 @@ struct Stage {
   }
 };
 
-// acc[j][i] += the products of W rows wrow[i] .. + 31 and X rows xrow + 32 j .. + 31 over
-// all of K.  The MFMA's rows are W's and its columns X's, so that lane l holds
-// four neighbouring outputs of X row l & 31 in every four registers.
-// w2: the second half of the W tile comes from there.
-template <typename T, int NW>
+// acc[j][i] += the products of x rows xrow + 32 j .. + 31 and weight rows wrow[i] .. + 31 of the stage
+// over all of K.
+template <typename T, typename S, bool ASYNC, int NW>
 __device__ __forceinline__ void products(const Rows<T>& x, int64_t x0, const Rows<T>& w,
                                          const Rows<T>* w2, int64_t w0, const int (&wrow)[NW],
-                                         int xrow, char* lds, floatx16 (&acc)[2][NW]) {
+                                         int xrow, char* lds, floatx16 (&acc)[S::XT][NW]) {
+  using Stg = Stage<T, S, ASYNC>;
   constexpr int STEP = kStagePieces * Mfma<T>::V;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
-  Stage<T> sx, sw;
-  auto fetch = [&](int k) {
-    sx.load(x, x0, k);
-    if (w2)
-      sw.load(w, *w2, w0, k);
-    else
-      sw.load(w, w0, k);
-  };
+  Stg stage;
   const int steps = (x.K + STEP - 1) / STEP;
-  fetch(0);
+  stage.start(x, x0, w, w2, w0, 0, lds);
   for (int s = 0; s < steps; ++s) {
-    char* bx = lds + (s & 1) * (2 * kStageBytes);
-    char* bw = bx + kStageBytes;
-    sx.store(bx);
-    sw.store(bw);
+    char* buf = lds + (s & 1) * S::BYTES;
+    stage.finish(buf);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
-    if (s + 1 < steps) fetch((s + 1) * STEP);
+    if (s + 1 < steps)
+      stage.start(x, x0, w, w2, w0, (s + 1) * STEP, lds + ((s + 1) & 1) * S::BYTES);
 #pragma unroll
     for (int c = 0; c < kStagePieces; c += 2) {
-      typename Mfma<T>::frag fx[2], fw[NW];
+      typename Mfma<T>::frag fx[S::XT], fw[NW];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fx[j] = Stage<T>::read(bx, xrow + 32 * j + lane, c + half);
+      for (int j = 0; j < S::XT; ++j) fx[j] = Stg::read(buf, xrow + 32 * j + lane, c + half);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) fw[i] = Stage<T>::read(bw, wrow[i] + lane, c + half);
+      for (int i = 0; i < NW; ++i) fw[i] = Stg::read(buf, S::X + wrow[i] + lane, c + half);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < S::XT; ++j)
 #pragma unroll
         for (int i = 0; i < NW; ++i) Mfma<T>::mma(fw[i], fx[j], acc[j][i]);
     }
@@ -102,93 +126,113 @@ __device__ __forceinline__ void products(const Rows<T>& x, int64_t x0, const Row
   __syncthreads();
 }
 
-// One 32 x 32 accumulator to LDS rows of `pitch` bytes, as values of type S.
-template <typename S, typename F>
-__device__ __forceinline__ void put_tile(char* lds, int pitch, int row, int col, F&& value) {
-  const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
+template <int M, int N>
+__device__ __forceinline__ void clear(floatx16 (&acc)[M][N]) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    struct alignas(sizeof(S) * 4) Four {
-      S v[4];
-    } f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.v[i] = S(value(4 * q + i));
-    *reinterpret_cast<Four*>(lds + (row + lane) * pitch + (col + 8 * q + 4 * half) * int(sizeof(S))) = f;
-  }
-}
-
-// LDS rows of COLS values to memory, columns below n.  (out rows start at 16 bytes, n is a
-// multiple of V.)
-template <typename T, int COLS>
-__device__ __forceinline__ void write_rows(const char* lds, int pitch, T* __restrict__ out,
-                                           int64_t ld, int64_t row0, int64_t rows, int col0,
-                                           int n) {
-  using frag = typename Mfma<T>::frag;
-  constexpr int V = Mfma<T>::V, PER = COLS / V;
-  for (int i = int(threadIdx.x); i < kTileRows * PER; i += kFfnThreads) {
-    const int r = i / PER, c = (i - r * PER) * V;
-    if (row0 + r < rows && col0 + c < n)
-      *reinterpret_cast<frag*>(out + (row0 + r) * ld + col0 + c) =
-          *reinterpret_cast<const frag*>(lds + r * pitch + c * int(sizeof(T)));
-  }
-}
-
-template <int N>
-__device__ __forceinline__ void clear(floatx16 (&acc)[2][N]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < M; ++j)
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < 16; ++k) acc[j][i][k] = 0.f;
 }
 
-// h = act(x Wg') * (x Wu'), 128 rows x 64 hidden units a workgroup; columns from F to the
-// padded width are zeros.
-template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_up(Rows<T> x, Rows<T> wg, Rows<T> wu, int act,
-                                                      T* __restrict__ h, int Fp) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * kStageBytes];
-  const int wave = int(threadIdx.x) >> 6, wm = wave >> 1, wn = wave & 1;
-  const int64_t x0 = int64_t(blockIdx.y) * kTileRows;
-  const int f0 = int(blockIdx.x) * kHiddenTile;
-  floatx16 acc[2][2];
-  clear(acc);
-  const int wrow[2] = {wn * 32, kHiddenTile + wn * 32};
-  products<T, 2>(x, x0, wg, &wu, f0, wrow, wm * 64, lds, acc);
-  constexpr int pitch = kHiddenTile * int(sizeof(T)) + 16;
-  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
+// The lane's outputs of an accumulator: pieces of V of row r, columns c0 .. c0 + 31, those below n.
+// value(i): of register i, or with a residual what is added to it.
+template <typename T, typename F>
+__device__ __forceinline__ void write_piece_row(T* out, int64_t ld, int64_t r, int64_t rows,
+                                                int c0, int n, bool vec, F&& value) {
+  using frag = typename Mfma<T>::frag;
+  constexpr int V = Mfma<T>::V;
+  const int half = (int(threadIdx.x) >> 5) & 1;
+  if (r >= rows) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      put_tile<T>(lds, pitch, wm * 64 + 32 * j, wn * 32, [&](int i) {
-        float value, slope;
-        gate(acc[j][0][i], value, slope);
-        return value * acc[j][1][i];
-      });
-  });
-  __syncthreads();
-  write_rows<T, kHiddenTile>(lds, pitch, h, Fp, x0, x.n, f0, Fp);
+  for (int p = 0; p < 16 / V; ++p) {
+    const int c = c0 + 2 * V * p + V * half;
+    if (c >= n) continue;
+    frag f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = from_f32<T>(value(p * V + i, c + i));
+    T* to = out + r * ld + c;
+    if (vec && c + V <= n) {
+      *reinterpret_cast<frag*>(to) = f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c + i < n) to[i] = f[i];
+    }
+  }
 }
 
-// dg, du and h of 128 rows x 64 hidden units, in rows of 3 Fp values.  wdt: Wd transposed.
-template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_grad_hidden(Rows<T> x, Rows<T> wg, Rows<T> wu,
-                                                               Rows<T> dy, Rows<T> wdt, int act,
-                                                               T* __restrict__ out, int Fp) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * kStageBytes];
-  const int wave = int(threadIdx.x) >> 6, wm = wave >> 1, wn = wave & 1;
-  const int64_t x0 = int64_t(blockIdx.y) * kTileRows;
-  const int f0 = int(blockIdx.x) * kHiddenTile;
-  floatx16 acc[2][2], dh[2][1];
+// Which tile a workgroup takes: consecutive workgroups go to the eight XCDs in turn, and an XCD goes through
+// the column tiles of a row tile one after the other, so that x's rows pass through one L2.
+__device__ __forceinline__ bool tile_of(int cols, int64_t rows, int64_t& row, int& col) {
+  const int64_t id = blockIdx.x, seq = id >> 3;
+  row = seq / cols * 8 + (id & 7);
+  col = int(seq % cols);
+  return row < rows;
+}
+
+// h = act(x Wg') * (x Wu'); columns from F to the padded width are zeros.
+template <typename T, typename S, bool ASYNC>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, Rows<T> wu, int act,
+                                                     T* __restrict__ h, int Fp) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
+  constexpr int NH = S::WT / 2, HIDDEN = S::W / 2;  // a wave's tiles of each, the workgroup's units
+  const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
+  const int lane = int(threadIdx.x) & 31;
+  int64_t row;
+  int col;
+  if (!tile_of((Fp + HIDDEN - 1) / HIDDEN, (x.n + S::X - 1) / S::X, row, col)) return;
+  const int64_t x0 = row * S::X;
+  const int f0 = col * HIDDEN, xrow = wm * 32 * S::XT;
+  floatx16 acc[S::XT][S::WT];
   clear(acc);
-  clear(dh);
-  const int wrow[2] = {wn * 32, kHiddenTile + wn * 32}, drow[1] = {wn * 32};
-  products<T, 2>(x, x0, wg, &wu, f0, wrow, wm * 64, lds, acc);
-  products<T, 1>(dy, x0, wdt, nullptr, f0, drow, wm * 64, lds, dh);
-  constexpr int pitch = kHiddenTile * int(sizeof(T)) + 16;
+  int wrow[S::WT];
+#pragma unroll
+  for (int i = 0; i < NH; ++i) {
+    wrow[i] = (wn * NH + i) * 32;
+    wrow[NH + i] = HIDDEN + (wn * NH + i) * 32;
+  }
+  products<T, S, ASYNC, S::WT>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
   with_gate<sizeof(T) == 2>(act, [&](auto gate) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+      for (int i = 0; i < NH; ++i)
+        write_piece_row<T>(h, Fp, x0 + xrow + 32 * j + lane, x.n, f0 + wrow[i], Fp, true,
+                           [&](int k, int) {
+                             float value, slope;
+                             gate(acc[j][i][k], value, slope);
+                             return value * acc[j][NH + i][k];
+                           });
+  });
+}
+
+// dg, du and h in rows of 3 Fp values.  wdt: Wd transposed.
+template <typename T, typename S, bool ASYNC>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows<T> wg, Rows<T> wu,
+                                                              Rows<T> dy, Rows<T> wdt, int act,
+                                                              T* __restrict__ out, int Fp) {
+  static_assert(S::WT == 2, "a gate and an up tile");
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
+  constexpr int HIDDEN = S::W / 2;
+  const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
+  const int lane = int(threadIdx.x) & 31;
+  int64_t row;
+  int col;
+  if (!tile_of((Fp + HIDDEN - 1) / HIDDEN, (x.n + S::X - 1) / S::X, row, col)) return;
+  const int64_t x0 = row * S::X;
+  const int f0 = col * HIDDEN, xrow = wm * 32 * S::XT;
+  floatx16 acc[S::XT][2], dh[S::XT][1];
+  clear(acc);
+  clear(dh);
+  const int wrow[2] = {wn * 32, HIDDEN + wn * 32}, drow[1] = {wn * 32};
+  products<T, S, ASYNC, 2>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
+  if (wdt.n > f0 + HIDDEN) wdt.n = f0 + HIDDEN;  // (half of a stage's weight rows)
+  products<T, S, ASYNC, 1>(dy, x0, wdt, nullptr, f0, drow, xrow, lds, dh);
+  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
+#pragma unroll
+    for (int j = 0; j < S::XT; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float value, slope;
@@ -200,49 +244,45 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_grad_hidden(Rows<T> x, Rows<T
       }
   });
 #pragma unroll
-  for (int part = 0; part < 3; ++part) {
-    if (part) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      put_tile<T>(lds, pitch, wm * 64 + 32 * j, wn * 32, [&](int i) {
-        return part == 0 ? acc[j][0][i] : part == 1 ? acc[j][1][i] : dh[j][0][i];
-      });
-    __syncthreads();
-    write_rows<T, kHiddenTile>(lds, pitch, out + int64_t(part) * Fp, 3 * int64_t(Fp), x0, x.n, f0,
-                               Fp);
+  for (int j = 0; j < S::XT; ++j) {
+    const int64_t r = x0 + xrow + 32 * j + lane, ld = 3 * int64_t(Fp);
+    const int f = f0 + wn * 32;
+    write_piece_row<T>(out, ld, r, x.n, f, Fp, true, [&](int k, int) { return acc[j][0][k]; });
+    write_piece_row<T>(out + Fp, ld, r, x.n, f, Fp, true, [&](int k, int) { return acc[j][1][k]; });
+    write_piece_row<T>(out + 2 * Fp, ld, r, x.n, f, Fp, true,
+                       [&](int k, int) { return dh[j][0][k]; });
   }
 }
 
-// out = a w' (+ residual), 128 rows x 128 columns a workgroup; fp32 until the residual is in.
-template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_rows(Rows<T> a, Rows<T> w,
-                                                        const T* __restrict__ residual,
-                                                        int64_t ldr, T* __restrict__ out, int n) {
-  constexpr int pitch = kTileRows * 4 + 16;
-  __shared__ __attribute__((aligned(16))) char
-      lds[4 * kStageBytes > kTileRows * pitch ? 4 * kStageBytes : kTileRows * pitch];
-  const int wave = int(threadIdx.x) >> 6, wm = wave >> 1, wn = wave & 1;
-  const int64_t x0 = int64_t(blockIdx.y) * kTileRows;
-  const int n0 = int(blockIdx.x) * kTileRows;
-  floatx16 acc[2][2];
+// out = a w' (+ residual, added in fp32).
+template <typename T, typename S, bool ASYNC>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
+                                                       const T* __restrict__ residual,
+                                                       int64_t ldr, T* __restrict__ out, int n,
+                                                       int vec) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
+  const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
+  const int lane = int(threadIdx.x) & 31;
+  int64_t row;
+  int col;
+  if (!tile_of((n + S::W - 1) / S::W, (a.n + S::X - 1) / S::X, row, col)) return;
+  const int64_t x0 = row * S::X;
+  const int n0 = col * S::W, xrow = wm * 32 * S::XT;
+  floatx16 acc[S::XT][S::WT];
   clear(acc);
-  const int wrow[2] = {wn * 64, wn * 64 + 32};
-  products<T, 2>(a, x0, w, nullptr, n0, wrow, wm * 64, lds, acc);
+  int wrow[S::WT];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < S::WT; ++i) wrow[i] = (wn * S::WT + i) * 32;
+  products<T, S, ASYNC, S::WT>(a, x0, w, nullptr, n0, wrow, xrow, lds, acc);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      put_tile<float>(lds, pitch, wm * 64 + 32 * j, wn * 64 + 32 * i,
-                      [&](int k) { return acc[j][i][k]; });
-  __syncthreads();
-  for (int i = int(threadIdx.x); i < kTileRows * kTileRows; i += kFfnThreads) {
-    const int r = i / kTileRows, c = i - r * kTileRows;
-    if (x0 + r < a.n && n0 + c < n) {
-      float v = *reinterpret_cast<const float*>(lds + r * pitch + c * 4);
-      if (residual) v += to_f32(residual[(x0 + r) * ldr + n0 + c]);
-      out[(x0 + r) * int64_t(n) + n0 + c] = from_f32<T>(v);
+  for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+    for (int i = 0; i < S::WT; ++i) {
+      const int64_t r = x0 + xrow + 32 * j + lane;
+      write_piece_row<T>(out, n, r, a.n, n0 + wrow[i], n, vec, [&](int k, int c) {
+        return residual && c < n ? acc[j][i][k] + to_f32(residual[r * ldr + c]) : acc[j][i][k];
+      });
     }
-  }
 }
 
 // dst [cols, ldd] = src [rows, cols] transposed, columns from rows to ldd's share as zeros:
@@ -270,7 +310,7 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_transpose(const T* __restrict
 
 // ---- weight gradients ------------------------------------------------------------
 // Partials of a' b over a share of the rows: a [rows, P] is of the hidden width, b [rows, Q] of x's
-// or dy's, 128 x TQ of the result a workgroup.  Rows are the MFMA's reduction: 64 of them
+// or dy's, TP x TQ of the result a workgroup.  Rows are the MFMA's reduction: 64 of them
 // (fp32: 32) a stage lie in LDS as in memory, 16-bit operands come out of it
 // transposed (ds_read_b64_tr_b16: sixteen lanes take a 4 x 16 block and get a column of it each),
 // fp32 ones value by value.
@@ -284,34 +324,32 @@ struct Gram {
   float* part;  // [shares][P][Q]
 };
 
-constexpr int kGramP = 128;
-constexpr int kGramStage = 16384;  // bytes of 128 columns in a stage
+constexpr int kGramStage = 128;  // bytes of a column in a stage
 
 template <typename T>
-constexpr int gram_rows() { return kGramStage / (kGramP * int(sizeof(T))); }
+constexpr int gram_rows() { return kGramStage / int(sizeof(T)); }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 
-// COLS columns of a stage in LDS.  16-bit rows hold their 16-byte pieces permuted: the four rows that
-// sixteen lanes read at once, 32 bytes of each, fall on different banks, and so do the 64 bytes of
-// each that 32 lanes read.
-template <typename T, int COLS>
+// COLS columns of a stage in LDS.  16-bit rows hold their 16-byte pieces permuted: the four rows that 32 lanes
+// read at once, 64 bytes of each, fall on different banks.
+template <typename T, int COLS, int THREADS>
 struct GramStage {
   using frag = typename Mfma<T>::frag;
   static constexpr int V = Mfma<T>::V, PER = COLS / V, ROWS = gram_rows<T>();
-  static constexpr int N = ROWS * PER / kFfnThreads;
+  static constexpr int N = ROWS * PER / THREADS;
   frag r[N];
 
   __device__ __forceinline__ static int slot(int row, int piece) {
     if constexpr (sizeof(T) == 4) return piece;
-    if constexpr (COLS == 128) return piece ^ ((row & 1) * 4 + ((row >> 1) & 1) * 10);
+    if constexpr (COLS % 128 == 0) return piece ^ ((row & 3) << 2);
     return piece ^ ((row & 3) << 1);
   }
   __device__ __forceinline__ void load(const T* p, int64_t ld, int vec, int64_t m, int64_t hi,
                                        int c0, int n) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = int(threadIdx.x) + j * kFfnThreads, row = i / PER;
+      const int i = int(threadIdx.x) + j * THREADS, row = i / PER;
       const int c = c0 + (i - row * PER) * V;
       r[j] = frag{};
       if (m + row >= hi || c >= n) continue;
@@ -328,7 +366,7 @@ struct GramStage {
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = int(threadIdx.x) + j * kFfnThreads, row = i / PER;
+      const int i = int(threadIdx.x) + j * THREADS, row = i / PER;
       *reinterpret_cast<frag*>(lds + (row * PER + slot(row, i - row * PER)) * 16) = r[j];
     }
   }
@@ -360,25 +398,32 @@ struct GramStage {
   }
 };
 
-template <typename T, int TQ>
-__global__ __launch_bounds__(kFfnThreads, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
-                                                           int64_t share) {
+// Waves of WP x 2, each with 64 x TQ / 2 of the tile.  The tiles of a share run on one XCD, one after the
+// other, so that its rows pass through one L2.
+template <typename T, int TP, int TQ>
+__global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
+                                                      int64_t share) {
   using frag = typename Mfma<T>::frag;
-  constexpr int ROWS = gram_rows<T>(), NQ = TQ / 64;
-  constexpr int STAGE = kGramStage + kGramStage / kGramP * TQ;
+  constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>(), NQ = TQ / 64;
+  constexpr int STAGE = kGramStage * (TP + TQ);
+  using SA = GramStage<T, TP, THREADS>;
+  using SB = GramStage<T, TQ, THREADS>;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
-  int tile = int(blockIdx.x);
+  const int tiles = g0.tiles + g1.tiles;
+  const int64_t id = blockIdx.x, seq = id >> 3;
+  const int64_t lo = (seq / tiles * 8 + (id & 7)) * share;
+  if (lo >= rows) return;
+  int tile = int(seq % tiles);
   const bool second = tile >= g0.tiles;
   if (second) tile -= g0.tiles;
   const Gram<T> g = second ? g1 : g0;
-  const int p0 = tile / g.tiles_q * kGramP, q0 = tile % g.tiles_q * TQ;
-  const int64_t lo = int64_t(blockIdx.y) * share;
+  const int p0 = tile / g.tiles_q * TP, q0 = tile % g.tiles_q * TQ;
   const int64_t hi = lo + share < rows ? lo + share : rows;
   const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 64, wq = (wave & 1) * (TQ / 2);
   floatx16 acc[2][NQ];
   clear(acc);
-  GramStage<T, kGramP> sa;
-  GramStage<T, TQ> sb;
+  SA sa;
+  SB sb;
   auto fetch = [&](int64_t m) {
     sa.load(g.a, g.lda, g.vec_a, m, hi, p0, g.P);
     sb.load(g.b, g.ldb, g.vec_b, m, hi, q0, g.Q);
@@ -387,25 +432,25 @@ __global__ __launch_bounds__(kFfnThreads, 2) void ffn_gram(Gram<T> g0, Gram<T> g
   int s = 0;
   for (int64_t m = lo; m < hi; m += ROWS, s ^= 1) {
     char* la = lds + s * STAGE;
-    char* lb = la + kGramStage;
+    char* lb = la + kGramStage * TP;
     sa.store(la);
     sb.store(lb);
-    __syncthreads();
+    __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) fetch(m + ROWS);
 #pragma unroll
     for (int k = 0; k < ROWS; k += 2 * Mfma<T>::V) {
       frag fa[2], fb[NQ];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) fa[i] = GramStage<T, kGramP>::read(la, k, wp + 32 * i);
+      for (int i = 0; i < 2; ++i) fa[i] = SA::read(la, k, wp + 32 * i);
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) fb[i] = GramStage<T, TQ>::read(lb, k, wq + 32 * i);
+      for (int i = 0; i < NQ; ++i) fb[i] = SB::read(lb, k, wq + 32 * i);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) Mfma<T>::mma(fa[i], fb[j], acc[i][j]);
     }
   }
-  float* part = g.part + int64_t(blockIdx.y) * g.P * g.Q;
+  float* part = g.part + lo / share * g.P * g.Q;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -453,16 +498,26 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restric
 }
 
 // ---- host ------------------------------------------------------------------------
-// Columns of a weight gradient's tile: 128, or 64 where both widths fit (half of a 128-wide tile would be
-// idle).
-static int gram_tile_q(int64_t C, int64_t Co) { return C <= 64 && Co <= 64 ? 64 : 128; }
+// Tiles of the weight gradients: 128 x 64 where both widths fit in 64 columns, 128 x 128, and for wider
+// rows 256 x 256, with which the L2 hands out half as much (50k rows of 512 channels, 1 376
+// hidden units: 1.7 GB for 3.3).
+struct GramShape {
+  int p, q;
+};
+static GramShape gram_shape(int64_t C, int64_t Co) {
+  const int64_t n = C > Co ? C : Co;
+  if (n <= 64) return {128, 64};
+  if (n <= 128) return {128, 128};
+  return {256, 256};
+}
 
-static int64_t gram_tiles(int64_t P, int64_t Q, int tq) { return cdiv(P, kGramP) * cdiv(Q, tq); }
+static int64_t gram_tiles(int64_t P, int64_t Q, GramShape t) { return cdiv(P, t.p) * cdiv(Q, t.q); }
 
-// Shares of the rows in the weight gradients: two workgroups a CU, each with at least 256 rows.
-static int64_t gram_shares(int64_t rows, int64_t tiles) {
-  const int64_t want = cdiv(512, tiles), most = cdiv(rows, 256);
-  return want < most ? want : most;
+// Shares of the rows in the weight gradients: two workgroups of 128 hidden units a CU or one of
+// 256, none of which waits for a second round, each with at least 256 rows.
+static int64_t gram_shares(int64_t rows, int64_t tiles, GramShape t) {
+  const int64_t want = (t.p == 256 ? 256 : 512) / tiles, most = cdiv(rows, 256);
+  return want < 1 ? 1 : want < most ? want : most;
 }
 
 // The backward pass's workspace, and which kernels it takes: for 16-bit rows of up to 128 channels two
@@ -485,10 +540,10 @@ static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t
   l.fused_weights = fused_weights_take(dtype, C, Co);
   l.Fp = int(cdiv(F, V) * V);
   l.Cop = int(cdiv(Co, V) * V);
-  const int tq = gram_tile_q(C, Co);
+  const GramShape t = gram_shape(C, Co);
   l.shares = l.fused_weights
                  ? fused_weights_shares(rows, C, F, Co)
-                 : gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C, tq) + gram_tiles(F, Co, tq));
+                 : gram_shares(rows, gram_tiles(2 * int64_t(l.Fp), C, t) + gram_tiles(F, Co, t), t);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -509,26 +564,79 @@ static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t
 }
 
 template <typename T>
-static int launch_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, int64_t ldr,
-                       void* out, int n, hipStream_t s) {
-  const dim3 grid(unsigned(cdiv(n, kTileRows)), unsigned(cdiv(a.n, kTileRows)));
-  ffn_rows<T><<<grid, kFfnThreads, 0, s>>>(a, w, static_cast<const T*>(residual), ldr,
-                                           static_cast<T*>(out), n);
+static bool whole(const Rows<T>& a) { return a.vec && a.K % Mfma<T>::V == 0; }
+
+// Workgroups of tiles of S: whole eights of row tiles (tile_of).
+template <typename S>
+static int64_t tile_groups(int64_t rows, int64_t cols) {
+  return cdiv(cdiv(rows, S::X), 8) * 8 * cols;
+}
+
+// The larger tiles where they still give every CU a workgroup or more: below that the smaller ones
+// spread the work further.
+template <typename S>
+static bool fills(int64_t rows, int64_t cols) { return cdiv(rows, S::X) * cols >= 256; }
+
+template <typename T, typename S, bool ASYNC>
+static int launch_up(const Rows<T>& x, const Rows<T>& wg, const Rows<T>& wu, int act, T* h,
+                     int Fp, hipStream_t s) {
+  const int64_t groups = tile_groups<S>(x.n, cdiv(Fp, S::W / 2));
+  SP_CHECK_ARG(groups <= kMaxGridX, "gated_ffn: too many rows");
+  ffn_up<T, S, ASYNC><<<unsigned(groups), S::THREADS, 0, s>>>(x, wg, wu, act, h, Fp);
   SP_LAUNCHED();
   return SP_OK;
+}
+
+template <typename T, typename S, bool ASYNC>
+static int launch_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, int64_t ldr,
+                       void* out, int n, hipStream_t s) {
+  const int64_t groups = tile_groups<S>(a.n, cdiv(n, S::W));
+  SP_CHECK_ARG(groups <= kMaxGridX, "gated_ffn: too many rows");
+  ffn_rows<T, S, ASYNC><<<unsigned(groups), S::THREADS, 0, s>>>(
+      a, w, static_cast<const T*>(residual), ldr, static_cast<T*>(out), n,
+      aligned(out) && n % Mfma<T>::V == 0);
+  SP_LAUNCHED();
+  return SP_OK;
+}
+
+template <typename T>
+static int run_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, int64_t ldr,
+                    void* out, int n, hipStream_t s) {
+  if (!whole(a) || !whole(w)) return launch_rows<T, SmallTile, false>(a, w, residual, ldr, out, n, s);
+  if (n > 128 && fills<LargeTile>(a.n, cdiv(n, LargeTile::W)))
+    return launch_rows<T, LargeTile, true>(a, w, residual, ldr, out, n, s);
+  if (fills<LongTile>(a.n, cdiv(n, LongTile::W)))
+    return launch_rows<T, LongTile, true>(a, w, residual, ldr, out, n, s);
+  return launch_rows<T, SmallTile, true>(a, w, residual, ldr, out, n, s);
 }
 
 template <typename T>
 static int forward(const FfnCall& a) {
   const int Fp = int(cdiv(a.F, Mfma<T>::V) * Mfma<T>::V);
   T* h = static_cast<T*>(a.ws);
-  const dim3 grid(unsigned(cdiv(a.F, kHiddenTile)), unsigned(cdiv(a.rows, kTileRows)));
-  ffn_up<T><<<grid, kFfnThreads, 0, a.stream>>>(
-      operand<T>(a.x, a.ldx, a.rows, a.C), operand<T>(a.wg, a.C, a.F, a.C),
-      operand<T>(a.wu, a.C, a.F, a.C), a.act, h, Fp);
+  const Rows<T> x = operand<T>(a.x, a.ldx, a.rows, a.C);
+  const Rows<T> wg = operand<T>(a.wg, a.C, a.F, a.C), wu = operand<T>(a.wu, a.C, a.F, a.C);
+  int rc;
+  if (!whole(x) || !whole(wg) || !whole(wu))
+    rc = launch_up<T, SmallTile, false>(x, wg, wu, a.act, h, Fp, a.stream);
+  else if (fills<LargeTile>(a.rows, cdiv(Fp, LargeTile::W / 2)))
+    rc = launch_up<T, LargeTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
+  else
+    rc = launch_up<T, SmallTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
+  if (rc) return rc;
+  return run_rows<T>(operand<T>(h, Fp, a.rows, a.F), operand<T>(a.wd, a.F, a.Co, a.F), a.residual,
+                     a.ldr, a.y, a.Co, a.stream);
+}
+
+template <typename T, typename S, bool ASYNC>
+static int launch_hidden(const Rows<T>& x, const Rows<T>& wg, const Rows<T>& wu, const Rows<T>& dy,
+                         const Rows<T>& wdt, int act, T* hid, int Fp, hipStream_t s) {
+  const int64_t groups = tile_groups<S>(x.n, cdiv(Fp, S::W / 2));
+  SP_CHECK_ARG(groups <= kMaxGridX, "gated_ffn_bwd: too many rows");
+  ffn_grad_hidden<T, S, ASYNC><<<unsigned(groups), S::THREADS, 0, s>>>(x, wg, wu, dy, wdt, act,
+                                                                       hid, Fp);
   SP_LAUNCHED();
-  return launch_rows<T>(operand<T>(h, Fp, a.rows, a.F), operand<T>(a.wd, a.F, a.Co, a.F),
-                        a.residual, a.ldr, a.y, a.Co, a.stream);
+  return SP_OK;
 }
 
 template <typename T>
@@ -548,17 +656,23 @@ static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
   T* wdt = reinterpret_cast<T*>(ws + l.wdt);
   T* wt = reinterpret_cast<T*>(ws + l.wt);
   if (int rc = transpose<T>(a.wd, a.Co, a.F, l.Cop, l.Cop, wdt, a.stream)) return rc;
-  const dim3 grid(unsigned(cdiv(a.F, kHiddenTile)), unsigned(cdiv(a.rows, kTileRows)));
-  ffn_grad_hidden<T><<<grid, kFfnThreads, 0, a.stream>>>(
-      operand<T>(a.x, a.ldx, a.rows, a.C), operand<T>(a.wg, a.C, a.F, a.C),
-      operand<T>(a.wu, a.C, a.F, a.C), operand<T>(a.dy, a.lddy, a.rows, a.Co),
-      operand<T>(wdt, l.Cop, a.F, a.Co), a.act, hid, l.Fp);
-  SP_LAUNCHED();
+  const Rows<T> x = operand<T>(a.x, a.ldx, a.rows, a.C), dy = operand<T>(a.dy, a.lddy, a.rows, a.Co);
+  const Rows<T> wg = operand<T>(a.wg, a.C, a.F, a.C), wu = operand<T>(a.wu, a.C, a.F, a.C);
+  // (Wd' has zeros past Co)
+  const Rows<T> d = operand<T>(wdt, l.Cop, a.F, a.Co);
+  int rc;
+  if (!whole(x) || !whole(wg) || !whole(wu) || !whole(dy))
+    rc = launch_hidden<T, SmallTile, false>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
+  else if (fills<LongTile>(a.rows, cdiv(l.Fp, LongTile::W / 2)))
+    rc = launch_hidden<T, LongTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
+  else
+    rc = launch_hidden<T, SmallTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
+  if (rc) return rc;
   if (!a.dx) return SP_OK;
   if (int rc = transpose<T>(a.wg, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt, a.stream)) return rc;
   if (int rc = transpose<T>(a.wu, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt + l.Fp, a.stream))
     return rc;
-  return launch_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
+  return run_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
                         operand<T>(wt, 2 * int64_t(l.Fp), a.C, 2 * int64_t(l.Fp)), nullptr, 0,
                         a.dx, a.C, a.stream);
 }
@@ -568,21 +682,23 @@ template <typename T>
 static int weight_products(const FfnCall& a, const FfnLayout& l, const T* hid, float* part0,
                            float* part1, int64_t* shares) {
   Gram<T> g0{}, g1{};
-  const int tq = gram_tile_q(a.C, a.Co);
+  const GramShape t = gram_shape(a.C, a.Co);
   auto gram = [&](const T* h, int P, const void* b, int64_t ldb, int Q, float* part) {
-    return Gram<T>{h, static_cast<const T*>(b), 3 * int64_t(l.Fp), ldb, P, Q, int(cdiv(Q, tq)),
-                   int(gram_tiles(P, Q, tq)), 1, aligned(b) && ldb % Mfma<T>::V == 0, part};
+    return Gram<T>{h, static_cast<const T*>(b), 3 * int64_t(l.Fp), ldb, P, Q, int(cdiv(Q, t.q)),
+                   int(gram_tiles(P, Q, t)), 1, aligned(b) && ldb % Mfma<T>::V == 0, part};
   };
   if (a.dwg || a.dwu) g0 = gram(hid, 2 * l.Fp, a.x, a.ldx, a.C, part0);
   if (a.dwd) g1 = gram(hid + 2 * int64_t(l.Fp), a.F, a.dy, a.lddy, a.Co, part1);
   constexpr int stage = gram_rows<T>();
   const int64_t share = cdiv(cdiv(a.rows, l.shares), stage) * stage;
   *shares = cdiv(a.rows, share);
-  const dim3 grid(unsigned(g0.tiles + g1.tiles), unsigned(*shares));
-  if (tq == 64)
-    ffn_gram<T, 64><<<grid, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
+  const unsigned groups = unsigned(cdiv(*shares, 8) * 8 * (g0.tiles + g1.tiles));
+  if (t.p == 256)
+    ffn_gram<T, 256, 256><<<groups, 512, 0, a.stream>>>(g0, g1, a.rows, share);
+  else if (t.q == 64)
+    ffn_gram<T, 128, 64><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share);
   else
-    ffn_gram<T, 128><<<grid, kFfnThreads, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 128, 128><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share);
   SP_LAUNCHED();
   return SP_OK;
 }
@@ -635,9 +751,7 @@ static int check_ffn(const char* what, int32_t dtype, int64_t rows, int64_t C, i
   SP_CHECK_ARG(rows >= 0 && C >= 1 && F >= 1 && Co >= 1 && C < 65536 && F < 65536 && Co < 65536,
                "%s: bad sizes rows=%lld C=%lld F=%lld Co=%lld", what, (long long)rows,
                (long long)C, (long long)F, (long long)Co);
-  // (workgroups along the rows are a grid's y)
-  SP_CHECK_ARG(cdiv(rows, kTileRows) <= 65535, "%s: more than %lld rows", what,
-               (long long)kTileRows * 65535);
+  SP_CHECK_ARG(rows < (int64_t(1) << 31), "%s: 2^31 rows or more", what);
   SP_CHECK_ARG(act >= kActSilu && act <= kActRelu, "%s: unknown activation %d", what, act);
   return SP_OK;
 }

@@ -8,27 +8,6 @@ namespace sp {
 
 constexpr int kFusedRows = 32;  // of a wave's tile
 
-// Row of a 32-row weight block that lies at operand row m: then accumulator register i of lane half b is
-// row 16 (i >> 3) + 8 b + (i & 7).
-__device__ __forceinline__ int unit_of(int m) {
-  return 16 * (m >> 4) + 8 * ((m >> 2) & 1) + 4 * ((m >> 3) & 1) + (m & 3);
-}
-
-__device__ const uint4 g_zero_piece = {0, 0, 0, 0};
-
-// 16 bytes from memory to LDS at `to` (the wave's first lane's) + 16 * lane.
-__device__ __forceinline__ void copy_piece(const void* from, char* to) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void*)from,
-      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-}
-
-// At most N of the wave's loads still on their way.
-template <int N>
-__device__ __forceinline__ void loads_in_flight() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
 // The weights as they lie in memory: rows of ldu (g, u) and ldd (d) elements.
 template <typename T>
 struct Weights {
