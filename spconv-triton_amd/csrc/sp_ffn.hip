@@ -163,13 +163,12 @@ __device__ __forceinline__ void write_piece_row(T* out, int64_t ld, int64_t r, i
   }
 }
 
-// Which tile a workgroup takes: consecutive workgroups go to the eight XCDs in turn, and an XCD goes through
-// the column tiles of a row tile one after the other, so that x's rows pass through one L2.
-__device__ __forceinline__ bool tile_of(int cols, int64_t rows, int64_t& row, int& col) {
-  const int64_t id = blockIdx.x, seq = id >> 3;
-  row = seq / cols * 8 + (id & 7);
-  col = int(seq % cols);
-  return row < rows;
+// The place of this workgroup among `total`: consecutive workgroups go to the eight XCDs in turn; here each XCD
+// gets an eighth of the places in a row, so that tiles which share rows meet in one L2.
+__device__ __forceinline__ int64_t place_of(int64_t total) {
+  const int64_t per = (total + 7) >> 3, id = blockIdx.x;
+  const int64_t k = (id >> 3) < per ? (id & 7) * per + (id >> 3) : total;
+  return k < total ? k : -1;
 }
 
 // h = act(x Wg') * (x Wu'); columns from F to the padded width are zeros.
@@ -180,11 +179,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, R
   constexpr int NH = S::WT / 2, HIDDEN = S::W / 2;  // a wave's tiles of each, the workgroup's units
   const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
   const int lane = int(threadIdx.x) & 31;
-  int64_t row;
-  int col;
-  if (!tile_of((Fp + HIDDEN - 1) / HIDDEN, (x.n + S::X - 1) / S::X, row, col)) return;
-  const int64_t x0 = row * S::X;
-  const int f0 = col * HIDDEN, xrow = wm * 32 * S::XT;
+  const int cols = (Fp + HIDDEN - 1) / HIDDEN;
+  const int64_t place = place_of((x.n + S::X - 1) / S::X * cols);
+  if (place < 0) return;
+  const int64_t x0 = place / cols * S::X;
+  const int f0 = int(place % cols) * HIDDEN, xrow = wm * 32 * S::XT;
   floatx16 acc[S::XT][S::WT];
   clear(acc);
   int wrow[S::WT];
@@ -213,45 +212,54 @@ template <typename T, typename S, bool ASYNC>
 __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows<T> wg, Rows<T> wu,
                                                               Rows<T> dy, Rows<T> wdt, int act,
                                                               T* __restrict__ out, int Fp) {
-  static_assert(S::WT == 2, "a gate and an up tile");
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
-  constexpr int HIDDEN = S::W / 2;
+  constexpr int NH = S::WT / 2, HIDDEN = S::W / 2;
   const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
   const int lane = int(threadIdx.x) & 31;
-  int64_t row;
-  int col;
-  if (!tile_of((Fp + HIDDEN - 1) / HIDDEN, (x.n + S::X - 1) / S::X, row, col)) return;
-  const int64_t x0 = row * S::X;
-  const int f0 = col * HIDDEN, xrow = wm * 32 * S::XT;
-  floatx16 acc[S::XT][2], dh[S::XT][1];
+  const int cols = (Fp + HIDDEN - 1) / HIDDEN;
+  const int64_t place = place_of((x.n + S::X - 1) / S::X * cols);
+  if (place < 0) return;
+  const int64_t x0 = place / cols * S::X;
+  const int f0 = int(place % cols) * HIDDEN, xrow = wm * 32 * S::XT;
+  floatx16 acc[S::XT][S::WT], dh[S::XT][NH];
   clear(acc);
   clear(dh);
-  const int wrow[2] = {wn * 32, HIDDEN + wn * 32}, drow[1] = {wn * 32};
-  products<T, S, ASYNC, 2>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
+  int wrow[S::WT], drow[NH];
+#pragma unroll
+  for (int i = 0; i < NH; ++i) {
+    drow[i] = wrow[i] = (wn * NH + i) * 32;
+    wrow[NH + i] = HIDDEN + wrow[i];
+  }
+  products<T, S, ASYNC, S::WT>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
   if (wdt.n > f0 + HIDDEN) wdt.n = f0 + HIDDEN;  // (half of a stage's weight rows)
-  products<T, S, ASYNC, 1>(dy, x0, wdt, nullptr, f0, drow, xrow, lds, dh);
+  products<T, S, ASYNC, NH>(dy, x0, wdt, nullptr, f0, drow, xrow, lds, dh);
   with_gate<sizeof(T) == 2>(act, [&](auto gate) {
 #pragma unroll
     for (int j = 0; j < S::XT; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float value, slope;
-        gate(acc[j][0][i], value, slope);
-        const float u = acc[j][1][i], d = dh[j][0][i];
-        acc[j][0][i] = d * u * slope;
-        acc[j][1][i] = d * value;
-        dh[j][0][i] = value * u;
-      }
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float value, slope;
+          gate(acc[j][n][i], value, slope);
+          const float u = acc[j][NH + n][i], d = dh[j][n][i];
+          acc[j][n][i] = d * u * slope;
+          acc[j][NH + n][i] = d * value;
+          dh[j][n][i] = value * u;
+        }
   });
 #pragma unroll
-  for (int j = 0; j < S::XT; ++j) {
-    const int64_t r = x0 + xrow + 32 * j + lane, ld = 3 * int64_t(Fp);
-    const int f = f0 + wn * 32;
-    write_piece_row<T>(out, ld, r, x.n, f, Fp, true, [&](int k, int) { return acc[j][0][k]; });
-    write_piece_row<T>(out + Fp, ld, r, x.n, f, Fp, true, [&](int k, int) { return acc[j][1][k]; });
-    write_piece_row<T>(out + 2 * Fp, ld, r, x.n, f, Fp, true,
-                       [&](int k, int) { return dh[j][0][k]; });
-  }
+  for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const int64_t r = x0 + xrow + 32 * j + lane, ld = 3 * int64_t(Fp);
+      const int f = f0 + drow[n];
+      write_piece_row<T>(out, ld, r, x.n, f, Fp, true, [&](int k, int) { return acc[j][n][k]; });
+      write_piece_row<T>(out + Fp, ld, r, x.n, f, Fp, true,
+                         [&](int k, int) { return acc[j][NH + n][k]; });
+      write_piece_row<T>(out + 2 * Fp, ld, r, x.n, f, Fp, true,
+                         [&](int k, int) { return dh[j][n][k]; });
+    }
 }
 
 // out = a w' (+ residual, added in fp32).
@@ -263,11 +271,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
   __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
   const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
   const int lane = int(threadIdx.x) & 31;
-  int64_t row;
-  int col;
-  if (!tile_of((n + S::W - 1) / S::W, (a.n + S::X - 1) / S::X, row, col)) return;
-  const int64_t x0 = row * S::X;
-  const int n0 = col * S::W, xrow = wm * 32 * S::XT;
+  const int cols = (n + S::W - 1) / S::W;
+  const int64_t place = place_of((a.n + S::X - 1) / S::X * cols);
+  if (place < 0) return;
+  const int64_t x0 = place / cols * S::X;
+  const int n0 = int(place % cols) * S::W, xrow = wm * 32 * S::XT;
   floatx16 acc[S::XT][S::WT];
   clear(acc);
   int wrow[S::WT];
@@ -398,11 +406,10 @@ struct GramStage {
   }
 };
 
-// Waves of WP x 2, each with 64 x TQ / 2 of the tile.  The tiles of a share run on one XCD, one after the
-// other, so that its rows pass through one L2.
+// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile.
 template <typename T, int TP, int TQ>
 __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
-                                                      int64_t share) {
+                                                      int64_t share, int shares) {
   using frag = typename Mfma<T>::frag;
   constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>(), NQ = TQ / 64;
   constexpr int STAGE = kGramStage * (TP + TQ);
@@ -410,10 +417,10 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
   using SB = GramStage<T, TQ, THREADS>;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   const int tiles = g0.tiles + g1.tiles;
-  const int64_t id = blockIdx.x, seq = id >> 3;
-  const int64_t lo = (seq / tiles * 8 + (id & 7)) * share;
-  if (lo >= rows) return;
-  int tile = int(seq % tiles);
+  const int64_t place = place_of(int64_t(tiles) * shares);
+  if (place < 0) return;
+  const int64_t lo = place / tiles * share;
+  int tile = int(place % tiles);
   const bool second = tile >= g0.tiles;
   if (second) tile -= g0.tiles;
   const Gram<T> g = second ? g1 : g0;
@@ -566,10 +573,10 @@ static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t
 template <typename T>
 static bool whole(const Rows<T>& a) { return a.vec && a.K % Mfma<T>::V == 0; }
 
-// Workgroups of tiles of S: whole eights of row tiles (tile_of).
+// Workgroups of tiles of S: whole eights (place_of).
 template <typename S>
 static int64_t tile_groups(int64_t rows, int64_t cols) {
-  return cdiv(cdiv(rows, S::X), 8) * 8 * cols;
+  return cdiv(cdiv(rows, S::X) * cols, 8) * 8;
 }
 
 // The larger tiles where they still give every CU a workgroup or more: below that the smaller ones
@@ -692,13 +699,13 @@ static int weight_products(const FfnCall& a, const FfnLayout& l, const T* hid, f
   constexpr int stage = gram_rows<T>();
   const int64_t share = cdiv(cdiv(a.rows, l.shares), stage) * stage;
   *shares = cdiv(a.rows, share);
-  const unsigned groups = unsigned(cdiv(*shares, 8) * 8 * (g0.tiles + g1.tiles));
+  const unsigned groups = unsigned(cdiv(*shares * (g0.tiles + g1.tiles), 8) * 8);
   if (t.p == 256)
-    ffn_gram<T, 256, 256><<<groups, 512, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 256, 256><<<groups, 512, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   else if (t.q == 64)
-    ffn_gram<T, 128, 64><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 128, 64><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   else
-    ffn_gram<T, 128, 128><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share);
+    ffn_gram<T, 128, 128><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   SP_LAUNCHED();
   return SP_OK;
 }
