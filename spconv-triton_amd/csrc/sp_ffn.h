@@ -121,6 +121,34 @@ __device__ __forceinline__ void loads_in_flight() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// STEPS steps of products whose operands F come from LDS, B steps' reads at a time: a batch is read while the
+// one before is in use.  Left to itself the compiler reads and waits step by step (LDS latency
+// each time; 1.6 times the time of a 256-channel call).  `start` may come early.
+template <typename F, int STEPS, int B>
+struct Batched {
+  static constexpr int BATCHES = (STEPS + B - 1) / B;
+  F f[2][B];
+  template <typename Read>
+  __device__ __forceinline__ void start(Read&& read) {
+#pragma unroll
+    for (int i = 0; i < B && i < STEPS; ++i) f[0][i] = read(i);
+  }
+  template <typename Read, typename Use>
+  __device__ __forceinline__ void run(Read&& read, Use&& use) {
+#pragma unroll
+    for (int b = 0; b < BATCHES; ++b) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if ((b + 1) * B + i < STEPS) f[(b + 1) & 1][i] = read((b + 1) * B + i);
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+        if (b * B + i < STEPS) use(b * B + i, f[b & 1][i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+};
+
 inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // A row-major operand: rows of K values; vec: rows start at multiples of 16 bytes.

@@ -92,6 +92,11 @@ struct Stage {
   }
 };
 
+template <typename T, int M, int N>
+struct Operands {
+  typename Mfma<T>::frag x[M], w[N];
+};
+
 // acc[j][i] += the products of x rows xrow + 32 j .. + 31 and weight rows wrow[i] .. + 31 of the stage
 // over all of K.
 template <typename T, typename S, bool ASYNC, int NW>
@@ -110,18 +115,22 @@ __device__ __forceinline__ void products(const Rows<T>& x, int64_t x0, const Row
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (s + 1 < steps)
       stage.start(x, x0, w, w2, w0, (s + 1) * STEP, lds + ((s + 1) & 1) * S::BYTES);
+    auto read = [&](int c) {
+      Operands<T, S::XT, NW> f;
 #pragma unroll
-    for (int c = 0; c < kStagePieces; c += 2) {
-      typename Mfma<T>::frag fx[S::XT], fw[NW];
+      for (int j = 0; j < S::XT; ++j) f.x[j] = Stg::read(buf, xrow + 32 * j + lane, 2 * c + half);
 #pragma unroll
-      for (int j = 0; j < S::XT; ++j) fx[j] = Stg::read(buf, xrow + 32 * j + lane, c + half);
-#pragma unroll
-      for (int i = 0; i < NW; ++i) fw[i] = Stg::read(buf, S::X + wrow[i] + lane, c + half);
+      for (int i = 0; i < NW; ++i) f.w[i] = Stg::read(buf, S::X + wrow[i] + lane, 2 * c + half);
+      return f;
+    };
+    Batched<Operands<T, S::XT, NW>, kStagePieces / 2, 1> steps_of;
+    steps_of.start(read);
+    steps_of.run(read, [&](int, const Operands<T, S::XT, NW>& f) {
 #pragma unroll
       for (int j = 0; j < S::XT; ++j)
 #pragma unroll
-        for (int i = 0; i < NW; ++i) Mfma<T>::mma(fw[i], fx[j], acc[j][i]);
-    }
+        for (int i = 0; i < NW; ++i) Mfma<T>::mma(f.w[i], f.x[j], acc[j][i]);
+    });
   }
   __syncthreads();
 }
@@ -410,7 +419,6 @@ struct GramStage {
 template <typename T, int TP, int TQ>
 __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
                                                       int64_t share, int shares) {
-  using frag = typename Mfma<T>::frag;
   constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>(), NQ = TQ / 64;
   constexpr int STAGE = kGramStage * (TP + TQ);
   using SA = GramStage<T, TP, THREADS>;
@@ -444,18 +452,22 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
     sb.store(lb);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) fetch(m + ROWS);
+    auto read = [&](int k) {
+      Operands<T, 2, NQ> f;
 #pragma unroll
-    for (int k = 0; k < ROWS; k += 2 * Mfma<T>::V) {
-      frag fa[2], fb[NQ];
+      for (int i = 0; i < 2; ++i) f.x[i] = SA::read(la, k * 2 * Mfma<T>::V, wp + 32 * i);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) fa[i] = SA::read(la, k, wp + 32 * i);
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) fb[i] = SB::read(lb, k, wq + 32 * i);
+      for (int i = 0; i < NQ; ++i) f.w[i] = SB::read(lb, k * 2 * Mfma<T>::V, wq + 32 * i);
+      return f;
+    };
+    Batched<Operands<T, 2, NQ>, ROWS / (2 * Mfma<T>::V), 1> steps;
+    steps.start(read);
+    steps.run(read, [&](int, const Operands<T, 2, NQ>& f) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) Mfma<T>::mma(fa[i], fb[j], acc[i][j]);
-    }
+        for (int j = 0; j < NQ; ++j) Mfma<T>::mma(f.x[i], f.w[j], acc[i][j]);
+    });
   }
   float* part = g.part + lo / share * g.P * g.Q;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;

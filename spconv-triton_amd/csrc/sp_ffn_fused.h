@@ -118,34 +118,6 @@ __device__ __forceinline__ void load_rows(const Rows<T>& x, int64_t r,
   }
 }
 
-// STEPS steps of products whose operands F come from LDS, B steps' reads at a time: a batch is read while the
-// one before is in use.  Left to itself the compiler reads and waits step by step (LDS latency
-// each time; 1.6 times the time of a 256-channel call).  `start` may come early.
-template <typename F, int STEPS, int B>
-struct Batched {
-  static constexpr int BATCHES = (STEPS + B - 1) / B;
-  F f[2][B];
-  template <typename Read>
-  __device__ __forceinline__ void start(Read&& read) {
-#pragma unroll
-    for (int i = 0; i < B && i < STEPS; ++i) f[0][i] = read(i);
-  }
-  template <typename Read, typename Use>
-  __device__ __forceinline__ void run(Read&& read, Use&& use) {
-#pragma unroll
-    for (int b = 0; b < BATCHES; ++b) {
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < B; ++i)
-        if ((b + 1) * B + i < STEPS) f[(b + 1) & 1][i] = read((b + 1) * B + i);
-#pragma unroll
-      for (int i = 0; i < B; ++i)
-        if (b * B + i < STEPS) use(b * B + i, f[b & 1][i]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-};
-
 template <typename T>
 struct FragPair {
   typename Mfma<T>::frag a, b;
