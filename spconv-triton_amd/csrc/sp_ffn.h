@@ -1,6 +1,8 @@
 // What the kernels of the gated feed-forward block share.
 #pragma once
 
+#include <type_traits>
+
 #include "sp_common.h"
 #include "sp_mfma.h"
 
@@ -50,9 +52,9 @@ __device__ __forceinline__ void gate(float z, float& value, float& slope) {
 
 // The gate of sixteen values of an accumulator, f(i, value, slope) for each, in stages, so that the
 // exponentials and reciprocals of one value do not wait for each other.
-template <int ACT, typename F>
+template <bool FAST, int ACT, typename F>
 __device__ __forceinline__ void gate16(const floatx16& z, F&& f) {
-  if constexpr (ACT == kActSilu) {
+  if constexpr (ACT == kActSilu && FAST) {
     float t[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) t[i] = __builtin_amdgcn_exp2f(z[i] * -1.4426950408889634f);
@@ -69,21 +71,21 @@ __device__ __forceinline__ void gate16(const floatx16& z, F&& f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float value, slope;
-      gate<true, ACT>(z[i], value, slope);
+      gate<FAST, ACT>(z[i], value, slope);
       f(i, value, slope);
     }
   }
 }
 
-// f(z, value, slope) for the call's activation: one branch around the whole of `loop`.
-template <bool FAST, typename Loop>
-__device__ __forceinline__ void with_gate(int act, Loop&& loop) {
+// loop(kind) with the call's activation as a constant: one branch around the whole of it.
+template <typename Loop>
+__device__ __forceinline__ void with_act(int act, Loop&& loop) {
   if (act == kActSilu)
-    loop([](float z, float& v, float& s) { gate<FAST, kActSilu>(z, v, s); });
+    loop(std::integral_constant<int, kActSilu>());
   else if (act == kActGelu)
-    loop([](float z, float& v, float& s) { gate<FAST, kActGelu>(z, v, s); });
+    loop(std::integral_constant<int, kActGelu>());
   else
-    loop([](float z, float& v, float& s) { gate<FAST, kActRelu>(z, v, s); });
+    loop(std::integral_constant<int, kActRelu>());
 }
 
 // Where piece c (16 bytes) of row r lies in LDS rows of PIECES pieces, so that no two lanes of a group
@@ -113,6 +115,11 @@ __device__ __forceinline__ void copy_piece(const void* from, char* to) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) void*)from,
       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// The wave's number in its workgroup, as one value for all of its lanes.
+__device__ __forceinline__ int wave_of() {
+  return __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
 }
 
 // At most N of the wave's loads still on their way.

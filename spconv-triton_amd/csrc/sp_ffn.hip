@@ -40,43 +40,75 @@ __device__ __forceinline__ int weight_row(int m) {
 
 // A stage: 128 bytes of X rows of x and of W weight rows, from w, or the first half of them from w and
 // the other from w2.  ASYNC: straight to LDS, for operands whose rows start at multiples of 16 bytes
-// and have whole pieces; else through registers.
+// and have whole pieces; rows past an operand's end are its last one, whose products no output
+// takes up (a hidden column past F meets zeros).  Else through registers, with zeros past the ends.
 template <typename T, typename S, bool ASYNC>
 struct Stage {
   using frag = typename Mfma<T>::frag;
   static constexpr int V = Mfma<T>::V, N = S::PIECES / S::THREADS;
+  const T* from[N];  // of this thread's pieces, at k
   frag r[ASYNC ? 1 : N];
+  unsigned in;  // whether a piece's row exists
+  int k, K;
 
-  // operand row i / 8 and piece i % 8 of LDS slot i
-  __device__ __forceinline__ static frag piece(const Rows<T>& a, int64_t row, int k) {
-    frag f = {};
-    if (row >= a.n || k >= a.K) return f;
-    const T* q = a.p + row * a.ld + k;
-    if (a.vec && k + V <= a.K) return *reinterpret_cast<const frag*>(q);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (k + i < a.K) f[i] = q[i];
-    return f;
+  // LDS slot i = j THREADS + thread holds piece i % 8 (permuted) of operand row i / 8
+  __device__ __forceinline__ static int first_k() {
+    const int row = int(threadIdx.x) >> 3;  // (j THREADS / 8 rows further the order is the same)
+    return swizzled<8>(row, int(threadIdx.x) & 7) * V;
   }
-  __device__ __forceinline__ void start(const Rows<T>& x, int64_t x0, const Rows<T>& w,
-                                        const Rows<T>* w2, int64_t w0, int k0, char* lds) {
+  __device__ __forceinline__ Stage(const Rows<T>& x, int64_t x0, const Rows<T>& w,
+                                   const Rows<T>* w2, int64_t w0)
+      : in(0u), k(first_k()), K(x.K) {
+    static_assert(S::THREADS % 256 == 0 && S::X * 8 % S::THREADS == 0 &&
+                      S::W * 4 % S::THREADS == 0, "whole rounds of an operand");
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = j * S::THREADS + int(threadIdx.x), row = i >> 3;
-      const int k = k0 + swizzled<8>(row, i & 7) * V;
-      const bool second = w2 && j * S::THREADS >= (S::X + S::W / 2) * 8;  // (whole rounds)
+      const int row = (j * S::THREADS + int(threadIdx.x)) >> 3;
+      const bool second = w2 && j * S::THREADS >= (S::X + S::W / 2) * 8;
       const bool weights = j * S::THREADS >= S::X * 8;
       const Rows<T>& a = second ? *w2 : weights ? w : x;
-      const int64_t at = !weights ? x0 + row
-                                  : w0 + weight_row<T>(row - S::X - (second ? S::W / 2 : 0));
-      if constexpr (ASYNC) {
-        const void* from = &g_zero_piece;
-        if (at < a.n && k < a.K) from = a.p + at * a.ld + k;
-        copy_piece(from, lds + (i - (int(threadIdx.x) & 63)) * 16);
-      } else {
-        r[j] = piece(a, at, k);
-      }
+      int64_t at = !weights ? x0 + row
+                            : w0 + weight_row<T>(row - S::X - (second ? S::W / 2 : 0));
+      if (at < a.n)
+        in |= 1u << j;
+      else
+        at = a.n - 1;
+      from[j] = a.p + at * a.ld + k;
     }
+  }
+  // tail: the operands end within this stage
+  __device__ __forceinline__ void start(const Rows<T>& x, const Rows<T>& w, char* lds, bool tail) {
+    const int at = wave_of() * 64;
+    if (ASYNC && !tail) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        copy_piece(from[j], lds + (j * S::THREADS + at) * 16);
+        from[j] += kStagePieces * V;
+      }
+      k += kStagePieces * V;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (ASYNC) {
+        copy_piece(k < K ? static_cast<const void*>(from[j]) : &g_zero_piece,
+                   lds + (j * S::THREADS + at) * 16);
+      } else {
+        const bool vec = j * S::THREADS >= S::X * 8 ? w.vec : x.vec;
+        r[j] = frag{};
+        if (in >> j & 1) {
+          if (vec && k + V <= K) {
+            r[j] = *reinterpret_cast<const frag*>(from[j]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (k + i < K) r[j][i] = from[j][i];
+          }
+        }
+      }
+      from[j] += kStagePieces * V;
+    }
+    k += kStagePieces * V;
   }
   __device__ __forceinline__ void finish(char* lds) const {
     if constexpr (ASYNC) {
@@ -106,15 +138,15 @@ __device__ __forceinline__ void products(const Rows<T>& x, int64_t x0, const Row
   using Stg = Stage<T, S, ASYNC>;
   constexpr int STEP = kStagePieces * Mfma<T>::V;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
-  Stg stage;
+  Stg stage(x, x0, w, w2, w0);
   const int steps = (x.K + STEP - 1) / STEP;
-  stage.start(x, x0, w, w2, w0, 0, lds);
+  stage.start(x, w, lds, x.K < STEP);
   for (int s = 0; s < steps; ++s) {
     char* buf = lds + (s & 1) * S::BYTES;
     stage.finish(buf);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (s + 1 < steps)
-      stage.start(x, x0, w, w2, w0, (s + 1) * STEP, lds + ((s + 1) & 1) * S::BYTES);
+      stage.start(x, w, lds + ((s + 1) & 1) * S::BYTES, (s + 2) * STEP > x.K);
     auto read = [&](int c) {
       Operands<T, S::XT, NW> f;
 #pragma unroll
@@ -202,17 +234,17 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, R
     wrow[NH + i] = HIDDEN + (wn * NH + i) * 32;
   }
   products<T, S, ASYNC, S::WT>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
-  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
+  with_act(act, [&](auto kind) {
 #pragma unroll
     for (int j = 0; j < S::XT; ++j)
 #pragma unroll
-      for (int i = 0; i < NH; ++i)
+      for (int i = 0; i < NH; ++i) {
+        const floatx16 z = acc[j][i];
+        gate16<sizeof(T) == 2, kind.value>(
+            z, [&](int k, float value, float) { acc[j][i][k] = value * acc[j][NH + i][k]; });
         write_piece_row<T>(h, Fp, x0 + xrow + 32 * j + lane, x.n, f0 + wrow[i], Fp, true,
-                           [&](int k, int) {
-                             float value, slope;
-                             gate(acc[j][i][k], value, slope);
-                             return value * acc[j][NH + i][k];
-                           });
+                           [&](int k, int) { return acc[j][i][k]; });
+      }
   });
 }
 
@@ -242,20 +274,19 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
   products<T, S, ASYNC, S::WT>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
   if (wdt.n > f0 + HIDDEN) wdt.n = f0 + HIDDEN;  // (half of a stage's weight rows)
   products<T, S, ASYNC, NH>(dy, x0, wdt, nullptr, f0, drow, xrow, lds, dh);
-  with_gate<sizeof(T) == 2>(act, [&](auto gate) {
+  with_act(act, [&](auto kind) {
 #pragma unroll
     for (int j = 0; j < S::XT; ++j)
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float value, slope;
-          gate(acc[j][n][i], value, slope);
+      for (int n = 0; n < NH; ++n) {
+        const floatx16 z = acc[j][n];
+        gate16<sizeof(T) == 2, kind.value>(z, [&](int i, float value, float slope) {
           const float u = acc[j][NH + n][i], d = dh[j][n][i];
           acc[j][n][i] = d * u * slope;
           acc[j][NH + n][i] = d * value;
           dh[j][n][i] = value * u;
-        }
+        });
+      }
   });
 #pragma unroll
   for (int j = 0; j < S::XT; ++j)

@@ -52,7 +52,7 @@ struct Chunk {
       const T* bg = w.g + int64_t(f0) * w.ldu;
       const T* bu = w.u + int64_t(f0) * w.ldu;
       const T* bd = w.d + f0;
-      char* at = to + (i - (tid & 63)) * 16;
+      char* at = to + (j * kFfnThreads + wave_of() * 64) * 16;
       if (whole) {
         copy_piece(bg + ou, at);
         copy_piece(bu + ou, at + STRIDE);

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
     Batched<frag, CP / 16, 4> down;
     down.start(read);
     frag h[2];
-    gate16<ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
+    gate16<true, ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
     down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i & 1], y[i >> 1]); });
   }
   chunks.done();

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a)
     Batched<FragPair<T>, CP / 16, 2> wgu;
     wgu.start(up);
     frag dg[2], du[2], h[2];
-    gate16<ACT>(g, [&](int i, float value, float slope) {
+    gate16<true, ACT>(g, [&](int i, float value, float slope) {
       dg[i >> 3][i & 7] = T(dh[i] * u[i] * slope);
       du[i >> 3][i & 7] = T(dh[i] * value);
       if (HIDDEN) h[i >> 3][i & 7] = T(value * u[i]);
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradAr
     for (int n = 0; n < U; ++n) {
       // register 8 s + j of lane half b holds row 16 s + 8 (j >> 2) + 4 b + (j & 3) of the tile
       frag dg[2], du[2], h[2];
-      gate16<ACT>(g[n], [&](int i, float value, float slope) {
+      gate16<true, ACT>(g[n], [&](int i, float value, float slope) {
         dg[i >> 3][i & 7] = T(dh[n][i] * u[n][i] * slope);
         du[i >> 3][i & 7] = T(dh[n][i] * value);
         h[i >> 3][i & 7] = T(value * u[n][i]);
