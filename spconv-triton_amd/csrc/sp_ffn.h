@@ -190,10 +190,10 @@ struct FfnCall {
 // The one-kernel passes, for 16-bit rows of at most kFusedWidth channels on either side
 // (sp_ffn_fused.hip, sp_ffn_grad.hip).  `weights`: what copies of weights may take whose rows do not
 // start at multiples of 16 bytes.
-constexpr int kFusedWidth = 256;
+constexpr int kFusedWidth = 192;
 constexpr int kFusedGramWidth = 128;  // the weight gradients' own kernel
 size_t fused_weights_bytes(int64_t C, int64_t F, int64_t Co);
-bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
+bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t Co);
 int fused_forward(int32_t dtype, const FfnCall& a);
 
 // The backward pass: dx, and either the weight gradients' partials or the hidden rows for a
@@ -204,8 +204,7 @@ struct FusedGrad {
   int64_t shares;
   int Fp;
 };
-bool fused_backward_takes(int32_t dtype, int64_t C, int64_t Co);
-bool fused_weights_take(int32_t dtype, int64_t C, int64_t Co);
+bool fused_backward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t Co);
 int64_t fused_weights_shares(int64_t rows, int64_t C, int64_t F, int64_t Co);
 // *shares: how many partials there are (at most o.shares)
 int fused_backward(int32_t dtype, const FfnCall& a, const FusedGrad& o, int64_t* shares);

@@ -547,6 +547,101 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restric
   dst[which == 2 ? (i - f * Co) * F + f : i] = from_f32<T>(v);
 }
 
+// ---- a few rows ------------------------------------------------------------------
+// For up to four rows the weights are read once and nothing else counts: a group of lanes takes an
+// output, each lane pieces of its weight row against the same pieces of every row, and h stays
+// fp32.  One row of 512 -> 1376 bf16 8.7 us (tiles 22.3), of 64 -> 172 fp16 6.5 (one kernel 9.7); four rows
+// 19 and 10, eight 34 and 16.
+constexpr int kFewRows = 4;
+
+// The sums of a over `lanes` lanes, on each of them.
+template <int N>
+__device__ __forceinline__ void sum_lanes(float (&a)[N], int lanes) {
+  for (int off = lanes >> 1; off >= 1; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] += __shfl_xor(a[i], off, 64);
+}
+
+template <typename T>
+__device__ __forceinline__ typename Mfma<T>::frag piece_of(const Rows<T>& a, int64_t r, int k) {
+  typename Mfma<T>::frag f = {};
+  constexpr int V = Mfma<T>::V;
+  const T* p = a.p + r * a.ld + k;
+  if (a.vec && k + V <= a.K) return *reinterpret_cast<const typename Mfma<T>::frag*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (k + i < a.K) f[i] = p[i];
+  return f;
+}
+
+template <typename T, int R>
+__global__ __launch_bounds__(kFfnThreads) void ffn_few_up(Rows<T> x, Rows<T> wg, Rows<T> wu,
+                                                          int act, int log_lanes,
+                                                          float* __restrict__ h) {
+  constexpr int V = Mfma<T>::V;
+  const int lanes = 1 << log_lanes, lane = int(threadIdx.x) & (lanes - 1);
+  const int64_t f = int64_t(blockIdx.x) * (kFfnThreads >> log_lanes) + (int(threadIdx.x) >> log_lanes);
+  float a[2 * R];
+#pragma unroll
+  for (int i = 0; i < 2 * R; ++i) a[i] = 0.f;
+  if (f < wg.n)
+    for (int k = lane * V; k < x.K; k += lanes * V) {
+      const auto g = piece_of(wg, f, k), u = piece_of(wu, f, k);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const auto v = piece_of(x, r < x.n ? r : x.n - 1, k);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          a[r] = __builtin_fmaf(to_f32(v[i]), to_f32(g[i]), a[r]);
+          a[R + r] = __builtin_fmaf(to_f32(v[i]), to_f32(u[i]), a[R + r]);
+        }
+      }
+    }
+  sum_lanes(a, lanes);
+  if (f >= wg.n || lane != 0) return;
+  with_act(act, [&](auto kind) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float value, slope;
+      gate<false, kind.value>(a[r], value, slope);
+      if (r < x.n) h[r * wg.n + f] = value * a[R + r];
+    }
+  });
+}
+
+template <typename T, int R>
+__global__ __launch_bounds__(kFfnThreads) void ffn_few_down(const float* __restrict__ h, int rows,
+                                                            Rows<T> wd,
+                                                            const T* __restrict__ residual,
+                                                            int64_t ldr, int log_lanes,
+                                                            T* __restrict__ y) {
+  constexpr int V = Mfma<T>::V;
+  const int lanes = 1 << log_lanes, lane = int(threadIdx.x) & (lanes - 1);
+  const int64_t c = int64_t(blockIdx.x) * (kFfnThreads >> log_lanes) + (int(threadIdx.x) >> log_lanes);
+  float a[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) a[i] = 0.f;
+  if (c < wd.n)
+    for (int k = lane * V; k < wd.K; k += lanes * V) {
+      const auto w = piece_of(wd, c, k);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (k + i < wd.K)
+            a[r] = __builtin_fmaf(h[int64_t(r < rows ? r : rows - 1) * wd.K + k + i], to_f32(w[i]),
+                                  a[r]);
+    }
+  sum_lanes(a, lanes);
+  if (c >= wd.n || lane != 0) return;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (r < rows) {
+      const float v = residual ? a[r] + to_f32(residual[r * ldr + c]) : a[r];
+      y[r * wd.n + c] = from_f32<T>(v);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------
 // Tiles of the weight gradients: 128 x 64 where both widths fit in 64 columns, 128 x 128, and for wider
 // rows 256 x 256, with which the L2 hands out half as much (50k rows of 512 channels, 1 376
@@ -571,7 +666,7 @@ static int64_t gram_shares(int64_t rows, int64_t tiles, GramShape t) {
 }
 
 // The backward pass's workspace, and which kernels it takes: for 16-bit rows of up to 128 channels two
-// that form everything again (fused, fused_weights), up to 256 one that also writes the hidden
+// that form everything again (fused, fused_weights), up to 192 one that also writes the hidden
 // rows, from which ffn_gram makes the weight gradients (fused); else ffn_grad_hidden,
 // ffn_rows and ffn_gram.
 struct FfnLayout {
@@ -586,8 +681,8 @@ static FfnLayout backward_layout(int32_t dtype, int64_t rows, int64_t C, int64_t
   FfnLayout l{};
   const int V = vec_of(dtype);
   const size_t z = size_of(dtype);
-  l.fused = fused_backward_takes(dtype, C, Co);
-  l.fused_weights = fused_weights_take(dtype, C, Co);
+  l.fused = fused_backward_takes(dtype, rows, C, Co);
+  l.fused_weights = l.fused && C <= kFusedGramWidth && Co <= kFusedGramWidth;
   l.Fp = int(cdiv(F, V) * V);
   l.Cop = int(cdiv(Co, V) * V);
   const GramShape t = gram_shape(C, Co);
@@ -676,6 +771,36 @@ static int forward(const FfnCall& a) {
   if (rc) return rc;
   return run_rows<T>(operand<T>(h, Fp, a.rows, a.F), operand<T>(a.wd, a.F, a.Co, a.F), a.residual,
                      a.ldr, a.y, a.Co, a.stream);
+}
+
+// Lanes of an output: as many as its weight row has pieces, up to a wave.
+static int few_lanes(int64_t K, int V) {
+  int l = 0;
+  while (l < 6 && (int64_t(V) << l) < K) ++l;
+  return l;
+}
+
+template <typename T, int R>
+static int launch_few(const FfnCall& a) {
+  constexpr int V = Mfma<T>::V;
+  float* h = static_cast<float*>(a.ws);
+  const int lu = few_lanes(a.C, V), ld = few_lanes(a.F, V);
+  ffn_few_up<T, R><<<unsigned(cdiv(a.F, kFfnThreads >> lu)), kFfnThreads, 0, a.stream>>>(
+      operand<T>(a.x, a.ldx, a.rows, a.C), operand<T>(a.wg, a.C, a.F, a.C),
+      operand<T>(a.wu, a.C, a.F, a.C), a.act, lu, h);
+  SP_LAUNCHED();
+  ffn_few_down<T, R><<<unsigned(cdiv(a.Co, kFfnThreads >> ld)), kFfnThreads, 0, a.stream>>>(
+      h, int(a.rows), operand<T>(a.wd, a.F, a.Co, a.F), static_cast<const T*>(a.residual), a.ldr,
+      ld, static_cast<T*>(a.y));
+  SP_LAUNCHED();
+  return SP_OK;
+}
+
+template <typename T>
+static int few_forward(const FfnCall& a) {
+  if (a.rows == 1) return launch_few<T, 1>(a);
+  if (a.rows == 2) return launch_few<T, 2>(a);
+  return launch_few<T, 4>(a);
 }
 
 template <typename T, typename S, bool ASYNC>
@@ -813,7 +938,8 @@ using namespace sp;
 extern "C" size_t sp_gated_ffn_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F,
                                          int64_t Co) {
   if (check_ffn("gated_ffn", dtype, rows, C, F, Co, 0) != SP_OK || rows == 0) return 0;
-  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_weights_bytes(C, F, Co);
+  if (rows <= kFewRows) return size_t(rows) * F * sizeof(float);
+  if (fused_forward_takes(dtype, rows, C, Co)) return fused_weights_bytes(C, F, Co);
   return size_t(rows) * (cdiv(F, vec_of(dtype)) * vec_of(dtype)) * size_of(dtype);
 }
 
@@ -835,7 +961,10 @@ extern "C" int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t r
   a.ldx = ldx, a.ldr = ldr, a.rows = rows;
   a.C = int(C), a.F = int(F), a.Co = int(Co), a.act = act;
   a.y = y, a.ws = ws, a.stream = as_stream(stream);
-  if (fused_forward_takes(dtype, rows, C, F, Co)) return fused_forward(dtype, a);
+  if (rows <= kFewRows)
+    return dtype == SP_F16 ? few_forward<_Float16>(a)
+                           : dtype == SP_BF16 ? few_forward<__bf16>(a) : few_forward<float>(a);
+  if (fused_forward_takes(dtype, rows, C, Co)) return fused_forward(dtype, a);
   return dtype == SP_F16 ? forward<_Float16>(a)
                          : dtype == SP_BF16 ? forward<__bf16>(a) : forward<float>(a);
 }

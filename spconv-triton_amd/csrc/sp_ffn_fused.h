@@ -23,30 +23,27 @@ template <int CP>
 struct Chunk {
   static constexpr int UP = CP / 8;      // pieces of a Wg or Wu row
   static constexpr int MATRIX = CP * 4;  // pieces of a matrix
-  static constexpr int ROUNDS = (MATRIX + kFfnThreads - 1) / kFfnThreads;
-  static constexpr int LOADS = 3 * ROUNDS;  // of every wave
-  // a matrix in LDS, with what the last round writes past it
-  static constexpr int STRIDE = ROUNDS * kFfnThreads * 16;
-  static constexpr int BYTES = 3 * STRIDE;
+  static constexpr int BYTES = 3 * MATRIX * 16;
 
   __device__ __forceinline__ static const char* up(const char* chunk, int which, int m, int c) {
-    return chunk + which * STRIDE + (m * UP + swizzled<UP>(m, c)) * 16;
+    return chunk + which * (MATRIX * 16) + (m * UP + swizzled<UP>(m, c)) * 16;
   }
   __device__ __forceinline__ static const char* down(const char* chunk, int m, int c) {
-    return chunk + 2 * STRIDE + (m * 4 + swizzled<4>(m, c)) * 16;
+    return chunk + 2 * (MATRIX * 16) + (m * 4 + swizzled<4>(m, c)) * 16;
   }
 
-  // Loads a chunk, every wave with as many loads, also past the last chunk and the matrices (zeros),
-  // so that a wave knows how many are younger than a chunk's.  Whole chunks of whole matrices take
-  // addresses of one part that is the wave's and one that is the lane's for good.
+  // Loads a chunk.  Whole chunks of whole matrices take addresses of one part that is the wave's
+  // and one that is the lane's for good; the others go by piece, with zeros past the ends.
   template <typename T>
   __device__ __forceinline__ static void load(const Weights<T>& w, int f0, char* to) {
+    constexpr int ROUNDS = (MATRIX + kFfnThreads - 1) / kFfnThreads;
     const int tid = int(threadIdx.x);
-    const bool whole = MATRIX % kFfnThreads == 0 && f0 + 32 <= w.Fw && w.C == CP && w.Cow == CP;
+    const bool whole = f0 + 32 <= w.Fw && w.C == CP && w.Cow == CP;
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j) {
       const int i = j * kFfnThreads + tid;
-      const int mu = i / UP, cu = swizzled<UP>(mu, i - mu * UP) * 8, fu = unit_of(mu & 31);
+      if (MATRIX % kFfnThreads != 0 && j * kFfnThreads + wave_of() * 64 >= MATRIX) break;
+      const int mu = i / UP, cu = swizzled<UP>(mu, i - mu * UP) * 8, fu = unit_of(mu);
       const int md = i >> 2, fd = swizzled<4>(md, i & 3) * 8, cd = (md & ~31) + unit_of(md & 31);
       const unsigned ou = unsigned(fu * w.ldu + cu), od = unsigned(cd * w.ldd + fd);
       const T* bg = w.g + int64_t(f0) * w.ldu;
@@ -55,44 +52,39 @@ struct Chunk {
       char* at = to + (j * kFfnThreads + wave_of() * 64) * 16;
       if (whole) {
         copy_piece(bg + ou, at);
-        copy_piece(bu + ou, at + STRIDE);
-        copy_piece(bd + od, at + 2 * STRIDE);
+        copy_piece(bu + ou, at + MATRIX * 16);
+        copy_piece(bd + od, at + 2 * MATRIX * 16);
       } else {
-        const bool in = i < MATRIX && f0 + fu < w.Fw && cu < w.C;
-        const bool ind = i < MATRIX && cd < w.Cow && f0 + fd < w.Fw;
+        const bool in = f0 + fu < w.Fw && cu < w.C, ind = cd < w.Cow && f0 + fd < w.Fw;
         const void* zero = &g_zero_piece;
         copy_piece(in ? static_cast<const void*>(bg + ou) : zero, at);
-        copy_piece(in ? static_cast<const void*>(bu + ou) : zero, at + STRIDE);
-        copy_piece(ind ? static_cast<const void*>(bd + od) : zero, at + 2 * STRIDE);
+        copy_piece(in ? static_cast<const void*>(bu + ou) : zero, at + MATRIX * 16);
+        copy_piece(ind ? static_cast<const void*>(bd + od) : zero, at + 2 * MATRIX * 16);
       }
     }
   }
 };
 
-// The chunks of a call's weights, N of them in LDS: `first` starts N - 1; `next` waits for a chunk, for all
-// waves' loads of it, and starts the one N - 1 further into the buffer that all waves have left; `done` waits for
-// the loads past the end, which may not outlive the workgroup.
-template <typename T, int CP, int N>
+// The chunks of a call's weights, two of them in LDS: `next` waits until a chunk is there, for all waves' loads
+// of it, and starts the following one into the buffer that all waves have left.
+template <typename T, int CP>
 struct Chunks {
   using C = Chunk<CP>;
   const Weights<T>& w;
   char* lds;
-  int f, at;
-  __device__ __forceinline__ Chunks(const Weights<T>& w_, char* lds_) : w(w_), lds(lds_), f(0), at(0) {
-#pragma unroll
-    for (int i = 0; i + 1 < N; ++i) C::load(w, 32 * i, lds + i * C::BYTES);
+  int f = 0, at = 0;
+  __device__ __forceinline__ Chunks(const Weights<T>& w_, char* lds_) : w(w_), lds(lds_) {
+    C::load(w, 0, lds);
   }
   __device__ __forceinline__ const char* next() {
-    loads_in_flight<(N - 2) * C::LOADS>();
+    loads_in_flight<0>();
     __syncthreads();
-    const int into = at == 0 ? N - 1 : at - 1;
-    C::load(w, f + 32 * (N - 1), lds + into * C::BYTES);
-    const char* chunk = lds + at * C::BYTES;
-    at = at + 1 == N ? 0 : at + 1;
     f += 32;
+    const char* chunk = lds + at * C::BYTES;
+    at ^= 1;
+    if (f < w.F) C::load(w, f, lds + at * C::BYTES);
     return chunk;
   }
-  __device__ __forceinline__ void done() { loads_in_flight<0>(); }
 };
 
 // A lane's 8 values of a row; past n zeros.

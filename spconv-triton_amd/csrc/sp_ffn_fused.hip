@@ -1,4 +1,4 @@
-// The gated feed-forward block's forward pass in one kernel, for 16-bit rows of at most 256
+// The gated feed-forward block's forward pass in one kernel, for 16-bit rows of at most 192
 // channels: hidden values exist in registers only.
 //
 // Everything is computed transposed, with the rows of x as the MFMAs' columns:
@@ -56,15 +56,15 @@ __device__ __forceinline__ void fused_store(const FusedArgs<T>& a, int64_t r,
     }
 }
 
-// CP: channels of x and y, rounded up to 32.  N: chunks in LDS.
-template <typename T, int ACT, int CP, int N, int MINW>
+// CP: channels of x and y, rounded up to 32.
+template <typename T, int ACT, int CP, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   using frag = typename Mfma<T>::frag;
-  __shared__ __attribute__((aligned(16))) char lds[N * Chunk<CP>::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds[2 * Chunk<CP>::BYTES];
   const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 31;
   const int half = (int(threadIdx.x) >> 5) & 1;
   const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * kFusedRows + lane;
-  Chunks<T, CP, N> chunks(a.w, lds);
+  Chunks<T, CP> chunks(a.w, lds);
   frag x[CP / 16];
   load_rows<T, CP>(a.x, r, x);
   floatx16 y[CP / 32];
@@ -83,7 +83,6 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
     gate16<true, ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
     down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i & 1], y[i >> 1]); });
   }
-  chunks.done();
   fused_store<T, CP>(a, r, y);
 }
 
@@ -111,22 +110,28 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_pad(const T* __restrict__ s0,
 
 static int up8(int64_t v) { return int(cdiv(v, 8) * 8); }
 
-bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co) {
-  return dtype != SP_F32 && C <= kFusedWidth && Co <= kFusedWidth && rows >= 1;
+// A wave goes through all hidden units one chunk after the other, so a call lasts as long as that at
+// least; the tiled kernels' chains are shorter, but write and read h.  Measured, one kernel against two
+// (us; 128 -> 344 fp16): 1 000 rows 14.9 / 12.3, 8 000 15.5 / 14.7, 16 000 16.1 / 19.3, 32 000 17.6 / 28.8;
+// 64 -> 256 8.7 / 10.6 at 1 000 rows; 192 -> 512 26.8 / 24.6 at 16 000 and 29.7 / 39.5 at 32 000;
+// 256 -> 688 bf16 at 75 000 rows 149 / 138 (a wave a SIMD: its registers hold no more).
+bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t Co) {
+  const int64_t n = C > Co ? C : Co;
+  return dtype != SP_F32 && n <= kFusedWidth && (n <= 64 || rows >= 96 * n);
 }
 
 size_t fused_weights_bytes(int64_t C, int64_t F, int64_t Co) {
   return (2 * size_t(up8(F)) * up8(C) + size_t(up8(Co)) * up8(F)) * 2;
 }
 
-template <typename T, int CP, int N, int MINW>
+template <typename T, int CP, int MINW>
 static int launch_fused(const FusedArgs<T>& a, int act, hipStream_t s) {
   const int64_t tiles = cdiv(a.x.n, kFusedRows);
   SP_CHECK_ARG(tiles <= kMaxGridX, "gated_ffn: too many rows");
   using Kern = void (*)(FusedArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused<T, kActSilu, CP, N, MINW>)
-                    : act == kActGelu ? Kern(ffn_fused<T, kActGelu, CP, N, MINW>)
-                                      : Kern(ffn_fused<T, kActRelu, CP, N, MINW>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused<T, kActSilu, CP, MINW>)
+                    : act == kActGelu ? Kern(ffn_fused<T, kActGelu, CP, MINW>)
+                                      : Kern(ffn_fused<T, kActRelu, CP, MINW>);
   kern<<<unsigned(cdiv(tiles, 4)), kFfnThreads, 0, s>>>(a);
   SP_LAUNCHED();
   return SP_OK;
@@ -168,13 +173,12 @@ static int run_fused(const FfnCall& c) {
   a.vec_y = aligned(c.y) && c.Co % 8 == 0;
   if (int rc = fused_weights(c, static_cast<T*>(c.ws), a.w)) return rc;
   const int widest = c.C > c.Co ? c.C : c.Co;
-  if (widest <= 32) return launch_fused<T, 32, 2, 4>(a, c.act, c.stream);
-  if (widest <= 64) return launch_fused<T, 64, 2, 4>(a, c.act, c.stream);
-  if (widest <= 96) return launch_fused<T, 96, 2, 3>(a, c.act, c.stream);
-  if (widest <= 128) return launch_fused<T, 128, 2, 2>(a, c.act, c.stream);
-  if (widest <= 160) return launch_fused<T, 160, 2, 2>(a, c.act, c.stream);
-  if (widest <= 192) return launch_fused<T, 192, 2, 2>(a, c.act, c.stream);
-  return launch_fused<T, 256, 2, 1>(a, c.act, c.stream);
+  if (widest <= 32) return launch_fused<T, 32, 4>(a, c.act, c.stream);
+  if (widest <= 64) return launch_fused<T, 64, 4>(a, c.act, c.stream);
+  if (widest <= 96) return launch_fused<T, 96, 3>(a, c.act, c.stream);
+  if (widest <= 128) return launch_fused<T, 128, 2>(a, c.act, c.stream);
+  if (widest <= 160) return launch_fused<T, 160, 2>(a, c.act, c.stream);
+  return launch_fused<T, 192, 2>(a, c.act, c.stream);
 }
 
 int fused_forward(int32_t dtype, const FfnCall& a) {

@@ -1,4 +1,4 @@
-// The gated feed-forward block's backward pass for 16-bit rows of up to 128 channels, and of up to 256 the
+// The gated feed-forward block's backward pass for 16-bit rows of up to 128 channels, and of up to 192 the
 // gradient of the hidden rows and of x in one kernel.  Nothing of the hidden width is in memory: both
 // kernels form g, u and dh again from x, dy and the weights.
 //
@@ -94,15 +94,15 @@ __device__ __forceinline__ typename Mfma<T>::frag x_piece(const GradArgs<T>& a, 
                       : row_piece<T>(a.x.p + r * a.x.ld, c, a.x.K, a.x.vec);
 }
 
-template <typename T, int ACT, int CP, int N, bool HIDDEN, int MINW>
+template <typename T, int ACT, int CP, bool HIDDEN, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a) {
   using frag = typename Mfma<T>::frag;
   using C = Chunk<CP>;
-  __shared__ __attribute__((aligned(16))) char lds[N * C::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds[2 * C::BYTES];
   const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 31;
   const int half = (int(threadIdx.x) >> 5) & 1;
   const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * kFusedRows + lane;
-  Chunks<T, CP, N> chunks(a.w, lds);
+  Chunks<T, CP> chunks(a.w, lds);
   frag x[CP / 16], dy[CP / 16];
 #pragma unroll
   for (int k = 0; k < CP / 16; ++k) x[k] = x_piece(a, r, k * 16 + half * 8);
@@ -151,7 +151,6 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a)
       }
     }
   }
-  chunks.done();
   if (!a.dx || r >= a.x.n) return;
 #pragma unroll
   for (int t = 0; t < CP / 32; ++t)
@@ -336,12 +335,12 @@ static int64_t widest(int64_t C, int64_t Co) { return C > Co ? C : Co; }
 // Rows of a tile of the weight gradients' kernel.
 static int tile_rows(int64_t C, int64_t Co) { return widest(C, Co) <= 64 ? 64 : 32; }
 
-bool fused_backward_takes(int32_t dtype, int64_t C, int64_t Co) {
-  return dtype != SP_F32 && widest(C, Co) <= kFusedWidth;
-}
-
-bool fused_weights_take(int32_t dtype, int64_t C, int64_t Co) {
-  return dtype != SP_F32 && widest(C, Co) <= kFusedGramWidth;
+// Measured, these kernels against the tiled ones (us, fp16): 64 -> 256 38 / 31 at 1 000 rows, 42 / 43 at 16 000,
+// 50 / 57 at 32 000; 128 -> 344 54 / 37, 67 / 64, 79 / 88; 192 -> 512 68 / 49, 90 / 87, 112 / 133; 32 -> 128
+// 24 / 27 at 1 000; 256 -> 688 bf16 at 75 000 rows 477 / 449.
+bool fused_backward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t Co) {
+  const int64_t n = widest(C, Co);
+  return dtype != SP_F32 && n <= kFusedWidth && (n <= 32 || rows >= 16384);
 }
 
 // Shares of the rows: one workgroup a CU, each with eight tiles at least.
@@ -350,14 +349,14 @@ int64_t fused_weights_shares(int64_t rows, int64_t C, int64_t F, int64_t Co) {
   return want < most ? want : most;
 }
 
-template <typename T, int CP, int N, bool HIDDEN, int MINW>
+template <typename T, int CP, bool HIDDEN, int MINW>
 static int launch_dx(const GradArgs<T>& a, int act, hipStream_t s) {
   const int64_t blocks = cdiv(a.x.n, 4 * kFusedRows);
   SP_CHECK_ARG(blocks <= kMaxGridX, "gated_ffn_bwd: too many rows");
   using Kern = void (*)(GradArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused_dx<T, kActSilu, CP, N, HIDDEN, MINW>)
-                    : act == kActGelu ? Kern(ffn_fused_dx<T, kActGelu, CP, N, HIDDEN, MINW>)
-                                      : Kern(ffn_fused_dx<T, kActRelu, CP, N, HIDDEN, MINW>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused_dx<T, kActSilu, CP, HIDDEN, MINW>)
+                    : act == kActGelu ? Kern(ffn_fused_dx<T, kActGelu, CP, HIDDEN, MINW>)
+                                      : Kern(ffn_fused_dx<T, kActRelu, CP, HIDDEN, MINW>);
   kern<<<unsigned(blocks), kFfnThreads, 0, s>>>(a);
   SP_LAUNCHED();
   return SP_OK;
@@ -394,14 +393,13 @@ static int run_grad(const FfnCall& c, const FusedGrad& o, int64_t* shares) {
   if (a.dx || a.hid) {
     int rc;
     if (n > kFusedGramWidth)
-      rc = n <= 160   ? launch_dx<T, 160, 2, true, 1>(a, c.act, c.stream)
-           : n <= 192 ? launch_dx<T, 192, 2, true, 1>(a, c.act, c.stream)
-                      : launch_dx<T, 256, 2, true, 1>(a, c.act, c.stream);
+      rc = n <= 160 ? launch_dx<T, 160, true, 1>(a, c.act, c.stream)
+                    : launch_dx<T, 192, true, 1>(a, c.act, c.stream);
     else
-      rc = n <= 32   ? launch_dx<T, 32, 2, false, 4>(a, c.act, c.stream)
-           : n <= 64 ? launch_dx<T, 64, 2, false, 3>(a, c.act, c.stream)
-           : n <= 96 ? launch_dx<T, 96, 2, false, 2>(a, c.act, c.stream)
-                     : launch_dx<T, 128, 2, false, 2>(a, c.act, c.stream);
+      rc = n <= 32   ? launch_dx<T, 32, false, 4>(a, c.act, c.stream)
+           : n <= 64 ? launch_dx<T, 64, false, 3>(a, c.act, c.stream)
+           : n <= 96 ? launch_dx<T, 96, false, 2>(a, c.act, c.stream)
+                     : launch_dx<T, 128, false, 2>(a, c.act, c.stream);
     if (rc) return rc;
   }
   if (!o.part0) return SP_OK;

@@ -114,8 +114,38 @@ def test_gated_ffn_matches_fp64(n, c, f, co, dtype, act):
     _check([y], _reference(*d, dy, act, residual=res)[:1])
 
 
+# rows enough for the one-kernel passes (16-bit, up to 192 channels) and for the larger tiles
+LONG = [(17001, 32, 72, 16, F16, "gelu"), (16500, 64, 96, 64, F16, "silu"),
+        (16384, 20, 53, 61, BF16, "silu"), (20003, 96, 136, 72, BF16, "relu"),
+        (16999, 128, 64, 128, F16, "gelu"), (18000, 100, 36, 99, F16, "silu"),
+        (16390, 160, 40, 152, BF16, "silu"), (21000, 130, 72, 192, F16, "gelu"),
+        (20100, 264, 520, 256, BF16, "silu"), (33000, 200, 136, 320, F16, "gelu"),
+        (20100, 96, 264, 96, F32, "silu"), (65700, 72, 40, 68, F32, "gelu"),
+        (20100, 202, 136, 264, BF16, "silu"), (3, 72, 40, 68, F32, "gelu"),
+        (4, 520, 1100, 99, BF16, "silu"), (5, 520, 1100, 99, F16, "relu")]
+
+
+@pytest.mark.parametrize("n,c,f,co,dtype,act", LONG)
+def test_gated_ffn_of_many_rows_matches_fp64(n, c, f, co, dtype, act):
+    from spconv_triton.pytorch import functional as Fsp
+
+    x, wg, wu, wd, dy, res = _inputs(n, c, f, co, dtype, n + c)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = Fsp.gated_ffn(*leaves, act=act, residual=res)
+    grads = torch.autograd.grad(y, leaves, dy)
+    d = [t.detach() for t in leaves]
+    _check([y.detach(), *grads], _reference(*d, dy, act, residual=res))
+    # (each on its own gives the same)
+    for i in range(4):
+        t = [v.detach().requires_grad_(i == j) for j, v in enumerate(d)]
+        g, = torch.autograd.grad(Fsp.gated_ffn(*t, act=act, residual=res), t[i], dy)
+        assert torch.equal(g, grads[i])
+
+
 @pytest.mark.parametrize("n,c,f,dtype", [(50, 64, 128, F16), (1000, 128, 256, BF16),
-                                         (200, 99, 100, F32), (77, 260, 96, F16)])
+                                         (200, 99, 100, F32), (77, 260, 96, F16),
+                                         (17000, 64, 96, F16), (16400, 99, 72, BF16),
+                                         (16600, 160, 72, F16)])
 def test_gated_ffn_from_8_bits(n, c, f, dtype):
     """The forward pass takes x as it is, the backward one the values of its 8-bit copy, made
     there or by the caller."""
