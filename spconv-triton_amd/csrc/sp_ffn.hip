@@ -333,26 +333,34 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
     }
 }
 
-// dst [cols, ldd] = src [rows, cols] transposed, columns from rows to ldd's share as zeros:
-// dst[c * ldd + r] for r < rows_out.
+// dst [cols][ldd] = src [rows][cols] transposed, zeros from rows to rows_out.
 template <typename T>
-__global__ __launch_bounds__(kFfnThreads) void ffn_transpose(const T* __restrict__ src, int rows,
-                                                             int cols, int rows_out,
-                                                             int cols_out, int64_t ldd,
-                                                             T* __restrict__ dst) {
+struct Transpose {
+  const T* src;
+  T* dst;
+  int rows, cols, rows_out;
+  int64_t ldd;
+};
+
+// Three matrices in one launch (a launch costs the host as much as the transposition takes).
+template <typename T>
+__global__ __launch_bounds__(kFfnThreads) void ffn_transpose(Transpose<T> m0, Transpose<T> m1,
+                                                             Transpose<T> m2) {
   __shared__ T tile[32][33];
+  const Transpose<T> m = blockIdx.z == 0 ? m0 : blockIdx.z == 1 ? m1 : m2;
   const int r0 = int(blockIdx.x) * 32, c0 = int(blockIdx.y) * 32;
+  if (r0 >= m.rows_out || c0 >= m.cols) return;
   const int tx = int(threadIdx.x) & 31, ty = int(threadIdx.x) >> 5;
 #pragma unroll
   for (int j = 0; j < 32; j += 8) {
     const int r = r0 + ty + j, c = c0 + tx;
-    tile[ty + j][tx] = r < rows && c < cols ? src[int64_t(r) * cols + c] : T(0.f);
+    tile[ty + j][tx] = r < m.rows && c < m.cols ? m.src[int64_t(r) * m.cols + c] : T(0.f);
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 32; j += 8) {
     const int c = c0 + ty + j, r = r0 + tx;
-    if (c < cols_out && r < rows_out) dst[int64_t(c) * ldd + r] = tile[tx][ty + j];
+    if (c < m.cols && r < m.rows_out) m.dst[int64_t(c) * m.ldd + r] = tile[tx][ty + j];
   }
 }
 
@@ -814,23 +822,21 @@ static int launch_hidden(const Rows<T>& x, const Rows<T>& wg, const Rows<T>& wu,
   return SP_OK;
 }
 
-template <typename T>
-static int transpose(const void* src, int rows, int cols, int rows_out, int64_t ldd, T* dst,
-                     hipStream_t s) {
-  const dim3 grid(unsigned(cdiv(rows_out, 32)), unsigned(cdiv(cols, 32)));
-  ffn_transpose<T><<<grid, kFfnThreads, 0, s>>>(static_cast<const T*>(src), rows, cols, rows_out,
-                                                cols, ldd, dst);
-  SP_LAUNCHED();
-  return SP_OK;
-}
-
 // dg, du and h of all rows, and dx, by the kernels of their own.
 template <typename T>
 static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
   char* ws = static_cast<char*>(a.ws);
   T* wdt = reinterpret_cast<T*>(ws + l.wdt);
   T* wt = reinterpret_cast<T*>(ws + l.wt);
-  if (int rc = transpose<T>(a.wd, a.Co, a.F, l.Cop, l.Cop, wdt, a.stream)) return rc;
+  const int64_t ld2 = 2 * int64_t(l.Fp);
+  const Transpose<T> d0{static_cast<const T*>(a.wd), wdt, a.Co, a.F, l.Cop, l.Cop};
+  const Transpose<T> d1{static_cast<const T*>(a.wg), wt, a.F, a.C, l.Fp, ld2};
+  const Transpose<T> d2{static_cast<const T*>(a.wu), wt + l.Fp, a.F, a.C, l.Fp, ld2};
+  const int most_rows = l.Cop > l.Fp ? l.Cop : l.Fp, most_cols = a.F > a.C ? a.F : a.C;
+  ffn_transpose<T><<<dim3(unsigned(cdiv(most_rows, 32)), unsigned(cdiv(most_cols, 32)),
+                          a.dx ? 3 : 1),
+                     kFfnThreads, 0, a.stream>>>(d0, d1, d2);
+  SP_LAUNCHED();
   const Rows<T> x = operand<T>(a.x, a.ldx, a.rows, a.C), dy = operand<T>(a.dy, a.lddy, a.rows, a.Co);
   const Rows<T> wg = operand<T>(a.wg, a.C, a.F, a.C), wu = operand<T>(a.wu, a.C, a.F, a.C);
   // (Wd' has zeros past Co)
@@ -844,9 +850,6 @@ static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
     rc = launch_hidden<T, SmallTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
   if (rc) return rc;
   if (!a.dx) return SP_OK;
-  if (int rc = transpose<T>(a.wg, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt, a.stream)) return rc;
-  if (int rc = transpose<T>(a.wu, a.F, a.C, l.Fp, 2 * int64_t(l.Fp), wt + l.Fp, a.stream))
-    return rc;
   return run_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
                         operand<T>(wt, 2 * int64_t(l.Fp), a.C, 2 * int64_t(l.Fp)), nullptr, 0,
                         a.dx, a.C, a.stream);

@@ -125,8 +125,14 @@ def rms_norm_backward(dy, dsum, total, weight=None, eps: float = 1e-6, need_weig
     """(gradient of x and of the residual, gradient of the weight or None).  ``total`` is x
     + residual as the forward pass returned it, ``dsum`` its own gradient or None."""
     check_norm(total, weight, eps, dsum)
-    dtype, device = total.dtype, total.device
     _check_like("rms_norm_backward", "dy", dy, total.shape, total)
+    return run_rms_norm_backward(dy, dsum, total, weight, eps, need_weight)
+
+
+def run_rms_norm_backward(dy, dsum, total, weight, eps, need_weight):
+    """``rms_norm_backward`` of tensors known to fit, as autograd's own do.  (It runs on autograd's
+    thread, where every Python step costs two to three times as much.)"""
+    dtype, device = total.dtype, total.device
     dy, py, lddy = _strided(dy)
     dsum, pd, ldds = _strided(dsum)
     total, pt, lds = _strided(total)
@@ -235,29 +241,40 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, act: str = "silu",
     """Gradients of x, w_gate, w_up and w_down (None where ``need`` is false).  ``x``: the rows,
     or their ``Int8Rows``, whose values then stand for them throughout."""
     check_ffn(x, w_gate, w_up, w_down, act, None)
-    n, c = x.shape
-    dtype, device = x.dtype, x.device
-    hidden, c_out = w_gate.shape[0], w_down.shape[0]
-    _check_like("gated_ffn_backward", "dy", dy, (n, c_out), x)
-    dy, py, lddy = _strided(dy)
-    px = codes = scales = None
-    ldx = 0
+    _check_like("gated_ffn_backward", "dy", dy, (x.shape[0], w_down.shape[0]), x)
     if isinstance(x, Int8Rows):
-        codes, scales = x.codes.data_ptr(), x.scales.data_ptr()
-    else:
+        return run_gated_ffn_backward(dy, None, x.codes, x.scales, w_gate, w_up, w_down, act, need)
+    return run_gated_ffn_backward(dy, x, None, None, w_gate, w_up, w_down, act, need)
+
+
+def run_gated_ffn_backward(dy, x, codes, scales, w_gate, w_up, w_down, act, need):
+    """``gated_ffn_backward`` of tensors known to fit: x, or its codes and scales."""
+    dtype, device = w_gate.dtype, w_gate.device
+    dy, py, lddy = _strided(dy)
+    px = pq = ps = None
+    ldx = 0
+    if codes is None:
+        n, c = x.shape
         x, px, ldx = _strided(x)
+    else:
+        n, c = codes.shape
+        pq, ps = codes.data_ptr(), scales.data_ptr()
+    hidden, c_out = w_gate.shape[0], w_down.shape[0]
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     make = torch.zeros_like if n == 0 else torch.empty_like
     dx = torch.empty((n, c), dtype=dtype, device=device) if need[0] else None
-    grads = [make(w) if k else None for w, k in zip((w_gate, w_up, w_down), need[1:])]
+    dwg = make(w_gate) if need[1] else None
+    dwu = make(w_up) if need[2] else None
+    dwd = make(w_down) if need[3] else None
     if n and any(need):
         L = _lib.lib()
         code = _lib.dtype_code(dtype)
         nbytes = L.sp_gated_ffn_bwd_workspace(code, n, c, hidden, c_out, codes is not None)
         ws = _lib.workspace(nbytes, device)
-        pdx, pdg, pdu, pdd = (None if t is None else t.data_ptr() for t in (dx, *grads))
         _lib.check(L.sp_gated_ffn_bwd(
-            py, lddy, px, ldx, codes, scales, code, n, c, w_gate.data_ptr(), w_up.data_ptr(),
-            hidden, w_down.data_ptr(), c_out, ACTIVATIONS[act], pdx, pdg, pdu, pdd,
+            py, lddy, px, ldx, pq, ps, code, n, c, w_gate.data_ptr(), w_up.data_ptr(),
+            hidden, w_down.data_ptr(), c_out, ACTIVATIONS[act],
+            dx.data_ptr() if need[0] else None, dwg.data_ptr() if need[1] else None,
+            dwu.data_ptr() if need[2] else None, dwd.data_ptr() if need[3] else None,
             ws.data_ptr(), nbytes, _lib.stream_of(device)), "sp_gated_ffn_bwd")
-    return (dx, *grads)
+    return dx, dwg, dwu, dwd

@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from spconv_triton.compat import tv
 from spconv_triton.pytorch import ops
+from spconv_triton.pytorch._impl import rows as _rows
 from spconv_triton.pytorch._impl.rows import Int8Rows
 from spconv_triton.pytorch.hash import HashTable
 from spconv_triton.tools import CUDAKernelTimer
@@ -235,7 +236,7 @@ class RMSNormFunction(Function):
         if dy is None:  # the sum alone was used
             ds, dw = dsum, torch.zeros_like(weight) if need_w else None
         else:
-            ds, dw = ops.rms_norm_backward(dy, dsum, total, weight, ctx.eps, need_w)
+            ds, dw = _rows.run_rms_norm_backward(dy, dsum, total, weight, ctx.eps, need_w)
         return ds if need_x else None, dw, None, ds if need_res else None, None
 
 
@@ -272,26 +273,24 @@ class GatedFFNFunction(Function):
     def forward(ctx, x, w_gate, w_up, w_down, act, residual, saved):
         y = ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
         ctx.act = act
-        ctx.kept_type = None
         if any(ctx.needs_input_grad[:4]):
             if saved == "int8":
                 saved = ops.quantize_rows(x)
             if saved is None:
-                ctx.save_for_backward(w_gate, w_up, w_down, x)
+                ctx.save_for_backward(w_gate, w_up, w_down, x, None, None)
             else:
-                ctx.kept_type = x.dtype
-                ctx.save_for_backward(w_gate, w_up, w_down, saved.codes, saved.scales)
+                ctx.save_for_backward(w_gate, w_up, w_down, None, saved.codes, saved.scales)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        grads = [None] * 4
+        grads = (None,) * 4
         if any(need[:4]):
-            w_gate, w_up, w_down, *x = ctx.saved_tensors
-            x = x[0] if ctx.kept_type is None else Int8Rows(*x, ctx.kept_type)
-            grads = ops.gated_ffn_backward(dy, x, w_gate, w_up, w_down, ctx.act, need[:4])
+            w_gate, w_up, w_down, x, codes, scales = ctx.saved_tensors
+            grads = _rows.run_gated_ffn_backward(dy, x, codes, scales, w_gate, w_up, w_down,
+                                                 ctx.act, need[:4])
         return (*grads, None, dy if need[5] else None, None)
 
 
