@@ -28,7 +28,11 @@ weights, and prints one JSON object per configuration:
   the rulebook cached, strided and transposed with pair generation, in fp16,
   fp32 and TF32-equivalent;
 * ``wgrad``: the weight gradient of each convolution of the ``resunet``
-  network, one call per layer, with its achieved algorithmic GB/s.
+  network, one call per layer, with its achieved algorithmic GB/s;
+* ``blocks``: training step of a stem and two ``SparseFFNBlock`` (SubMConv3d
+  64 -> 64, norm with residual, gated feed-forward 64 -> 256 -> 64), fp16
+  autocast, batch 2 x ~120k voxels in [128, 2048, 2048], the activations of the
+  feed-forward blocks kept as they are and in 8 bits, with the peak memory.
 
 Usage: ``python bench_configs.py [--config NAME ...] [--reps R]``.
 """
@@ -456,9 +460,45 @@ def cfg_wgrad(reps):
             "frac_of_8TBps": round(tot_bytes / tot_ms / 1e6 / 8000.0, 3)}
 
 
+def cfg_blocks(reps):
+    import spconv_triton.pytorch as spconv
+
+    shape = [128, 2048, 2048]
+    idx = urban_cloud(120000, batch=2, seed=9, shape=shape)
+    it = torch.from_numpy(idx).to(DEV)
+    n = idx.shape[0]
+    feats = torch.rand(n, 4, device=DEV)
+    target = torch.rand(n, 64, device=DEV)
+    out = {"voxels": int(n)}
+    for int8 in (False, True):
+        torch.manual_seed(0)
+        net = spconv.SparseSequential(
+            spconv.SubMConv3d(4, 64, 3, padding=1, indice_key="s"),
+            *(spconv.SparseFFNBlock(spconv.SubMConv3d(64, 64, 3, padding=1, indice_key="s"), 64,
+                                    256, int8_activations=int8) for _ in range(2))).to(DEV)
+
+        def step():
+            x = spconv.SparseConvTensor(feats, it, shape, 2)
+            with torch.autocast("cuda", dtype=torch.float16):
+                y = net(x).features
+                loss = torch.nn.functional.mse_loss(y.float(), target)
+            loss.backward()
+            for p in net.parameters():
+                p.grad = None
+
+        for _ in range(3):
+            step()
+        torch.cuda.reset_peak_memory_stats()
+        key = "int8" if int8 else "plain"
+        out[f"{key}_median_ms"] = median_ms(step, reps)
+        out[f"{key}_peak_MiB"] = torch.cuda.max_memory_allocated() / 2 ** 20
+    return {**out, "what": "training step (forward + backward), fp16 autocast, rulebook rebuilt"}
+
+
 CONFIGS = {"encoder": cfg_encoder, "resunet": cfg_resunet, "subm4d": cfg_subm4d,
            "wide": cfg_wide, "config1": cfg_config1, "quickstart": cfg_quickstart,
-           "lidar_c256": cfg_lidar_c256, "ref_c256": cfg_ref_c256, "wgrad": cfg_wgrad}
+           "lidar_c256": cfg_lidar_c256, "ref_c256": cfg_ref_c256, "wgrad": cfg_wgrad,
+           "blocks": cfg_blocks}
 
 
 def main() -> int:

@@ -27,7 +27,9 @@ struct TileShape {
   static constexpr int THREADS = 64 * WX * WW;
   static constexpr int PIECES = (X + W) * kStagePieces, BYTES = PIECES * 16;
 };
+using ThinTile = TileShape<1, 2, 2, 2>;    // 64 x 128, four waves
 using SmallTile = TileShape<2, 2, 2, 2>;   // 128 x 128, four waves
+using QuickTile = TileShape<1, 2, 4, 2>;   // 128 x 128, eight waves, two such workgroups a CU
 using LongTile = TileShape<2, 2, 4, 2>;    // 256 x 128, eight waves
 using LargeTile = TileShape<2, 4, 4, 2>;   // 256 x 256, eight waves
 
@@ -760,7 +762,7 @@ static int run_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, in
     return launch_rows<T, LargeTile, true>(a, w, residual, ldr, out, n, s);
   if (fills<LongTile>(a.n, cdiv(n, LongTile::W)))
     return launch_rows<T, LongTile, true>(a, w, residual, ldr, out, n, s);
-  return launch_rows<T, SmallTile, true>(a, w, residual, ldr, out, n, s);
+  return launch_rows<T, ThinTile, true>(a, w, residual, ldr, out, n, s);
 }
 
 template <typename T>
@@ -774,8 +776,10 @@ static int forward(const FfnCall& a) {
     rc = launch_up<T, SmallTile, false>(x, wg, wu, a.act, h, Fp, a.stream);
   else if (fills<LargeTile>(a.rows, cdiv(Fp, LargeTile::W / 2)))
     rc = launch_up<T, LargeTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
+  else if (fills<QuickTile>(a.rows, cdiv(Fp, QuickTile::W / 2)))
+    rc = launch_up<T, QuickTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
   else
-    rc = launch_up<T, SmallTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
+    rc = launch_up<T, ThinTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
   if (rc) return rc;
   return run_rows<T>(operand<T>(h, Fp, a.rows, a.F), operand<T>(a.wd, a.F, a.Co, a.F), a.residual,
                      a.ldr, a.y, a.Co, a.stream);
@@ -844,10 +848,10 @@ static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
   int rc;
   if (!whole(x) || !whole(wg) || !whole(wu) || !whole(dy))
     rc = launch_hidden<T, SmallTile, false>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
-  else if (fills<LongTile>(a.rows, cdiv(l.Fp, LongTile::W / 2)))
-    rc = launch_hidden<T, LongTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
   else
-    rc = launch_hidden<T, SmallTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
+    // (one workgroup's epilogue, three arrays, beside another's products: 75k x 256 -> 688 backward 428
+    // us, with 256-row tiles, of which a CU holds one, 458)
+    rc = launch_hidden<T, QuickTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
   if (rc) return rc;
   if (!a.dx) return SP_OK;
   return run_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
