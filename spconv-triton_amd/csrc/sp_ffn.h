@@ -19,6 +19,25 @@ __device__ __forceinline__ float sigmoid_fast(float z) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
 
+// gelu(z) = z * cdf(z) by Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erfc(x) =
+// (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0, to 1.5e-7; the exponential is the
+// derivative's too.
+__device__ __forceinline__ void gelu_start(float z, float& t, float& e) {
+  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+  t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+  e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
+}
+__device__ __forceinline__ void gelu_finish(float z, float t, float e, float& value,
+                                            float& slope) {
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f) * t;
+  const float tail = 0.5f * p * e, cdf = z < 0.f ? tail : 1.f - tail;
+  value = z * cdf;
+  slope = __builtin_fmaf(z * 0.39894228040143268f, e, cdf);
+}
+
 // The gate's activation and its derivative, FAST for 16-bit rows.
 template <bool FAST, int ACT>
 __device__ __forceinline__ void gate(float z, float& value, float& slope) {
@@ -27,19 +46,9 @@ __device__ __forceinline__ void gate(float z, float& value, float& slope) {
     value = z * sig;
     slope = __builtin_fmaf(value, 1.f - sig, sig);
   } else if constexpr (ACT == kActGelu && FAST) {
-    // Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erfc(x) =
-    // (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0, to 1.5e-7; the exponential is
-    // the derivative's too.
-    const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
-    const float e = __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f);
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f) * t;
-    const float tail = 0.5f * p * e, cdf = z < 0.f ? tail : 1.f - tail;
-    value = z * cdf;
-    slope = __builtin_fmaf(z * 0.39894228040143268f, e, cdf);
+    float t, e;
+    gelu_start(z, t, e);
+    gelu_finish(z, t, e, value, slope);
   } else if constexpr (ACT == kActGelu) {
     const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
     value = z * cdf;
@@ -66,6 +75,20 @@ __device__ __forceinline__ void gate16(const floatx16& z, F&& f) {
     for (int i = 0; i < 16; ++i) {
       const float value = z[i] * t[i];
       f(i, value, __builtin_fmaf(value, 1.f - t[i], t[i]));
+    }
+  } else if constexpr (ACT == kActGelu && FAST) {
+#pragma unroll
+    for (int b = 0; b < 16; b += 8) {
+      float t[8], e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gelu_start(z[b + i], t[i], e[i]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float value, slope;
+        gelu_finish(z[b + i], t[i], e[i], value, slope);
+        f(b + i, value, slope);
+      }
     }
   } else {
 #pragma unroll
