@@ -151,9 +151,10 @@ __device__ __forceinline__ void loads_in_flight() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// STEPS steps of products whose operands F come from LDS, B steps' reads at a time: a batch is read while the
-// one before is in use.  Left to itself the compiler reads and waits step by step (LDS latency
-// each time; 1.6 times the time of a 256-channel call).  `start` may come early.
+// STEPS steps of products whose operands F come from LDS, B steps' reads at a time: a batch is read while
+// the one before is in use.  Left to itself the compiler reads and waits step by step, for the
+// LDS's latency each time (75k x 256 -> 688 bf16 in one kernel: 193 us, 168 so).  `start` may come
+// early.
 template <typename F, int STEPS, int B>
 struct Batched {
   static constexpr int BATCHES = (STEPS + B - 1) / B;

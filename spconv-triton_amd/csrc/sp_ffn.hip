@@ -16,10 +16,12 @@ namespace sp {
 // ---- products of rows with weight rows -------------------------------------------
 // A workgroup's tile: WX x WW waves, each with XT x WT tiles of 32 rows of x and of 32 weight rows.  The
 // MFMA's rows are the weights' and its columns x's, so that a lane holds one row of x and
-// neighbouring outputs of it.  Every operand byte that the LDS gives serves 32 XT or 32 WT products:
-// with 2 x 2 tiles a wave the reads of four waves alone take the LDS as long as the MFMAs
-// take, and the L2 hands out 2.2 GB for the gate and up products of 50k rows of 512 channels
-// (64 hidden units a workgroup), 1.1 GB with 256 rows and 128 hidden units.
+// neighbouring outputs of it.  With 128 rows and 64 hidden units a workgroup the L2 hands out 2.2
+// GB for the gate and up products of 50k rows of 512 channels and 1 376 hidden units, with 256 and
+// 128 half of that: 307 and 200 us (700 TFLOP/s bf16).  What bounds them then: the eight waves of a CU
+// meet at a barrier each stage, and read its first operands with the matrix cores idle; of the time
+// that a CU is busy these take 47 %, and 50k rows leave the last round of workgroups half empty
+// (1.5 rounds for w_down).  Four stages of half the length, with three in flight: 7 % slower.
 template <int XT_, int WT_, int WX_, int WW_>
 struct TileShape {
   static constexpr int XT = XT_, WT = WT_, WX = WX_, WW = WW_;
@@ -774,7 +776,9 @@ static int forward(const FfnCall& a) {
   int rc;
   if (!whole(x) || !whole(wg) || !whole(wu))
     rc = launch_up<T, SmallTile, false>(x, wg, wu, a.act, h, Fp, a.stream);
-  else if (fills<LargeTile>(a.rows, cdiv(Fp, LargeTile::W / 2)))
+  // (four stages and less: one workgroup's epilogue beside another's products is worth more than fewer
+  // reads; 75k x 256 -> 688 142 us with QuickTile, 151 with LargeTile, 50k x 512 -> 1 376 269 and 257)
+  else if (a.C > 4 * kStagePieces * Mfma<T>::V && fills<LargeTile>(a.rows, cdiv(Fp, LargeTile::W / 2)))
     rc = launch_up<T, LargeTile, true>(x, wg, wu, a.act, h, Fp, a.stream);
   else if (fills<QuickTile>(a.rows, cdiv(Fp, QuickTile::W / 2)))
     rc = launch_up<T, QuickTile, true>(x, wg, wu, a.act, h, Fp, a.stream);

@@ -60,6 +60,7 @@ __device__ __forceinline__ void fused_store(const FusedArgs<T>& a, int64_t r,
 template <typename T, int ACT, int CP, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   using frag = typename Mfma<T>::frag;
+  constexpr int TILES = CP / 32;
   __shared__ __attribute__((aligned(16))) char lds[2 * Chunk<CP>::BYTES];
   const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 31;
   const int half = (int(threadIdx.x) >> 5) & 1;
@@ -73,15 +74,17 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
     const char* chunk = chunks.next();
     floatx16 g, u;
     fused_up<T, CP>(chunk, x, g, u);
-    auto read = [&](int i) {  // Wd's 32 channels i / 2, its 16 hidden units i % 2
+    // Wd's 32 channels i % TILES, its 16 hidden units i / TILES: an MFMA that adds to the result of the one
+    // before it waits for it (84 clocks for 32)
+    auto read = [&](int i) {
       return *reinterpret_cast<const frag*>(
-          Chunk<CP>::down(chunk, (i >> 1) * 32 + lane, 2 * (i & 1) + half));
+          Chunk<CP>::down(chunk, i % TILES * 32 + lane, 2 * (i / TILES) + half));
     };
     Batched<frag, CP / 16, 4> down;
     down.start(read);
     frag h[2];
     gate16<true, ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
-    down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i & 1], y[i >> 1]); });
+    down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i / TILES], y[i % TILES]); });
   }
   fused_store<T, CP>(a, r, y);
 }

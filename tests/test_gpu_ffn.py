@@ -191,11 +191,13 @@ def test_gated_ffn_gradient_against_differences():
             assert abs(num - got) <= 1e-5 * size
 
 
-@pytest.mark.parametrize("dtype,c,shift", [(F16, 64, 8), (BF16, 64, 3), (F32, 40, 1)])
-def test_strided_and_misaligned_rows(dtype, c, shift):
+@pytest.mark.parametrize("n,dtype,c,shift", [(201, F16, 64, 8), (201, BF16, 64, 3), (201, F32, 40, 1),
+                                             (17003, F16, 64, 8), (16400, BF16, 72, 3),
+                                             (2, F16, 40, 5), (300, F16, 264, 8)])
+def test_strided_and_misaligned_rows(n, dtype, c, shift):
     from spconv_triton.pytorch import functional as Fsp
 
-    n, f = 201, 96
+    f = 96
     x, wg, wu, wd, dy, res = _inputs(n, c + 24, f, c + 24, dtype, 9)
     wg, wu, wd = wg[:, :c], wu[:, shift:shift + c], wd[:c]  # weights with strides of their own
     x, dy, res = (t[:, shift:shift + c].detach() for t in (x, dy, res))
@@ -237,7 +239,8 @@ def test_empty_rows():
 def test_not_finite_rows_stay_in_their_rows():
     from spconv_triton.pytorch import functional as Fsp
 
-    for dtype, n, c, f in ((F16, 300, 64, 128), (F32, 200, 99, 100), (BF16, 70, 264, 77)):
+    for dtype, n, c, f in ((F16, 300, 64, 128), (F32, 200, 99, 100), (BF16, 70, 264, 77),
+                           (F16, 17000, 64, 72), (BF16, 16500, 144, 72), (F16, 20100, 264, 136)):
         x, wg, wu, wd, dy, _ = _inputs(n, c, f, c, dtype, 2)
         x[5, 3], x[44, 0], x[66, c - 1] = float("nan"), float("inf"), -float("inf")
         x.requires_grad_(True)
@@ -249,20 +252,23 @@ def test_not_finite_rows_stay_in_their_rows():
         assert torch.isnan(y[5]).all() and not torch.isfinite(y[44]).any()
 
 
-def test_the_same_every_time():
+@pytest.mark.parametrize("n,c,f,dtype", [(20011, 64, 160, F16), (20011, 160, 72, BF16),
+                                         (20011, 264, 136, F16), (5003, 96, 72, F32)])
+def test_the_same_every_time(n, c, f, dtype):
     from spconv_triton.pytorch import ops
 
-    x, wg, wu, wd, dy, _ = _inputs(20011, 64, 160, 64, F16, 4)
+    x, wg, wu, wd, dy, _ = _inputs(n, c, f, c, dtype, 4)
     first = ops.gated_ffn_backward(dy, x, wg, wu, wd)
     for _ in range(3):
         again = ops.gated_ffn_backward(dy, x, wg, wu, wd)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
-def test_on_another_stream_and_in_a_graph():
+@pytest.mark.parametrize("n", [3, 3001, 17001])
+def test_on_another_stream_and_in_a_graph(n):
     from spconv_triton.pytorch import ops
 
-    x, wg, wu, wd, dy, _ = _inputs(3001, 64, 160, 64, BF16, 4)
+    x, wg, wu, wd, dy, _ = _inputs(n, 64, 160, 64, BF16, 4)
 
     def both():
         return [ops.gated_ffn(x, wg, wu, wd), *ops.gated_ffn_backward(dy, x, wg, wu, wd)]
@@ -278,7 +284,7 @@ def test_on_another_stream_and_in_a_graph():
     with torch.cuda.graph(graph):
         got = both()
     for i in range(3):
-        x.copy_(_inputs(3001, 64, 160, 64, BF16, 50 + i)[0])
+        x.copy_(_inputs(n, 64, 160, 64, BF16, 50 + i)[0])
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, both()))
