@@ -8,7 +8,13 @@
 // Both projections share the tiles of x and end in one epilogue, so that g and u
 // never leave the registers.  The backward pass forms g, u and dh again in one
 // kernel whose epilogue writes h, dg and du; nothing of the hidden width is kept
-// between the passes.
+// between the passes.  In 16-bit calls h, dg and du are rounded to the rows' type, for they
+// are operands of the products that follow, as they are where each step is a call of its
+// own; g, u, dh, the gate and every sum stay in fp32.
+//
+// This file has the kernels for rows of any type and width, a tile of the product a workgroup,
+// and the choice between them and the one-kernel passes of narrow 16-bit rows
+// (sp_ffn_fused.hip, sp_ffn_grad.hip).
 #include "sp_ffn.h"
 
 namespace sp {
@@ -16,12 +22,14 @@ namespace sp {
 // ---- products of rows with weight rows -------------------------------------------
 // A workgroup's tile: WX x WW waves, each with XT x WT tiles of 32 rows of x and of 32 weight rows.  The
 // MFMA's rows are the weights' and its columns x's, so that a lane holds one row of x and
-// neighbouring outputs of it.  With 128 rows and 64 hidden units a workgroup the L2 hands out 2.2
-// GB for the gate and up products of 50k rows of 512 channels and 1 376 hidden units, with 256 and
-// 128 half of that: 307 and 200 us (700 TFLOP/s bf16).  What bounds them then: the eight waves of a CU
-// meet at a barrier each stage, and read its first operands with the matrix cores idle; of the time
-// that a CU is busy these take 47 %, and 50k rows leave the last round of workgroups half empty
-// (1.5 rounds for w_down).  Four stages of half the length, with three in flight: 7 % slower.
+// neighbouring outputs of it, which it writes in 16 bytes.  Larger tiles read less: with 128 rows and
+// 64 hidden units a workgroup the L2 hands out 2.2 GB for the gate and up products of 50k rows of 512
+// channels and 1 376 hidden units, with 256 and 128 half of that, 307 and 200 us (700 TFLOP/s bf16,
+// where the library's product of these sizes without the gate reaches 500).  What bounds the large
+// tiles then: the eight waves of a CU meet at a barrier each stage and read its first operands with
+// the matrix cores idle (these work for 47 % of the time that a CU is busy), and 50k rows leave the last
+// round of workgroups half empty (1.5 rounds for w_down).  Four stages of half the length, with
+// three in flight: 7 % slower.
 template <int XT_, int WT_, int WX_, int WW_>
 struct TileShape {
   static constexpr int XT = XT_, WT = WT_, WX = WX_, WW = WW_;
@@ -30,7 +38,7 @@ struct TileShape {
   static constexpr int PIECES = (X + W) * kStagePieces, BYTES = PIECES * 16;
 };
 using ThinTile = TileShape<1, 2, 2, 2>;    // 64 x 128, four waves
-using SmallTile = TileShape<2, 2, 2, 2>;   // 128 x 128, four waves
+using SmallTile = TileShape<2, 2, 2, 2>;   // 128 x 128, four waves, for operands that go through registers
 using QuickTile = TileShape<1, 2, 4, 2>;   // 128 x 128, eight waves, two such workgroups a CU
 using LongTile = TileShape<2, 2, 4, 2>;    // 256 x 128, eight waves
 using LargeTile = TileShape<2, 4, 4, 2>;   // 256 x 256, eight waves
@@ -181,6 +189,15 @@ __device__ __forceinline__ void clear(floatx16 (&acc)[M][N]) {
       for (int k = 0; k < 16; ++k) acc[j][i][k] = 0.f;
 }
 
+// f(register, column) for the lane's outputs of an accumulator of columns from c0 on (write_piece_row's order).
+template <typename T, typename F>
+__device__ __forceinline__ void each_column(int c0, F&& f) {
+  constexpr int V = Mfma<T>::V;
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f(i, c0 + i / V * 2 * V + V * half + i % V);
+}
+
 // The lane's outputs of an accumulator: pieces of V of row r, columns c0 .. c0 + 31, those below n.
 // value(i): of register i, or with a residual what is added to it.
 template <typename T, typename F>
@@ -216,7 +233,8 @@ __device__ __forceinline__ int64_t place_of(int64_t total) {
   return k < total ? k : -1;
 }
 
-// h = act(x Wg') * (x Wu'); columns from F to the padded width are zeros.
+// h = act(x Wg') * (x Wu'), rows of Fp values, of which those from F on stand for nothing: who reads h
+// stops at F.  50k x 512 -> 1 376 bf16 200 us (700 TFLOP/s), 75k x 256 -> 688 107.
 template <typename T, typename S, bool ASYNC>
 __global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, Rows<T> wu, int act,
                                                      T* __restrict__ h, int Fp) {
@@ -252,7 +270,11 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, R
   });
 }
 
-// dg, du and h in rows of 3 Fp values.  wdt: Wd transposed.
+// dg, du and h in rows of 3 Fp values, zeros from F to Fp.  wdt: Wd transposed.  The operands of dh take a
+// second pass over the same stages, so that the three accumulators of a unit meet in one epilogue: 16-bit
+// writes of three arrays (413 MB for 50k rows and 1 376 units: 84 us of 413 at a copy's rate), which
+// only another workgroup on the CU hides.  Those 413 us are 510 TFLOP/s bf16; fp32, 30k rows
+// of 96 -> 256, takes 68 (65 TFLOP/s, the matrix cores give 154).
 template <typename T, typename S, bool ASYNC>
 __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows<T> wg, Rows<T> wu,
                                                               Rows<T> dy, Rows<T> wdt, int act,
@@ -266,6 +288,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
   if (place < 0) return;
   const int64_t x0 = place / cols * S::X;
   const int f0 = int(place % cols) * HIDDEN, xrow = wm * 32 * S::XT;
+  const int F = int(wg.n);
   floatx16 acc[S::XT][S::WT], dh[S::XT][NH];
   clear(acc);
   clear(dh);
@@ -278,6 +301,15 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
   products<T, S, ASYNC, S::WT>(x, x0, wg, &wu, f0, wrow, xrow, lds, acc);
   if (wdt.n > f0 + HIDDEN) wdt.n = f0 + HIDDEN;  // (half of a stage's weight rows)
   products<T, S, ASYNC, NH>(dy, x0, wdt, nullptr, f0, drow, xrow, lds, dh);
+  if (F < Fp && f0 + HIDDEN > F) {  // (else infinities of unit F - 1 would meet the zeros of Wg and Wu)
+#pragma unroll
+    for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+        each_column<T>(f0 + drow[n], [&](int i, int c) {
+          if (c >= F) acc[j][n][i] = acc[j][NH + n][i] = dh[j][n][i] = 0.f;
+        });
+  }
   with_act(act, [&](auto kind) {
 #pragma unroll
     for (int j = 0; j < S::XT; ++j)
@@ -306,7 +338,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
     }
 }
 
-// out = a w' (+ residual, added in fp32).
+// out = a w' (+ residual, added in fp32).  50k x 1 376 -> 512 bf16 150 us (470 TFLOP/s: 1.5 rounds of
+// workgroups), 75k x 688 -> 256 85 (310: one column of tiles, short reductions).
 template <typename T, typename S, bool ASYNC>
 __global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
                                                        const T* __restrict__ residual,
@@ -458,7 +491,10 @@ struct GramStage {
   }
 };
 
-// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile.
+// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile.  The partials of a share of the rows are
+// fp32 and joined in a fixed order, so that two calls give the same gradients.  50k rows, 512 channels,
+// 1 376 units bf16: 317 us, 667 TFLOP/s, bound as the products above, and by the transposed
+// reads, two for each operand; 75k rows, 256, 688: 130. fp32, 30k rows, 96, 256: 66 (67 TFLOP/s).
 template <typename T, int TP, int TQ>
 __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
                                                       int64_t share, int shares) {
@@ -528,7 +564,8 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
 
 // The three weight gradients from their partials: dWg and dWu [F][C] from rows 0 and Fp on of the
 // first product, dWd [Co][F] from the second, [F][Co].  64 values a workgroup, four runs of the shares
-// summed apart and then in order.
+// summed apart and then in order.  Bound by the partials' reads, which come from the L2s and the cache behind
+// them: 75k x 256 -> 688, 16 shares of 2.1 MB, 16.5 us.
 template <typename T>
 __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part0,
                                                           const float* __restrict__ part1,
@@ -858,9 +895,8 @@ static int hidden_and_dx(const FfnCall& a, const FfnLayout& l, T* hid) {
     rc = launch_hidden<T, QuickTile, true>(x, wg, wu, dy, d, a.act, hid, l.Fp, a.stream);
   if (rc) return rc;
   if (!a.dx) return SP_OK;
-  return run_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, 2 * int64_t(l.Fp)),
-                        operand<T>(wt, 2 * int64_t(l.Fp), a.C, 2 * int64_t(l.Fp)), nullptr, 0,
-                        a.dx, a.C, a.stream);
+  return run_rows<T>(operand<T>(hid, 3 * int64_t(l.Fp), a.rows, ld2),
+                     operand<T>(wt, ld2, a.C, ld2), nullptr, 0, a.dx, a.C, a.stream);
 }
 
 // The weight gradients' partials from the hidden rows.

@@ -252,6 +252,23 @@ def test_not_finite_rows_stay_in_their_rows():
         assert torch.isnan(y[5]).all() and not torch.isfinite(y[44]).any()
 
 
+@pytest.mark.parametrize("n,c", [(100, 64), (100, 60), (17000, 64), (17000, 160)])
+def test_an_infinity_of_the_last_unit_stays_one(n, c):
+    from spconv_triton.pytorch import ops
+
+    # 172 hidden units are no whole pieces of eight; the last unit's gradient passes 65504
+    f = 172
+    x = torch.ones(n, c, dtype=F16, device=DEV)
+    wg = torch.full((f, c), 0.5, dtype=F16, device=DEV)
+    wd = torch.zeros(c, f, dtype=F16, device=DEV)
+    wd[:, f - 1] = 100
+    dy = torch.full((n, c), 100., dtype=F16, device=DEV)
+    dx, dwg, dwu, dwd = ops.gated_ffn_backward(dy, x, wg, wg, wd, "silu")
+    assert torch.isposinf(dx).all()
+    assert torch.isposinf(dwg[f - 1]).all() and torch.isposinf(dwu[f - 1]).all()
+    assert (dwg[:f - 1] == 0).all() and (dwu[:f - 1] == 0).all()
+
+
 @pytest.mark.parametrize("n,c,f,dtype", [(20011, 64, 160, F16), (20011, 160, 72, BF16),
                                          (20011, 264, 136, F16), (5003, 96, 72, F32)])
 def test_the_same_every_time(n, c, f, dtype):
