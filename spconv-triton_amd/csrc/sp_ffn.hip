@@ -227,8 +227,8 @@ __device__ __forceinline__ void write_piece_row(T* out, int64_t ld, int64_t r, i
 
 // The place of this workgroup among `total`: consecutive workgroups go to the eight XCDs in turn; here each XCD
 // gets an eighth of the places in a row, so that tiles which share rows meet in one L2.
-__device__ __forceinline__ int64_t place_of(int64_t total) {
-  const int64_t per = (total + 7) >> 3, id = blockIdx.x;
+__device__ __forceinline__ int64_t place_of(int64_t total, int64_t id = blockIdx.x) {
+  const int64_t per = (total + 7) >> 3;
   const int64_t k = (id >> 3) < per ? (id & 7) * per + (id >> 3) : total;
   return k < total ? k : -1;
 }
@@ -338,21 +338,22 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
     }
 }
 
-// out = a w' (+ residual, added in fp32).  50k x 1 376 -> 512 bf16 150 us (470 TFLOP/s: 1.5 rounds of
-// workgroups), 75k x 688 -> 256 85 (310: one column of tiles, short reductions).
+// out = a w' (+ residual, added in fp32).  50k x 1 376 -> 512 bf16 109 us and x 2 752 -> 512 190 (645 and 740
+// TFLOP/s; 392 tiles are 1.5 rounds of workgroups); fp32 30k x 256 -> 96 25 us and x 512 -> 96 44 (67,
+// the rate of one wave's products in turn with its loads).
+template <typename T>
+struct RowsOut {
+  const T* residual;
+  int64_t ldr;
+  T* out;
+  int n, vec;
+};
+
 template <typename T, typename S, bool ASYNC>
-__global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
-                                                       const T* __restrict__ residual,
-                                                       int64_t ldr, T* __restrict__ out, int n,
-                                                       int vec) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
+__device__ __forceinline__ void rows_tile(const Rows<T>& a, const Rows<T>& w, const RowsOut<T>& o,
+                                          int64_t x0, int n0, char* lds) {
   const int wave = int(threadIdx.x) >> 6, wm = wave / S::WW, wn = wave % S::WW;
-  const int lane = int(threadIdx.x) & 31;
-  const int cols = (n + S::W - 1) / S::W;
-  const int64_t place = place_of((a.n + S::X - 1) / S::X * cols);
-  if (place < 0) return;
-  const int64_t x0 = place / cols * S::X;
-  const int n0 = int(place % cols) * S::W, xrow = wm * 32 * S::XT;
+  const int lane = int(threadIdx.x) & 31, xrow = wm * 32 * S::XT;
   floatx16 acc[S::XT][S::WT];
   clear(acc);
   int wrow[S::WT];
@@ -364,10 +365,44 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w,
 #pragma unroll
     for (int i = 0; i < S::WT; ++i) {
       const int64_t r = x0 + xrow + 32 * j + lane;
-      write_piece_row<T>(out, n, r, a.n, n0 + wrow[i], n, vec, [&](int k, int c) {
-        return residual && c < n ? acc[j][i][k] + to_f32(residual[r * ldr + c]) : acc[j][i][k];
+      write_piece_row<T>(o.out, o.n, r, a.n, n0 + wrow[i], o.n, o.vec, [&](int k, int c) {
+        return o.residual && c < o.n ? acc[j][i][k] + to_f32(o.residual[r * o.ldr + c])
+                                     : acc[j][i][k];
       });
     }
+}
+
+template <typename T, typename S, bool ASYNC>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_rows(Rows<T> a, Rows<T> w, RowsOut<T> o) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::BYTES];
+  const int cols = (o.n + S::W - 1) / S::W;
+  const int64_t place = place_of((a.n + S::X - 1) / S::X * cols);
+  if (place < 0) return;
+  rows_tile<T, S, ASYNC>(a, w, o, place / cols * S::X, int(place % cols) * S::W, lds);
+}
+
+// The same with `whole` large tiles (a multiple of 256: full rounds of the CUs) and each of the others as
+// four of a quarter its size.
+template <typename T>
+__global__ __launch_bounds__(LargeTile::THREADS, 2) void ffn_rows_split(Rows<T> a, Rows<T> w,
+                                                                        RowsOut<T> o, int whole) {
+  static_assert(QuickTile::THREADS == LargeTile::THREADS && 2 * QuickTile::X == LargeTile::X &&
+                    2 * QuickTile::W == LargeTile::W, "quarters");
+  __shared__ __attribute__((aligned(16))) char lds[2 * LargeTile::BYTES];
+  const int cols = (o.n + LargeTile::W - 1) / LargeTile::W;
+  const int64_t tiles = (a.n + LargeTile::X - 1) / LargeTile::X * cols;
+  if (int(blockIdx.x) < whole) {
+    const int64_t place = place_of(whole);
+    rows_tile<T, LargeTile, true>(a, w, o, place / cols * LargeTile::X,
+                                  int(place % cols) * LargeTile::W, lds);
+    return;
+  }
+  const int64_t place = place_of(4 * (tiles - whole), int64_t(blockIdx.x) - whole);
+  if (place < 0) return;
+  const int64_t tile = whole + place / 4;
+  const int64_t x0 = tile / cols * LargeTile::X + (place >> 1 & 1) * QuickTile::X;
+  const int n0 = int(tile % cols) * LargeTile::W + int(place & 1) * QuickTile::W;
+  if (x0 < a.n && n0 < o.n) rows_tile<T, QuickTile, true>(a, w, o, x0, n0, lds);
 }
 
 // dst [cols][ldd] = src [rows][cols] transposed, zeros from rows to rows_out.
@@ -782,13 +817,10 @@ static int launch_up(const Rows<T>& x, const Rows<T>& wg, const Rows<T>& wu, int
 }
 
 template <typename T, typename S, bool ASYNC>
-static int launch_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, int64_t ldr,
-                       void* out, int n, hipStream_t s) {
-  const int64_t groups = tile_groups<S>(a.n, cdiv(n, S::W));
+static int launch_rows(const Rows<T>& a, const Rows<T>& w, const RowsOut<T>& o, hipStream_t s) {
+  const int64_t groups = tile_groups<S>(a.n, cdiv(o.n, S::W));
   SP_CHECK_ARG(groups <= kMaxGridX, "gated_ffn: too many rows");
-  ffn_rows<T, S, ASYNC><<<unsigned(groups), S::THREADS, 0, s>>>(
-      a, w, static_cast<const T*>(residual), ldr, static_cast<T*>(out), n,
-      aligned(out) && n % Mfma<T>::V == 0);
+  ffn_rows<T, S, ASYNC><<<unsigned(groups), S::THREADS, 0, s>>>(a, w, o);
   SP_LAUNCHED();
   return SP_OK;
 }
@@ -796,12 +828,23 @@ static int launch_rows(const Rows<T>& a, const Rows<T>& w, const void* residual,
 template <typename T>
 static int run_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, int64_t ldr,
                     void* out, int n, hipStream_t s) {
-  if (!whole(a) || !whole(w)) return launch_rows<T, SmallTile, false>(a, w, residual, ldr, out, n, s);
-  if (n > 128 && fills<LargeTile>(a.n, cdiv(n, LargeTile::W)))
-    return launch_rows<T, LargeTile, true>(a, w, residual, ldr, out, n, s);
-  if (fills<LongTile>(a.n, cdiv(n, LongTile::W)))
-    return launch_rows<T, LongTile, true>(a, w, residual, ldr, out, n, s);
-  return launch_rows<T, ThinTile, true>(a, w, residual, ldr, out, n, s);
+  const RowsOut<T> o{static_cast<const T*>(residual), ldr, static_cast<T*>(out), n,
+                     aligned(out) && n % Mfma<T>::V == 0};
+  if (!whole(a) || !whole(w)) return launch_rows<T, SmallTile, false>(a, w, o, s);
+  const int64_t tiles = cdiv(a.n, LargeTile::X) * cdiv(n, LargeTile::W), last = tiles % 256;
+  if (n > 128 && tiles >= 256) {
+    // (a last round of up to 64 tiles is one of up to 256 quarters: forward and backward pass 119 and 396 us
+    // for 107 and 377 at 70k x 256 -> 688, last 18; 203 and 684 for 187 and 663 at 40k x 512 -> 1 376, last 58;
+    // 140 and 478 for 137 and 479 with 96 left, 242 and 818 for 259 and 843 with 136)
+    if (last == 0 || last > 64) return launch_rows<T, LargeTile, true>(a, w, o, s);
+    const int64_t groups = tiles - last + cdiv(4 * last, 8) * 8;
+    SP_CHECK_ARG(groups <= kMaxGridX, "gated_ffn: too many rows");
+    ffn_rows_split<T><<<unsigned(groups), LargeTile::THREADS, 0, s>>>(a, w, o, int(tiles - last));
+    SP_LAUNCHED();
+    return SP_OK;
+  }
+  if (fills<LongTile>(a.n, cdiv(n, LongTile::W))) return launch_rows<T, LongTile, true>(a, w, o, s);
+  return launch_rows<T, ThinTile, true>(a, w, o, s);
 }
 
 template <typename T>
