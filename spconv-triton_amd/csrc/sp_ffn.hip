@@ -40,6 +40,7 @@ struct TileShape {
 using ThinTile = TileShape<1, 2, 2, 2>;    // 64 x 128, four waves
 using SmallTile = TileShape<2, 2, 2, 2>;   // 128 x 128, four waves, for operands that go through registers
 using QuickTile = TileShape<1, 2, 4, 2>;   // 128 x 128, eight waves, two such workgroups a CU
+using NarrowTile = TileShape<1, 3, 4, 1>;  // 128 x 96, four waves
 using LongTile = TileShape<2, 2, 4, 2>;    // 256 x 128, eight waves
 using LargeTile = TileShape<2, 4, 4, 2>;   // 256 x 256, eight waves
 
@@ -72,7 +73,7 @@ struct Stage {
                                    const Rows<T>* w2, int64_t w0)
       : in(0u), k(first_k()), K(x.K) {
     static_assert(S::THREADS % 256 == 0 && S::X * 8 % S::THREADS == 0 &&
-                      S::W * 4 % S::THREADS == 0, "whole rounds of an operand");
+                      S::W * 8 % S::THREADS == 0, "whole rounds of an operand");
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int row = (j * S::THREADS + int(threadIdx.x)) >> 3;
@@ -339,8 +340,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
 }
 
 // out = a w' (+ residual, added in fp32).  50k x 1 376 -> 512 bf16 109 us and x 2 752 -> 512 190 (645 and 740
-// TFLOP/s; 392 tiles are 1.5 rounds of workgroups); fp32 30k x 256 -> 96 25 us and x 512 -> 96 44 (67,
-// the rate of one wave's products in turn with its loads).
+// TFLOP/s; 392 tiles are 1.5 rounds of workgroups); fp32 30k x 256 -> 96 21 us and x 512 -> 96 35 (71 and
+// 83, of 154: one tile a CU, whose waves take loads and products in turn).
 template <typename T>
 struct RowsOut {
   const T* residual;
@@ -469,7 +470,7 @@ struct GramStage {
   frag r[N];
 
   __device__ __forceinline__ static int slot(int row, int piece) {
-    if constexpr (sizeof(T) == 4) return piece;
+    if constexpr (sizeof(T) == 4 || COLS == 96) return piece;  // (rows of 192 bytes fall apart by themselves)
     if constexpr (COLS % 128 == 0) return piece ^ ((row & 3) << 2);
     return piece ^ ((row & 3) << 1);
   }
@@ -526,14 +527,16 @@ struct GramStage {
   }
 };
 
-// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile.  The partials of a share of the rows are
+// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile, or where TQ is 96 of 32 x 96.  The partials of a share of the rows are
 // fp32 and joined in a fixed order, so that two calls give the same gradients.  50k rows, 512 channels,
 // 1 376 units bf16: 317 us, 667 TFLOP/s, bound as the products above, and by the transposed
-// reads, two for each operand; 75k rows, 256, 688: 130. fp32, 30k rows, 96, 256: 66 (67 TFLOP/s).
+// reads, two for each operand; 75k rows, 256, 688: 130.  fp32, 30k rows, 96, 256: 57 (78 TFLOP/s; 66 us
+// with 128 columns, a quarter of them empty).
 template <typename T, int TP, int TQ>
 __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
                                                       int64_t share, int shares) {
-  constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>(), NQ = TQ / 64;
+  constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>();
+  constexpr int NP = TQ == 96 ? 1 : 2, NQ = TQ == 96 ? 3 : TQ / 64;
   constexpr int STAGE = kGramStage * (TP + TQ);
   using SA = GramStage<T, TP, THREADS>;
   using SB = GramStage<T, TQ, THREADS>;
@@ -548,8 +551,9 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
   const Gram<T> g = second ? g1 : g0;
   const int p0 = tile / g.tiles_q * TP, q0 = tile % g.tiles_q * TQ;
   const int64_t hi = lo + share < rows ? lo + share : rows;
-  const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 64, wq = (wave & 1) * (TQ / 2);
-  floatx16 acc[2][NQ];
+  const int wave = int(threadIdx.x) >> 6, wp = TQ == 96 ? wave * 32 : (wave >> 1) * 64;
+  const int wq = TQ == 96 ? 0 : (wave & 1) * (TQ / 2);
+  floatx16 acc[NP][NQ];
   clear(acc);
   SA sa;
   SB sb;
@@ -567,18 +571,18 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) fetch(m + ROWS);
     auto read = [&](int k) {
-      Operands<T, 2, NQ> f;
+      Operands<T, NP, NQ> f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) f.x[i] = SA::read(la, k * 2 * Mfma<T>::V, wp + 32 * i);
+      for (int i = 0; i < NP; ++i) f.x[i] = SA::read(la, k * 2 * Mfma<T>::V, wp + 32 * i);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) f.w[i] = SB::read(lb, k * 2 * Mfma<T>::V, wq + 32 * i);
       return f;
     };
-    Batched<Operands<T, 2, NQ>, ROWS / (2 * Mfma<T>::V), 1> steps;
+    Batched<Operands<T, NP, NQ>, ROWS / (2 * Mfma<T>::V), 1> steps;
     steps.start(read);
-    steps.run(read, [&](int, const Operands<T, 2, NQ>& f) {
+    steps.run(read, [&](int, const Operands<T, NP, NQ>& f) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < NP; ++i)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) Mfma<T>::mma(f.x[i], f.w[j], acc[i][j]);
     });
@@ -586,7 +590,7 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
   float* part = g.part + lo / share * g.P * g.Q;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NP; ++i)
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -600,7 +604,7 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
 // The three weight gradients from their partials: dWg and dWu [F][C] from rows 0 and Fp on of the
 // first product, dWd [Co][F] from the second, [F][Co].  64 values a workgroup, four runs of the shares
 // summed apart and then in order.  Bound by the partials' reads, which come from the L2s and the cache behind
-// them: 75k x 256 -> 688, 16 shares of 2.1 MB, 16.5 us.
+// them: 75k x 256 -> 688, 28 shares of 2.1 MB, 16.5 us (3.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part0,
                                                           const float* __restrict__ part1,
@@ -727,7 +731,7 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_few_down(const float* __restr
 }
 
 // ---- host ------------------------------------------------------------------------
-// Tiles of the weight gradients: 128 x 64 where both widths fit in 64 columns, 128 x 128, and for wider
+// Tiles of the weight gradients: 128 x 64, 96 or 128, the fewest columns that both widths fit in, and for wider
 // rows 256 x 256, with which the L2 hands out half as much (50k rows of 512 channels, 1 376
 // hidden units: 1.7 GB for 3.3).
 struct GramShape {
@@ -736,6 +740,7 @@ struct GramShape {
 static GramShape gram_shape(int64_t C, int64_t Co) {
   const int64_t n = C > Co ? C : Co;
   if (n <= 64) return {128, 64};
+  if (n <= 96) return {128, 96};
   if (n <= 128) return {128, 128};
   return {256, 256};
 }
@@ -843,6 +848,10 @@ static int run_rows(const Rows<T>& a, const Rows<T>& w, const void* residual, in
     SP_LAUNCHED();
     return SP_OK;
   }
+  // (the wider of the low tiles once the others would give a CU two: 30k rows fp32, 256 -> 96 24.6 us for 20.7,
+  // 512 -> 96 43.6 for 35.4; 10k rows 15 for 20)
+  if (n > 64 && n <= 96 && cdiv(a.n, ThinTile::X) > 256)
+    return launch_rows<T, NarrowTile, true>(a, w, o, s);
   if (fills<LongTile>(a.n, cdiv(n, LongTile::W))) return launch_rows<T, LongTile, true>(a, w, o, s);
   return launch_rows<T, ThinTile, true>(a, w, o, s);
 }
@@ -962,6 +971,8 @@ static int weight_products(const FfnCall& a, const FfnLayout& l, const T* hid, f
     ffn_gram<T, 256, 256><<<groups, 512, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   else if (t.q == 64)
     ffn_gram<T, 128, 64><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
+  else if (t.q == 96)
+    ffn_gram<T, 128, 96><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   else
     ffn_gram<T, 128, 128><<<groups, 256, 0, a.stream>>>(g0, g1, a.rows, share, int(*shares));
   SP_LAUNCHED();

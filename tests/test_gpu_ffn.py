@@ -123,6 +123,7 @@ LONG = [(17001, 32, 72, 16, F16, "gelu"), (16500, 64, 96, 64, F16, "silu"),
         (20100, 96, 264, 96, F32, "silu"), (65700, 72, 40, 68, F32, "gelu"),
         (20100, 202, 136, 264, BF16, "silu"), (3, 72, 40, 68, F32, "gelu"),
         (65700, 200, 40, 136, BF16, "relu"), (65600, 132, 24, 200, F32, "silu"),
+        (65700, 104, 20, 40, F32, "gelu"),
         (4, 520, 1100, 99, BF16, "silu"), (5, 520, 1100, 99, F16, "relu")]
 
 
