@@ -527,11 +527,11 @@ struct GramStage {
   }
 };
 
-// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile, or where TQ is 96 of 32 x 96.  The partials of a share of the rows are
-// fp32 and joined in a fixed order, so that two calls give the same gradients.  50k rows, 512 channels,
-// 1 376 units bf16: 317 us, 667 TFLOP/s, bound as the products above, and by the transposed
-// reads, two for each operand; 75k rows, 256, 688: 130.  fp32, 30k rows, 96, 256: 57 (78 TFLOP/s; 66 us
-// with 128 columns, a quarter of them empty).
+// Waves of TP / 64 x 2, each with 64 x TQ / 2 of the tile, or where TQ is 96 of 32 x 96.  The partials of
+// a share of the rows are fp32 and joined in a fixed order, so that two calls give the same gradients.
+// 50k rows, 512 channels, 1 376 units bf16: 317 us, 667 TFLOP/s, bound as the products above, and by the
+// transposed reads, two for each operand; 75k rows, 256, 688: 130.  fp32, 30k rows, 96, 256: 57 (78
+// TFLOP/s; 66 us with 128 columns, a quarter of them empty).
 template <typename T, int TP, int TQ>
 __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, int64_t rows,
                                                       int64_t share, int shares) {

@@ -12,6 +12,9 @@
 //
 // The weights pass through LDS in chunks of 32 hidden units, loaded by direct loads to LDS while the
 // chunk before is in use, and are read by all four waves.
+//
+// h is rounded to the rows' type on its way into the last products, as a stored h would be; the sums
+// of y are fp32 and the residual is added to them before their one rounding.
 #include "sp_ffn_fused.h"
 
 namespace sp {
@@ -56,7 +59,11 @@ __device__ __forceinline__ void fused_store(const FusedArgs<T>& a, int64_t r,
     }
 }
 
-// CP: channels of x and y, rounded up to 32.
+// CP: channels of x and y, rounded up to 32.  200k x 64 -> 256 fp16 31-36 us (51 MB of rows would take 10,
+// the products 14 at the rate of large ones; the two kernels that store h took 137 in their first form).
+// A wave's gate, 16 exponentials and reciprocals for each 32 x 32 block, is as long as the block's
+// MFMAs; other waves' MFMAs run beside it, four waves a SIMD.  About 15 us are the first rows' loads
+// and the last ones' writes, with no products beside them: all workgroups are resident at once.
 template <typename T, int ACT, int CP, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   using frag = typename Mfma<T>::frag;
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   fused_store<T, CP>(a, r, y);
 }
 
-// dst [rows_out][ldd] = src [rows][cols] with zeros around, both wg and wu or wd alone.
+// dst = Wg and Wu as [Fp][Cp] and Wd as [Cop][Fp], with zeros past F, C and Co.
 template <typename T>
 __global__ __launch_bounds__(kFfnThreads) void ffn_pad(const T* __restrict__ s0,
                                                        const T* __restrict__ s1,

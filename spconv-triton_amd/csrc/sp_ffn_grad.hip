@@ -94,6 +94,9 @@ __device__ __forceinline__ typename Mfma<T>::frag x_piece(const GradArgs<T>& a, 
                       : row_piece<T>(a.x.p + r * a.x.ld, c, a.x.K, a.x.vec);
 }
 
+// dg and du are rounded to the rows' type as operands of the last products.  240k x 64 -> 256 fp16 64 us: five
+// products, 39 GFLOP, 615 TFLOP/s; bound as the forward pass, by the gate's instructions beside the
+// MFMAs.  HIDDEN: writes dg, du and h as well, for rows whose weight gradients do not fit in registers.
 template <typename T, int ACT, int CP, bool HIDDEN, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a) {
   using frag = typename Mfma<T>::frag;
@@ -205,12 +208,15 @@ struct RowTile {
   }
 };
 
-// A workgroup: 128 hidden units (four waves of 32) and a share of the rows, HALVES * U tiles of 32 rows
-// between barriers, U of them for each four waves.
-template <typename T, int ACT, int CP, int HALVES, int U>
+// A workgroup: 128 hidden units (four waves of 32) and a share of the rows, HALVES tiles of 32 rows
+// between barriers, one for each four waves.  240k x 64 -> 256 fp16 87 us: six products, 47 GFLOP, 543
+// TFLOP/s.  Weights and gradients fill the registers of two waves a SIMD, so that little runs beside a
+// wave's gate and its waits at the barrier; one wave a SIMD with two tiles was slower.  Storing the
+// hidden rows and multiplying them instead moves 1.5 KB a row.
+template <typename T, int ACT, int CP, int HALVES>
 __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradArgs<T> a) {
   using frag = typename Mfma<T>::frag;
-  constexpr int THREADS = kFfnThreads * HALVES, ROWS = kFusedRows * HALVES * U, UP = CP / 8;
+  constexpr int THREADS = kFfnThreads * HALVES, ROWS = kFusedRows * HALVES, UP = CP / 8;
   constexpr int K = CP / 16, TILES = CP / 32;
   using Tile = RowTile<T, CP, THREADS, ROWS>;
   constexpr int JOIN = HALVES > 1 ? 4 * TILES * 4096 : 0;  // a matrix of four waves
@@ -245,49 +251,43 @@ __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradAr
     tile.store(at);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) tile.load(a, m + ROWS, hi);
-    const char* xs = at + (wave >> 2) * (U * kFusedRows * UP * 16);
+    const char* xs = at + (wave >> 2) * (kFusedRows * UP * 16);
     const char* ds = xs + Tile::BYTES;
-    floatx16 g[U], u[U], dh[U];
+    floatx16 g, u, dh;
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
+    for (int i = 0; i < 16; ++i) g[i] = u[i] = dh[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) g[n][i] = u[n][i] = dh[n][i] = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const int piece = (lane * UP + swizzled<UP>(lane, 2 * k + half)) * 16;
+      const frag fx = *reinterpret_cast<const frag*>(xs + piece);
+      const frag fd = *reinterpret_cast<const frag*>(ds + piece);
+      Mfma<T>::mma(fx, wg[k], g);
+      Mfma<T>::mma(fx, wu[k], u);
+      Mfma<T>::mma(fd, wd[k], dh);
+    }
+    // register 8 s + j of lane half b holds row 16 s + 8 (j >> 2) + 4 b + (j & 3) of the tile
+    frag dg[2], du[2], h[2];
+    gate16<true, ACT>(g, [&](int i, float value, float slope) {
+      dg[i >> 3][i & 7] = T(dh[i] * u[i] * slope);
+      du[i >> 3][i & 7] = T(dh[i] * value);
+      h[i >> 3][i & 7] = T(value * u[i]);
+    });
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int piece = ((n * kFusedRows + lane) * UP + swizzled<UP>(lane, 2 * k + half)) * 16;
-        const frag fx = *reinterpret_cast<const frag*>(xs + piece);
-        const frag fd = *reinterpret_cast<const frag*>(ds + piece);
-        Mfma<T>::mma(fx, wg[k], g[n]);
-        Mfma<T>::mma(fx, wu[k], u[n]);
-        Mfma<T>::mma(fd, wd[k], dh[n]);
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        // columns 32 t .. of those rows
+        const int l = int(threadIdx.x) & 15;
+        const int col = 4 * t + 2 * ((int(threadIdx.x) >> 4) & 1) + ((l >> 1) & 1);
+        const int row = 16 * s + 4 * half + (l >> 2);
+        const int p0 = (row * UP + swizzled<UP>(row, col)) * 16 + (l & 1) * 8;
+        const int p1 = ((row + 8) * UP + swizzled<UP>(row + 8, col)) * 16 + (l & 1) * 8;
+        const frag fx = read_transposed<T>(xs + p0, xs + p1);
+        const frag fd = read_transposed<T>(ds + p0, ds + p1);
+        Mfma<T>::mma(dg[s], fx, dwg[t]);
+        Mfma<T>::mma(du[s], fx, dwu[t]);
+        Mfma<T>::mma(h[s], fd, dwd[t]);
       }
-    }
-#pragma unroll
-    for (int n = 0; n < U; ++n) {
-      // register 8 s + j of lane half b holds row 16 s + 8 (j >> 2) + 4 b + (j & 3) of the tile
-      frag dg[2], du[2], h[2];
-      gate16<true, ACT>(g[n], [&](int i, float value, float slope) {
-        dg[i >> 3][i & 7] = T(dh[n][i] * u[n][i] * slope);
-        du[i >> 3][i & 7] = T(dh[n][i] * value);
-        h[i >> 3][i & 7] = T(value * u[n][i]);
-      });
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          // columns 32 t .. of those rows
-          const int l = int(threadIdx.x) & 15;
-          const int col = 4 * t + 2 * ((int(threadIdx.x) >> 4) & 1) + ((l >> 1) & 1);
-          const int row = n * kFusedRows + 16 * s + 4 * half + (l >> 2);
-          const int p0 = (row * UP + swizzled<UP>(row, col)) * 16 + (l & 1) * 8;
-          const int p1 = ((row + 8) * UP + swizzled<UP>(row + 8, col)) * 16 + (l & 1) * 8;
-          const frag fx = read_transposed<T>(xs + p0, xs + p1);
-          const frag fd = read_transposed<T>(ds + p0, ds + p1);
-          Mfma<T>::mma(dg[s], fx, dwg[t]);
-          Mfma<T>::mma(du[s], fx, dwu[t]);
-          Mfma<T>::mma(h[s], fd, dwd[t]);
-        }
-    }
   }
   // the second four waves' sums through LDS to the first's
   auto join = [&](floatx16(&d)[TILES]) {
@@ -362,12 +362,12 @@ static int launch_dx(const GradArgs<T>& a, int act, hipStream_t s) {
   return SP_OK;
 }
 
-template <typename T, int CP, int HALVES, int U>
+template <typename T, int CP, int HALVES>
 static int launch_weights(const GradArgs<T>& a, int act, hipStream_t s) {
   using Kern = void (*)(GradArgs<T>);
-  const Kern kern = act == kActSilu   ? Kern(ffn_fused_weights<T, kActSilu, CP, HALVES, U>)
-                    : act == kActGelu ? Kern(ffn_fused_weights<T, kActGelu, CP, HALVES, U>)
-                                      : Kern(ffn_fused_weights<T, kActRelu, CP, HALVES, U>);
+  const Kern kern = act == kActSilu   ? Kern(ffn_fused_weights<T, kActSilu, CP, HALVES>)
+                    : act == kActGelu ? Kern(ffn_fused_weights<T, kActGelu, CP, HALVES>)
+                                      : Kern(ffn_fused_weights<T, kActRelu, CP, HALVES>);
   const dim3 grid(unsigned(cdiv(a.w.F, 128)), unsigned(cdiv(a.x.n, a.share)));
   kern<<<grid, kFfnThreads * HALVES, 0, s>>>(a);
   SP_LAUNCHED();
@@ -406,10 +406,10 @@ static int run_grad(const FfnCall& c, const FusedGrad& o, int64_t* shares) {
   const int tile = tile_rows(c.C, c.Co);
   a.share = cdiv(cdiv(c.rows, o.shares), tile) * tile;
   *shares = cdiv(c.rows, a.share);
-  return n <= 32   ? launch_weights<T, 32, 2, 1>(a, c.act, c.stream)
-         : n <= 64 ? launch_weights<T, 64, 2, 1>(a, c.act, c.stream)
-         : n <= 96 ? launch_weights<T, 96, 1, 1>(a, c.act, c.stream)
-                   : launch_weights<T, 128, 1, 1>(a, c.act, c.stream);
+  return n <= 32   ? launch_weights<T, 32, 2>(a, c.act, c.stream)
+         : n <= 64 ? launch_weights<T, 64, 2>(a, c.act, c.stream)
+         : n <= 96 ? launch_weights<T, 96, 1>(a, c.act, c.stream)
+                   : launch_weights<T, 128, 1>(a, c.act, c.stream);
 }
 
 int fused_backward(int32_t dtype, const FfnCall& a, const FusedGrad& o, int64_t* shares) {
