@@ -602,18 +602,20 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
 }
 
 // The three weight gradients from their partials: dWg and dWu [F][C] from rows 0 and Fp on of the
-// first product, dWd [Co][F] from the second, [F][Co].  64 values a workgroup, four runs of the shares
-// summed apart and then in order.  Bound by the partials' reads, which come from the L2s and the cache behind
-// them: 75k x 256 -> 688, 28 shares of 2.1 MB, 16.5 us (3.6 TB/s).
-template <typename T>
+// first product, dWd [Co][F] from the second, [F][Co].  64 V values a workgroup, four runs of the shares
+// summed apart and then in order.  Bound by the partials' reads, which come from the cache behind the L2s: 59 MB
+// each for 75k x 256 -> 688 (28 shares) 13.3 us, value by value 16.5, and for 50k x 512 -> 1 376 (7 shares) 15.5
+// and 24.5; 240k x 64 -> 256 (125 shares, 25 MB) 7.2 and 6.5.
+template <typename T, int V>
 __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restrict__ part0,
                                                           const float* __restrict__ part1,
                                                           int shares, int C, int F, int Fp, int Co,
                                                           T* __restrict__ dwg, T* __restrict__ dwu,
                                                           T* __restrict__ dwd) {
-  __shared__ float lds[4][64];
+  typedef float vec __attribute__((ext_vector_type(V)));
+  __shared__ vec lds[4][64];
   const int lane = int(threadIdx.x) & 63, run = int(threadIdx.x) >> 6;
-  const int64_t i = int64_t(blockIdx.x) * 64 + lane;
+  const int64_t i = (int64_t(blockIdx.x) * 64 + lane) * V;
   const int64_t n0 = int64_t(F) * C, n1 = int64_t(F) * Co;
   const int which = int(blockIdx.y);
   T* dst = which == 0 ? dwg : which == 1 ? dwu : dwd;
@@ -621,18 +623,20 @@ __global__ __launch_bounds__(kFfnThreads) void ffn_reduce(const float* __restric
   const bool in = i < (which == 2 ? n1 : n0);
   const float* p = which == 2 ? part1 + i : part0 + (which ? int64_t(Fp) * C : 0) + i;
   const int64_t stride = which == 2 ? n1 : 2 * int64_t(Fp) * C;
-  float v = 0.f;
+  vec v = vec(0.f);
   if (in) {
     const int per = (shares + 3) / 4, end = (run + 1) * per < shares ? (run + 1) * per : shares;
 #pragma unroll 8
-    for (int s = run * per; s < end; ++s) v += p[int64_t(s) * stride];
+    for (int s = run * per; s < end; ++s) v += *reinterpret_cast<const vec*>(p + int64_t(s) * stride);
   }
   lds[run][lane] = v;
   __syncthreads();
   if (run != 0 || !in) return;
   v = ((lds[0][lane] + lds[1][lane]) + lds[2][lane]) + lds[3][lane];
-  const int64_t f = i / Co;
-  dst[which == 2 ? (i - f * Co) * F + f : i] = from_f32<T>(v);
+  const int64_t f = i / Co;  // (a piece lies in one row of Wd')
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    dst[which == 2 ? (i + k - f * Co) * F + f : i + k] = from_f32<T>(v[k]);
 }
 
 // ---- a few rows ------------------------------------------------------------------
@@ -1013,9 +1017,17 @@ static int backward(int32_t dtype, FfnCall a, const FfnLayout& l) {
   if (!l.fused_weights)
     if (int rc = weight_products<T>(a, l, hid, part0, part1, &shares)) return rc;
   const int64_t most = int64_t(a.F) * (a.C > a.Co ? a.C : a.Co);
-  ffn_reduce<T><<<dim3(unsigned(cdiv(most, 64)), 3), kFfnThreads, 0, a.stream>>>(
-      part0, part1, int(shares), a.C, a.F, l.Fp, a.Co, static_cast<T*>(a.dwg),
-      static_cast<T*>(a.dwu), static_cast<T*>(a.dwd));
+  // (four values a lane where that still gives every CU a workgroup for each gradient)
+  const bool vec = a.C % 4 == 0 && a.Co % 4 == 0 && most >= 65536;
+  auto reduce = [&](auto kernel, int V) {
+    kernel<<<dim3(unsigned(cdiv(most, 64 * V)), 3), kFfnThreads, 0, a.stream>>>(
+        part0, part1, int(shares), a.C, a.F, l.Fp, a.Co, static_cast<T*>(a.dwg),
+        static_cast<T*>(a.dwu), static_cast<T*>(a.dwd));
+  };
+  if (vec)
+    reduce(ffn_reduce<T, 4>, 4);
+  else
+    reduce(ffn_reduce<T, 1>, 1);
   SP_LAUNCHED();
   return SP_OK;
 }
