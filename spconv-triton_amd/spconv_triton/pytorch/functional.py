@@ -214,6 +214,17 @@ indice_maxpool_implicit_gemm = SparseMaxPoolImplicitGemmFunction.apply
 indice_avgpool_implicit_gemm = SparseAvgPoolImplicitGemmFunction.apply
 
 
+def _inference() -> bool:
+    """No gradient, transform or autocast concerns a call made now: it needs no autograd node,
+    which costs the host as much as the kernel's launch."""
+    if torch.compiler.is_compiling():  # (first: Dynamo cannot trace the questions below)
+        return False
+    return not (torch.is_grad_enabled() or torch.is_autocast_enabled("cuda")
+                or torch._C._functorch.peek_interpreter_stack() is not None
+                or torch.autograd.forward_ad._current_level >= 0)
+
+
+
 # ---------------------------------------------------------------------------
 # the channel half of a block: norm, gated feed-forward, rows in 8 bits
 # ---------------------------------------------------------------------------
@@ -248,7 +259,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     Returns ``y``; with ``residual`` also ``s``; with ``int8`` also y's :class:`Int8Rows` (which
     carries no gradient).  ``weight`` has the rows' type or float32; statistics are float32.
     """
-    y, total, kept = RMSNormFunction.apply(x, weight, eps, residual, int8)
+    run = ops.rms_norm if _inference() else RMSNormFunction.apply
+    y, total, kept = run(x, weight, eps, residual, int8)
     out = (y,) if residual is None else (y, total)
     if int8:
         out += (kept,)
@@ -311,6 +323,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
                              f"x {tuple(x.shape)} on {x.device}")
     elif saved not in (None, "int8"):
         raise ValueError(f"gated_ffn: saved is None, 'int8' or Int8Rows, got {saved!r}")
+    if _inference():
+        return ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
     return GatedFFNFunction.apply(x, w_gate, w_up, w_down, act, residual, saved)
 
 
