@@ -456,7 +456,7 @@ int sp_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, i
 /* Gradients of sp_rms_norm from those of y (dy) and of s (dsum, nullable), with s as stored:
  * ds [rows, C] (of x and of the residual alike) and dweight [C] of type
  * param_dtype (nullable; its sums over rows have a fixed order).  The workspace, 16-byte
- * aligned, is read only with dweight. */
+ * aligned, is read only with dweight and where the query is not 0 (a few rows need none). */
 size_t sp_rms_norm_bwd_workspace(int64_t rows, int64_t C);
 int sp_rms_norm_bwd(const void* dy, int64_t lddy, const void* dsum, int64_t ldds, const void* s,
                     int64_t lds, int32_t dtype, int64_t rows, int64_t C, const void* weight,

@@ -263,7 +263,7 @@ template <typename T, typename P, int V, int PIECES, int ROWS>
 __global__ __launch_bounds__(kRowThreads) void rms_rows_bwd(
     const T* __restrict__ dy, int64_t lddy, const T* __restrict__ dsum, int64_t ldds,
     const T* __restrict__ s, int64_t lds_, const void* __restrict__ w, float eps, int64_t rows,
-    int C, int log_lanes, T* __restrict__ ds, float* __restrict__ part) {
+    int C, int log_lanes, T* __restrict__ ds, float* __restrict__ part, P* __restrict__ dw) {
   using vec = Piece<T, V>;
   constexpr int NW = kRowThreads / 64;
   __shared__ float lds[NW][64 * V * PIECES];
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kRowThreads) void rms_rows_bwd(
       }
     }
   }
-  if (!part) return;
+  if (!part && !dw) return;
   const int wave = int(threadIdx.x) >> 6;
 #pragma unroll
   for (int p = 0; p < PIECES; ++p)
@@ -340,7 +340,10 @@ __global__ __launch_bounds__(kRowThreads) void rms_rows_bwd(
     float v = lds[0][c];
 #pragma unroll
     for (int q = 1; q < NW; ++q) v += lds[q][c];
-    part[int64_t(blockIdx.x) * C + c] = v;
+    if (dw)  // (the only workgroup)
+      dw[c] = P(v);
+    else
+      part[int64_t(blockIdx.x) * C + c] = v;
   }
 }
 
@@ -519,16 +522,22 @@ static int reduce_dw(const float* part, int64_t n, const NormGrad& a) {
   return SP_OK;
 }
 
+// A few rows (64 of 64 channels, two turns of a workgroup) go to one workgroup, which needs no partials: the
+// other launch and the workspace cost the host 4 us of the call's 13.
+static bool one_workgroup(int64_t rows, int64_t C) { return C <= 256 && rows * C <= 4096; }
+
 template <typename T, typename P, int V, int PIECES>
 static int launch_bwd(const NormGrad& a, int log_lanes) {
   constexpr int ROWS = PIECES == 1 ? 2 : 1;
   int64_t blocks = cdiv(a.rows, int64_t(kRowThreads >> log_lanes) * ROWS);
   if (blocks > kRowPartials) blocks = kRowPartials;
-  float* part = a.dw ? static_cast<float*>(a.ws) : nullptr;
+  const bool alone = a.dw && one_workgroup(a.rows, a.C);
+  if (alone) blocks = 1;
+  float* part = a.dw && !alone ? static_cast<float*>(a.ws) : nullptr;
   rms_rows_bwd<T, P, V, PIECES, ROWS><<<unsigned(blocks), kRowThreads, 0, a.stream>>>(
       static_cast<const T*>(a.dy), a.lddy, static_cast<const T*>(a.dsum), a.ldds,
       static_cast<const T*>(a.s), a.lds, a.w, a.eps, a.rows, a.C, log_lanes,
-      static_cast<T*>(a.ds), part);
+      static_cast<T*>(a.ds), part, alone ? static_cast<P*>(a.dw) : nullptr);
   SP_LAUNCHED();
   return part ? reduce_dw<P>(part, blocks, a) : SP_OK;
 }
@@ -628,7 +637,7 @@ extern "C" int sp_rms_norm(const void* x, int64_t ldx, const void* residual, int
 }
 
 extern "C" size_t sp_rms_norm_bwd_workspace(int64_t rows, int64_t C) {
-  if (rows <= 0 || C <= 0) return 0;
+  if (rows <= 0 || C <= 0 || one_workgroup(rows, C)) return 0;
   const size_t fast = size_t(rows < kRowPartials ? rows : kRowPartials) * size_t(C);
   const size_t wide = size_t(wide_shares(rows)) * size_t(C) + size_t(rows);
   return (fast > wide ? fast : wide) * sizeof(float);
@@ -646,7 +655,7 @@ extern "C" int sp_rms_norm_bwd(const void* dy, int64_t lddy, const void* dsum, i
   if (rows == 0) return SP_OK;
   SP_CHECK_ARG(dy && s && ds, "rms_norm_bwd: null pointer");
   SP_CHECK_ARG(lddy >= C && lds >= C && (!dsum || ldds >= C), "rms_norm_bwd: rows overlap");
-  if (dweight) {
+  if (dweight && !one_workgroup(rows, C)) {
     SP_CHECK_ARG(ws && aligned16(ws), "rms_norm_bwd: the workspace must be 16-byte aligned");
     if (ws_bytes < sp_rms_norm_bwd_workspace(rows, C))
       return set_error(SP_ERR_WORKSPACE, "rms_norm_bwd: workspace of %zu bytes, needs %zu",

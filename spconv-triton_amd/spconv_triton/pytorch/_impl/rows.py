@@ -150,8 +150,10 @@ def run_rms_norm_backward(dy, dsum, total, weight, eps, need_weight):
                 return ds, torch.zeros_like(weight)
             dw = torch.empty_like(weight)
             nbytes = L.sp_rms_norm_bwd_workspace(n, c)
-            ws = _lib.workspace(nbytes, device)
-            pdw, pws = dw.data_ptr(), ws.data_ptr()
+            pdw = dw.data_ptr()
+            if nbytes:
+                ws = _lib.workspace(nbytes, device)
+                pws = ws.data_ptr()
     _lib.check(L.sp_rms_norm_bwd(py, lddy, pd, ldds, pt, lds, code, n, c, pw, pcode, eps,
                                  ds.data_ptr(), pdw, pws, nbytes, _lib.stream_of(device)),
                "sp_rms_norm_bwd")
