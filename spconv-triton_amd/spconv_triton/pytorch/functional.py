@@ -279,10 +279,21 @@ def restore_rows(rows: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tens
     return ops.restore_rows(rows, dtype)
 
 
+def _as_autocast_takes(*tensors):
+    """Floating tensors in the type of the autocast region around the call, as ``nn.Linear``'s are.
+    (The convolutions take fp16 under any autocast, as the reference's do; rows in bf16 would
+    lose their range by that.)"""
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    dtype = torch.get_autocast_dtype("cuda")
+    return tuple(t.to(dtype) if t is not None and t.is_cuda and t.is_floating_point()
+                 and t.dtype is not torch.float64 else t for t in tensors)
+
+
 class GatedFFNFunction(Function):
     @staticmethod
-    @_FWD
     def forward(ctx, x, w_gate, w_up, w_down, act, residual, saved):
+        x, w_gate, w_up, w_down, residual = _as_autocast_takes(x, w_gate, w_up, w_down, residual)
         y = ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
         ctx.act = act
         if any(ctx.needs_input_grad[:4]):
@@ -316,6 +327,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     copy made here (``saved="int8"``), or as a copy that the caller has (``saved`` an
     :class:`Int8Rows`, as ``rms_norm`` returns).  With a copy the gradients are those at the
     values that it stands for.
+
+    Under autocast x, the weights and the residual are taken, and y returned, in autocast's type.
     """
     if isinstance(saved, Int8Rows):
         if saved.shape != x.shape or saved.device != x.device:
