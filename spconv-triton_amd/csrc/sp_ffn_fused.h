@@ -110,6 +110,16 @@ __device__ __forceinline__ void load_rows(const Rows<T>& x, int64_t r,
   }
 }
 
+// Operands of 32 hidden units from f0 on, with zeros from F on: the weights there are zeros, but an
+// infinity of x or dy makes their values NaN, which would meet other zeros in the next product.
+template <typename Frag>
+__device__ __forceinline__ void end_units(Frag (&h)[2], int f0, int F) {
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (f0 + 16 * (i >> 3) + 8 * half + (i & 7) >= F) h[i >> 3][i & 7] = 0;
+}
+
 template <typename T>
 struct FragPair {
   typename Mfma<T>::frag a, b;

@@ -91,6 +91,7 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
     down.start(read);
     frag h[2];
     gate16<true, ACT>(g, [&](int i, float value, float) { h[i >> 3][i & 7] = T(value * u[i]); });
+    if (f0 + 32 > a.w.F) end_units(h, f0, a.w.F);
     down.run(read, [&](int i, const frag& f) { Mfma<T>::mma(f, h[i / TILES], y[i % TILES]); });
   }
   fused_store<T, CP>(a, r, y);

@@ -137,6 +137,10 @@ __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused_dx(GradArgs<T> a)
       du[i >> 3][i & 7] = T(dh[i] * value);
       if (HIDDEN) h[i >> 3][i & 7] = T(value * u[i]);
     });
+    if (f0 + 32 > a.w.F) {  // (h's are not read)
+      end_units(dg, f0, a.w.F);
+      end_units(du, f0, a.w.F);
+    }
     wgu.run(up, [&](int i, const FragPair<T>& f) {
       Mfma<T>::mma(f.a, dg[i & 1], dx[i >> 1]);
       Mfma<T>::mma(f.b, du[i & 1], dx[i >> 1]);
