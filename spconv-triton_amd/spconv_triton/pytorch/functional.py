@@ -214,14 +214,20 @@ indice_maxpool_implicit_gemm = SparseMaxPoolImplicitGemmFunction.apply
 indice_avgpool_implicit_gemm = SparseAvgPoolImplicitGemmFunction.apply
 
 
+def _recorded() -> bool:
+    """A trace records this call: outside a Function it would record the results' allocation
+    alone, for a kernel fills them behind PyTorch's back."""
+    return not torch.compiler.is_compiling() and torch.jit.is_tracing()
+
+
 def _inference() -> bool:
-    """No gradient, transform or autocast concerns a call made now: it needs no autograd node,
-    which costs the host as much as the kernel's launch."""
+    """No gradient, transform, trace or autocast concerns a call made now: it needs no autograd
+    node, which costs the host as much as the kernel's launch."""
     if torch.compiler.is_compiling():  # (first: Dynamo cannot trace the questions below)
         return False
     return not (torch.is_grad_enabled() or torch.is_autocast_enabled("cuda")
                 or torch._C._functorch.peek_interpreter_stack() is not None
-                or torch.autograd.forward_ad._current_level >= 0)
+                or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing())
 
 
 
@@ -229,7 +235,8 @@ def _inference() -> bool:
 # the channel half of a block: norm, gated feed-forward, rows in 8 bits
 # ---------------------------------------------------------------------------
 
-# (the backward passes below run no operation that autocast looks at, and go without custom_bwd)
+# (the backward passes below run no operation that autocast looks at, and go without custom_bwd;
+# 8-bit rows go in and out as the tensors they are made of, which a trace can follow)
 class RMSNormFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, eps, residual, int8):
@@ -237,11 +244,14 @@ class RMSNormFunction(Function):
         ctx.save_for_backward(x if residual is None else total, weight)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
-        return y, total, kept
+        if not int8:
+            return y, total, None, None
+        ctx.mark_non_differentiable(kept.codes, kept.scales)
+        return y, total, kept.codes, kept.scales
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dsum, _):
+    def backward(ctx, dy, dsum, *_):
         total, weight = ctx.saved_tensors
         need_x, need_w, _, need_res, _ = ctx.needs_input_grad
         if dy is None:  # the sum alone was used
@@ -259,23 +269,51 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     Returns ``y``; with ``residual`` also ``s``; with ``int8`` also y's :class:`Int8Rows` (which
     carries no gradient).  ``weight`` has the rows' type or float32; statistics are float32.
     """
-    run = ops.rms_norm if _inference() else RMSNormFunction.apply
-    y, total, kept = run(x, weight, eps, residual, int8)
+    if _inference():
+        y, total, kept = ops.rms_norm(x, weight, eps, residual, int8)
+    else:
+        y, total, codes, scales = RMSNormFunction.apply(x, weight, eps, residual, int8)
+        kept = Int8Rows(codes, scales, y.dtype) if int8 else None
     out = (y,) if residual is None else (y, total)
     if int8:
         out += (kept,)
     return out[0] if len(out) == 1 else out
 
 
+class QuantizeRowsFunction(Function):
+    """``quantize_rows`` of a trace."""
+
+    @staticmethod
+    def forward(ctx, x):
+        kept = ops.quantize_rows(x)
+        ctx.mark_non_differentiable(kept.codes, kept.scales)
+        return kept.codes, kept.scales
+
+
+class RestoreRowsFunction(Function):
+    """``restore_rows`` of a trace."""
+
+    @staticmethod
+    def forward(ctx, codes, scales, dtype, to):
+        out = ops.restore_rows(Int8Rows(codes, scales, dtype), to)
+        ctx.mark_non_differentiable(out)
+        return out
+
+
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """Feature rows in 8 bits, one scale for each row and 128 channels: ``scale = max|x| / 127``,
     ``code = rint(x * (127 / max|x|))``.  A group with an infinity or a NaN is NaN when restored.
     No gradient passes."""
+    if _recorded():
+        codes, scales = QuantizeRowsFunction.apply(x.detach())
+        return Int8Rows(codes, scales, x.dtype)
     return ops.quantize_rows(x.detach())
 
 
 def restore_rows(rows: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values that 8-bit rows stand for, in ``dtype`` (default: the type they came from)."""
+    if isinstance(rows, Int8Rows) and _recorded():
+        return RestoreRowsFunction.apply(rows.codes, rows.scales, rows.dtype, dtype)
     return ops.restore_rows(rows, dtype)
 
 
@@ -292,17 +330,15 @@ def _as_autocast_takes(*tensors):
 
 class GatedFFNFunction(Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, act, residual, saved):
+    def forward(ctx, x, w_gate, w_up, w_down, act, residual, int8, codes, scales):
         x, w_gate, w_up, w_down, residual = _as_autocast_takes(x, w_gate, w_up, w_down, residual)
         y = ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
         ctx.act = act
         if any(ctx.needs_input_grad[:4]):
-            if saved == "int8":
-                saved = ops.quantize_rows(x)
-            if saved is None:
-                ctx.save_for_backward(w_gate, w_up, w_down, x, None, None)
-            else:
-                ctx.save_for_backward(w_gate, w_up, w_down, None, saved.codes, saved.scales)
+            if int8 and codes is None:
+                kept = ops.quantize_rows(x)
+                codes, scales = kept.codes, kept.scales
+            ctx.save_for_backward(w_gate, w_up, w_down, None if int8 else x, codes, scales)
         return y
 
     @staticmethod
@@ -314,7 +350,7 @@ class GatedFFNFunction(Function):
             w_gate, w_up, w_down, x, codes, scales = ctx.saved_tensors
             grads = _rows.run_gated_ffn_backward(dy, x, codes, scales, w_gate, w_up, w_down,
                                                  ctx.act, need[:4])
-        return (*grads, None, dy if need[5] else None, None)
+        return (*grads, None, dy if need[5] else None, None, None, None)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -330,7 +366,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     Under autocast x, the weights and the residual are taken, and y returned, in autocast's type.
     """
+    codes = scales = None
     if isinstance(saved, Int8Rows):
+        codes, scales = saved.codes, saved.scales
         if saved.shape != x.shape or saved.device != x.device:
             raise ValueError(f"gated_ffn: saved has shape {tuple(saved.shape)} on {saved.device}, "
                              f"x {tuple(x.shape)} on {x.device}")
@@ -338,7 +376,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         raise ValueError(f"gated_ffn: saved is None, 'int8' or Int8Rows, got {saved!r}")
     if _inference():
         return ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
-    return GatedFFNFunction.apply(x, w_gate, w_up, w_down, act, residual, saved)
+    return GatedFFNFunction.apply(x, w_gate, w_up, w_down, act, residual, saved is not None, codes,
+                                  scales)
 
 
 _MAX_INT32 = 2 ** 31 - 1
