@@ -201,7 +201,7 @@ def restore_rows(kept: Int8Rows, dtype: torch.dtype | None = None) -> torch.Tens
 # ---------------------------------------------------------------------------
 
 def check_ffn(x, w_gate, w_up, w_down, act, residual) -> None:
-    if isinstance(x, Int8Rows):
+    if isinstance(x, Int8Rows):  # (the backward pass's)
         _lib.require_gpu(x.codes)
     else:
         _check_rows("gated_ffn", "x", x)
@@ -219,6 +219,9 @@ def check_ffn(x, w_gate, w_up, w_down, act, residual) -> None:
 
 def gated_ffn(x, w_gate, w_up, w_down, act: str = "silu", residual=None) -> torch.Tensor:
     """(act(x w_gate') * (x w_up')) w_down' (+ residual)."""
+    if isinstance(x, Int8Rows):
+        raise ValueError("gated_ffn: x is Int8Rows; only the backward pass takes rows in 8 bits "
+                         "(restore_rows gives their values)")
     check_ffn(x, w_gate, w_up, w_down, act, residual)
     dtype, device = x.dtype, x.device
     x, px, ldx = _strided(x)

@@ -96,3 +96,23 @@ def test_modules_build_and_reload():
     assert spconv.RMSNorm(16, affine=False).weight is None
     block.load_state_dict(block.state_dict())
     assert "gelu" in repr(block)
+
+
+def test_rows_in_8_bits_are_refused_as_input(monkeypatch):
+    """By the forward pass, in every way to call it; before a library or a GPU is asked for."""
+    import spconv_triton.pytorch as spconv
+    from spconv_triton.pytorch import functional as Fsp
+    from spconv_triton.pytorch import ops
+    from spconv_triton.pytorch._impl import _lib
+
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+    kept = ops.Int8Rows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4, 1), torch.float32)
+    w, wd = torch.zeros(12, 8), torch.zeros(8, 12)
+    block = spconv.GatedFFN(8, 12)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            for call in (lambda: ops.gated_ffn(kept, w, w, wd), lambda: block(kept),
+                         lambda: Fsp.gated_ffn(kept, w, w, wd),
+                         lambda: Fsp.gated_ffn(kept, w, w, wd, saved=kept)):
+                with pytest.raises(ValueError, match="8 bits"):
+                    call()
