@@ -276,6 +276,14 @@ __global__ __launch_bounds__(kFfnThreads * HALVES) void ffn_fused_weights(GradAr
       du[i >> 3][i & 7] = T(dh[i] * value);
       h[i >> 3][i & 7] = T(value * u[i]);
     });
+    if (m + ROWS > hi) {
+      // rows past the end are zeros, of which an infinity in a weight makes NaN
+      const int left = int(hi - m) - (wave >> 2) * kFusedRows;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + 8 * ((i >> 2) & 1) + 4 * half + (i & 3) >= left)
+          dg[i >> 3][i & 7] = du[i >> 3][i & 7] = h[i >> 3][i & 7] = 0;
+    }
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll

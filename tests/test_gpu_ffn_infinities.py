@@ -53,3 +53,28 @@ def test_an_infinity_in_the_gradient(n, c, f, dtype):
     hit = torch.zeros(c, dtype=torch.bool, device=DEV)
     hit[2] = True
     assert torch.isposinf(dwd[hit]).all() and torch.isfinite(dwd[~hit]).all()
+
+
+@pytest.mark.parametrize("f", [8, 53, 64])
+@pytest.mark.parametrize("n,c", [(3, 64), (300, 20), (17001, 20), (17001, 64), (17001, 99), (17001, 128),
+                                 (16385, 160), (300, 264)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_an_infinity_in_a_weight(n, c, f, dtype):
+    """Rows that only fill up a kernel's last tile make no NaN of it."""
+    from spconv_triton.pytorch import ops
+
+    x, w, wd, dy = _positive(n, c, f, dtype)
+    wg, other = w.clone(), torch.ones(f, dtype=torch.bool, device=DEV)
+    wg[3, 2], other[3] = float("inf"), False
+    # g and h of unit 3 are infinite; dh, and dg at relu's slope 1, are finite
+    _, dwg, dwu, dwd = ops.gated_ffn_backward(dy, x, wg, w, wd, "relu")
+    assert torch.isfinite(dwg).all()
+    assert torch.isposinf(dwu[3]).all() and torch.isfinite(dwu[other]).all()
+    assert torch.isposinf(dwd[:, 3]).all() and torch.isfinite(dwd[:, other]).all()
+    down = wd.clone()
+    down[2, 3] = float("inf")
+    # dh of unit 3 is infinite
+    _, dwg, dwu, dwd = ops.gated_ffn_backward(dy, x, w, w, down, "relu")
+    for g in (dwg, dwu):
+        assert torch.isposinf(g[3]).all() and torch.isfinite(g[other]).all()
+    assert torch.isfinite(dwd).all()
