@@ -23,6 +23,8 @@ constexpr int kRowGroup = 128;   // channels that share a scale
 constexpr int kRowPieces = 4;    // pieces of a lane at most: wider rows take the looping kernels
 constexpr int kRowPartials = 1024;  // workgroups of the norm's backward pass at most
 constexpr int kWideStrip = 64;   // channels of a workgroup in the wide weight gradient
+// Workgroups of a launch at most: HIP takes grids of fewer than 2^32 threads.
+constexpr int64_t kRowGrid = 0xffffffffLL / kRowThreads;
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Piece {
@@ -467,12 +469,19 @@ struct NormCall {
 template <typename T, typename P, int V, int PIECES, bool NORM>
 static int launch_rows(const NormCall& a, int log_lanes) {
   constexpr int ROWS = PIECES == 1 ? 2 : 1;
-  const int64_t blocks = cdiv(a.rows, int64_t(kRowThreads >> log_lanes) * ROWS);
-  SP_CHECK_ARG(blocks <= kMaxGridX, "rms_norm: too many rows");
-  rms_rows<T, P, V, PIECES, ROWS, NORM><<<unsigned(blocks), kRowThreads, 0, a.stream>>>(
-      static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.res), a.ldr, a.w, a.eps, a.rows,
-      a.C, log_lanes, static_cast<T*>(a.y), static_cast<T*>(a.sum), a.codes, a.scales);
-  SP_LAUNCHED();
+  const int64_t per = int64_t(kRowThreads >> log_lanes) * ROWS, most = kRowGrid * per;
+  const int groups = int(cdiv(a.C, kRowGroup));
+  auto from = [](auto* p, int64_t at) { return p ? p + at : nullptr; };
+  for (int64_t r = 0; r < a.rows; r += most) {
+    const int64_t rows = a.rows - r < most ? a.rows - r : most;
+    rms_rows<T, P, V, PIECES, ROWS, NORM>
+        <<<unsigned(cdiv(rows, per)), kRowThreads, 0, a.stream>>>(
+            static_cast<const T*>(a.x) + r * a.ldx, a.ldx,
+            from(static_cast<const T*>(a.res), r * a.ldr), a.ldr, a.w, a.eps, rows, a.C, log_lanes,
+            from(static_cast<T*>(a.y), r * a.C), from(static_cast<T*>(a.sum), r * a.C),
+            from(a.codes, r * a.C), from(a.scales, r * groups));
+    SP_LAUNCHED();
+  }
   return SP_OK;
 }
 
@@ -583,7 +592,7 @@ static int run_restore(const int8_t* codes, const float* scales, int64_t rows, i
       C % V == 0 && aligned16(out) && (reinterpret_cast<uintptr_t>(codes) & (V - 1)) == 0;
   const int64_t pieces = rows * (vec ? C / V : C);
   const int64_t blocks = cdiv(pieces, kRowThreads);
-  const unsigned grid = unsigned(blocks < kMaxGridX ? blocks : kMaxGridX);
+  const unsigned grid = unsigned(blocks < kRowGrid ? blocks : kRowGrid);
   if (vec)
     restore_rows<T, V><<<grid, kRowThreads, 0, s>>>(codes, scales, pieces, C,
                                                     static_cast<T*>(out));
