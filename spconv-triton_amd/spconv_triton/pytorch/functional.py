@@ -324,8 +324,9 @@ def _as_autocast_takes(*tensors):
     if not torch.is_autocast_enabled("cuda"):
         return tensors
     dtype = torch.get_autocast_dtype("cuda")
-    return tuple(t.to(dtype) if t is not None and t.is_cuda and t.is_floating_point()
-                 and t.dtype is not torch.float64 else t for t in tensors)
+    return tuple(t.to(dtype) if isinstance(t, torch.Tensor) and t.is_cuda
+                 and t.is_floating_point() and t.dtype is not torch.float64 else t
+                 for t in tensors)
 
 
 class GatedFFNFunction(Function):

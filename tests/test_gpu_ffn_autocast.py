@@ -80,3 +80,18 @@ def test_a_block_in_a_bf16_region():
     y.float().square().sum().backward()
     assert all(p.grad is not None and p.grad.dtype is F32 and torch.isfinite(p.grad).all()
                for p in block.parameters())
+
+
+def test_refusals_are_the_same():
+    from spconv_triton.pytorch import functional as Fsp
+
+    x, wg, wu, wd, res, _ = _inputs()
+    with torch.autocast("cuda", dtype=BF16):
+        with pytest.raises(ValueError, match="8 bits"):
+            Fsp.gated_ffn(Fsp.quantize_rows(x), wg, wu, wd)
+        with pytest.raises(ValueError):
+            Fsp.gated_ffn(x, wg[:, 1:], wu, wd)
+        with pytest.raises(ValueError):
+            Fsp.gated_ffn(x, wg, wu.cpu(), wd)
+        with pytest.raises(NotImplementedError):
+            Fsp.gated_ffn(*(t.double() for t in (x, wg, wu, wd)))
