@@ -443,7 +443,8 @@ int sp_point2voxel(const void* points, int32_t dtype, int64_t n_points, int64_t 
 /* ---- whole rows: norm and 8-bit copies --------------------------------- */
 /* Operators of this library's own (the reference has none of this kind) on
  * feature rows of f16, bf16 or f32.  ld*: elements from row to row (>= C); rows without
- * one are contiguous.  Sums and statistics are fp32.
+ * one are contiguous.  Sums and statistics are fp32.  Calls of so many rows that a grid would pass
+ * 2^32 threads are several launches.
  *
  * s = x + residual (residual null: s = x), y = s / sqrt(mean(s^2) + eps) *
  * weight, each rounded once to the rows' type; weight [C] of type param_dtype
@@ -476,8 +477,9 @@ int sp_restore_rows(const int8_t* codes, const float* scales, int64_t rows, int6
 /* g = x w_gate', u = x w_up', y = (act(g) * u) w_down' (+ residual, nullable),
  * for rows x [rows, C] and weights w_gate, w_up [F, C], w_down [Co, F] of one
  * type (f16, bf16 or f32), contiguous; y [rows, Co].  act: 0 silu, 1 gelu (the exact one), 2 relu.  Sums are
- * fp32; act(g) * u is rounded to the type between the products.  Workspaces are 16-byte
- * aligned. */
+ * fp32; act(g) * u is rounded to the type between the products (in f16 infinite past 65504) from five
+ * rows on, and stays fp32 for up to four, so that a row's result may depend on how many there
+ * are.  Workspaces are 16-byte aligned; wide or f32 rows take F values a row of them. */
 size_t sp_gated_ffn_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co);
 int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
                  const void* w_gate, const void* w_up, int64_t F, const void* w_down, int64_t Co,
@@ -487,7 +489,8 @@ int sp_gated_ffn(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_
  * codes and scales as sp_quantize_rows makes them (ldx is not read), whose values then stand for
  * x throughout; `int8` of the workspace query says which.  g, u and the gradient of the
  * hidden rows are formed again; the latter's parts are rounded to the type between the products.
- * Sums over rows have a fixed order. */
+ * Sums over rows have a fixed order.  The workspace holds 3 F values a row where the hidden rows
+ * pass through memory (f32, more than 128 channels, or 33 to 128 and fewer than 16384 rows). */
 size_t sp_gated_ffn_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t F, int64_t Co,
                                   int32_t int8);
 int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,

@@ -27,7 +27,7 @@ namespace sp {
 // channels and 1 376 hidden units, with 256 and 128 half of that, 307 and 200 us (700 TFLOP/s bf16,
 // where the library's product of these sizes without the gate reaches 500).  What bounds the large
 // tiles then: the eight waves of a CU meet at a barrier each stage and read its first operands with
-// the matrix cores idle (these work for 47 % of the time that a CU is busy), and 50k rows leave the last
+// the matrix cores idle (these work for 44 % of the time that a CU is busy), and 50k rows leave the last
 // round of workgroups half empty (1.5 rounds for w_down).  Four stages of half the length, with
 // three in flight: 7 % slower.
 template <int XT_, int WT_, int WX_, int WW_>
@@ -235,7 +235,7 @@ __device__ __forceinline__ int64_t place_of(int64_t total, int64_t id = blockIdx
 }
 
 // h = act(x Wg') * (x Wu'), rows of Fp values, of which those from F on stand for nothing: who reads h
-// stops at F.  50k x 512 -> 1 376 bf16 200 us (700 TFLOP/s), 75k x 256 -> 688 107.
+// stops at F.  50k x 512 -> 1 376 bf16 194 us (725 TFLOP/s), 75k x 256 -> 688 111.
 template <typename T, typename S, bool ASYNC>
 __global__ __launch_bounds__(S::THREADS, 2) void ffn_up(Rows<T> x, Rows<T> wg, Rows<T> wu, int act,
                                                      T* __restrict__ h, int Fp) {
@@ -341,7 +341,10 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_grad_hidden(Rows<T> x, Rows
 
 // out = a w' (+ residual, added in fp32).  50k x 1 376 -> 512 bf16 109 us and x 2 752 -> 512 190 (645 and 740
 // TFLOP/s; 392 tiles are 1.5 rounds of workgroups); fp32 30k x 256 -> 96 21 us and x 512 -> 96 35 (71 and
-// 83, of 154: one tile a CU, whose waves take loads and products in turn).
+// 83, of 154: one tile a CU, whose waves take loads and products in turn).  The residual is read value by value
+// in the epilogue: 40 us more at 75k x 688 -> 256, 60 at 50k x 1 376 -> 512, for 8 and 10 of its bytes' own.
+// Rows of w whose width V does not divide go through registers value by value: 75k x 256 -> 682 291 us in all
+// for 120 at 688, 50k x 512 -> 1 365 727 for 259 at 1 360.
 template <typename T>
 struct RowsOut {
   const T* residual;

@@ -62,8 +62,9 @@ __device__ __forceinline__ void fused_store(const FusedArgs<T>& a, int64_t r,
 // CP: channels of x and y, rounded up to 32.  200k x 64 -> 256 fp16 31-36 us (51 MB of rows would take 10,
 // the products 14 at the rate of large ones; the two kernels that store h took 137 in their first form).
 // A wave's gate, 16 exponentials and reciprocals for each 32 x 32 block, is as long as the block's
-// MFMAs; other waves' MFMAs run beside it, four waves a SIMD.  About 15 us are the first rows' loads
-// and the last ones' writes, with no products beside them: all workgroups are resident at once.
+// MFMAs; other waves' MFMAs run beside it, four waves a SIMD, whose 128 registers are two to seven too
+// few for silu and gelu (these go to scratch memory).  The 1 563 workgroups of those 200k rows are a round and
+// a half of the 1 024 that are resident at a time: the second round is half empty.
 template <typename T, int ACT, int CP, int MINW>
 __global__ __launch_bounds__(kFfnThreads, MINW) void ffn_fused(FusedArgs<T> a) {
   using frag = typename Mfma<T>::frag;
@@ -125,7 +126,8 @@ static int up8(int64_t v) { return int(cdiv(v, 8) * 8); }
 // least; the tiled kernels' chains are shorter, but write and read h.  Measured, one kernel against two
 // (us; 128 -> 344 fp16): 1 000 rows 14.9 / 12.3, 8 000 15.5 / 14.7, 16 000 16.1 / 19.3, 32 000 17.6 / 28.8;
 // 64 -> 256 8.7 / 10.6 at 1 000 rows; 192 -> 512 26.8 / 24.6 at 16 000 and 29.7 / 39.5 at 32 000;
-// 256 -> 688 bf16 at 75 000 rows 149 / 138 (a wave a SIMD: its registers hold no more).
+// 256 -> 688 bf16 at 75 000 rows 149 / 138 (a wave a SIMD: its registers hold no more).  All of these have
+// hidden widths of 2.7 to 4 times the channels; other ratios were not measured.
 bool fused_forward_takes(int32_t dtype, int64_t rows, int64_t C, int64_t Co) {
   const int64_t n = C > Co ? C : Co;
   return dtype != SP_F32 && n <= kFusedWidth && (n <= 64 || rows >= 96 * n);

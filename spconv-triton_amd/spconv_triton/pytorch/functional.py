@@ -230,7 +230,6 @@ def _inference() -> bool:
                 or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing())
 
 
-
 # ---------------------------------------------------------------------------
 # the channel half of a block: norm, gated feed-forward, rows in 8 bits
 # ---------------------------------------------------------------------------
@@ -365,7 +364,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     :class:`Int8Rows`, as ``rms_norm`` returns).  With a copy the gradients are those at the
     values that it stands for.
 
-    Under autocast x, the weights and the residual are taken, and y returned, in autocast's type.
+    Sums are float32; 16-bit calls of five rows or more round ``act(x w_gate') * (x w_up')`` to
+    their type between the products (up to four rows keep it in float32).  Under autocast x, the
+    weights and the residual are taken, and y returned, in autocast's type.
     """
     codes = scales = None
     if isinstance(saved, Int8Rows):
