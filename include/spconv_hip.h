@@ -499,6 +499,45 @@ int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
                      const void* w_down, int64_t Co, int32_t act, void* dx, void* dw_gate,
                      void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- attention ----------------------------------------------------------- */
+/* O = softmax(scale q k') v for each of `heads` query heads, within each sequence of rows.  Key head h
+ * serves the heads / kv_heads query heads from h (heads / kv_heads) on.  q [nq, heads, dim], k and v
+ * [nk, kv_heads, dim] of f16, bf16 or f32: *_row elements from row to row, *_head from head to
+ * head, all multiples of 16 bytes, as dim (<= 128) is; the values of a head are neighbours.
+ * Sequence s has the queries q_offsets[s] .. q_offsets[s + 1] - 1 and the keys of k_offsets likewise
+ * (device memory, [sequences + 1], ascending; both null: one sequence of all rows).
+ * Offsets are not checked; whatever they hold, no access leaves the rows.  causal: a query sees
+ * the keys up to its own place counted from the sequence's end (the last query sees all).  A query that sees no key, as
+ * those outside all sequences, gets zeros.  Sums and the softmax's statistics are fp32, its
+ * weights are rounded to the type between the products. */
+typedef struct sp_attn {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int64_t nq, nk, heads, kv_heads, dim, sequences;
+  const int32_t *q_offsets, *k_offsets;
+  float scale; /* > 0 */
+  int32_t causal, dtype;
+} sp_attn;
+/* out [nq, heads, dim]; lse [heads, nq] (nullable, for the backward pass) receives the base-2 logarithm
+ * of the sum of 2^(log2(e) score).  The workspace (16-byte aligned) holds partial results where
+ * few queries have many keys. */
+size_t sp_attention_workspace(const sp_attn* call);
+int sp_attention(const sp_attn* call, void* out, int64_t out_row, int64_t out_head, float* lse,
+                 void* ws, size_t ws_bytes, void* stream);
+/* Gradients from that of out (dout), with out (o) and lse as the forward pass gave them: dq, dk and dv
+ * (each nullable), laid out as the strides say.  Rows outside all sequences get zeros.  Sums have a fixed
+ * order. */
+typedef struct sp_attn_grad {
+  const void *o, *dout;
+  const float* lse;
+  void *dq, *dk, *dv;
+  int64_t o_row, o_head, dout_row, dout_head;
+  int64_t dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+} sp_attn_grad;
+size_t sp_attention_bwd_workspace(const sp_attn* call);
+int sp_attention_bwd(const sp_attn* call, const sp_attn_grad* grad, void* ws, size_t ws_bytes,
+                     void* stream);
+
 /* ---- hash table (spconv_triton/pytorch/hash.py:15-110) ----------------- */
 /* A table of `capacity` (a power of two) slots lives in one caller-owned
  * device buffer of sp_hash_table_bytes(capacity).  Keys are int32 (key64 = 0)

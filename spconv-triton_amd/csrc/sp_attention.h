@@ -1,0 +1,419 @@
+// What the attention kernels share: sequences in packed rows, tiles of rows in LDS and the
+// operands that the matrix instructions take from them.
+#pragma once
+
+#include "sp_ffn.h"  // LDS order, loads to LDS, batched operand reads
+
+namespace sp {
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnWaves = kAttnThreads / 64;
+constexpr int kAttnBatch = 2;  // operands read from LDS at a time, while as many are in use
+
+// Rows [rows] in `parts` sequences, sequence p at bound(p) .. bound(p + 1).  With offsets the first and the
+// last part are the rows before the first sequence and behind the last one: they have no keys, and
+// no queries.  Whatever the offsets hold, a bound lies in the rows.
+struct Seqs {
+  const int32_t* off;
+  int64_t rows;
+  int parts;
+  __device__ __forceinline__ int64_t bound(int p) const {
+    if (p == 0) return 0;
+    if (!off || p >= parts) return rows;
+    const int64_t b = off[p - 1];
+    return b < 0 ? 0 : b < rows ? b : rows;
+  }
+  __device__ __forceinline__ bool outside(int p) const { return off && (p == 0 || p + 1 == parts); }
+};
+
+// A sequence's tile of `tile` of its rows: `at` is the first one's place among the sequence's rows, lo the
+// sequence's first row.  Each row counts `mult` times (the query heads that share a key head are rows of
+// one tile).
+struct Tile {
+  int part;
+  int64_t lo, len, at;  // len: the sequence's rows, times mult; at < len where there is a tile
+};
+
+// Tile number `slot` of start(p) = bound(p) mult / tile + p on: a sequence has at least as many slots
+// as tiles, and no table of tiles is needed.  All lanes of a wave look 64 ways at a time.
+__device__ __forceinline__ Tile find_tile(const Seqs& s, int mult, int tile, int64_t slot) {
+  int lo = 0, size = s.parts;
+  const int lane = int(threadIdx.x) & 63;
+  while (size > 1) {
+    const int step = (size + 63) >> 6, at = lane * step;
+    const bool before = at < size && s.bound(lo + at) * mult / tile + lo + at <= slot;
+    const int n = __popcll(__ballot(before));
+    const int skip = n > 1 ? (n - 1) * step : 0;
+    lo += skip;
+    size = size - skip < step ? size - skip : step;
+  }
+  Tile t;
+  t.part = lo;
+  t.lo = s.bound(lo);
+  const int64_t hi = s.bound(lo + 1);
+  t.len = hi > t.lo ? (hi - t.lo) * mult : 0;
+  t.at = (slot - (t.lo * mult / tile + lo)) * tile;
+  if (t.at < 0) t.at = t.len;
+  return t;
+}
+
+inline int64_t tile_slots(const Seqs& s, int mult, int tile) {
+  return s.rows * mult / tile + s.parts;
+}
+
+// The keys of the queries of part p.
+__device__ __forceinline__ int keys_of(const Seqs& q, const Seqs& k, int p, int64_t klo) {
+  const int64_t n = q.outside(p) ? 0 : k.bound(p + 1) - klo;
+  return n > 0 ? int(n) : 0;
+}
+
+// How many of Lk keys the i-th of Lq queries sees, causal: the last one sees all.
+__device__ __forceinline__ int keys_seen(int64_t i, int Lq, int Lk) {
+  const int64_t n = i + 1 + Lk - Lq;
+  return n < 0 ? 0 : n < Lk ? int(n) : Lk;
+}
+
+// Rows of a head: row r, head h at p + r * row + h * head.
+template <typename T>
+struct Heads {
+  T* p;
+  int64_t row, head;
+};
+
+// ---- tiles in LDS ----------------------------------------------------------------
+// ROWS rows of DP values (the head's, then zeros) in 16-byte pieces, permuted within a row so that neither
+// whole pieces of 32 rows nor transposed reads meet on a bank.  Rows lie in their own order.
+template <typename T, int DP, int ROWS>
+struct HeadTile {
+  using frag = typename Mfma<T>::frag;
+  static constexpr int V = Mfma<T>::V, KSTEP = Mfma<T>::KSTEP;
+  static constexpr int PIECES = DP / V, BYTES = ROWS * PIECES * 16;
+  static constexpr int N = ROWS * PIECES / kAttnThreads;  // pieces of a thread
+  static_assert(ROWS * PIECES % kAttnThreads == 0, "whole rounds");
+
+  // The operand row that MFMA row m of a 32-row block takes: then the accumulator's register i of lane half
+  // h is row 2 V (i / V) + V h + i % V, which is the order of the next product's operand.
+  __device__ __forceinline__ static int row_of(int m) { return sizeof(T) == 2 ? unit_of(m) : m; }
+
+  // rows r0 .. r0 + 31, values k .. k + KSTEP - 1 (step k of the reduction)
+  __device__ __forceinline__ static frag read(const char* lds, int r0, int step) {
+    const int lane = int(threadIdx.x) & 63, r = r0 + row_of(lane & 31);
+    return *reinterpret_cast<const frag*>(
+        lds + (r * PIECES + swizzled<PIECES>(r, 2 * step + (lane >> 5))) * 16);
+  }
+  // transposed: values c0 .. c0 + 31 (permuted as row_of) of rows r0 .. r0 + KSTEP - 1, which are
+  // the reduction
+  __device__ __forceinline__ static frag read_t(const char* lds, int r0, int c0) {
+    const int lane = int(threadIdx.x) & 63, half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      frag f;
+      const int c = c0 + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int r = r0 + half * V + i;
+        f[i] = *reinterpret_cast<const T*>(
+            lds + (r * PIECES + swizzled<PIECES>(r, c / V)) * 16 + c % V * 4);
+      }
+      return f;
+    } else {
+      typedef short short4 __attribute__((ext_vector_type(4)));
+      const int t = lane & 15;
+      const int c = c0 + (lane & 16) + ((t & 1) << 3) + ((t & 2) << 1);
+      union {
+        short4 q[2];
+        frag f;
+      } u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = r0 + 8 * half + 4 * j + (t >> 2);
+        u.q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4*)(lds + (r * PIECES +
+                swizzled<PIECES>(r, c >> 3)) * 16 + (c & 7) * 2));
+      }
+      return u.f;
+    }
+  }
+};
+
+// The row (reduction index of the next product) of an accumulator's register i.
+template <typename T>
+__device__ __forceinline__ int acc_row(int i) {
+  constexpr int V = Mfma<T>::V;
+  return i / V * 2 * V + V * ((int(threadIdx.x) >> 5) & 1) + i % V;
+}
+
+// Loads of a thread's pieces of tiles of a head's rows.  Whole tiles take an address of the workgroup's and
+// an offset of the lane's for good; the pieces past the head's width are zeroed once and never
+// written.  A tile that passes the last row goes by piece, with zeros past the end (0 times what
+// lies there could be NaN).
+template <typename T, int DP, int ROWS>
+struct TileLoads {
+  using L = HeadTile<T, DP, ROWS>;
+  const T* p;  // the sequence's first row
+  int64_t row;
+  int len, D;
+  unsigned off[L::N];  // of this thread's pieces, in bytes (rows of less than 2^23 values)
+
+  __device__ __forceinline__ TileLoads(const T* p_, int64_t row_, int len_, int D_)
+      : p(p_), row(row_), len(len_), D(D_) {
+#pragma unroll
+    for (int j = 0; j < L::N; ++j) off[j] = unsigned(at_row(j) * int(row) + at_value(j)) * unsigned(sizeof(T));
+  }
+  __device__ __forceinline__ static int at_row(int j) {
+    return (j * kAttnThreads + int(threadIdx.x)) / L::PIECES;
+  }
+  __device__ __forceinline__ static int at_value(int j) {
+    const int m = at_row(j);
+    return swizzled<L::PIECES>(m, j * kAttnThreads + int(threadIdx.x) - m * L::PIECES) * L::V;
+  }
+  // zeros past the head's width, before the first tile (a barrier follows)
+  __device__ __forceinline__ void clear(char* lds) const {
+#pragma unroll
+    for (int j = 0; j < L::N; ++j)
+      if (at_value(j) >= D)
+        *reinterpret_cast<uint4*>(lds + (j * kAttnThreads + int(threadIdx.x)) * 16) =
+            uint4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void start(int at, char* lds) const {
+    const char* base = reinterpret_cast<const char*>(p + at * row);
+    if (at + ROWS <= len) {
+#pragma unroll
+      for (int j = 0; j < L::N; ++j)
+        if (DP == D || at_value(j) < D)
+          copy_piece(base + off[j], lds + (j * kAttnThreads + wave_of() * 64) * 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < L::N; ++j)
+        if (DP == D || at_value(j) < D)
+          copy_piece(at + at_row(j) < len ? static_cast<const void*>(base + off[j]) : &g_zero_piece,
+                     lds + (j * kAttnThreads + wave_of() * 64) * 16);
+    }
+  }
+};
+
+// A row's operands for the whole head (zeros past D).
+template <typename T, int DP>
+__device__ __forceinline__ void load_head(const T* p, bool live, int D,
+                                          typename Mfma<T>::frag (&f)[DP / Mfma<T>::KSTEP]) {
+  using frag = typename Mfma<T>::frag;
+  constexpr int V = Mfma<T>::V;
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int s = 0; s < DP / Mfma<T>::KSTEP; ++s) {
+    const int c = (2 * s + half) * V;
+    f[s] = frag{};
+    if (live && c < D) f[s] = *reinterpret_cast<const frag*>(p + c);
+  }
+}
+
+template <typename T>
+struct Both {
+  typename Mfma<T>::frag a, b;
+};
+
+__device__ __forceinline__ void zero(floatx16& a) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a[i] = 0.f;
+}
+
+// The other half's value of the same row.
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// acc[t] += (values 32 t .. of rows r0 .. r0 + 31)' p: the second product of attention and of its gradients.
+template <typename T, int DP, int ROWS, int B>
+__device__ __forceinline__ void add_rows(const char* lds, int r0,
+                                         const typename Mfma<T>::frag (&p)[32 / Mfma<T>::KSTEP],
+                                         floatx16 (&acc)[DP / 32]) {
+  using L = HeadTile<T, DP, ROWS>;
+  constexpr int TILES = DP / 32, STEPS = 32 / Mfma<T>::KSTEP;
+  // (neighbouring products go to different accumulators)
+  auto read = [&](int i) {
+    return L::read_t(lds, r0 + i / TILES * Mfma<T>::KSTEP, i % TILES * 32);
+  };
+  Batched<typename Mfma<T>::frag, TILES * STEPS, B> f;
+  f.start(read);
+  f.run(read, [&](int i, const typename Mfma<T>::frag& a) {
+    Mfma<T>::mma(a, p[i / TILES], acc[i % TILES]);
+  });
+}
+
+// The same where a lane sees the rows lo .. hi - 1 only and the others may hold infinities or NaN, which times
+// the zeros of p would be NaN: one row at a time, added where it is seen.  Slow, and run
+// for tiles whose results came out not finite only.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void add_rows_seen(const char* lds, int r0, int lo, int hi,
+                                           const typename Mfma<T>::frag (&p)[32 / Mfma<T>::KSTEP],
+                                           floatx16 (&acc)[DP / 32]) {
+  using L = HeadTile<T, DP, ROWS>;
+  using frag = typename Mfma<T>::frag;
+  constexpr int V = Mfma<T>::V, STEPS = 32 / Mfma<T>::KSTEP;
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const bool seen = r0 + j >= lo && r0 + j < hi;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+      floatx16 one;
+      zero(one);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        frag f = L::read_t(lds, r0 + s * Mfma<T>::KSTEP, 32 * t), g = p[s];
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (s * Mfma<T>::KSTEP + half * V + i != j) f[i] = g[i] = T(0.f);
+        Mfma<T>::mma(f, g, one);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][i] += seen ? one[i] : 0.f;
+    }
+  }
+}
+
+// Whether any lane of the wave holds a value that is not finite.
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const floatx16 (&acc)[N]) {
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      bad |= !(__builtin_fabsf(acc[t][i]) < __builtin_inff());
+  return __ballot(bad) != 0;
+}
+
+// The lane's row of results, value(t, i) for register i of tile t.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void store_head(T* p, int D, F&& value) {
+  using frag = typename Mfma<T>::frag;
+  constexpr int V = Mfma<T>::V;
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int b = 0; b < 16 / V; ++b) {
+      const int c = 32 * t + 2 * V * b + V * half;
+      if (c >= D) continue;
+      frag f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = from_f32<T>(value(t, V * b + i));
+      *reinterpret_cast<frag*>(p + c) = f;
+    }
+}
+
+// fp32 partials of a share, D values a row.
+template <int DP, int V, typename F>
+__device__ __forceinline__ void store_part(float* p, int D, F&& value) {
+  const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int b = 0; b < 16 / V; ++b) {
+      const int c = 32 * t + 2 * V * b + V * half;
+      if (c >= D) continue;
+#pragma unroll
+      for (int i = 0; i < V; i += 4)
+        *reinterpret_cast<float4v*>(p + c + i) =
+            float4v{value(t, V * b + i), value(t, V * b + i + 1), value(t, V * b + i + 2),
+                    value(t, V * b + i + 3)};
+    }
+}
+
+template <typename T>
+struct AttnArgs {
+  Heads<const T> q, k, v, o, dout;  // o: the forward pass's result, in the backward pass
+  Heads<T> out, dq, dk, dv;
+  Seqs qs, ks;
+  int H, Hk, G, D, causal;
+  float scale, scale2;  // of the scores, and times log2(e)
+  float* lse;           // [H][rows of q], base 2; +inf for a row without keys
+  const float* top;     // partial maxima of the rows' norms (fp16 gradients)
+  int tops;
+  int shares;
+  float *part, *part_ml;
+  int* again;  // causal: one a workgroup, whether its results are not finite
+};
+
+// Causal tiles run in two launches.  Where a query does not see a key, the product's operand is zero, but the
+// key's value may be an infinity or NaN, and a result that is not finite may come from there. The first
+// launch says which workgroups have such results, the second (STRICT) makes those again and adds
+// only what is seen; it costs the time of a launch.
+template <bool CAUSAL, bool STRICT>
+__device__ __forceinline__ bool skips(const int* again) {
+  return STRICT && !again[blockIdx.x];
+}
+template <bool CAUSAL, bool STRICT>
+__device__ __forceinline__ void report(int* again, bool bad, int* lds) {
+  if (!CAUSAL || STRICT) return;
+  if (threadIdx.x == 0) *lds = 0;
+  __syncthreads();
+  if (bad) *lds = 1;
+  __syncthreads();
+  if (threadIdx.x == 0) again[blockIdx.x] = *lds;
+}
+
+// The workgroup's tile: slot, key head and share of the other axis.
+struct Place {
+  int64_t slot;
+  int head, share;
+};
+// (an XCD's workgroups are an eighth of the places in a row: those of a key head share its L2)
+__device__ __forceinline__ bool find_place(int64_t slots, int heads, int shares, int64_t id,
+                                           Place& p) {
+  const int64_t total = slots * heads * shares, per = (total + 7) >> 3;
+  const int64_t k = (id >> 3) < per ? (id & 7) * per + (id >> 3) : total;
+  if (k >= total) return false;
+  const int64_t a = k / shares;
+  p.share = int(k - a * shares);
+  p.head = int(a / slots);
+  p.slot = a - p.head * slots;
+  return true;
+}
+
+// ---- host ------------------------------------------------------------------------
+constexpr int kAttnMaxDim = 128;
+
+// Rows of a tile that passes through LDS.
+template <typename T>
+constexpr int attn_stage() { return sizeof(T) == 4 ? 32 : 64; }
+
+// How many shares the other axis, of `len` rows on average, is cut into where `tiles` tiles do not fill
+// the CUs; a share keeps 256 rows.
+inline int attn_shares(int64_t tiles, int64_t len) {
+  const int64_t want = 768 / (tiles < 1 ? 1 : tiles), most = len / 256;
+  const int64_t n = want < most ? want : most;
+  return n < 1 ? 1 : int(n);
+}
+
+inline int64_t attn_tiles(const Seqs& s, int mult, int heads, int tile) {
+  return cdiv(s.rows * mult, tile) * heads;
+}
+
+inline int64_t attn_length(const Seqs& s) {
+  return s.off && s.parts > 2 ? s.rows / (s.parts - 2) : s.rows;
+}
+
+// f(padded head width as a constant)
+template <typename F>
+int with_width(int D, F&& f) {
+  if (D <= 32) return f(std::integral_constant<int, 32>());
+  if (D <= 64) return f(std::integral_constant<int, 64>());
+  if (D <= 96) return f(std::integral_constant<int, 96>());
+  return f(std::integral_constant<int, 128>());
+}
+
+// The workgroups of a launch: whole eights (find_place).
+inline int64_t attn_groups(int64_t slots, int heads, int shares) {
+  return cdiv(slots * heads * shares, 8) * 8;
+}
+
+struct AttnGradLayout {
+  size_t nl, nd, tops, part, again, total;
+  int dq_shares, dkv_shares;
+};
+AttnGradLayout attn_grad_layout(const Seqs& q, const Seqs& k, int H, int Hk, int D,
+                                bool causal);
+template <typename T>
+int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq, bool need_dkv,
+                  hipStream_t s);
+
+}  // namespace sp

@@ -1,0 +1,453 @@
+// Softmax attention of packed sequences of rows, forward pass:
+//
+//   S = scale q k', P = softmax(S) over the keys that a query sees, O = P v
+//
+// Everything is computed transposed, with the queries as the MFMAs' columns: S' = K Q', O' += V' P'.
+// A lane then holds one query, and the accumulators of the first product are the second one's operand:
+// P exists in registers only.  Keys pass through LDS a tile at a time with the running maximum
+// and sum of the softmax; the query heads that share a key head are rows of one tile.
+//
+// Statistics and sums are fp32.  P is rounded to the rows' type between the products, as the matrix
+// instructions take it; relative to a running maximum no value exceeds 2^8, and what fp16 loses below 2^-14
+// is less than 2^-25 of the largest term.
+#include "sp_attention.h"
+
+namespace sp {
+
+// A maximum that grows by less than this (in powers of two) does not rescale what is summed up.
+constexpr float kLazyMax = 8.f;
+
+// Waves a SIMD.
+template <typename T>
+constexpr int attend_waves(int DP, int QT) {
+  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : QT == 2 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : 2;
+}
+
+template <typename T, int DP, int QT, int BK, bool CAUSAL, bool STRICT>
+__global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, QT)) void attend(AttnArgs<T> a,
+                                                                                int64_t slots) {
+  using frag = typename Mfma<T>::frag;
+  using L = HeadTile<T, DP, BK>;
+  constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
+  constexpr int NK = BK / 32, BQ = kAttnWaves * QT * 32;
+  __shared__ __attribute__((aligned(16))) char lds[4 * L::BYTES];
+  __shared__ int bad_lds;
+  Place place;
+  if (!find_place(slots, a.Hk, a.shares, blockIdx.x, place)) return;
+  if (skips<CAUSAL, STRICT>(a.again)) return;
+  if (CAUSAL) place.slot = slots - 1 - place.slot;  // (the longest rows first)
+  const Tile t = find_tile(a.qs, a.G, BQ, place.slot);
+  if (t.at >= t.len) {
+    if (CAUSAL && !STRICT && threadIdx.x == 0) a.again[blockIdx.x] = 0;
+    return;
+  }
+  const int64_t klo = a.ks.bound(t.part);
+  const int Lk = keys_of(a.qs, a.ks, t.part, klo), Lq = int(t.len / a.G);
+
+  // this lane's queries
+  const int wave = wave_of(), lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
+  frag q[QT][STEPS];
+  int row[QT], seen[QT], head[QT];  // the query's row in its sequence; how many keys it sees
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    const int64_t r = t.at + (wave * QT + u) * 32 + lane;
+    const bool live = r < t.len;
+    const int i = int(r / a.G);
+    head[u] = place.head * a.G + int(r - int64_t(i) * a.G);
+    row[u] = live ? i : -1;
+    seen[u] = CAUSAL ? keys_seen(i, Lq, Lk) : Lk;
+    load_head<T, DP>(a.q.p + (t.lo + i) * a.q.row + head[u] * a.q.head, live, a.D, q[u]);
+  }
+  // keys that some query of the workgroup or wave sees, and that every one of the wave sees
+  int most = Lk, wave_most = Lk, wave_least = Lk;
+  if (CAUSAL) {
+    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * QT * 32;
+    most = keys_seen(int((last - 1) / a.G), Lq, Lk);
+    wave_least = keys_seen(int(w / a.G), Lq, Lk);
+    wave_most = keys_seen(int((w + QT * 32 - 1) / a.G), Lq, Lk);
+    wave_most = wave_most < most ? wave_most : most;
+  }
+
+  // this share's tiles
+  const int tiles = (most + BK - 1) / BK, per = (tiles + a.shares - 1) / a.shares;
+  const int first = place.share * per, end = first + per < tiles ? first + per : tiles;
+  const TileLoads<T, DP, BK> lk(a.k.p + klo * a.k.row + place.head * a.k.head, a.k.row, Lk, a.D);
+  const TileLoads<T, DP, BK> lv(a.v.p + klo * a.v.row + place.head * a.v.head, a.v.row, Lk, a.D);
+  const float c = a.scale2;
+  if (DP != a.D) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
+  }
+  floatx16 o[QT][DP / 32];
+  float m[QT], neg[QT], l[QT];
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    m[u] = -__builtin_inff();
+    neg[u] = l[u] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) zero(o[u][d]);
+  }
+  if (first < end) {
+    lk.start(first * BK, lds);
+    lv.start(first * BK, lds + L::BYTES);
+  }
+  for (int n = first; n < end; ++n) {
+    char* buf = lds + ((n - first) & 1) * 2 * L::BYTES;
+    loads_in_flight<0>();
+    __syncthreads();
+    if (n + 1 < end) {
+      char* next = lds + ((n + 1 - first) & 1) * 2 * L::BYTES;
+      lk.start((n + 1) * BK, next);
+      lv.start((n + 1) * BK, next + L::BYTES);
+    }
+    const int key0 = n * BK;
+    if (CAUSAL && key0 >= wave_most) continue;
+    const bool edge = key0 + BK > wave_least;
+    floatx16 s[QT][NK];
+#pragma unroll
+    for (int x = 0; x < NK; ++x) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u) zero(s[u][x]);
+      auto read = [&](int k) { return L::read(buf, 32 * x, k); };
+      Batched<frag, STEPS, kAttnBatch> f;
+      f.start(read);
+      f.run(read, [&](int k, const frag& kf) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) Mfma<T>::mma(kf, q[u][k], s[u][x]);
+      });
+    }
+    frag p[QT][NK][PS];
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < NK; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (key0 + 32 * x + acc_row<T>(i) >= seen[u]) s[u][x][i] = -__builtin_inff();
+      }
+      float mx = s[u][0][0];
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, s[u][x][i]);
+      mx = __builtin_fmaxf(mx, other_half(mx)) * c;
+      if (__ballot(mx > m[u] + kLazyMax)) {
+        const float now = __builtin_fmaxf(mx, m[u]);
+        const float safe = now == -__builtin_inff() ? 0.f : now;
+        const float down = __builtin_amdgcn_exp2f(m[u] - safe);
+        m[u] = now;
+        neg[u] = -safe;
+        l[u] *= down;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[u][d][i] *= down;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x][i], c, neg[u]));
+          sum += e;
+          p[u][x][i / V][i % V] = T(e);
+        }
+      l[u] += sum;
+    }
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        if (STRICT && edge)
+          add_rows_seen<T, DP, BK>(buf + L::BYTES, 32 * x, 0, seen[u] - key0, p[u][x], o[u]);
+        else
+          add_rows<T, DP, BK, kAttnBatch>(buf + L::BYTES, 32 * x, p[u][x], o[u]);
+      }
+  }
+  bool bad = false;
+  if (CAUSAL && !STRICT) {
+#pragma unroll
+    for (int u = 0; u < QT; ++u) bad |= any_not_finite(o[u]);
+  }
+  report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+
+  const int64_t rows = a.qs.rows;
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    const float sum = l[u] + other_half(l[u]);
+    if (row[u] < 0) continue;
+    const int64_t r = t.lo + row[u];
+    if (a.shares > 1) {
+      const int64_t at = (place.share * rows + r) * a.H + head[u];
+      store_part<DP, V>(a.part + at * a.D, a.D, [&](int d, int i) { return o[u][d][i]; });
+      if (half == 0) {
+        a.part_ml[2 * at] = m[u];
+        a.part_ml[2 * at + 1] = sum;
+      }
+      continue;
+    }
+    // (a row without keys is zeros)
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    store_head<T, DP>(a.out.p + r * a.out.row + head[u] * a.out.head, a.D,
+                      [&](int d, int i) { return o[u][d][i] * inv; });
+    if (a.lse && half == 0)
+      a.lse[head[u] * rows + r] =
+          sum == 0.f ? __builtin_inff() : m[u] + __builtin_amdgcn_logf(sum);
+  }
+}
+
+// The shares' results of a row joined: a workgroup of 64 lanes a row and head.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attend_join(AttnArgs<T> a) {
+  const int64_t n = a.qs.rows * a.H, at = int64_t(blockIdx.x) * kAttnWaves + wave_of();
+  if (at >= n) return;
+  const int lane = int(threadIdx.x) & 63;
+  const int64_t r = at / a.H;
+  const int h = int(at - r * a.H);
+  float m = -__builtin_inff();
+  for (int s = 0; s < a.shares; ++s) m = __builtin_fmaxf(m, a.part_ml[2 * (s * n + at)]);
+  const float safe = m == -__builtin_inff() ? 0.f : m;
+  float sum = 0.f, v[2] = {0.f, 0.f};
+  for (int s = 0; s < a.shares; ++s) {
+    const int64_t i = s * n + at;
+    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * i] - safe);
+    sum = __builtin_fmaf(w, a.part_ml[2 * i + 1], sum);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (lane + 64 * j < a.D)
+        v[j] = __builtin_fmaf(w, a.part[i * a.D + lane + 64 * j], v[j]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* to = a.out.p + r * a.out.row + h * a.out.head;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (lane + 64 * j < a.D) to[lane + 64 * j] = from_f32<T>(v[j] * inv);
+  if (a.lse && lane == 0)
+    a.lse[h * a.qs.rows + r] =
+        sum == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(sum);
+}
+
+// ---- host ------------------------------------------------------------------------
+constexpr int kForwardTiles = 1;  // query tiles of 32 a wave
+constexpr int kForwardRows = kAttnWaves * kForwardTiles * 32;
+
+template <typename T>
+static int launch_attend(AttnArgs<T> a, hipStream_t s) {
+  const int64_t slots = tile_slots(a.qs, a.G, kForwardRows);
+  const int64_t groups = attn_groups(slots, a.Hk, a.shares);
+  SP_CHECK_ARG(groups <= kMaxGridX, "attention: too many rows");
+  with_width(a.D, [&](auto w) {
+    constexpr int DP = w.value, QT = kForwardTiles, BK = attn_stage<T>();
+    const dim3 grid{unsigned(groups)}, block{kAttnThreads};
+    if (!a.causal) {
+      attend<T, DP, QT, BK, false, false><<<grid, block, 0, s>>>(a, slots);
+    } else {
+      attend<T, DP, QT, BK, true, false><<<grid, block, 0, s>>>(a, slots);
+      attend<T, DP, QT, BK, true, true><<<grid, block, 0, s>>>(a, slots);
+    }
+    return 0;
+  });
+  SP_LAUNCHED();
+  if (a.shares == 1) return SP_OK;
+  const int64_t joins = cdiv(a.qs.rows * a.H, kAttnWaves);
+  SP_CHECK_ARG(joins <= kMaxGridX, "attention: too many rows");
+  attend_join<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
+  SP_LAUNCHED();
+  return SP_OK;
+}
+
+static int check_heads(const char* what, const char* name, const void* p, int64_t row,
+                       int64_t head, int64_t heads, int64_t dim, int V) {
+  SP_CHECK_ARG(p, "%s: %s is null", what, name);
+  SP_CHECK_ARG(aligned(p) && row % V == 0 && head % V == 0,
+               "%s: heads of %s do not start at multiples of 16 bytes", what, name);
+  SP_CHECK_ARG((heads == 1 || head >= dim) && row >= 0, "%s: heads of %s overlap", what, name);
+  SP_CHECK_ARG(row < (1 << 23), "%s: %s has 2^23 values or more from row to row", what, name);
+  return SP_OK;
+}
+
+static int check_call(const char* what, const sp_attn* a) {
+  SP_CHECK_ARG(a, "%s: null arguments", what);
+  SP_CHECK_ARG(a->dtype == SP_F16 || a->dtype == SP_BF16 || a->dtype == SP_F32,
+               "%s: dtype %d not supported (f16/bf16/f32)", what, a->dtype);
+  const int V = vec_of(a->dtype);
+  SP_CHECK_ARG(a->heads >= 1 && a->kv_heads >= 1 && a->heads < 65536 &&
+                   a->heads % a->kv_heads == 0,
+               "%s: %lld query heads for %lld key heads", what, (long long)a->heads,
+               (long long)a->kv_heads);
+  SP_CHECK_ARG(a->dim >= 1 && a->dim % V == 0, "%s: head width %lld is no multiple of %d", what,
+               (long long)a->dim, V);
+  if (a->dim > kAttnMaxDim)
+    return set_error(SP_ERR_UNSUPPORTED, "%s: heads wider than %d", what, kAttnMaxDim);
+  SP_CHECK_ARG(a->nq >= 0 && a->nk >= 0 && a->nq < (int64_t(1) << 31) &&
+                   a->nk < (int64_t(1) << 31),
+               "%s: bad row counts %lld and %lld", what, (long long)a->nq, (long long)a->nk);
+  SP_CHECK_ARG((a->q_offsets == nullptr) == (a->k_offsets == nullptr),
+               "%s: offsets of queries and keys go together", what);
+  SP_CHECK_ARG(!a->q_offsets || (a->sequences >= 0 && a->sequences < (1 << 30)),
+               "%s: bad number of sequences %lld", what, (long long)a->sequences);
+  SP_CHECK_ARG(a->scale > 0.f && a->scale < __builtin_inff(), "%s: the scale must be positive",
+               what);
+  if (a->nq) {
+    if (int rc = check_heads(what, "q", a->q, a->q_row, a->q_head, a->heads, a->dim, V)) return rc;
+  }
+  if (a->nk) {
+    if (int rc = check_heads(what, "k", a->k, a->k_row, a->k_head, a->kv_heads, a->dim, V))
+      return rc;
+    if (int rc = check_heads(what, "v", a->v, a->v_row, a->v_head, a->kv_heads, a->dim, V))
+      return rc;
+  }
+  return SP_OK;
+}
+
+static Seqs seqs(const int32_t* off, int64_t rows, int64_t n) {
+  return Seqs{off, rows, off ? int(n) + 2 : 1};
+}
+
+template <typename T>
+static AttnArgs<T> arguments(const sp_attn& c) {
+  AttnArgs<T> a{};
+  a.q = {static_cast<const T*>(c.q), c.q_row, c.q_head};
+  a.k = {static_cast<const T*>(c.k), c.k_row, c.k_head};
+  a.v = {static_cast<const T*>(c.v), c.v_row, c.v_head};
+  a.qs = seqs(c.q_offsets, c.nq, c.sequences);
+  a.ks = seqs(c.k_offsets, c.nk, c.sequences);
+  a.H = int(c.heads);
+  a.Hk = int(c.kv_heads);
+  a.G = a.H / a.Hk;
+  a.D = int(c.dim);
+  a.causal = c.causal != 0;
+  a.scale = c.scale;
+  a.scale2 = c.scale * 1.4426950408889634f;
+  a.shares = 1;
+  return a;
+}
+
+struct ForwardLayout {
+  size_t part, ml, again, total;
+  int shares;
+};
+
+static ForwardLayout forward_layout(const sp_attn& c) {
+  const Seqs q = seqs(c.q_offsets, c.nq, c.sequences), k = seqs(c.k_offsets, c.nk, c.sequences);
+  const int G = int(c.heads / c.kv_heads), Hk = int(c.kv_heads);
+  ForwardLayout l{};
+  l.shares = attn_shares(attn_tiles(q, G, Hk, kForwardRows), attn_length(k));
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = align_up(off + bytes, 256);
+    return at;
+  };
+  const size_t rows = l.shares > 1 ? size_t(l.shares) * c.nq * c.heads : 0;
+  l.part = take(rows * c.dim * sizeof(float));
+  l.ml = take(rows * 2 * sizeof(float));
+  if (c.causal)
+    l.again = take(size_t(attn_groups(tile_slots(q, G, kForwardRows), Hk, l.shares)) * sizeof(int));
+  l.total = off;
+  return l;
+}
+
+template <typename T>
+static int run_forward(const sp_attn& c, void* out, int64_t row, int64_t head, float* lse,
+                       char* ws, hipStream_t s) {
+  AttnArgs<T> a = arguments<T>(c);
+  a.out = {static_cast<T*>(out), row, head};
+  a.lse = lse;
+  const ForwardLayout l = forward_layout(c);
+  a.shares = l.shares;
+  a.part = reinterpret_cast<float*>(ws + l.part);
+  a.part_ml = reinterpret_cast<float*>(ws + l.ml);
+  a.again = reinterpret_cast<int*>(ws + l.again);
+  return launch_attend(a, s);
+}
+
+template <typename T>
+static int run_backward(const sp_attn& c, const sp_attn_grad& g, const AttnGradLayout& l, char* ws,
+                        hipStream_t s) {
+  AttnArgs<T> a = arguments<T>(c);
+  a.o = {static_cast<const T*>(g.o), g.o_row, g.o_head};
+  a.dout = {static_cast<const T*>(g.dout), g.dout_row, g.dout_head};
+  a.lse = const_cast<float*>(g.lse);
+  a.dq = {static_cast<T*>(g.dq), g.dq_row, g.dq_head};
+  a.dk = {static_cast<T*>(g.dk), g.dk_row, g.dk_head};
+  a.dv = {static_cast<T*>(g.dv), g.dv_row, g.dv_head};
+  return attn_backward<T>(a, l, ws, g.dq != nullptr && c.nq > 0,
+                          (g.dk != nullptr || g.dv != nullptr) && c.nk > 0, s);
+}
+
+}  // namespace sp
+
+using namespace sp;
+
+extern "C" size_t sp_attention_workspace(const sp_attn* c) {
+  if (check_call("attention", c) != SP_OK || c->nq == 0) return 0;
+  return forward_layout(*c).total;
+}
+
+extern "C" int sp_attention(const sp_attn* c, void* out, int64_t out_row, int64_t out_head,
+                            float* lse, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_call("attention", c)) return rc;
+  if (c->nq == 0) return SP_OK;
+  if (int rc = check_heads("attention", "out", out, out_row, out_head, c->heads, c->dim,
+                           vec_of(c->dtype)))
+    return rc;
+  const size_t need = sp_attention_workspace(c);
+  if (ws_bytes < need)
+    return set_error(SP_ERR_WORKSPACE, "attention: workspace of %zu bytes, needs %zu", ws_bytes,
+                     need);
+  SP_CHECK_ARG(!need || (ws && aligned(ws)), "attention: the workspace must be 16-byte aligned");
+  char* w = static_cast<char*>(ws);
+  const hipStream_t s = as_stream(stream);
+  if (c->dtype == SP_F16)
+    return run_forward<_Float16>(*c, out, out_row, out_head, lse, w, s);
+  if (c->dtype == SP_BF16) return run_forward<__bf16>(*c, out, out_row, out_head, lse, w, s);
+  return run_forward<float>(*c, out, out_row, out_head, lse, w, s);
+}
+
+static AttnGradLayout grad_layout(const sp_attn* c) {
+  return attn_grad_layout(seqs(c->q_offsets, c->nq, c->sequences),
+                          seqs(c->k_offsets, c->nk, c->sequences), int(c->heads),
+                          int(c->kv_heads), int(c->dim), c->causal != 0);
+}
+
+extern "C" size_t sp_attention_bwd_workspace(const sp_attn* c) {
+  if (check_call("attention_bwd", c) != SP_OK || (c->nq == 0 && c->nk == 0)) return 0;
+  return grad_layout(c).total;
+}
+
+extern "C" int sp_attention_bwd(const sp_attn* c, const sp_attn_grad* g, void* ws, size_t ws_bytes,
+                                void* stream) {
+  if (int rc = check_call("attention_bwd", c)) return rc;
+  SP_CHECK_ARG(g, "attention_bwd: null arguments");
+  if (c->nq == 0 && c->nk == 0) return SP_OK;
+  const int V = vec_of(c->dtype);
+  auto check = [&](const char* name, const void* p, int64_t row, int64_t head, int64_t heads) {
+    return check_heads("attention_bwd", name, p, row, head, heads, c->dim, V);
+  };
+  if (c->nq) {
+    if (int rc = check("o", g->o, g->o_row, g->o_head, c->heads)) return rc;
+    if (int rc = check("dout", g->dout, g->dout_row, g->dout_head, c->heads)) return rc;
+    SP_CHECK_ARG(g->lse, "attention_bwd: lse is null");
+  }
+  if (g->dq) {
+    if (int rc = check("dq", g->dq, g->dq_row, g->dq_head, c->heads)) return rc;
+  }
+  if (g->dk) {
+    if (int rc = check("dk", g->dk, g->dk_row, g->dk_head, c->kv_heads)) return rc;
+  }
+  if (g->dv) {
+    if (int rc = check("dv", g->dv, g->dv_row, g->dv_head, c->kv_heads)) return rc;
+  }
+  const AttnGradLayout l = grad_layout(c);
+  if (ws_bytes < l.total)
+    return set_error(SP_ERR_WORKSPACE, "attention_bwd: workspace of %zu bytes, needs %zu",
+                     ws_bytes, l.total);
+  SP_CHECK_ARG(ws && aligned(ws), "attention_bwd: the workspace must be 16-byte aligned");
+  char* w = static_cast<char*>(ws);
+  const hipStream_t s = as_stream(stream);
+  if (c->dtype == SP_F16) return run_backward<_Float16>(*c, *g, l, w, s);
+  if (c->dtype == SP_BF16) return run_backward<__bf16>(*c, *g, l, w, s);
+  return run_backward<float>(*c, *g, l, w, s);
+}

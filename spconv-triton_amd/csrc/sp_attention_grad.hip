@@ -1,0 +1,604 @@
+// Gradients of softmax attention (sp_attention.hip) from that of its result, dO:
+//
+//   P = 2^(c S - lse), delta = sum(dO * O) over a head's values
+//   dV = P' dO, dP = dO V', dS = P * (dP - delta), dQ = scale dS K, dK = scale dS' Q
+//
+// S and P are formed again from q, k and the forward pass's lse, in two kernels: one with a tile of
+// queries a workgroup, which goes through the keys for dQ (S, dP, dQ), and one with a tile of keys, which
+// goes through the queries for dK and dV (S, dP, dV, dK).  That is seven products for the five that one
+// kernel would need, but no sums by atomics: two calls give the same gradients.
+//
+// P and dS are rounded to the rows' type as operands of the products that follow.  In fp16, P of a long
+// row (1 / its keys) and dS would lie below the normal range: P goes in times 2^15 (it is at most 1), and dS times the
+// power of two that the bound |dS| <= 2 |dO| max|v| (lengths of rows) leaves: for dQ from the
+// query's own |dO|, for dK, whose sums are over queries, from the largest.
+#include "sp_attention.h"
+
+namespace sp {
+
+constexpr int kTops = 256;  // workgroups of attend_grad_rows at most
+
+// Waves a SIMD.
+template <typename T>
+constexpr int grad_waves(int DP) {
+  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 3 : DP <= 64 ? 2 : 1;
+}
+
+template <typename T>
+constexpr float kLift = sizeof(T) == 2 && std::is_same<T, _Float16>::value ? 15.f : 0.f;
+
+__device__ const float g_no_row[2] = {-__builtin_inff(), 0.f};  // of a row past the end: P = 0
+
+// What both kernels need of each query and head: nl = lift - lse and nd = -delta, [H][rows].  In fp16 also
+// the largest squares of |dO| and |v| over the rows of the sequences, one pair a workgroup (those that
+// are not finite do not count: their rows' gradients are not finite either).
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attend_grad_rows(AttnArgs<T> a, int log_lanes,
+                                                                 float* __restrict__ nl,
+                                                                 float* __restrict__ nd,
+                                                                 float* __restrict__ tops) {
+  constexpr int V = Mfma<T>::V;
+  using frag = typename Mfma<T>::frag;
+  const int lanes = 1 << log_lanes, lane = int(threadIdx.x) & (lanes - 1);
+  const int per = kAttnThreads >> log_lanes;
+  const int64_t stride = int64_t(gridDim.x) * per;
+  const int64_t start = int64_t(blockIdx.x) * per + (int(threadIdx.x) >> log_lanes);
+  float top[2] = {0.f, 0.f};
+  auto sum = [&](float v) {
+    for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+  };
+  const int64_t n = a.qs.rows * a.H;
+  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < n; b += stride) {
+    const int64_t at = b + (int(threadIdx.x) >> log_lanes), r = at / a.H;
+    const int h = int(at - r * a.H);
+    float dot = 0.f, sq = 0.f;
+    if (at < n)
+      for (int c = lane * V; c < a.D; c += lanes * V) {
+        const frag x = *reinterpret_cast<const frag*>(a.dout.p + r * a.dout.row + h * a.dout.head + c);
+        const frag y = *reinterpret_cast<const frag*>(a.o.p + r * a.o.row + h * a.o.head + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          dot = __builtin_fmaf(to_f32(x[i]), to_f32(y[i]), dot);
+          sq = __builtin_fmaf(to_f32(x[i]), to_f32(x[i]), sq);
+        }
+      }
+    dot = sum(dot);
+    if (kLift<T> != 0.f) {
+      sq = sum(sq);
+      const bool in = !a.qs.off || (r >= a.qs.bound(1) && r < a.qs.bound(a.qs.parts - 1));
+      if (at < n && in && sq < __builtin_inff()) top[0] = __builtin_fmaxf(top[0], sq);
+    }
+    if (at < n && lane == 0) {
+      nl[h * a.qs.rows + r] = kLift<T> - a.lse[h * a.qs.rows + r];
+      nd[h * a.qs.rows + r] = -dot;
+    }
+  }
+  if (kLift<T> == 0.f) return;
+  const int64_t nv = a.ks.rows * a.Hk;
+  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < nv; b += stride) {
+    const int64_t at = b + (int(threadIdx.x) >> log_lanes), r = at / a.Hk;
+    const int h = int(at - r * a.Hk);
+    float sq = 0.f;
+    if (at < nv)
+      for (int c = lane * V; c < a.D; c += lanes * V) {
+        const frag x = *reinterpret_cast<const frag*>(a.v.p + r * a.v.row + h * a.v.head + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq = __builtin_fmaf(to_f32(x[i]), to_f32(x[i]), sq);
+      }
+    sq = sum(sq);
+    const bool in = !a.ks.off || (r >= a.ks.bound(1) && r < a.ks.bound(a.ks.parts - 1));
+    if (at < nv && in && sq < __builtin_inff()) top[1] = __builtin_fmaxf(top[1], sq);
+  }
+  __shared__ float lds[2][kAttnWaves];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+      top[j] = __builtin_fmaxf(top[j], __shfl_xor(top[j], off, 64));
+    if ((threadIdx.x & 63) == 0) lds[j][wave_of()] = top[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) v = __builtin_fmaxf(v, lds[threadIdx.x][w]);
+    tops[2 * blockIdx.x + threadIdx.x] = v;
+  }
+}
+
+// The largest of the workgroups' pairs, on every lane of the wave.
+__device__ __forceinline__ void read_tops(const float* tops, int n, float& grad, float& value) {
+  grad = value = 0.f;
+  for (int i = int(threadIdx.x) & 63; i < n; i += 64) {
+    grad = __builtin_fmaxf(grad, tops[2 * i]);
+    value = __builtin_fmaxf(value, tops[2 * i + 1]);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    grad = __builtin_fmaxf(grad, __shfl_xor(grad, off, 64));
+    value = __builtin_fmaxf(value, __shfl_xor(value, off, 64));
+  }
+}
+
+// The exponent e with 2 |dO| |v| 2^e <= 2^15, from the squares of the lengths.
+__device__ __forceinline__ float lift_of(float grad_sq, float value_sq) {
+  const float e = __builtin_floorf(
+      14.f - 0.5f * (__builtin_amdgcn_logf(grad_sq) + __builtin_amdgcn_logf(value_sq)));
+  return e > -100.f ? (e < 100.f ? e : 100.f) : 0.f;  // (a length of 0 makes e infinite)
+}
+
+template <typename T, int DP, int QT, int BK, bool CAUSAL, bool STRICT>
+__global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dq(
+    AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
+  using frag = typename Mfma<T>::frag;
+  using L = HeadTile<T, DP, BK>;
+  constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
+  constexpr int BQ = kAttnWaves * QT * 32;
+  __shared__ __attribute__((aligned(16))) char lds[4 * L::BYTES];
+  __shared__ int bad_lds;
+  Place place;
+  if (!find_place(slots, a.Hk, a.shares, blockIdx.x, place)) return;
+  if (skips<CAUSAL, STRICT>(a.again)) return;
+  if (CAUSAL) place.slot = slots - 1 - place.slot;
+  const Tile t = find_tile(a.qs, a.G, BQ, place.slot);
+  if (t.at >= t.len) {
+    if (CAUSAL && !STRICT && threadIdx.x == 0) a.again[blockIdx.x] = 0;
+    return;
+  }
+  const int64_t klo = a.ks.bound(t.part);
+  const int Lk = keys_of(a.qs, a.ks, t.part, klo), Lq = int(t.len / a.G);
+  const int wave = wave_of(), lane = int(threadIdx.x) & 31;
+  float top_grad = 0.f, top_value = 0.f;
+  if (kLift<T> != 0.f) read_tops(a.top, a.tops, top_grad, top_value);
+
+  frag q[QT][STEPS], g[QT][STEPS];
+  int row[QT], seen[QT], head[QT];
+  float base[QT], minus[QT], lift[QT];
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    const int64_t r = t.at + (wave * QT + u) * 32 + lane;
+    const bool live = r < t.len;
+    const int i = int(r / a.G);
+    head[u] = place.head * a.G + int(r - int64_t(i) * a.G);
+    row[u] = live ? i : -1;
+    seen[u] = CAUSAL ? keys_seen(i, Lq, Lk) : Lk;
+    const int64_t at = t.lo + i;
+    load_head<T, DP>(a.q.p + at * a.q.row + head[u] * a.q.head, live, a.D, q[u]);
+    load_head<T, DP>(a.dout.p + at * a.dout.row + head[u] * a.dout.head, live, a.D, g[u]);
+    base[u] = live ? nl[head[u] * a.qs.rows + at] : -__builtin_inff();
+    minus[u] = live ? nd[head[u] * a.qs.rows + at] : 0.f;
+    lift[u] = 0.f;
+    if (kLift<T> != 0.f) {
+      float sq = 0.f;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float v = to_f32(g[u][s][j]);
+          sq = __builtin_fmaf(v, v, sq);
+        }
+      lift[u] = lift_of(sq + other_half(sq), top_value);
+      base[u] += lift[u] - kLift<T>;
+    }
+  }
+  int most = Lk, wave_most = Lk, wave_least = Lk;
+  if (CAUSAL) {
+    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * QT * 32;
+    most = keys_seen((last - 1) / a.G, Lq, Lk);
+    wave_least = keys_seen(w / a.G, Lq, Lk);
+    wave_most = keys_seen((w + QT * 32 - 1) / a.G, Lq, Lk);
+    wave_most = wave_most < most ? wave_most : most;
+  }
+  const int tiles = (most + BK - 1) / BK, per = (tiles + a.shares - 1) / a.shares;
+  const int first = place.share * per, end = first + per < tiles ? first + per : tiles;
+  const TileLoads<T, DP, BK> lk(a.k.p + klo * a.k.row + place.head * a.k.head, a.k.row, Lk, a.D);
+  const TileLoads<T, DP, BK> lv(a.v.p + klo * a.v.row + place.head * a.v.head, a.v.row, Lk, a.D);
+  const float c = a.scale2;
+  if (DP != a.D) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
+  }
+  floatx16 acc[QT][DP / 32];
+#pragma unroll
+  for (int u = 0; u < QT; ++u)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) zero(acc[u][d]);
+  if (first < end) {
+    lk.start(first * BK, lds);
+    lv.start(first * BK, lds + L::BYTES);
+  }
+  for (int n = first; n < end; ++n) {
+    char* buf = lds + ((n - first) & 1) * 2 * L::BYTES;
+    loads_in_flight<0>();
+    __syncthreads();
+    if (n + 1 < end) {
+      char* next = lds + ((n + 1 - first) & 1) * 2 * L::BYTES;
+      lk.start((n + 1) * BK, next);
+      lv.start((n + 1) * BK, next + L::BYTES);
+    }
+    const int key0 = n * BK;
+    if (CAUSAL && key0 >= wave_most) continue;
+    const bool edge = key0 + BK > wave_least;
+#pragma unroll
+    for (int x = 0; x < BK / 32; ++x) {
+      floatx16 s[QT], dp[QT];
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        zero(s[u]);
+        zero(dp[u]);
+      }
+      auto read = [&](int k) {
+        return Both<T>{L::read(buf, 32 * x, k), L::read(buf + L::BYTES, 32 * x, k)};
+      };
+      Batched<Both<T>, STEPS, 1> f;
+      f.start(read);
+      f.run(read, [&](int k, const Both<T>& kv) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+          Mfma<T>::mma(kv.a, q[u][k], s[u]);
+          Mfma<T>::mma(kv.b, g[u][k], dp[u]);
+        }
+      });
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        frag ds[PS];
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (key0 + 32 * x + acc_row<T>(i) >= seen[u]) {
+              s[u][i] = -__builtin_inff();
+              dp[u][i] = 0.f;  // (not what a NaN there makes of it)
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, base[u]));
+          ds[i / V][i % V] = T(p * (dp[u][i] + minus[u]));
+        }
+        if (STRICT && edge)
+          add_rows_seen<T, DP, BK>(buf, 32 * x, 0, seen[u] - key0, ds, acc[u]);
+        else
+          add_rows<T, DP, BK, kAttnBatch>(buf, 32 * x, ds, acc[u]);
+      }
+    }
+  }
+  bool bad = false;
+  if (CAUSAL && !STRICT) {
+#pragma unroll
+    for (int u = 0; u < QT; ++u) bad |= any_not_finite(acc[u]);
+  }
+  report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    if (row[u] < 0) continue;
+    const int64_t r = t.lo + row[u];
+    const float f = a.scale * __builtin_amdgcn_exp2f(-lift[u]);
+    if (a.shares > 1) {
+      const int64_t at = (place.share * a.qs.rows + r) * a.H + head[u];
+      store_part<DP, V>(a.part + at * a.D, a.D, [&](int d, int i) { return acc[u][d][i] * f; });
+    } else {
+      store_head<T, DP>(a.dq.p + r * a.dq.row + head[u] * a.dq.head, a.D,
+                        [&](int d, int i) { return acc[u][d][i] * f; });
+    }
+  }
+}
+
+// A tile of keys goes through the queries of its head's G query heads, one head after the other.
+template <typename T, int DP, int KT, int BQ, bool CAUSAL, bool STRICT>
+__global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
+    AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
+  using frag = typename Mfma<T>::frag;
+  using L = HeadTile<T, DP, BQ>;
+  constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
+  constexpr int BK = kAttnWaves * KT * 32, STAGE = 2 * L::BYTES + 2 * BQ * 4;
+  static_assert(BQ <= 64, "a wave loads a tile's statistics at once");
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  __shared__ int bad_lds;
+  Place place;
+  if (!find_place(slots, a.Hk, a.shares, blockIdx.x, place)) return;
+  if (skips<CAUSAL, STRICT>(a.again)) return;
+  const Tile t = find_tile(a.ks, 1, BK, place.slot);
+  if (t.at >= t.len) {
+    if (CAUSAL && !STRICT && threadIdx.x == 0) a.again[blockIdx.x] = 0;
+    return;
+  }
+  const int64_t qlo = a.qs.bound(t.part);
+  const int Lk = int(t.len), Lq = keys_of(a.ks, a.qs, t.part, qlo);
+  const int wave = wave_of(), lane = int(threadIdx.x) & 31, lane64 = int(threadIdx.x) & 63;
+  float g = 1.f, lift = 0.f;
+  if (kLift<T> != 0.f) {
+    float top_grad, top_value;
+    read_tops(a.top, a.tops, top_grad, top_value);
+    lift = lift_of(top_grad, top_value);
+    g = __builtin_amdgcn_exp2f(lift - kLift<T>);
+  }
+
+  frag k[KT][STEPS], v[KT][STEPS];
+  int row[KT], from[KT];  // the key's place in its sequence; its first query
+#pragma unroll
+  for (int u = 0; u < KT; ++u) {
+    const int j = int(t.at) + (wave * KT + u) * 32 + lane;
+    row[u] = j < Lk ? j : -1;
+    from[u] = CAUSAL && j > Lk - Lq ? j - Lk + Lq : 0;
+    const int64_t at = t.lo + j;
+    load_head<T, DP>(a.k.p + at * a.k.row + place.head * a.k.head, j < Lk, a.D, k[u]);
+    load_head<T, DP>(a.v.p + at * a.v.row + place.head * a.v.head, j < Lk, a.D, v[u]);
+  }
+  // first queries: of the workgroup's keys, of the wave's, of its last key
+  int least = 0, wave_least = 0, wave_most = 0;
+  if (CAUSAL) {
+    const int shift = Lq - Lk, j = int(t.at) + wave * KT * 32;
+    least = t.at + shift > 0 ? int(t.at) + shift : 0;
+    wave_least = j + shift > 0 ? j + shift : 0;
+    wave_most = j + KT * 32 - 1 + shift > 0 ? j + KT * 32 - 1 + shift : 0;
+  }
+  const int begin = least / BQ, last = (Lq + BQ - 1) / BQ;  // tiles of a head
+  const int64_t tiles = last > begin ? int64_t(last - begin) * a.G : 0;
+  const int64_t per = (tiles + a.shares - 1) / a.shares;
+  int64_t n = place.share * per;
+  const int64_t end = n + per < tiles ? n + per : tiles;
+  int qh = 0, qt = begin;  // the tile's head and place
+  if (n < end) {
+    qh = int(n / (last - begin));
+    qt = begin + int(n - int64_t(qh) * (last - begin));
+  }
+  const int64_t h0 = int64_t(place.head) * a.G;
+  TileLoads<T, DP, BQ> lq(a.q.p + qlo * a.q.row, a.q.row, Lq, a.D);
+  TileLoads<T, DP, BQ> lg(a.dout.p + qlo * a.dout.row, a.dout.row, Lq, a.D);
+  const T *q0 = lq.p, *g0 = lg.p;
+  auto start = [&](int head, int tile, char* to) {
+    lq.p = q0 + (h0 + head) * a.q.head;
+    lg.p = g0 + (h0 + head) * a.dout.head;
+    lq.start(tile * BQ, to);
+    lg.start(tile * BQ, to + L::BYTES);
+    if (wave < 2 && lane64 < BQ) {
+      const int r = tile * BQ + lane64;
+      const float* from_ =
+          r < Lq ? (wave ? nd : nl) + (h0 + head) * a.qs.rows + qlo + r : &g_no_row[wave];
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)from_,
+          (__attribute__((address_space(3))) void*)(to + 2 * L::BYTES + wave * (BQ * 4)), 4, 0, 0);
+    }
+  };
+  const float c = a.scale2;
+  if (DP != a.D) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lq.clear(lds + (i >> 1) * STAGE + (i & 1) * L::BYTES);
+  }
+  floatx16 dk[KT][DP / 32], dv[KT][DP / 32];
+#pragma unroll
+  for (int u = 0; u < KT; ++u)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+      zero(dk[u][d]);
+      zero(dv[u][d]);
+    }
+  if (n < end) start(qh, qt, lds);
+  for (int stage = 0; n < end; ++n, stage ^= 1) {
+    char* buf = lds + stage * STAGE;
+    loads_in_flight<0>();
+    __syncthreads();
+    const int query0 = qt * BQ;
+    if (++qt == last) {
+      qt = begin;
+      ++qh;
+    }
+    if (n + 1 < end) start(qh, qt, lds + (stage ^ 1) * STAGE);
+    if (CAUSAL && query0 + BQ <= wave_least) continue;
+    const bool edge = CAUSAL && query0 < wave_most;
+    const float* stats = reinterpret_cast<const float*>(buf + 2 * L::BYTES);
+#pragma unroll
+    for (int x = 0; x < BQ / 32; ++x) {
+      floatx16 s[KT], dp[KT];
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        zero(s[u]);
+        zero(dp[u]);
+      }
+      auto read = [&](int i) {
+        return Both<T>{L::read(buf, 32 * x, i), L::read(buf + L::BYTES, 32 * x, i)};
+      };
+      Batched<Both<T>, STEPS, 1> f;
+      f.start(read);
+      f.run(read, [&](int i, const Both<T>& qg) {
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          Mfma<T>::mma(qg.a, k[u][i], s[u]);
+          Mfma<T>::mma(qg.b, v[u][i], dp[u]);
+        }
+      });
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        frag p[PS], ds[PS];
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (query0 + 32 * x + acc_row<T>(i) < from[u]) {
+              s[u][i] = -__builtin_inff();
+              dp[u][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int r = 32 * x + acc_row<T>(i);
+          const float4v base = *reinterpret_cast<const float4v*>(stats + r);
+          const float4v minus = *reinterpret_cast<const float4v*>(stats + BQ + r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + j], c, base[j]));
+            float d = dp[u][i + j] + minus[j];
+            if (kLift<T> != 0.f) d *= g;
+            p[(i + j) / V][(i + j) % V] = T(e);
+            ds[(i + j) / V][(i + j) % V] = T(e * d);
+          }
+        }
+        if (STRICT && edge) {
+          add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from[u] - query0, BQ, p, dv[u]);
+          add_rows_seen<T, DP, BQ>(buf, 32 * x, from[u] - query0, BQ, ds, dk[u]);
+        } else {
+          add_rows<T, DP, BQ, kAttnBatch>(buf + L::BYTES, 32 * x, p, dv[u]);
+          add_rows<T, DP, BQ, kAttnBatch>(buf, 32 * x, ds, dk[u]);
+        }
+      }
+    }
+  }
+  bool bad = false;
+  if (CAUSAL && !STRICT) {
+#pragma unroll
+    for (int u = 0; u < KT; ++u) bad |= any_not_finite(dk[u]) || any_not_finite(dv[u]);
+  }
+  report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+  const float fk = a.scale * __builtin_amdgcn_exp2f(-lift), fv = __builtin_amdgcn_exp2f(-kLift<T>);
+#pragma unroll
+  for (int u = 0; u < KT; ++u) {
+    if (row[u] < 0) continue;
+    const int64_t r = t.lo + row[u];
+    if (a.shares > 1) {
+      float* to = a.part + (((place.share * 2) * a.ks.rows + r) * a.Hk + place.head) * a.D;
+      store_part<DP, V>(to, a.D, [&](int d, int i) { return dk[u][d][i] * fk; });
+      store_part<DP, V>(to + a.ks.rows * a.Hk * a.D, a.D,
+                        [&](int d, int i) { return dv[u][d][i] * fv; });
+      continue;
+    }
+    if (a.dk.p)
+      store_head<T, DP>(a.dk.p + r * a.dk.row + place.head * a.dk.head, a.D,
+                        [&](int d, int i) { return dk[u][d][i] * fk; });
+    if (a.dv.p)
+      store_head<T, DP>(a.dv.p + r * a.dv.row + place.head * a.dv.head, a.D,
+                        [&](int d, int i) { return dv[u][d][i] * fv; });
+  }
+}
+
+// out[r][h] = the sum of the shares' partials, which lie `stride` values apart, in their order.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attend_sum(const float* __restrict__ part,
+                                                           int64_t stride, int shares,
+                                                           int64_t rows, int heads, int D,
+                                                           Heads<T> out) {
+  const int quads = D / 4;
+  const int64_t n = rows * heads * quads;
+  for (int64_t i = int64_t(blockIdx.x) * kAttnThreads + threadIdx.x; i < n;
+       i += int64_t(gridDim.x) * kAttnThreads) {
+    const int64_t at = i / quads, r = at / heads;
+    const int c = int(i - at * quads) * 4, h = int(at - r * heads);
+    float4v v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < shares; ++s)
+      v += *reinterpret_cast<const float4v*>(part + s * stride + at * D + c);
+    T* to = out.p + r * out.row + h * out.head + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = from_f32<T>(v[j]);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+constexpr int kGradTiles = 1;  // tiles of 32 of its own axis a wave
+constexpr int kGradRows = kAttnWaves * kGradTiles * 32;
+
+AttnGradLayout attn_grad_layout(const Seqs& q, const Seqs& k, int H, int Hk, int D,
+                                bool causal) {
+  AttnGradLayout l{};
+  l.dq_shares = attn_shares(attn_tiles(q, H / Hk, Hk, kGradRows), attn_length(k));
+  l.dkv_shares = attn_shares(attn_tiles(k, 1, Hk, kGradRows), attn_length(q) * (H / Hk));
+  size_t off = 0;
+  auto take = [&](size_t floats) {
+    const size_t at = off;
+    off = align_up(off + floats * sizeof(float), 256);
+    return at;
+  };
+  l.nl = take(size_t(q.rows) * H);
+  l.nd = take(size_t(q.rows) * H);
+  l.tops = take(2 * kTops);
+  // (one after the other)
+  const size_t dq = l.dq_shares > 1 ? size_t(l.dq_shares) * q.rows * H * D : 0;
+  const size_t dkv = l.dkv_shares > 1 ? size_t(l.dkv_shares) * 2 * k.rows * Hk * D : 0;
+  l.part = take(dq > dkv ? dq : dkv);
+  if (causal) {
+    const int64_t gq = attn_groups(tile_slots(q, H / Hk, kGradRows), Hk, l.dq_shares);
+    const int64_t gk = attn_groups(tile_slots(k, 1, kGradRows), Hk, l.dkv_shares);
+    l.again = take(size_t(gq > gk ? gq : gk));
+  }
+  l.total = off;
+  return l;
+}
+
+template <typename T>
+int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq, bool need_dkv,
+                  hipStream_t s) {
+  float* nl = reinterpret_cast<float*>(ws + l.nl);
+  float* nd = reinterpret_cast<float*>(ws + l.nd);
+  float* tops = reinterpret_cast<float*>(ws + l.tops);
+  a.part = reinterpret_cast<float*>(ws + l.part);
+  a.again = reinterpret_cast<int*>(ws + l.again);
+  a.top = tops;
+  if (!need_dq && !need_dkv) return SP_OK;
+  int lanes = 0;
+  while ((Mfma<T>::V << lanes) < a.D) ++lanes;
+  const int64_t most = a.qs.rows * a.H > a.ks.rows * a.Hk ? a.qs.rows * a.H : a.ks.rows * a.Hk;
+  const int64_t rows = cdiv(most, kAttnThreads >> lanes);
+  a.tops = int(rows < kTops ? rows : kTops);
+  attend_grad_rows<T><<<unsigned(a.tops), kAttnThreads, 0, s>>>(a, lanes, nl, nd, tops);
+  SP_LAUNCHED();
+  auto sum = [&](const float* part, int64_t stride, int shares, int64_t n, int heads,
+                 const Heads<T>& out) {
+    if (!out.p) return;
+    const int64_t groups = cdiv(n * heads * (a.D / 4), kAttnThreads);
+    attend_sum<T><<<unsigned(groups < 4096 ? groups : 4096), kAttnThreads, 0, s>>>(
+        part, stride, shares, n, heads, a.D, out);
+  };
+  if (need_dq) {
+    const int64_t slots = tile_slots(a.qs, a.G, kGradRows);
+    a.shares = l.dq_shares;
+    const int64_t groups = attn_groups(slots, a.Hk, a.shares);
+    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
+    with_width(a.D, [&](auto w) {
+      constexpr int DP = w.value, N = kGradTiles, B = attn_stage<T>();
+      const dim3 grid{unsigned(groups)}, block{kAttnThreads};
+      if (!a.causal) {
+        attend_dq<T, DP, N, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+      } else {
+        attend_dq<T, DP, N, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dq<T, DP, N, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
+      }
+      return 0;
+    });
+    SP_LAUNCHED();
+    if (a.shares > 1)
+      sum(a.part, a.qs.rows * a.H * a.D, a.shares, a.qs.rows, a.H, a.dq);
+    SP_LAUNCHED();
+  }
+  if (need_dkv) {
+    const int64_t slots = tile_slots(a.ks, 1, kGradRows);
+    a.shares = l.dkv_shares;
+    const int64_t groups = attn_groups(slots, a.Hk, a.shares);
+    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
+    with_width(a.D, [&](auto w) {
+      constexpr int DP = w.value, N = kGradTiles, B = attn_stage<T>();
+      const dim3 grid{unsigned(groups)}, block{kAttnThreads};
+      if (!a.causal) {
+        attend_dkv<T, DP, N, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+      } else {
+        attend_dkv<T, DP, N, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dkv<T, DP, N, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
+      }
+      return 0;
+    });
+    SP_LAUNCHED();
+    if (a.shares > 1) {
+      const int64_t one = a.ks.rows * a.Hk * a.D;
+      sum(a.part, 2 * one, a.shares, a.ks.rows, a.Hk, a.dk);
+      sum(a.part + one, 2 * one, a.shares, a.ks.rows, a.Hk, a.dv);
+    }
+    SP_LAUNCHED();
+  }
+  return SP_OK;
+}
+
+template int attn_backward<_Float16>(AttnArgs<_Float16>, const AttnGradLayout&, char*, bool, bool,
+                                     hipStream_t);
+template int attn_backward<__bf16>(AttnArgs<__bf16>, const AttnGradLayout&, char*, bool, bool,
+                                   hipStream_t);
+template int attn_backward<float>(AttnArgs<float>, const AttnGradLayout&, char*, bool, bool,
+                                  hipStream_t);
+
+}  // namespace sp

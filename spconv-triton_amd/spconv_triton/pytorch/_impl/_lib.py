@@ -149,6 +149,10 @@ _SIGNATURES = {
     "sp_gated_ffn_bwd_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I32]),
     "sp_gated_ffn_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _I32, _I64, _I64, _P, _P, _I64,
                                         _P, _I64, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "sp_attention_workspace": (_SZ, [_P]),
+    "sp_attention": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P, _SZ, _P]),
+    "sp_attention_bwd_workspace": (_SZ, [_P]),
+    "sp_attention_bwd": (ctypes.c_int, [_P, _P, _P, _SZ, _P]),
     "sp_maxpool_fwd": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P]),
     "sp_maxpool_bwd": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P]),
     "sp_avgpool_fwd": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I64, _I64, _P, _P, _P]),
@@ -252,6 +256,14 @@ def stream_of(device: torch.device):
     if _raw_stream is None or device.index is None:
         return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
     return ctypes.c_void_p(_raw_stream(device.index))
+
+
+def launch(device: torch.device, fn, *args) -> int:
+    """``fn(*args)`` with ``device`` as the current one: a kernel starts on its stream's device."""
+    if device.type != "cuda" or torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from spconv_triton.compat import tv
 from spconv_triton.pytorch import ops
+from spconv_triton.pytorch._impl import attention as _attention
 from spconv_triton.pytorch._impl import rows as _rows
 from spconv_triton.pytorch._impl.rows import Int8Rows
 from spconv_triton.pytorch.hash import HashTable
@@ -380,6 +381,90 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         return ops.gated_ffn(x, w_gate, w_up, w_down, act, residual)
     return GatedFFNFunction.apply(x, w_gate, w_up, w_down, act, residual, saved is not None, codes,
                                   scales)
+
+
+# ---------------------------------------------------------------------------
+# the attention half of a block
+# ---------------------------------------------------------------------------
+
+class AttentionFunction(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, key_offsets, causal, scale):
+        q, k, v = _as_autocast_takes(q, k, v)
+        need = any(ctx.needs_input_grad[:3])
+        out, lse = ops.attention(q, k, v, offsets, key_offsets, causal, scale, need)
+        if need:
+            ctx.save_for_backward(q, k, v, out, lse, offsets, key_offsets)
+            ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, offsets, key_offsets = ctx.saved_tensors
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
+                 for t, need in zip((q, k, v), ctx.needs_input_grad)]
+        return (*_attention.run_attention_backward(dout, q, k, v, out, lse, offsets, key_offsets,
+                                                   ctx.causal, ctx.scale, grads), *(None,) * 4)
+
+
+class PackedAttentionFunction(Function):
+    @staticmethod
+    def forward(ctx, qkv, heads, kv_heads, offsets, causal, scale):
+        qkv, = _as_autocast_takes(qkv)
+        need = ctx.needs_input_grad[0]
+        out, lse = ops.attention(*_attention.split_packed(qkv, heads, kv_heads), offsets, None,
+                                 causal, scale, need)
+        if need:
+            ctx.save_for_backward(qkv, out, lse, offsets)
+            ctx.call = heads, kv_heads, causal, scale
+        return out.flatten(1)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lse, offsets = ctx.saved_tensors
+        heads, kv_heads, causal, scale = ctx.call
+        grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _attention.run_attention_backward(
+            dout.unflatten(1, (heads, -1)), *_attention.split_packed(qkv, heads, kv_heads), out,
+            lse, offsets, None, causal, scale, _attention.split_packed(grad, heads, kv_heads))
+        return grad, None, None, None, None, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+              offsets: torch.Tensor | None = None, key_offsets: torch.Tensor | None = None,
+              causal: bool = False, scale: float | None = None):
+    """Softmax attention between feature rows, ``softmax(scale * q k') v`` for each head.
+
+    ``q`` is ``[rows, heads, dim]``, ``k`` and ``v`` ``[key rows, kv_heads, dim]``, with dim up to 128;
+    key head h serves the ``heads / kv_heads`` query heads from ``h * heads / kv_heads`` on.  ``offsets``
+    (int32, ``[sequences + 1]``, ascending, on the rows' device) say where each sequence of rows begins
+    and ends: queries see the keys of their own sequence, whose rows ``key_offsets`` give
+    (default: the same).  Without them all rows are one sequence.  With ``causal`` the last query of a
+    sequence sees all of its keys, the one before it all but the last, and so on.  ``scale`` is
+    ``dim ** -0.5`` by default.
+
+    A query that sees no key, or lies outside all sequences, gets zeros and passes no gradient.
+    Sums and the softmax's statistics are float32; its weights are rounded to the rows' type.
+    Offsets are not checked (they are on the device); ones that descend give rows without meaning.
+    Under autocast q, k and v are taken in autocast's type.
+    """
+    if _inference():
+        return ops.attention(q, k, v, offsets, key_offsets, causal, scale, False)[0]
+    return AttentionFunction.apply(q, k, v, offsets, key_offsets, causal, scale)
+
+
+def packed_attention(qkv: torch.Tensor, heads: int, kv_heads: int | None = None,
+                     offsets: torch.Tensor | None = None, causal: bool = False,
+                     scale: float | None = None):
+    """``attention`` of rows with themselves, queries, keys and values in rows ``[q | k | v]`` of ``heads``,
+    ``kv_heads`` (default: as many) and ``kv_heads`` heads, as one projection makes them.  Returns
+    ``[rows, heads * dim]``."""
+    if _inference():
+        return ops.attention(*_attention.split_packed(qkv, heads, kv_heads), offsets, None, causal,
+                             scale, False)[0].flatten(1)
+    return PackedAttentionFunction.apply(qkv, heads, kv_heads, offsets, causal, scale)
 
 
 _MAX_INT32 = 2 ** 31 - 1

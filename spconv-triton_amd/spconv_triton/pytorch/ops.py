@@ -27,6 +27,7 @@ from spconv_triton.core import AlgoHint, ConvAlgo  # noqa: F401
 from spconv_triton.pytorch._impl import gemm as _gemm
 from spconv_triton.pytorch._impl import pairs as _pairs
 from spconv_triton.pytorch._impl import pool as _pool
+from spconv_triton.pytorch._impl.attention import attention, attention_backward
 from spconv_triton.pytorch._impl.pairs import get_conv_output_size, get_deconv_output_size
 from spconv_triton.pytorch._impl.rows import (
     Int8Rows,
@@ -49,6 +50,8 @@ DEBUG_INT64_HASH_K = False
 __all__ = [
     "ConvAlgo",
     "Int8Rows",
+    "attention",
+    "attention_backward",
     "gated_ffn",
     "gated_ffn_backward",
     "get_conv_output_size",

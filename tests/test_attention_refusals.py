@@ -1,0 +1,106 @@
+"""Attention on the host: calls that are refused before any launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def no_gpu_needed(monkeypatch):
+    from spconv_triton.pytorch._impl import _lib
+
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+
+
+def test_cpu_tensors_are_refused():
+    from spconv_triton.pytorch import functional as Fsp
+
+    x = torch.zeros(4, 2, 8)
+    for call in (lambda: Fsp.attention(x, x, x), lambda: Fsp.packed_attention(torch.zeros(4, 24), 1)):
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), pytest.raises(AssertionError):
+                call()
+
+
+def test_arguments_that_do_not_fit(no_gpu_needed):
+    from spconv_triton.pytorch import functional as Fsp
+    from spconv_triton.pytorch import ops
+
+    x, off = torch.zeros(6, 4, 8), torch.tensor([0, 6], dtype=torch.int32)
+    bad = [
+        (ValueError, (x[0], x, x)), (ValueError, (x, x, x[:5])), (ValueError, (x, x[..., :4], x[..., :4])),
+        (ValueError, (x, x[:, :3], x[:, :3])), (ValueError, (x, x.half(), x)),
+        (NotImplementedError, (x.double(),) * 3), (NotImplementedError, (torch.zeros(2, 1, 129),) * 3),
+        (ValueError, (x[:, :0], x[:, :0], x[:, :0])), (ValueError, (x, x, x, off.long())),
+        (ValueError, (x, x, x, off[None])), (ValueError, (x, x, x, off[:0])),
+        (ValueError, (x, x, x, None, off)), (ValueError, (x, x, x, off, off[:1])),
+        (ValueError, (x, x[:3], x[:3], off)), (ValueError, (x, x, x, [0, 6])),
+    ]
+    for kind, args in bad:
+        for call in (Fsp.attention, ops.attention):
+            with pytest.raises(kind):
+                call(*args)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            Fsp.attention(x, x, x, scale=scale)
+    lse = torch.zeros(4, 6)
+    for args in ((x[:5], x, x, x, x, lse), (x, x, x, x, x.half(), lse), (x, x, x, x, x, lse.t())):
+        with pytest.raises(ValueError):
+            ops.attention_backward(*args)
+    qkv = torch.zeros(4, 24)
+    for args in ((qkv, 5), (qkv, 0), (qkv, 1, -1), (qkv[0], 1), (qkv[:, :0], 1), (qkv, 2, 3)):
+        with pytest.raises(ValueError):
+            Fsp.packed_attention(*args)
+
+
+def test_bad_sizes_and_workspaces_are_refused():
+    """By the C entry points, before the pointers are used (they are not device memory here)."""
+    from spconv_triton.pytorch._impl import _lib
+    from spconv_triton.pytorch._impl.attention import _Call, _Grad
+
+    L = _lib.load_library()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+
+    def call(**kw):
+        c = _Call(p, p, p, 64, 32, 64, 32, 64, 32, 1, 5000, 2, 2, 32, 0, None, None, 0.1, 0, 0)
+        for k, val in kw.items():
+            setattr(c, k, val)
+        return c
+
+    def forward(c, ws=p, nbytes=1 << 30, out=p):
+        return L.sp_attention(ctypes.byref(c), out, 64, 32, None, ws, nbytes, None)
+
+    bad = [dict(dtype=3), dict(dtype=-1), dict(heads=3), dict(kv_heads=0), dict(dim=12), dict(dim=0),
+           dict(nq=-1), dict(nk=1 << 31), dict(scale=0.0), dict(scale=float("nan")),
+           dict(scale=float("inf")), dict(q=None), dict(v=None), dict(k=p + 2), dict(q_row=63),
+           dict(k_head=16), dict(v_row=1 << 23), dict(q_row=-64), dict(q_offsets=p),
+           dict(q_offsets=p, k_offsets=p, sequences=-1)]
+    for kw in bad:
+        assert forward(call(**kw)) == _lib.SP_ERR_INVALID_ARG, kw
+    assert forward(call(dim=136, q_row=272, q_head=136, k_row=272, k_head=136, v_row=272,
+                        v_head=136)) == _lib.SP_ERR_UNSUPPORTED
+    c = call()
+    need = L.sp_attention_workspace(ctypes.byref(c))
+    assert need > 0 and forward(c, nbytes=need - 1) == _lib.SP_ERR_WORKSPACE
+    assert forward(c, ws=None) == forward(c, ws=p + 2) == _lib.SP_ERR_INVALID_ARG
+    assert forward(c, out=None) == forward(c, out=p + 2) == _lib.SP_ERR_INVALID_ARG
+    assert forward(call(nq=0)) == _lib.SP_OK
+    assert L.sp_attention_workspace(None) == 0
+    assert L.sp_attention(None, p, 64, 32, None, p, 1 << 30, None) == _lib.SP_ERR_INVALID_ARG
+
+    need = L.sp_attention_bwd_workspace(ctypes.byref(c))
+
+    def backward(c, ws=p, nbytes=1 << 30, **kw):
+        g = _Grad(p, p, p, p, p, p, *(64, 32) * 5)
+        for k, val in kw.items():
+            setattr(g, k, val)
+        return L.sp_attention_bwd(ctypes.byref(c), ctypes.byref(g), ws, nbytes, None)
+
+    assert need > 0 and backward(c, nbytes=need - 1) == _lib.SP_ERR_WORKSPACE
+    for kw in (dict(o=None), dict(dout=None), dict(lse=None), dict(dq=p + 2), dict(dk_row=63),
+               dict(dv_head=16), dict(ws=None), dict(ws=p + 8)):
+        assert backward(c, **kw) == _lib.SP_ERR_INVALID_ARG, kw
+    assert L.sp_attention_bwd(ctypes.byref(c), None, p, 1 << 30, None) == _lib.SP_ERR_INVALID_ARG
+    assert backward(call(nq=0, nk=0)) == _lib.SP_OK
