@@ -499,6 +499,46 @@ int sp_gated_ffn_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
                      const void* w_down, int64_t Co, int32_t act, void* dx, void* dw_gate,
                      void* dw_up, void* dw_down, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- group norm ----------------------------------------------------------- */
+/* y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and var over the rows of a sample and the
+ * C / groups channels of a group.  Rows [rows, C] of f16, bf16 or f32, ldx elements from row to
+ * row; weight and bias [C] (nullable) of param_dtype, the rows' or SP_F32; act as in
+ * sp_gated_ffn, 3 none.  Sample s has the rows offsets[s] .. offsets[s + 1] - 1 (device memory, [samples
+ * + 1], ascending; null: one sample of all rows); rows outside all samples become zeros.  Offsets are not
+ * checked; whatever they hold, no access leaves the rows.  stats receives mean and 1 / sqrt(var + eps)
+ * of each part and group, 2 * groups * (offsets ? samples + 2 : 1) floats, for the backward
+ * pass.  Statistics are fp32 and joined in a fixed order.  samples of the query: -1 without
+ * offsets. */
+size_t sp_group_norm_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t groups,
+                               int64_t samples, int32_t backward);
+int sp_group_norm(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
+                  int64_t groups, const void* weight, const void* bias, int32_t param_dtype,
+                  float eps, int32_t act, const int32_t* offsets, int64_t samples, void* y,
+                  float* stats, void* ws, size_t ws_bytes, void* stream);
+/* Gradients from that of y: dx [rows, C], dweight and dbias [C] of param_dtype (each nullable). */
+int sp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                      int64_t rows, int64_t C, int64_t groups, const void* weight,
+                      const void* bias, int32_t param_dtype, int32_t act, const int32_t* offsets,
+                      int64_t samples, const float* stats, void* dx, void* dweight, void* dbias,
+                      void* ws, size_t ws_bytes, void* stream);
+
+/* ---- linear layer --------------------------------------------------------- */
+/* y = act(x weight' + bias) + residual for rows x [rows, C], weight [Co, C], bias [Co] and residual
+ * [rows, Co] (both nullable) of one type (f16, bf16 or f32); weight, bias and y contiguous.  act as
+ * in sp_gated_ffn, 3 none.  Sums are fp32, y is rounded once. */
+int sp_linear(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
+              const void* weight, int64_t Co, const void* bias, int32_t act, const void* residual,
+              int64_t ldr, void* y, void* stream);
+/* Gradients from that of y (the residual's is dy): dx [rows, C], dweight [Co, C], dbias [Co] (each
+ * nullable).  With an activation x weight' + bias is formed again and the gradient of it,
+ * rounded to the type, takes rows * Co values of the workspace (16-byte aligned).  Sums over rows
+ * have a fixed order. */
+size_t sp_linear_bwd_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t Co, int32_t act);
+int sp_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                  int64_t rows, int64_t C, const void* weight, int64_t Co, const void* bias,
+                  int32_t act, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
+                  void* stream);
+
 /* ---- attention ----------------------------------------------------------- */
 /* O = softmax(scale q k') v for each of `heads` query heads, within each sequence of rows.  Key head h
  * serves the heads / kv_heads query heads from h (heads / kv_heads) on.  q [nq, heads, dim], k and v

@@ -1,0 +1,820 @@
+// Group norm of feature rows, sample by sample, with an activation after it:
+//
+//   mean, var of a sample's rows in a group of C / groups channels, inv = 1 / sqrt(var + eps)
+//   u = (x - mean) inv, z = u w + b, y = act(z)
+//   dz = dy act'(z), dw = sum dz u, db = sum dz
+//   dx = inv (w dz - mean(w dz) - u mean(w dz u))      (means over the same rows and group)
+//
+// Bound by memory.  x passes twice (the statistics, then the values), in the backward pass x and dy do; the second
+// time comes from the caches as far as they hold it.  A thread has V channels (16 bytes) of some rows of
+// a chunk.  The statistics of a chunk are each channel's mean and sum of squares about it, formed
+// from a few rows in registers and joined by Chan, Golub and LeVeque's formula, so that a mean far
+// from zero costs no digits; everything is fp32 and joined in a fixed order.
+#include "sp_attention.h"  // sequences in packed rows
+
+namespace sp {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormRows = 4;       // rows of a thread at a time
+constexpr int kNormChunks = 1024;  // chunks that a call is cut into, about
+// Calls of so many values and parts at most go through one workgroup, in one launch: 60 x 64 fp16 ...
+constexpr int64_t kNormSmall = 16384;
+constexpr int kNormSmallParts = 3;
+
+enum { kActNone = 3 };  // beside the feed-forward block's activations
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) NormPiece {
+  T v[V];
+};
+
+// n values' mean and their sum of squares about it.
+struct Moments {
+  float n, mean, m2;
+  __device__ __forceinline__ void join(float on, float omean, float om2) {
+    const float all = n + on;
+    if (on == 0.f) return;
+    const float d = omean - mean, w = on / all;
+    mean = __builtin_fmaf(d, w, mean);
+    m2 += __builtin_fmaf(d * d, n * w, om2);
+    n = all;
+  }
+};
+
+template <bool FAST, int ACT>
+__device__ __forceinline__ void norm_act(float z, float& value, float& slope) {
+  if constexpr (ACT == kActNone) {
+    value = z;
+    slope = 1.f;
+  } else {
+    gate<FAST, ACT>(z, value, slope);
+  }
+}
+
+// How the threads of a workgroup lie over rows and channels: L threads of V channels a row, `per` rows
+// at a time; blocks of L V channels where a row has more.
+struct NormShape {
+  int C, groups, cg, L, per, blocks;
+  int64_t chunk;  // rows
+};
+
+template <typename T, typename P>
+struct NormArgs {
+  const T *x, *dy;
+  int64_t ldx, lddy;
+  Seqs seqs;
+  NormShape s;
+  const P *w, *b;
+  float eps;
+  T *y, *dx;
+  P *dw, *db;
+  float2* stats;  // [parts][groups]: mean, inv
+  float2* part;   // [slots][C]: a chunk's moments; sums of dz and dz u
+  float2* sums;   // [parts][C]: sums of dz and dz u
+  float2* back;   // [parts][groups]: mean(w dz), mean(w dz u)
+};
+
+// This thread's channels and rows.
+struct NormLane {
+  int c, row;  // first channel; first row of the chunk, per rows apart
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ NormLane norm_lane(const NormShape& s, int block) {
+  const int row = int(threadIdx.x) / s.L, c = (block * s.L + int(threadIdx.x) - row * s.L) * V;
+  return NormLane{c, row, row < s.per && c < s.C};
+}
+
+// Moments of V channels over rows first, first + per, ... below end.
+template <typename T, int V>
+__device__ __forceinline__ void row_moments(const T* x, int64_t ldx, int64_t first, int64_t end,
+                                            int per, int c, Moments (&m)[V]) {
+  using vec = NormPiece<T, V>;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m[i] = Moments{0.f, 0.f, 0.f};
+  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
+    vec a[kNormRows];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j) {
+      a[j] = vec{};
+      if (r + int64_t(j) * per < end) {
+        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
+        n = j + 1;
+      }
+    }
+    const float one = 1.f / float(n);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float sum = 0.f, sq = 0.f;
+#pragma unroll
+      for (int j = 0; j < kNormRows; ++j) sum += to_f32(a[j].v[i]);
+      const float mean = sum * one;
+#pragma unroll
+      for (int j = 0; j < kNormRows; ++j) {
+        const float d = j < n ? to_f32(a[j].v[i]) - mean : 0.f;
+        sq = __builtin_fmaf(d, d, sq);
+      }
+      m[i].join(float(n), mean, sq);
+    }
+  }
+}
+
+// Channel c's moments over the workgroup's `per` rows of threads, from LDS [per][L V].
+__device__ __forceinline__ Moments column_moments(const float2* lds, const float* counts, int per,
+                                                  int width, int c) {
+  Moments m{0.f, 0.f, 0.f};
+  for (int r = 0; r < per; ++r) {
+    const float2 v = lds[r * width + c];
+    m.join(counts[r], v.x, v.y);
+  }
+  return m;
+}
+
+template <typename T, typename P, int V>
+__global__ __launch_bounds__(kNormThreads) void norm_moments(NormArgs<T, P> a) {
+  __shared__ float2 lds[kNormThreads * V];
+  __shared__ float counts[kNormThreads];
+  const Tile t = find_tile(a.seqs, 1, int(a.s.chunk), blockIdx.x);
+  if (t.at >= t.len || a.seqs.outside(t.part)) return;
+  const int64_t end = t.at + a.s.chunk < t.len ? t.at + a.s.chunk : t.len;
+  const NormLane l = norm_lane<V>(a.s, int(blockIdx.y));
+  const int width = a.s.L * V;
+  if (l.on) {
+    Moments m[V];
+    row_moments<T, V>(a.x + t.lo * a.ldx, a.ldx, t.at + l.row, end, a.s.per, l.c, m);
+    const int at = l.c - int(blockIdx.y) * width;
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[l.row * width + at + i] = float2{m[i].mean, m[i].m2};
+    if (at == 0) counts[l.row] = m[0].n;
+  }
+  __syncthreads();
+  for (int c = int(threadIdx.x); c < width; c += kNormThreads) {
+    const int channel = int(blockIdx.y) * width + c;
+    if (channel >= a.s.C) break;
+    const Moments m = column_moments(lds, counts, a.s.per, width, c);
+    a.part[int64_t(blockIdx.x) * a.s.C + channel] = float2{m.mean, m.m2};
+  }
+}
+
+// Sums of two values, or joined moments, over a workgroup, on every thread.
+__device__ __forceinline__ Moments block_moments(Moments m, float* lds) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const float n = __shfl_xor(m.n, off, 64), mean = __shfl_xor(m.mean, off, 64);
+    const float m2 = __shfl_xor(m.m2, off, 64);
+    // (both partners join in one order, so that they agree)
+    Moments lo = m, hi{n, mean, m2};
+    if ((int(threadIdx.x) & off) != 0) {
+      lo = hi;
+      hi = m;
+    }
+    lo.join(hi.n, hi.mean, hi.m2);
+    m = lo;
+  }
+  const int wave = int(threadIdx.x) >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    lds[3 * wave] = m.n;
+    lds[3 * wave + 1] = m.mean;
+    lds[3 * wave + 2] = m.m2;
+  }
+  __syncthreads();
+  Moments all{0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kNormThreads / 64; ++w) all.join(lds[3 * w], lds[3 * w + 1], lds[3 * w + 2]);
+  return all;
+}
+
+// The chunks of part p: the first one's slot, and how many.
+struct PartChunks {
+  int64_t slot, n, len;
+};
+__device__ __forceinline__ PartChunks part_chunks(const Seqs& s, int64_t chunk, int p) {
+  const int64_t lo = s.bound(p), hi = s.bound(p + 1), len = hi > lo ? hi - lo : 0;
+  return PartChunks{lo / chunk + p, (len + chunk - 1) / chunk, len};
+}
+
+// A part's group: its chunks' and channels' moments joined.
+template <typename T, typename P>
+__global__ __launch_bounds__(kNormThreads) void norm_stats(NormArgs<T, P> a) {
+  __shared__ float lds[3 * kNormThreads / 64];
+  const int p = int(blockIdx.x) / a.s.groups, g = int(blockIdx.x) % a.s.groups;
+  if (a.seqs.outside(p)) return;
+  const PartChunks k = part_chunks(a.seqs, a.s.chunk, p);
+  if (k.len == 0) return;
+  Moments m{0.f, 0.f, 0.f};
+  const int64_t n = k.n * a.s.cg;
+  for (int64_t i = threadIdx.x; i < n; i += kNormThreads) {
+    const int64_t j = i / a.s.cg;
+    const int c = g * a.s.cg + int(i - j * a.s.cg);
+    const float2 v = a.part[(k.slot + j) * a.s.C + c];
+    m.join(float(j + 1 < k.n ? a.s.chunk : k.len - j * a.s.chunk), v.x, v.y);
+  }
+  m = block_moments(m, lds);
+  if (threadIdx.x == 0)
+    a.stats[blockIdx.x] = float2{m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps)};
+}
+
+// What a thread needs of its channels.
+template <int V>
+struct NormChannels {
+  float mean[V], inv[V], w[V], b[V];
+  template <typename P>
+  __device__ __forceinline__ NormChannels(const NormShape& s, const float2* stats, const P* wt,
+                                          const P* bt, int c) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 st = stats[(c + i) / s.cg];
+      mean[i] = st.x;
+      inv[i] = st.y;
+      w[i] = wt ? to_f32(wt[c + i]) : 1.f;
+      b[i] = bt ? to_f32(bt[c + i]) : 0.f;
+    }
+  }
+};
+
+// f(pointer offset row) over a thread's rows, kNormRows at a time.
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void norm_rows(const T* x, int64_t ldx, T* y, int64_t ldy, int64_t first,
+                                          int64_t end, int per, int c, const NormChannels<V>& k) {
+  using vec = NormPiece<T, V>;
+  constexpr bool FAST = sizeof(T) == 2;
+  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
+    vec a[kNormRows];
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j)
+      if (r + int64_t(j) * per < end)
+        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j) {
+      if (r + int64_t(j) * per >= end) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float u = (to_f32(a[j].v[i]) - k.mean[i]) * k.inv[i];
+        float value, slope;
+        norm_act<FAST, ACT>(__builtin_fmaf(u, k.w[i], k.b[i]), value, slope);
+        a[j].v[i] = from_f32<T>(value);
+      }
+      *reinterpret_cast<vec*>(y + (r + int64_t(j) * per) * ldy + c) = a[j];
+    }
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void zero_rows(T* y, int64_t ld, int64_t first, int64_t end, int per,
+                                          int c) {
+  for (int64_t r = first; r < end; r += per)
+    *reinterpret_cast<NormPiece<T, V>*>(y + r * ld + c) = NormPiece<T, V>{};
+}
+
+template <typename T, typename P, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void norm_apply(NormArgs<T, P> a) {
+  const Tile t = find_tile(a.seqs, 1, int(a.s.chunk), blockIdx.x);
+  if (t.at >= t.len) return;
+  const int64_t end = t.at + a.s.chunk < t.len ? t.at + a.s.chunk : t.len;
+  const NormLane l = norm_lane<V>(a.s, int(blockIdx.y));
+  if (!l.on) return;
+  T* y = a.y + t.lo * a.s.C;
+  if (a.seqs.outside(t.part)) {
+    zero_rows<T, V>(y, a.s.C, t.at + l.row, end, a.s.per, l.c);
+    return;
+  }
+  const NormChannels<V> k(a.s, a.stats + int64_t(t.part) * a.s.groups, a.w, a.b, l.c);
+  norm_rows<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, y, a.s.C, t.at + l.row, end, a.s.per, l.c, k);
+}
+
+// ---- gradients ---------------------------------------------------------------------
+// Sums of dz and dz u of V channels over rows first, first + per, ...
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, int64_t lddy,
+                                         int64_t first, int64_t end, int per, int c,
+                                         const NormChannels<V>& k, float (&s1)[V],
+                                         float (&s2)[V]) {
+  using vec = NormPiece<T, V>;
+  constexpr bool FAST = sizeof(T) == 2;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
+  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
+    vec a[kNormRows], d[kNormRows];
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j)
+      if (r + int64_t(j) * per < end) {
+        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
+        d[j] = *reinterpret_cast<const vec*>(dy + (r + int64_t(j) * per) * lddy + c);
+      }
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j) {
+      if (r + int64_t(j) * per >= end) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float u = (to_f32(a[j].v[i]) - k.mean[i]) * k.inv[i];
+        float value, slope;
+        norm_act<FAST, ACT>(__builtin_fmaf(u, k.w[i], k.b[i]), value, slope);
+        const float dz = to_f32(d[j].v[i]) * slope;
+        s1[i] += dz;
+        s2[i] = __builtin_fmaf(dz, u, s2[i]);
+      }
+    }
+  }
+}
+
+// a b - c with the product rounded, as it was when c was summed up: where c is the mean of one value, the
+// difference is zero.
+__device__ __forceinline__ float less(float a, float b, float c) {
+#pragma clang fp contract(off)
+  const float p = a * b;
+  return p - c;
+}
+
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void grad_rows(const T* x, int64_t ldx, const T* dy, int64_t lddy, T* dx,
+                                          int64_t lddx, int64_t first, int64_t end, int per, int c,
+                                          const NormChannels<V>& k, const float (&m1)[V],
+                                          const float (&m2)[V]) {
+  using vec = NormPiece<T, V>;
+  constexpr bool FAST = sizeof(T) == 2;
+  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
+    vec a[kNormRows], d[kNormRows];
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j)
+      if (r + int64_t(j) * per < end) {
+        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
+        d[j] = *reinterpret_cast<const vec*>(dy + (r + int64_t(j) * per) * lddy + c);
+      }
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j) {
+      if (r + int64_t(j) * per >= end) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float u = (to_f32(a[j].v[i]) - k.mean[i]) * k.inv[i];
+        float value, slope;
+        norm_act<FAST, ACT>(__builtin_fmaf(u, k.w[i], k.b[i]), value, slope);
+        a[j].v[i] = from_f32<T>(
+            k.inv[i] * __builtin_fmaf(-u, m2[i], less(to_f32(d[j].v[i]) * slope, k.w[i], m1[i])));
+      }
+      *reinterpret_cast<vec*>(dx + (r + int64_t(j) * per) * lddx + c) = a[j];
+    }
+  }
+}
+
+template <typename T, typename P, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_sums(NormArgs<T, P> a) {
+  __shared__ float2 lds[kNormThreads * V];
+  const Tile t = find_tile(a.seqs, 1, int(a.s.chunk), blockIdx.x);
+  if (t.at >= t.len || a.seqs.outside(t.part)) return;
+  const int64_t end = t.at + a.s.chunk < t.len ? t.at + a.s.chunk : t.len;
+  const NormLane l = norm_lane<V>(a.s, int(blockIdx.y));
+  const int width = a.s.L * V;
+  if (l.on) {
+    const NormChannels<V> k(a.s, a.stats + int64_t(t.part) * a.s.groups, a.w, a.b, l.c);
+    float s1[V], s2[V];
+    row_sums<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, t.at + l.row, end,
+                        a.s.per, l.c, k, s1, s2);
+    const int at = l.c - int(blockIdx.y) * width;
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[l.row * width + at + i] = float2{s1[i], s2[i]};
+  }
+  __syncthreads();
+  for (int c = int(threadIdx.x); c < width; c += kNormThreads) {
+    const int channel = int(blockIdx.y) * width + c;
+    if (channel >= a.s.C) break;
+    float2 v{0.f, 0.f};
+    for (int r = 0; r < a.s.per; ++r) {
+      v.x += lds[r * width + c].x;
+      v.y += lds[r * width + c].y;
+    }
+    a.part[int64_t(blockIdx.x) * a.s.C + channel] = v;
+  }
+}
+
+// A part's group: its channels' sums over the chunks, and from them the group's means.  A wave a
+// channel at a time.
+template <typename T, typename P>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_join(NormArgs<T, P> a) {
+  __shared__ float2 lds[kNormThreads / 64];
+  const int p = int(blockIdx.x) / a.s.groups, g = int(blockIdx.x) % a.s.groups;
+  const PartChunks k = part_chunks(a.seqs, a.s.chunk, p);
+  const int64_t n = a.seqs.outside(p) ? 0 : k.n;
+  const int wave = int(threadIdx.x) >> 6, lane = int(threadIdx.x) & 63;
+  float2 mine{0.f, 0.f};
+  for (int j = wave; j < a.s.cg; j += kNormThreads / 64) {
+    const int c = g * a.s.cg + j;
+    float2 v{0.f, 0.f};
+    for (int64_t i = lane; i < n; i += 64) {
+      const float2 o = a.part[(k.slot + i) * a.s.C + c];
+      v.x += o.x;
+      v.y += o.y;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      v.x += __shfl_xor(v.x, off, 64);
+      v.y += __shfl_xor(v.y, off, 64);
+    }
+    if (lane == 0) a.sums[int64_t(p) * a.s.C + c] = v;
+    const float w = a.w ? to_f32(a.w[c]) : 1.f;
+    mine.x = __builtin_fmaf(v.x, w, mine.x);
+    mine.y = __builtin_fmaf(v.y, w, mine.y);
+  }
+  if (lane == 0) lds[wave] = mine;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  float2 all = lds[0];
+#pragma unroll
+  for (int w = 1; w < kNormThreads / 64; ++w) {
+    all.x += lds[w].x;
+    all.y += lds[w].y;
+  }
+  const float count = float(k.len) * float(a.s.cg);
+  a.back[blockIdx.x] = n ? float2{all.x / count, all.y / count} : float2{0.f, 0.f};
+}
+
+// dx; the workgroups from `slots` on sum the parameters' gradients over the parts.
+template <typename T, typename P, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_apply(NormArgs<T, P> a, int64_t slots) {
+  if (int64_t(blockIdx.x) >= slots) {
+    const int c = int(blockIdx.x - slots) * kNormThreads + int(threadIdx.x);
+    if (blockIdx.y != 0 || c >= a.s.C) return;
+    float2 v{0.f, 0.f};
+    for (int p = 0; p < a.seqs.parts; ++p) {
+      const float2 o = a.sums[int64_t(p) * a.s.C + c];
+      v.x += o.x;
+      v.y += o.y;
+    }
+    if (a.dw) a.dw[c] = from_f32<P>(v.y);
+    if (a.db) a.db[c] = from_f32<P>(v.x);
+    return;
+  }
+  if (!a.dx) return;
+  const Tile t = find_tile(a.seqs, 1, int(a.s.chunk), blockIdx.x);
+  if (t.at >= t.len) return;
+  const int64_t end = t.at + a.s.chunk < t.len ? t.at + a.s.chunk : t.len;
+  const NormLane l = norm_lane<V>(a.s, int(blockIdx.y));
+  if (!l.on) return;
+  T* dx = a.dx + t.lo * a.s.C;
+  if (a.seqs.outside(t.part)) {
+    zero_rows<T, V>(dx, a.s.C, t.at + l.row, end, a.s.per, l.c);
+    return;
+  }
+  const NormChannels<V> k(a.s, a.stats + int64_t(t.part) * a.s.groups, a.w, a.b, l.c);
+  float m1[V], m2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float2 v = a.back[int64_t(t.part) * a.s.groups + (l.c + i) / a.s.cg];
+    m1[i] = v.x;
+    m2[i] = v.y;
+  }
+  grad_rows<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, dx, a.s.C,
+                       t.at + l.row, end, a.s.per, l.c, k, m1, m2);
+}
+
+// ---- small calls: one workgroup, part after part -------------------------------------
+template <typename T, typename P, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void norm_small(NormArgs<T, P> a) {
+  __shared__ float2 lds[kNormThreads * V];
+  __shared__ float counts[kNormThreads];
+  const NormLane l = norm_lane<V>(a.s, 0);
+  const int width = a.s.L * V;
+  for (int p = 0; p < a.seqs.parts; ++p) {
+    const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
+    if (len == 0) continue;
+    if (a.seqs.outside(p)) {
+      if (l.on) zero_rows<T, V>(a.y + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c);
+      continue;
+    }
+    if (l.on) {
+      Moments m[V];
+      row_moments<T, V>(a.x + lo * a.ldx, a.ldx, l.row, len, a.s.per, l.c, m);
+#pragma unroll
+      for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{m[i].mean, m[i].m2};
+      if (l.c == 0) counts[l.row] = m[0].n;
+    }
+    __syncthreads();
+    for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
+      const Moments m = column_moments(lds, counts, a.s.per, width, c);
+      lds[c] = float2{m.mean, m.m2};  // (its own column's first place)
+    }
+    __syncthreads();
+    float2* stats = a.stats + int64_t(p) * a.s.groups;
+    for (int g = int(threadIdx.x); g < a.s.groups; g += kNormThreads) {
+      Moments m{0.f, 0.f, 0.f};
+      for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) m.join(float(len), lds[c].x, lds[c].y);
+      stats[g] = float2{m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps)};
+    }
+    __syncthreads();  // (which makes the workgroup's own stores to memory visible to it)
+    if (l.on) {
+      const NormChannels<V> k(a.s, stats, a.w, a.b, l.c);
+      norm_rows<T, V, ACT>(a.x + lo * a.ldx, a.ldx, a.y + lo * a.s.C, a.s.C, l.row, len, a.s.per,
+                           l.c, k);
+    }
+  }
+}
+
+template <typename T, typename P, int V, int ACT>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_small(NormArgs<T, P> a) {
+  __shared__ float2 lds[kNormThreads * V];
+  __shared__ float2 total[kNormThreads * V];
+  const NormLane l = norm_lane<V>(a.s, 0);
+  const int width = a.s.L * V;
+  for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) total[c] = float2{0.f, 0.f};
+  for (int p = 0; p < a.seqs.parts; ++p) {
+    const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
+    if (len == 0) continue;
+    if (a.seqs.outside(p)) {
+      if (l.on && a.dx) zero_rows<T, V>(a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c);
+      continue;
+    }
+    const float2* stats = a.stats + int64_t(p) * a.s.groups;
+    const NormChannels<V> k(a.s, stats, a.w, a.b, l.on ? l.c : 0);
+    const T* x = a.x + lo * a.ldx;
+    const T* dy = a.dy + lo * a.lddy;
+    __syncthreads();
+    if (l.on) {
+      float s1[V], s2[V];
+      row_sums<T, V, ACT>(x, a.ldx, dy, a.lddy, l.row, len, a.s.per, l.c, k, s1, s2);
+#pragma unroll
+      for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{s1[i], s2[i]};
+    }
+    __syncthreads();
+    for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
+      float2 v{0.f, 0.f};
+      for (int r = 0; r < a.s.per; ++r) {
+        v.x += lds[r * width + c].x;
+        v.y += lds[r * width + c].y;
+      }
+      lds[c] = v;
+      total[c].x += v.x;
+      total[c].y += v.y;
+    }
+    __syncthreads();
+    if (l.on && a.dx) {
+      const float count = float(len) * float(a.s.cg);
+      float m1[V], m2[V];
+      int at = -1;
+      float2 all{0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int g = (l.c + i) / a.s.cg;
+        if (g != at) {
+          all = float2{0.f, 0.f};
+          for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) {
+            const float w = a.w ? to_f32(a.w[c]) : 1.f;
+            all.x = __builtin_fmaf(lds[c].x, w, all.x);
+            all.y = __builtin_fmaf(lds[c].y, w, all.y);
+          }
+          at = g;
+        }
+        m1[i] = all.x / count;
+        m2[i] = all.y / count;
+      }
+      grad_rows<T, V, ACT>(x, a.ldx, dy, a.lddy, a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c,
+                           k, m1, m2);
+    }
+  }
+  __syncthreads();
+  for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
+    if (a.dw) a.dw[c] = from_f32<P>(total[c].y);
+    if (a.db) a.db[c] = from_f32<P>(total[c].x);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+static NormShape norm_shape(int64_t rows, int C, int groups, int V) {
+  NormShape s{};
+  s.C = C;
+  s.groups = groups;
+  s.cg = C / groups;
+  s.L = C / V < kNormThreads ? C / V : kNormThreads;
+  s.per = kNormThreads / s.L;
+  s.blocks = int(cdiv(C, s.L * V));
+  const int64_t step = int64_t(s.per) * kNormRows;
+  s.chunk = cdiv(cdiv(rows, kNormChunks), step) * step;
+  return s;
+}
+
+static bool norm_is_small(int64_t rows, const NormShape& s, const Seqs& q) {
+  return rows * s.C <= kNormSmall && q.parts <= kNormSmallParts && s.blocks == 1;
+}
+
+static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
+  return Seqs{off, rows, off ? int(n) + 2 : 1};
+}
+
+// (the sizes do not depend on V, which the tensors' addresses decide)
+static size_t norm_workspace(int64_t rows, int64_t C, int64_t groups, const Seqs& q, int V,
+                             bool grad) {
+  const NormShape s = norm_shape(rows, int(C), int(groups), V);
+  if (norm_is_small(rows, s, q)) return 0;
+  size_t n = align_up(size_t(tile_slots(q, 1, int(s.chunk))) * C * sizeof(float2), 256);
+  if (grad)
+    n += align_up(size_t(q.parts) * C * sizeof(float2), 256) +
+         align_up(size_t(q.parts) * groups * sizeof(float2), 256);
+  return n;
+}
+
+template <typename F>
+static int norm_act_of(int act, F&& f) {
+  switch (act) {
+    case kActSilu: return f(std::integral_constant<int, kActSilu>());
+    case kActGelu: return f(std::integral_constant<int, kActGelu>());
+    case kActRelu: return f(std::integral_constant<int, kActRelu>());
+    default: return f(std::integral_constant<int, kActNone>());
+  }
+}
+
+template <typename T, typename P, int V>
+static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
+  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
+  if (norm_is_small(a.seqs.rows, a.s, a.seqs)) {
+    norm_act_of(act, [&](auto k) {
+      norm_small<T, P, V, k.value><<<1, kNormThreads, 0, st>>>(a);
+      return 0;
+    });
+    SP_LAUNCHED();
+    return SP_OK;
+  }
+  const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
+  const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
+  SP_CHECK_ARG(slots <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
+  a.part = reinterpret_cast<float2*>(ws);
+  const dim3 grid(unsigned(slots), unsigned(a.s.blocks));
+  norm_moments<T, P, V><<<grid, kNormThreads, 0, st>>>(a);
+  SP_LAUNCHED();
+  norm_stats<T, P><<<unsigned(joins), kNormThreads, 0, st>>>(a);
+  SP_LAUNCHED();
+  norm_act_of(act, [&](auto k) {
+    norm_apply<T, P, V, k.value><<<grid, kNormThreads, 0, st>>>(a);
+    return 0;
+  });
+  SP_LAUNCHED();
+  return SP_OK;
+}
+
+template <typename T, typename P, int V>
+static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
+  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
+  if (norm_is_small(a.seqs.rows, a.s, a.seqs)) {
+    norm_act_of(act, [&](auto k) {
+      norm_grad_small<T, P, V, k.value><<<1, kNormThreads, 0, st>>>(a);
+      return 0;
+    });
+    SP_LAUNCHED();
+    return SP_OK;
+  }
+  const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
+  const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
+  const int64_t extra = cdiv(a.s.C, kNormThreads);
+  SP_CHECK_ARG(slots + extra <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
+  a.part = reinterpret_cast<float2*>(ws);
+  ws += align_up(size_t(slots) * a.s.C * sizeof(float2), 256);
+  a.sums = reinterpret_cast<float2*>(ws);
+  ws += align_up(size_t(a.seqs.parts) * a.s.C * sizeof(float2), 256);
+  a.back = reinterpret_cast<float2*>(ws);
+  const dim3 grid(unsigned(slots), unsigned(a.s.blocks));
+  norm_act_of(act, [&](auto k) {
+    norm_grad_sums<T, P, V, k.value><<<grid, kNormThreads, 0, st>>>(a);
+    return 0;
+  });
+  SP_LAUNCHED();
+  norm_grad_join<T, P><<<unsigned(joins), kNormThreads, 0, st>>>(a);
+  SP_LAUNCHED();
+  const dim3 last(unsigned(slots + extra), unsigned(a.s.blocks));
+  norm_act_of(act, [&](auto k) {
+    norm_grad_apply<T, P, V, k.value><<<last, kNormThreads, 0, st>>>(a, slots);
+    return 0;
+  });
+  SP_LAUNCHED();
+  return SP_OK;
+}
+
+static int check_norm(const char* what, int32_t dtype, int64_t rows, int64_t C, int64_t groups,
+                      int32_t param_dtype, float eps, int32_t act, const int32_t* offsets,
+                      int64_t samples) {
+  SP_CHECK_ARG(dtype == SP_F16 || dtype == SP_BF16 || dtype == SP_F32,
+               "%s: dtype %d not supported (f16/bf16/f32)", what, dtype);
+  SP_CHECK_ARG(param_dtype == dtype || param_dtype == SP_F32,
+               "%s: parameters of type %d for rows of type %d", what, param_dtype, dtype);
+  SP_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 31) && C >= 1 && C < 65536,
+               "%s: bad sizes rows=%lld C=%lld", what, (long long)rows, (long long)C);
+  SP_CHECK_ARG(groups >= 1 && groups <= C && C % groups == 0, "%s: %lld channels in %lld groups",
+               what, (long long)C, (long long)groups);
+  SP_CHECK_ARG(eps >= 0.f && eps < __builtin_inff(), "%s: bad eps", what);
+  SP_CHECK_ARG(act >= kActSilu && act <= kActNone, "%s: unknown activation %d", what, act);
+  SP_CHECK_ARG(!offsets || (samples >= 0 && samples < (1 << 24)), "%s: bad number of samples %lld",
+               what, (long long)samples);
+  return SP_OK;
+}
+
+template <typename T, typename P, typename F>
+static int norm_width(const NormArgs<T, P>& a, bool vec, F&& run) {
+  constexpr int V = Mfma<T>::V;
+  if (vec) return run(a, std::integral_constant<int, V>());
+  return run(a, std::integral_constant<int, 1>());
+}
+
+template <typename F>
+static int norm_types(int32_t dtype, int32_t param_dtype, F&& f) {
+  if (dtype == SP_F32) return f(float(), float());
+  if (dtype == SP_F16)
+    return param_dtype == SP_F16 ? f(_Float16(), _Float16()) : f(_Float16(), float());
+  return param_dtype == SP_BF16 ? f(__bf16(), __bf16()) : f(__bf16(), float());
+}
+
+}  // namespace sp
+
+using namespace sp;
+
+extern "C" size_t sp_group_norm_workspace(int32_t dtype, int64_t rows, int64_t C, int64_t groups,
+                                          int64_t samples, int32_t backward) {
+  if (check_norm("group_norm", dtype, rows, C, groups, dtype, 0.f, kActNone, nullptr, 0) != SP_OK ||
+      rows == 0 || samples >= (1 << 24))
+    return 0;
+  const Seqs q{nullptr, rows, samples >= 0 ? int(samples) + 2 : 1};
+  const size_t one = norm_workspace(rows, C, groups, q, 1, backward != 0);
+  if (C % vec_of(dtype) != 0) return one;
+  const size_t vec = norm_workspace(rows, C, groups, q, vec_of(dtype), backward != 0);
+  return one > vec ? one : vec;
+}
+
+extern "C" int sp_group_norm(const void* x, int64_t ldx, int32_t dtype, int64_t rows, int64_t C,
+                             int64_t groups, const void* weight, const void* bias,
+                             int32_t param_dtype, float eps, int32_t act, const int32_t* offsets,
+                             int64_t samples, void* y, float* stats, void* ws, size_t ws_bytes,
+                             void* stream) {
+  if (int rc = check_norm("group_norm", dtype, rows, C, groups, param_dtype, eps, act, offsets,
+                          samples))
+    return rc;
+  if (rows == 0) return SP_OK;
+  SP_CHECK_ARG(x && y && stats, "group_norm: null pointer");
+  SP_CHECK_ARG(ldx >= C, "group_norm: rows overlap");
+  const size_t need =
+      sp_group_norm_workspace(dtype, rows, C, groups, offsets ? samples : -1, 0);
+  if (ws_bytes < need)
+    return set_error(SP_ERR_WORKSPACE, "group_norm: workspace of %zu bytes, needs %zu", ws_bytes,
+                     need);
+  SP_CHECK_ARG(!need || (ws && aligned(ws)), "group_norm: the workspace must be 16-byte aligned");
+  return norm_types(dtype, param_dtype, [&](auto t, auto p) {
+    using T = decltype(t);
+    using P = decltype(p);
+    NormArgs<T, P> a{};
+    a.x = static_cast<const T*>(x);
+    a.ldx = ldx;
+    a.seqs = norm_seqs(offsets, rows, samples);
+    a.s.C = int(C);
+    a.s.groups = int(groups);
+    a.w = static_cast<const P*>(weight);
+    a.b = static_cast<const P*>(bias);
+    a.eps = eps;
+    a.y = static_cast<T*>(y);
+    a.stats = reinterpret_cast<float2*>(stats);
+    const int V = vec_of(dtype);
+    const bool vec = C % V == 0 && ldx % V == 0 && aligned(x) && aligned(y);
+    return norm_width(a, vec, [&](const auto& args, auto v) {
+      return norm_forward<T, P, v.value>(args, act, static_cast<char*>(ws), as_stream(stream));
+    });
+  });
+}
+
+extern "C" int sp_group_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                 int32_t dtype, int64_t rows, int64_t C, int64_t groups,
+                                 const void* weight, const void* bias, int32_t param_dtype,
+                                 int32_t act, const int32_t* offsets, int64_t samples,
+                                 const float* stats, void* dx, void* dweight, void* dbias, void* ws,
+                                 size_t ws_bytes, void* stream) {
+  if (int rc = check_norm("group_norm_bwd", dtype, rows, C, groups, param_dtype, 0.f, act, offsets,
+                          samples))
+    return rc;
+  if (rows == 0) return SP_OK;
+  SP_CHECK_ARG(dy && x && stats, "group_norm_bwd: null pointer");
+  SP_CHECK_ARG(ldx >= C && lddy >= C, "group_norm_bwd: rows overlap");
+  const size_t need =
+      sp_group_norm_workspace(dtype, rows, C, groups, offsets ? samples : -1, 1);
+  if (ws_bytes < need)
+    return set_error(SP_ERR_WORKSPACE, "group_norm_bwd: workspace of %zu bytes, needs %zu",
+                     ws_bytes, need);
+  SP_CHECK_ARG(!need || (ws && aligned(ws)),
+               "group_norm_bwd: the workspace must be 16-byte aligned");
+  return norm_types(dtype, param_dtype, [&](auto t, auto p) {
+    using T = decltype(t);
+    using P = decltype(p);
+    NormArgs<T, P> a{};
+    a.x = static_cast<const T*>(x);
+    a.dy = static_cast<const T*>(dy);
+    a.ldx = ldx;
+    a.lddy = lddy;
+    a.seqs = norm_seqs(offsets, rows, samples);
+    a.s.C = int(C);
+    a.s.groups = int(groups);
+    a.w = static_cast<const P*>(weight);
+    a.b = static_cast<const P*>(bias);
+    a.dx = static_cast<T*>(dx);
+    a.dw = static_cast<P*>(dweight);
+    a.db = static_cast<P*>(dbias);
+    a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+    const int V = vec_of(dtype);
+    const bool vec = C % V == 0 && ldx % V == 0 && lddy % V == 0 && aligned(x) && aligned(dy) &&
+                     (!dx || aligned(dx));
+    return norm_width(a, vec, [&](const auto& args, auto v) {
+      return norm_backward<T, P, v.value>(args, act, static_cast<char*>(ws), as_stream(stream));
+    });
+  });
+}

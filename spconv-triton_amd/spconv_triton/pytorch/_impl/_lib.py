@@ -149,6 +149,16 @@ _SIGNATURES = {
     "sp_gated_ffn_bwd_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I32]),
     "sp_gated_ffn_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _I32, _I64, _I64, _P, _P, _I64,
                                         _P, _I64, _I32, _P, _P, _P, _P, _P, _SZ, _P]),
+    "sp_group_norm_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I32]),
+    "sp_group_norm": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _I64, _P, _P, _I32,
+                                     ctypes.c_float, _I32, _P, _I64, _P, _P, _P, _SZ, _P]),
+    "sp_group_norm_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _I64, _P, _P, _I32,
+                                         _I32, _P, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
+    "sp_linear": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _I64, _P, _I32, _P, _I64, _P,
+                                 _P]),
+    "sp_linear_bwd_workspace": (_SZ, [_I32, _I64, _I64, _I64, _I32]),
+    "sp_linear_bwd": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I64, _P, _I64, _P, _I32, _P,
+                                     _P, _P, _P, _SZ, _P]),
     "sp_attention_workspace": (_SZ, [_P]),
     "sp_attention": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P, _SZ, _P]),
     "sp_attention_bwd_workspace": (_SZ, [_P]),

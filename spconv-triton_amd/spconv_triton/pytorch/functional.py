@@ -20,6 +20,8 @@ from torch.autograd.function import once_differentiable
 from spconv_triton.compat import tv
 from spconv_triton.pytorch import ops
 from spconv_triton.pytorch._impl import attention as _attention
+from spconv_triton.pytorch._impl import group_norm as _group_norm
+from spconv_triton.pytorch._impl import linear as _linear
 from spconv_triton.pytorch._impl import rows as _rows
 from spconv_triton.pytorch._impl.rows import Int8Rows
 from spconv_triton.pytorch.hash import HashTable
@@ -386,6 +388,79 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 # ---------------------------------------------------------------------------
 # the attention half of a block
 # ---------------------------------------------------------------------------
+
+class GroupNormFunction(Function):
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps, act, offsets):
+        y, stats = ops.group_norm(x, groups, weight, bias, eps, act, offsets)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(x, weight, bias, stats, offsets)
+            ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats, offsets = ctx.saved_tensors
+        need_x, _, need_w, need_b = ctx.needs_input_grad[:4]
+        dx, dw, db = _group_norm.run_group_norm_backward(
+            dy, x, ctx.groups, stats, weight, bias, ctx.act, offsets, (need_x, need_w, need_b))
+        return dx, None, dw, db, None, None, None
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5, act: str | None = None,
+               offsets: torch.Tensor | None = None):
+    """Group norm of feature rows with an activation after it: ``act((x - mean) / sqrt(var + eps) *
+    weight + bias)``, mean and variance over all rows of a sample and the ``channels / groups``
+    channels of a group.
+
+    ``offsets`` (int32, ``[samples + 1]``, ascending, on the rows' device; ``ops.sample_offsets`` makes
+    them from indices) say where each sample's rows begin and end; without them all rows are one
+    sample.  Rows outside all samples become zeros and pass no gradient.  ``act`` is ``"silu"``,
+    ``"gelu"`` (exact), ``"relu"`` or None.  ``weight`` and ``bias`` have the rows' type or float32;
+    statistics are float32.
+    """
+    if _inference():
+        return ops.group_norm(x, groups, weight, bias, eps, act, offsets)[0]
+    return GroupNormFunction.apply(x, groups, weight, bias, eps, act, offsets)
+
+
+class LinearFunction(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        x, weight, bias, residual = _as_autocast_takes(x, weight, bias, residual)
+        y = ops.linear(x, weight, bias, act, residual)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(x, weight, bias)
+            ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        grads = (None,) * 3
+        if any(need[:3]):
+            x, weight, bias = ctx.saved_tensors
+            grads = _linear.run_linear_backward(dy, x, weight, bias, ctx.act, need[:3])
+        return (*grads, None, dy if need[4] else None)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+           act: str | None = None, residual: torch.Tensor | None = None):
+    """Linear layer of feature rows, ``act(x weight' + bias)``, plus ``residual`` where one is given, in
+    one product.  ``weight`` is ``[out, in]`` like ``nn.Linear``'s; ``act`` is ``"silu"``, ``"gelu"``
+    (exact), ``"relu"`` or None.
+
+    Of the activations x is kept for the backward pass, which forms the activation's argument
+    again.  Sums are float32 and the result is rounded once.  Under autocast x, the parameters and the
+    residual are taken, and y returned, in autocast's type.
+    """
+    if _inference():
+        return ops.linear(x, weight, bias, act, residual)
+    return LinearFunction.apply(x, weight, bias, act, residual)
+
 
 class AttentionFunction(Function):
     @staticmethod

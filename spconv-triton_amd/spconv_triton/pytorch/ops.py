@@ -28,6 +28,8 @@ from spconv_triton.pytorch._impl import gemm as _gemm
 from spconv_triton.pytorch._impl import pairs as _pairs
 from spconv_triton.pytorch._impl import pool as _pool
 from spconv_triton.pytorch._impl.attention import attention, attention_backward
+from spconv_triton.pytorch._impl.group_norm import group_norm, group_norm_backward
+from spconv_triton.pytorch._impl.linear import linear, linear_backward
 from spconv_triton.pytorch._impl.pairs import get_conv_output_size, get_deconv_output_size
 from spconv_triton.pytorch._impl.rows import (
     Int8Rows,
@@ -59,6 +61,8 @@ __all__ = [
     "get_indice_pairs",
     "get_indice_pairs_implicit_gemm",
     "global_pool_rearrange",
+    "group_norm",
+    "group_norm_backward",
     "implicit_gemm",
     "implicit_gemm_backward",
     "indice_avgpool_implicit_gemm",
@@ -69,12 +73,34 @@ __all__ = [
     "indice_maxpool_backward",
     "indice_maxpool_implicit_gemm",
     "indice_maxpool_implicit_gemm_backward",
+    "linear",
+    "linear_backward",
     "maximum_value_int_",
     "quantize_rows",
     "restore_rows",
     "rms_norm",
     "rms_norm_backward",
+    "sample_offsets",
 ]
+
+
+def sample_offsets(indices: torch.Tensor, batch_size: int) -> torch.Tensor:
+    """Where the rows of each sample begin and end, int32 ``[batch_size + 1]`` on the indices'
+    device: sample b has the rows ``offsets[b] .. offsets[b + 1] - 1``.  The rows have to lie in the
+    samples' order, as the rulebooks' outputs and concatenated voxelisations do; others raise a
+    ValueError.  (Reading that from the device blocks the host once.)"""
+    if indices.dim() != 2 or indices.dtype != torch.int32:
+        raise ValueError(f"sample_offsets: indices are an int32 [rows, ndim + 1] tensor, got "
+                         f"{indices.dtype} {tuple(indices.shape)}")
+    if batch_size < 1:
+        raise ValueError(f"sample_offsets: batch_size is {batch_size}")
+    batch = indices[:, 0].contiguous()
+    if batch.numel():
+        good = (batch[1:] >= batch[:-1]).all() & (batch[0] >= 0) & (batch[-1] < batch_size)
+        if not bool(good):
+            raise ValueError("sample_offsets: the rows are not in the order of their samples")
+    samples = torch.arange(batch_size + 1, dtype=torch.int32, device=indices.device)
+    return torch.searchsorted(batch, samples, out_int32=True)
 
 
 def _apply_act_inplace(out: torch.Tensor, act_type, act_alpha: float, act_beta: float):
