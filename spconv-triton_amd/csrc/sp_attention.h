@@ -142,6 +142,14 @@ __device__ __forceinline__ int acc_row(int i) {
   return i / V * 2 * V + V * ((int(threadIdx.x) >> 5) & 1) + i % V;
 }
 
+// A pointer that is the same on all lanes, in scalar registers.
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(u >> 32));
+  return reinterpret_cast<const char*>(uint64_t(hi) << 32 | lo);
+}
+
 // Loads of a thread's pieces of tiles of a head's rows.  Whole tiles take an address of the workgroup's and
 // an offset of the lane's for good; the pieces past the head's width are zeroed once and never
 // written.  A tile that passes the last row goes by piece, with zeros past the end (0 times what
@@ -175,19 +183,18 @@ struct TileLoads {
             uint4{0, 0, 0, 0};
   }
   __device__ __forceinline__ void start(int at, char* lds) const {
-    const char* base = reinterpret_cast<const char*>(p + at * row);
-    if (at + ROWS <= len) {
+    const char* base = uniform(reinterpret_cast<const char*>(p + at * row));
+    if (DP == D && at + ROWS <= len) {
 #pragma unroll
       for (int j = 0; j < L::N; ++j)
-        if (DP == D || at_value(j) < D)
-          copy_piece(base + off[j], lds + (j * kAttnThreads + wave_of() * 64) * 16);
-    } else {
-#pragma unroll
-      for (int j = 0; j < L::N; ++j)
-        if (DP == D || at_value(j) < D)
-          copy_piece(at + at_row(j) < len ? static_cast<const void*>(base + off[j]) : &g_zero_piece,
-                     lds + (j * kAttnThreads + wave_of() * 64) * 16);
+        copy_piece(base + off[j], lds + (j * kAttnThreads + wave_of() * 64) * 16);
+      return;
     }
+#pragma unroll
+    for (int j = 0; j < L::N; ++j)
+      if (at_value(j) < D)
+        copy_piece(at + at_row(j) < len ? static_cast<const void*>(base + off[j]) : &g_zero_piece,
+                   lds + (j * kAttnThreads + wave_of() * 64) * 16);
   }
 };
 
@@ -216,8 +223,36 @@ __device__ __forceinline__ void zero(floatx16& a) {
   for (int i = 0; i < 16; ++i) a[i] = 0.f;
 }
 
-// The other half's value of the same row.
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// Both halves' values of a row on each of them, joined by f.
+template <typename F>
+__device__ __forceinline__ float join_halves(float v, F&& f) {
+  const auto r =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  return join_halves(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float half_max(float v) {
+  return join_halves(v, [](float a, float b) { return __builtin_fmaxf(a, b); });
+}
+
+// N products whose operands come from LDS, AHEAD of them on their way: use(i, operand) issues the product and
+// some vector instructions that run beside it.  The order is the one written here (the compiler's
+// puts the products first, and then the matrix cores wait for the vector unit and the other way round).
+template <typename F, int N, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void beside(Read&& read, Use&& use) {
+  F f[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD && i < N; ++i) f[i] = read(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    use(i, f[i % AHEAD]);
+    if (i + AHEAD < N) f[i % AHEAD] = read(i + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 // acc[t] += (values 32 t .. of rows r0 .. r0 + 31)' p: the second product of attention and of its gradients.
 template <typename T, int DP, int ROWS, int B>

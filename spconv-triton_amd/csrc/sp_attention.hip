@@ -8,28 +8,29 @@
 // and sum of the softmax; the query heads that share a key head are rows of one tile.
 //
 // Statistics and sums are fp32.  P is rounded to the rows' type between the products, as the matrix
-// instructions take it; relative to a running maximum no value exceeds 2^8, and what fp16 loses below 2^-14
-// is less than 2^-25 of the largest term.
+// instructions take it; relative to a maximum that is at most 2^14 below the
+// largest no weight exceeds 2^14, and what fp16 loses below 2^-14 is less than 2^-25 of the maximum's term.
 #include "sp_attention.h"
 
 namespace sp {
 
-// A maximum that grows by less than this (in powers of two) does not rescale what is summed up.
-constexpr float kLazyMax = 8.f;
+// A lane's weights of a tile may sum up to this before they are put relative to a new maximum (fp16 holds
+// weights up to 2^16).
+constexpr float kMostWeight = 16384.f;
 
 // Waves a SIMD.
 template <typename T>
-constexpr int attend_waves(int DP, int QT) {
-  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : QT == 2 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : 2;
+constexpr int attend_waves(int DP) {
+  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
 }
 
-template <typename T, int DP, int QT, int BK, bool CAUSAL, bool STRICT>
-__global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, QT)) void attend(AttnArgs<T> a,
-                                                                                int64_t slots) {
+template <typename T, int DP, int BK, bool CAUSAL, bool STRICT>
+__global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP)) void attend(AttnArgs<T> a,
+                                                                            int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BK>;
   constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
-  constexpr int NK = BK / 32, BQ = kAttnWaves * QT * 32;
+  constexpr int NK = BK / 32, BQ = kAttnWaves * 32, TILES = DP / 32;
   __shared__ __attribute__((aligned(16))) char lds[4 * L::BYTES];
   __shared__ int bad_lds;
   Place place;
@@ -44,27 +45,21 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, QT)) void attend(
   const int64_t klo = a.ks.bound(t.part);
   const int Lk = keys_of(a.qs, a.ks, t.part, klo), Lq = int(t.len / a.G);
 
-  // this lane's queries
+  // this lane's query
   const int wave = wave_of(), lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
-  frag q[QT][STEPS];
-  int row[QT], seen[QT], head[QT];  // the query's row in its sequence; how many keys it sees
-#pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    const int64_t r = t.at + (wave * QT + u) * 32 + lane;
-    const bool live = r < t.len;
-    const int i = int(r / a.G);
-    head[u] = place.head * a.G + int(r - int64_t(i) * a.G);
-    row[u] = live ? i : -1;
-    seen[u] = CAUSAL ? keys_seen(i, Lq, Lk) : Lk;
-    load_head<T, DP>(a.q.p + (t.lo + i) * a.q.row + head[u] * a.q.head, live, a.D, q[u]);
-  }
+  const int64_t r = t.at + wave * 32 + lane;
+  const bool live = r < t.len;
+  const int row = int(r / a.G), head = place.head * a.G + int(r - int64_t(row) * a.G);
+  const int seen = CAUSAL ? keys_seen(row, Lq, Lk) : Lk;  // how many keys it sees
+  frag q[STEPS];
+  load_head<T, DP>(a.q.p + (t.lo + row) * a.q.row + head * a.q.head, live, a.D, q);
   // keys that some query of the workgroup or wave sees, and that every one of the wave sees
   int most = Lk, wave_most = Lk, wave_least = Lk;
   if (CAUSAL) {
-    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * QT * 32;
-    most = keys_seen(int((last - 1) / a.G), Lq, Lk);
-    wave_least = keys_seen(int(w / a.G), Lq, Lk);
-    wave_most = keys_seen(int((w + QT * 32 - 1) / a.G), Lq, Lk);
+    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * 32;
+    most = keys_seen((last - 1) / a.G, Lq, Lk);
+    wave_least = keys_seen(w / a.G, Lq, Lk);
+    wave_most = keys_seen((w + 31) / a.G, Lq, Lk);
     wave_most = wave_most < most ? wave_most : most;
   }
 
@@ -78,159 +73,176 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, QT)) void attend(
 #pragma unroll
     for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
   }
-  floatx16 o[QT][DP / 32];
-  float m[QT], neg[QT], l[QT];
+  floatx16 o[TILES];
+  float m = -__builtin_inff(), neg = 0.f, l = 0.f;
 #pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    m[u] = -__builtin_inff();
-    neg[u] = l[u] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) zero(o[u][d]);
-  }
-  if (first < end) {
-    lk.start(first * BK, lds);
-    lv.start(first * BK, lds + L::BYTES);
-  }
-  for (int n = first; n < end; ++n) {
-    char* buf = lds + ((n - first) & 1) * 2 * L::BYTES;
+  for (int d = 0; d < TILES; ++d) zero(o[d]);
+  // Tile n, in buffer B (constants, so that the reads' addresses stay in registers).
+  auto step = [&](int n, auto buffer) {
+    char* buf = lds + buffer.value * 2 * L::BYTES;
     loads_in_flight<0>();
     __syncthreads();
     if (n + 1 < end) {
-      char* next = lds + ((n + 1 - first) & 1) * 2 * L::BYTES;
+      char* next = lds + (1 - buffer.value) * 2 * L::BYTES;
       lk.start((n + 1) * BK, next);
       lv.start((n + 1) * BK, next + L::BYTES);
     }
     const int key0 = n * BK;
-    if (CAUSAL && key0 >= wave_most) continue;
+    if (CAUSAL && key0 >= wave_most) return;
     const bool edge = key0 + BK > wave_least;
-    floatx16 s[QT][NK];
+    floatx16 s[NK];
 #pragma unroll
-    for (int x = 0; x < NK; ++x) {
-#pragma unroll
-      for (int u = 0; u < QT; ++u) zero(s[u][x]);
-      auto read = [&](int k) { return L::read(buf, 32 * x, k); };
-      Batched<frag, STEPS, kAttnBatch> f;
-      f.start(read);
-      f.run(read, [&](int k, const frag& kf) {
-#pragma unroll
-        for (int u = 0; u < QT; ++u) Mfma<T>::mma(kf, q[u][k], s[u][x]);
-      });
-    }
-    frag p[QT][NK][PS];
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      if (edge) {
-#pragma unroll
-        for (int x = 0; x < NK; ++x)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (key0 + 32 * x + acc_row<T>(i) >= seen[u]) s[u][x][i] = -__builtin_inff();
-      }
-      float mx = s[u][0][0];
+    for (int x = 0; x < NK; ++x) zero(s[x]);
+    // (products of neighbouring keys in turn: one that adds to the result of the one before waits for it)
+    auto read = [&](int i) { return L::read(buf, 32 * (i % NK), i / NK); };
+    Batched<frag, STEPS * NK, kAttnBatch> f;
+    f.start(read);
+    f.run(read, [&](int i, const frag& kf) { Mfma<T>::mma(kf, q[i / NK], s[i % NK]); });
+    if (edge) {
 #pragma unroll
       for (int x = 0; x < NK; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, s[u][x][i]);
-      mx = __builtin_fmaxf(mx, other_half(mx)) * c;
-      if (__ballot(mx > m[u] + kLazyMax)) {
-        const float now = __builtin_fmaxf(mx, m[u]);
-        const float safe = now == -__builtin_inff() ? 0.f : now;
-        const float down = __builtin_amdgcn_exp2f(m[u] - safe);
-        m[u] = now;
-        neg[u] = -safe;
-        l[u] *= down;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[u][d][i] *= down;
-      }
-      float sum = 0.f;
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 32 * x + acc_row<T>(i) >= seen) s[x][i] = -__builtin_inff();
+    }
+    // Weights relative to the maximum so far.  Only where their sum grows out of hand (or there is no
+    // maximum yet) is the tile's maximum found and everything put relative to it.
+    frag p[NK][PS];
+    float sum[2];
+    auto weigh = [&]() {
+      sum[0] = sum[1] = 0.f;
 #pragma unroll
       for (int x = 0; x < NK; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][x][i], c, neg[u]));
-          sum += e;
-          p[u][x][i / V][i % V] = T(e);
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, neg));
+          sum[i & 1] += e;
+          p[x][i / V][i % V] = T(e);
         }
-      l[u] += sum;
+      sum[0] += sum[1];
+    };
+    weigh();
+    if (__ballot(sum[0] > kMostWeight || m == -__builtin_inff())) {
+      float mx = s[0][0];
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, s[x][i]);
+      const float now = __builtin_fmaxf(half_max(mx) * c, m);
+      const float safe = now == -__builtin_inff() ? 0.f : now;
+      const float down = __builtin_amdgcn_exp2f(m - safe);
+      m = now;
+      neg = -safe;
+      l *= down;
+#pragma unroll
+      for (int d = 0; d < TILES; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= down;
+      weigh();
     }
+    l += sum[0];
 #pragma unroll
-    for (int x = 0; x < NK; ++x)
-#pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        if (STRICT && edge)
-          add_rows_seen<T, DP, BK>(buf + L::BYTES, 32 * x, 0, seen[u] - key0, p[u][x], o[u]);
-        else
-          add_rows<T, DP, BK, kAttnBatch>(buf + L::BYTES, 32 * x, p[u][x], o[u]);
-      }
+    for (int x = 0; x < NK; ++x) {
+      if (STRICT && edge)
+        add_rows_seen<T, DP, BK>(buf + L::BYTES, 32 * x, 0, seen - key0, p[x], o);
+      else
+        add_rows<T, DP, BK, kAttnBatch>(buf + L::BYTES, 32 * x, p[x], o);
+    }
+  };
+  if (first < end) {
+    lk.start(first * BK, lds);
+    lv.start(first * BK, lds + L::BYTES);
   }
-  bool bad = false;
-  if (CAUSAL && !STRICT) {
-#pragma unroll
-    for (int u = 0; u < QT; ++u) bad |= any_not_finite(o[u]);
+  for (int n = first; n < end; n += 2) {
+    step(n, std::integral_constant<int, 0>());
+    if (n + 1 < end) step(n + 1, std::integral_constant<int, 1>());
   }
-  report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+  report<CAUSAL, STRICT>(a.again, CAUSAL && !STRICT && any_not_finite(o), &bad_lds);
 
-  const int64_t rows = a.qs.rows;
-#pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    const float sum = l[u] + other_half(l[u]);
-    if (row[u] < 0) continue;
-    const int64_t r = t.lo + row[u];
-    if (a.shares > 1) {
-      const int64_t at = (place.share * rows + r) * a.H + head[u];
-      store_part<DP, V>(a.part + at * a.D, a.D, [&](int d, int i) { return o[u][d][i]; });
-      if (half == 0) {
-        a.part_ml[2 * at] = m[u];
-        a.part_ml[2 * at + 1] = sum;
-      }
-      continue;
+  const float sum = half_sum(l);
+  if (!live) return;
+  const int64_t rows = a.qs.rows, at = t.lo + row;
+  if (a.shares > 1) {
+    const int64_t i = (place.share * rows + at) * a.H + head;
+    store_part<DP, V>(a.part + i * a.D, a.D, [&](int d, int j) { return o[d][j]; });
+    if (half == 0) {
+      a.part_ml[2 * i] = m;
+      a.part_ml[2 * i + 1] = sum;
     }
-    // (a row without keys is zeros)
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    store_head<T, DP>(a.out.p + r * a.out.row + head[u] * a.out.head, a.D,
-                      [&](int d, int i) { return o[u][d][i] * inv; });
-    if (a.lse && half == 0)
-      a.lse[head[u] * rows + r] =
-          sum == 0.f ? __builtin_inff() : m[u] + __builtin_amdgcn_logf(sum);
+    return;
   }
+  // (a row without keys is zeros)
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store_head<T, DP>(a.out.p + at * a.out.row + head * a.out.head, a.D,
+                    [&](int d, int j) { return o[d][j] * inv; });
+  if (a.lse && half == 0)
+    a.lse[head * rows + at] = sum == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(sum);
 }
 
-// The shares' results of a row joined: a workgroup of 64 lanes a row and head.
+// The shares' results of a row and head joined, a workgroup each.  Every thread weighs some shares, then adds
+// up four values over some of them (one wave going through all shares by itself took 54 us for one
+// query's 8 heads of 32 in 96 shares, where the pass over 120k keys took 45).
+constexpr int kMostShares = 1024;
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attend_join(AttnArgs<T> a) {
-  const int64_t n = a.qs.rows * a.H, at = int64_t(blockIdx.x) * kAttnWaves + wave_of();
-  if (at >= n) return;
-  const int lane = int(threadIdx.x) & 63;
-  const int64_t r = at / a.H;
-  const int h = int(at - r * a.H);
+  __shared__ float weight[kMostShares];
+  __shared__ float4v lds[kAttnThreads];
+  __shared__ float wave_max[kAttnWaves], wave_sum[kAttnWaves];
+  const int64_t n = a.qs.rows * a.H, at = blockIdx.x;
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = wave_of();
   float m = -__builtin_inff();
-  for (int s = 0; s < a.shares; ++s) m = __builtin_fmaxf(m, a.part_ml[2 * (s * n + at)]);
-  const float safe = m == -__builtin_inff() ? 0.f : m;
-  float sum = 0.f, v[2] = {0.f, 0.f};
-  for (int s = 0; s < a.shares; ++s) {
-    const int64_t i = s * n + at;
-    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * i] - safe);
-    sum = __builtin_fmaf(w, a.part_ml[2 * i + 1], sum);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (lane + 64 * j < a.D)
-        v[j] = __builtin_fmaf(w, a.part[i * a.D + lane + 64 * j], v[j]);
+  for (int s = tid; s < a.shares; s += kAttnThreads) {
+    const float v = a.part_ml[2 * (s * n + at)];
+    weight[s] = v;
+    m = __builtin_fmaxf(m, v);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* to = a.out.p + r * a.out.row + h * a.out.head;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (lane + 64 * j < a.D) to[lane + 64 * j] = from_f32<T>(v[j] * inv);
-  if (a.lse && lane == 0)
-    a.lse[h * a.qs.rows + r] =
+  for (int off = 32; off >= 1; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off, 64));
+  if (lane == 0) wave_max[wave] = m;
+  __syncthreads();
+  m = wave_max[0];
+#pragma unroll
+  for (int w = 1; w < kAttnWaves; ++w) m = __builtin_fmaxf(m, wave_max[w]);
+  const float safe = m == -__builtin_inff() ? 0.f : m;
+  float sum = 0.f;
+  for (int s = tid; s < a.shares; s += kAttnThreads) {
+    const float w = __builtin_amdgcn_exp2f(weight[s] - safe);
+    weight[s] = w;
+    sum = __builtin_fmaf(w, a.part_ml[2 * (s * n + at) + 1], sum);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) wave_sum[wave] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) sum += wave_sum[w];
+  const int quads = a.D / 4, runs = kAttnThreads / quads, run = tid / quads, c = tid - run * quads;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+  if (run < runs) {
+#pragma unroll 4
+    for (int s = run; s < a.shares; s += runs)
+      v += weight[s] * *reinterpret_cast<const float4v*>(a.part + (s * n + at) * a.D + 4 * c);
+  }
+  lds[tid] = v;
+  __syncthreads();
+  if (run == 0) {
+    for (int r = 1; r < runs; ++r) v += lds[r * quads + c];
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t r = at / a.H;
+    T* to = a.out.p + r * a.out.row + (at - r * a.H) * a.out.head + 4 * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = from_f32<T>(v[i] * inv);
+  }
+  if (a.lse && tid == 0) {
+    const int64_t r = at / a.H;
+    a.lse[(at - r * a.H) * a.qs.rows + r] =
         sum == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(sum);
+  }
 }
 
 // ---- host ------------------------------------------------------------------------
-constexpr int kForwardTiles = 1;  // query tiles of 32 a wave
-constexpr int kForwardRows = kAttnWaves * kForwardTiles * 32;
+constexpr int kForwardRows = kAttnWaves * 32;
 
 template <typename T>
 static int launch_attend(AttnArgs<T> a, hipStream_t s) {
@@ -238,19 +250,19 @@ static int launch_attend(AttnArgs<T> a, hipStream_t s) {
   const int64_t groups = attn_groups(slots, a.Hk, a.shares);
   SP_CHECK_ARG(groups <= kMaxGridX, "attention: too many rows");
   with_width(a.D, [&](auto w) {
-    constexpr int DP = w.value, QT = kForwardTiles, BK = attn_stage<T>();
+    constexpr int DP = w.value, BK = attn_stage<T>();
     const dim3 grid{unsigned(groups)}, block{kAttnThreads};
     if (!a.causal) {
-      attend<T, DP, QT, BK, false, false><<<grid, block, 0, s>>>(a, slots);
+      attend<T, DP, BK, false, false><<<grid, block, 0, s>>>(a, slots);
     } else {
-      attend<T, DP, QT, BK, true, false><<<grid, block, 0, s>>>(a, slots);
-      attend<T, DP, QT, BK, true, true><<<grid, block, 0, s>>>(a, slots);
+      attend<T, DP, BK, true, false><<<grid, block, 0, s>>>(a, slots);
+      attend<T, DP, BK, true, true><<<grid, block, 0, s>>>(a, slots);
     }
     return 0;
   });
   SP_LAUNCHED();
   if (a.shares == 1) return SP_OK;
-  const int64_t joins = cdiv(a.qs.rows * a.H, kAttnWaves);
+  const int64_t joins = a.qs.rows * a.H;
   SP_CHECK_ARG(joins <= kMaxGridX, "attention: too many rows");
   attend_join<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
   SP_LAUNCHED();

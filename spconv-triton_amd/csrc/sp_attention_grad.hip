@@ -16,12 +16,28 @@
 
 namespace sp {
 
-constexpr int kTops = 256;  // workgroups of attend_grad_rows at most
+constexpr int kGradLoads = 4;  // rows of a group of lanes at a time in attend_grad_rows
+constexpr int kTops = 512;  // workgroups of attend_grad_rows at most
+
+constexpr int kAhead = 3;  // operands on their way from LDS
+
+// Whether 32 rows' products are written beside the weights of the 32 rows before, with two tiles' scores in
+// registers.  That pays where a SIMD has one wave in any case (128 values a head, causal, fp16: dQ 451 us
+// and 415 so, dK and dV 563 and 442) and for dK and dV of 64 values (bf16, 1 520 and 1 470); elsewhere more waves are
+// worth more (dQ of 64 values 1 032 and 1 130; of 32 values 460 and 475, dK and dV 581 and 670).
+template <typename T>
+constexpr bool dq_beside(int DP) { return DP > 64 || sizeof(T) == 4; }
+template <typename T>
+constexpr bool dkv_beside(int DP) { return DP >= 64 || sizeof(T) == 4; }
 
 // Waves a SIMD.
 template <typename T>
+constexpr int dq_waves(int DP) {
+  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 1;
+}
+template <typename T>
 constexpr int grad_waves(int DP) {
-  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 3 : DP <= 64 ? 2 : 1;
+  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 2 : 1;
 }
 
 template <typename T>
@@ -48,47 +64,65 @@ __global__ __launch_bounds__(kAttnThreads) void attend_grad_rows(AttnArgs<T> a, 
     for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
   };
+  // (kGradLoads rows' loads start before the first one's sum; the bounds are the workgroup's)
   const int64_t n = a.qs.rows * a.H;
-  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < n; b += stride) {
-    const int64_t at = b + (int(threadIdx.x) >> log_lanes), r = at / a.H;
-    const int h = int(at - r * a.H);
-    float dot = 0.f, sq = 0.f;
-    if (at < n)
-      for (int c = lane * V; c < a.D; c += lanes * V) {
-        const frag x = *reinterpret_cast<const frag*>(a.dout.p + r * a.dout.row + h * a.dout.head + c);
-        const frag y = *reinterpret_cast<const frag*>(a.o.p + r * a.o.row + h * a.o.head + c);
+  const int c = lane * V;
+  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < n; b += stride * kGradLoads) {
+    frag x[kGradLoads], y[kGradLoads];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          dot = __builtin_fmaf(to_f32(x[i]), to_f32(y[i]), dot);
-          sq = __builtin_fmaf(to_f32(x[i]), to_f32(x[i]), sq);
-        }
+    for (int j = 0; j < kGradLoads; ++j) {
+      const int64_t at = b + j * stride + (int(threadIdx.x) >> log_lanes), r = at / a.H;
+      const int h = int(at - r * a.H);
+      x[j] = y[j] = frag{};
+      if (at < n && c < a.D) {
+        x[j] = *reinterpret_cast<const frag*>(a.dout.p + r * a.dout.row + h * a.dout.head + c);
+        y[j] = *reinterpret_cast<const frag*>(a.o.p + r * a.o.row + h * a.o.head + c);
       }
-    dot = sum(dot);
-    if (kLift<T> != 0.f) {
-      sq = sum(sq);
-      const bool in = !a.qs.off || (r >= a.qs.bound(1) && r < a.qs.bound(a.qs.parts - 1));
-      if (at < n && in && sq < __builtin_inff()) top[0] = __builtin_fmaxf(top[0], sq);
     }
-    if (at < n && lane == 0) {
-      nl[h * a.qs.rows + r] = kLift<T> - a.lse[h * a.qs.rows + r];
-      nd[h * a.qs.rows + r] = -dot;
+#pragma unroll
+    for (int j = 0; j < kGradLoads; ++j) {
+      const int64_t at = b + j * stride + (int(threadIdx.x) >> log_lanes), r = at / a.H;
+      const int h = int(at - r * a.H);
+      float dot = 0.f, sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        dot = __builtin_fmaf(to_f32(x[j][i]), to_f32(y[j][i]), dot);
+        sq = __builtin_fmaf(to_f32(x[j][i]), to_f32(x[j][i]), sq);
+      }
+      dot = sum(dot);
+      if (kLift<T> != 0.f) {
+        sq = sum(sq);
+        const bool in = !a.qs.off || (r >= a.qs.bound(1) && r < a.qs.bound(a.qs.parts - 1));
+        if (at < n && in && sq < __builtin_inff()) top[0] = __builtin_fmaxf(top[0], sq);
+      }
+      if (at < n && lane == 0) {
+        nl[h * a.qs.rows + r] = kLift<T> - a.lse[h * a.qs.rows + r];
+        nd[h * a.qs.rows + r] = -dot;
+      }
     }
   }
   if (kLift<T> == 0.f) return;
   const int64_t nv = a.ks.rows * a.Hk;
-  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < nv; b += stride) {
-    const int64_t at = b + (int(threadIdx.x) >> log_lanes), r = at / a.Hk;
-    const int h = int(at - r * a.Hk);
-    float sq = 0.f;
-    if (at < nv)
-      for (int c = lane * V; c < a.D; c += lanes * V) {
-        const frag x = *reinterpret_cast<const frag*>(a.v.p + r * a.v.row + h * a.v.head + c);
+  for (int64_t b = start - (int(threadIdx.x) >> log_lanes); b < nv; b += stride * kGradLoads) {
+    frag x[kGradLoads];
 #pragma unroll
-        for (int i = 0; i < V; ++i) sq = __builtin_fmaf(to_f32(x[i]), to_f32(x[i]), sq);
-      }
-    sq = sum(sq);
-    const bool in = !a.ks.off || (r >= a.ks.bound(1) && r < a.ks.bound(a.ks.parts - 1));
-    if (at < nv && in && sq < __builtin_inff()) top[1] = __builtin_fmaxf(top[1], sq);
+    for (int j = 0; j < kGradLoads; ++j) {
+      const int64_t at = b + j * stride + (int(threadIdx.x) >> log_lanes), r = at / a.Hk;
+      const int h = int(at - r * a.Hk);
+      x[j] = frag{};
+      if (at < nv && c < a.D)
+        x[j] = *reinterpret_cast<const frag*>(a.v.p + r * a.v.row + h * a.v.head + c);
+    }
+#pragma unroll
+    for (int j = 0; j < kGradLoads; ++j) {
+      const int64_t at = b + j * stride + (int(threadIdx.x) >> log_lanes), r = at / a.Hk;
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) sq = __builtin_fmaf(to_f32(x[j][i]), to_f32(x[j][i]), sq);
+      sq = sum(sq);
+      const bool in = !a.ks.off || (r >= a.ks.bound(1) && r < a.ks.bound(a.ks.parts - 1));
+      if (at < nv && in && sq < __builtin_inff()) top[1] = __builtin_fmaxf(top[1], sq);
+    }
   }
   __shared__ float lds[2][kAttnWaves];
 #pragma unroll
@@ -128,13 +162,14 @@ __device__ __forceinline__ float lift_of(float grad_sq, float value_sq) {
   return e > -100.f ? (e < 100.f ? e : 100.f) : 0.f;  // (a length of 0 makes e infinite)
 }
 
-template <typename T, int DP, int QT, int BK, bool CAUSAL, bool STRICT>
-__global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dq(
+template <typename T, int DP, int BK, bool CAUSAL, bool STRICT>
+__global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
     AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BK>;
   constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
-  constexpr int BQ = kAttnWaves * QT * 32;
+  constexpr int BQ = kAttnWaves * 32, TILES = DP / 32, NX = BK / 32;
+  static_assert(NX <= 2, "a step holds one tile's weights while the next one's are formed");
   __shared__ __attribute__((aligned(16))) char lds[4 * L::BYTES];
   __shared__ int bad_lds;
   Place place;
@@ -152,42 +187,36 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dq(
   float top_grad = 0.f, top_value = 0.f;
   if (kLift<T> != 0.f) read_tops(a.top, a.tops, top_grad, top_value);
 
-  frag q[QT][STEPS], g[QT][STEPS];
-  int row[QT], seen[QT], head[QT];
-  float base[QT], minus[QT], lift[QT];
+  // this lane's query
+  const int64_t r = t.at + wave * 32 + lane;
+  const bool live = r < t.len;
+  const int row = int(r / a.G), head = place.head * a.G + int(r - int64_t(row) * a.G);
+  const int seen = a.causal ? keys_seen(row, Lq, Lk) : Lk;
+  const int64_t at = t.lo + row;
+  frag q[STEPS], g[STEPS];
+  load_head<T, DP>(a.q.p + at * a.q.row + head * a.q.head, live, a.D, q);
+  load_head<T, DP>(a.dout.p + at * a.dout.row + head * a.dout.head, live, a.D, g);
+  float base = live ? nl[head * a.qs.rows + at] : -__builtin_inff();
+  const float minus = live ? nd[head * a.qs.rows + at] : 0.f;
+  float lift = 0.f;
+  if (kLift<T> != 0.f) {
+    float sq = 0.f;
 #pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    const int64_t r = t.at + (wave * QT + u) * 32 + lane;
-    const bool live = r < t.len;
-    const int i = int(r / a.G);
-    head[u] = place.head * a.G + int(r - int64_t(i) * a.G);
-    row[u] = live ? i : -1;
-    seen[u] = CAUSAL ? keys_seen(i, Lq, Lk) : Lk;
-    const int64_t at = t.lo + i;
-    load_head<T, DP>(a.q.p + at * a.q.row + head[u] * a.q.head, live, a.D, q[u]);
-    load_head<T, DP>(a.dout.p + at * a.dout.row + head[u] * a.dout.head, live, a.D, g[u]);
-    base[u] = live ? nl[head[u] * a.qs.rows + at] : -__builtin_inff();
-    minus[u] = live ? nd[head[u] * a.qs.rows + at] : 0.f;
-    lift[u] = 0.f;
-    if (kLift<T> != 0.f) {
-      float sq = 0.f;
+    for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float v = to_f32(g[u][s][j]);
-          sq = __builtin_fmaf(v, v, sq);
-        }
-      lift[u] = lift_of(sq + other_half(sq), top_value);
-      base[u] += lift[u] - kLift<T>;
-    }
+      for (int j = 0; j < V; ++j) {
+        const float v = to_f32(g[s][j]);
+        sq = __builtin_fmaf(v, v, sq);
+      }
+    lift = lift_of(half_sum(sq), top_value);
+    base += lift - kLift<T>;
   }
   int most = Lk, wave_most = Lk, wave_least = Lk;
-  if (CAUSAL) {
-    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * QT * 32;
+  if (a.causal) {
+    const int64_t last = t.at + BQ < t.len ? t.at + BQ : t.len, w = t.at + wave * 32;
     most = keys_seen((last - 1) / a.G, Lq, Lk);
     wave_least = keys_seen(w / a.G, Lq, Lk);
-    wave_most = keys_seen((w + QT * 32 - 1) / a.G, Lq, Lk);
+    wave_most = keys_seen((w + 31) / a.G, Lq, Lk);
     wave_most = wave_most < most ? wave_most : most;
   }
   const int tiles = (most + BK - 1) / BK, per = (tiles + a.shares - 1) / a.shares;
@@ -199,99 +228,136 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dq(
 #pragma unroll
     for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
   }
-  floatx16 acc[QT][DP / 32];
+  floatx16 acc[TILES];
 #pragma unroll
-  for (int u = 0; u < QT; ++u)
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) zero(acc[u][d]);
-  if (first < end) {
-    lk.start(first * BK, lds);
-    lv.start(first * BK, lds + L::BYTES);
-  }
-  for (int n = first; n < end; ++n) {
-    char* buf = lds + ((n - first) & 1) * 2 * L::BYTES;
+  for (int d = 0; d < TILES; ++d) zero(acc[d]);
+  // A tile of keys in buffer B, in the order of attend_dkv's step.
+  auto step = [&](int n, auto buffer) {
+    char* buf = lds + buffer.value * 2 * L::BYTES;
     loads_in_flight<0>();
     __syncthreads();
     if (n + 1 < end) {
-      char* next = lds + ((n + 1 - first) & 1) * 2 * L::BYTES;
+      char* next = lds + (1 - buffer.value) * 2 * L::BYTES;
       lk.start((n + 1) * BK, next);
       lv.start((n + 1) * BK, next + L::BYTES);
     }
     const int key0 = n * BK;
-    if (CAUSAL && key0 >= wave_most) continue;
+    if (key0 >= wave_most) return;
     const bool edge = key0 + BK > wave_least;
+    floatx16 s[NX], dp[NX];
+    frag ds[NX][PS];
+    auto read = [&](int x) {
+      return [=](int i) { return L::read(buf + (i & 1) * L::BYTES, 32 * x, i >> 1); };
+    };
+    auto form = [&](int x, int i, const frag& f) {
+      if (i & 1)
+        Mfma<T>::mma(f, g[i >> 1], dp[x]);
+      else
+        Mfma<T>::mma(f, q[i >> 1], s[x]);
+    };
+    auto prepare = [&](int x) {
+      if (!edge) return;
 #pragma unroll
-    for (int x = 0; x < BK / 32; ++x) {
-      floatx16 s[QT], dp[QT];
+      for (int i = 0; i < 16; ++i)
+        if (key0 + 32 * x + acc_row<T>(i) >= seen) {
+          s[x][i] = -__builtin_inff();
+          dp[x][i] = 0.f;  // (not what a NaN there makes of it)
+        }
+    };
+    auto weigh = [&](int x, int lo, int hi) {
 #pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        zero(s[u]);
-        zero(dp[u]);
+      for (int i = lo; i < hi; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, base));
+        ds[x][i / V][i % V] = T(p * (dp[x][i] + minus));
       }
-      auto read = [&](int k) {
-        return Both<T>{L::read(buf, 32 * x, k), L::read(buf + L::BYTES, 32 * x, k)};
+    };
+    auto read_t = [&](int x) {
+      return [=](int i) {
+        return L::read_t(buf, 32 * x + i / TILES * Mfma<T>::KSTEP, 32 * (i % TILES));
       };
-      Batched<Both<T>, STEPS, 1> f;
-      f.start(read);
-      f.run(read, [&](int k, const Both<T>& kv) {
+    };
+    auto add = [&](int x, int i, const frag& f) {
+      Mfma<T>::mma(f, ds[x][i / TILES], acc[i % TILES]);
+    };
+    constexpr int FORM = 2 * STEPS, ADD = PS * TILES;
+    if constexpr (!dq_beside<T>(DP)) {
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-          Mfma<T>::mma(kv.a, q[u][k], s[u]);
-          Mfma<T>::mma(kv.b, g[u][k], dp[u]);
-        }
-      });
-#pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        frag ds[PS];
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (key0 + 32 * x + acc_row<T>(i) >= seen[u]) {
-              s[u][i] = -__builtin_inff();
-              dp[u][i] = 0.f;  // (not what a NaN there makes of it)
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, base[u]));
-          ds[i / V][i % V] = T(p * (dp[u][i] + minus[u]));
-        }
+      for (int x = 0; x < NX; ++x) {
+        zero(s[x]);
+        zero(dp[x]);
+        beside<frag, FORM, kAhead>(read(x), [&](int i, const frag& f) { form(x, i, f); });
+        prepare(x);
+        weigh(x, 0, 16);
         if (STRICT && edge)
-          add_rows_seen<T, DP, BK>(buf, 32 * x, 0, seen[u] - key0, ds, acc[u]);
+          add_rows_seen<T, DP, BK>(buf, 32 * x, 0, seen - key0, ds[x], acc);
         else
-          add_rows<T, DP, BK, kAttnBatch>(buf, 32 * x, ds, acc[u]);
+          beside<frag, ADD, kAhead>(read_t(x), [&](int i, const frag& f) { add(x, i, f); });
+      }
+      return;
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      zero(s[x]);
+      zero(dp[x]);
+    }
+    beside<frag, FORM, kAhead>(read(0), [&](int i, const frag& f) { form(0, i, f); });
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      prepare(x);
+      if (x + 1 < NX) {
+        beside<frag, FORM, kAhead>(read(x + 1), [&](int i, const frag& f) {
+          form(x + 1, i, f);
+          weigh(x, 16 * i / FORM, 16 * (i + 1) / FORM);
+        });
+      } else if (x > 0 && !(STRICT && edge)) {
+        beside<frag, ADD, kAhead>(read_t(x - 1), [&](int i, const frag& f) {
+          add(x - 1, i, f);
+          weigh(x, 16 * i / ADD, 16 * (i + 1) / ADD);
+        });
+      } else {
+        weigh(x, 0, 16);
       }
     }
+    if (STRICT && edge) {
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        add_rows_seen<T, DP, BK>(buf, 32 * x, 0, seen - key0, ds[x], acc);
+    } else {
+      beside<frag, ADD, kAhead>(read_t(NX - 1), [&](int i, const frag& f) { add(NX - 1, i, f); });
+    }
+  };
+  if (first < end) {
+    lk.start(first * BK, lds);
+    lv.start(first * BK, lds + L::BYTES);
+  }
+  for (int n = first; n < end; n += 2) {
+    step(n, std::integral_constant<int, 0>());
+    if (n + 1 < end) step(n + 1, std::integral_constant<int, 1>());
   }
   bool bad = false;
-  if (CAUSAL && !STRICT) {
-#pragma unroll
-    for (int u = 0; u < QT; ++u) bad |= any_not_finite(acc[u]);
-  }
+  if (CAUSAL && !STRICT) bad = any_not_finite(acc);
   report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
-#pragma unroll
-  for (int u = 0; u < QT; ++u) {
-    if (row[u] < 0) continue;
-    const int64_t r = t.lo + row[u];
-    const float f = a.scale * __builtin_amdgcn_exp2f(-lift[u]);
-    if (a.shares > 1) {
-      const int64_t at = (place.share * a.qs.rows + r) * a.H + head[u];
-      store_part<DP, V>(a.part + at * a.D, a.D, [&](int d, int i) { return acc[u][d][i] * f; });
-    } else {
-      store_head<T, DP>(a.dq.p + r * a.dq.row + head[u] * a.dq.head, a.D,
-                        [&](int d, int i) { return acc[u][d][i] * f; });
-    }
+  if (!live) return;
+  const float f = a.scale * __builtin_amdgcn_exp2f(-lift);
+  if (a.shares > 1) {
+    const int64_t i = (place.share * a.qs.rows + at) * a.H + head;
+    store_part<DP, V>(a.part + i * a.D, a.D, [&](int d, int j) { return acc[d][j] * f; });
+  } else {
+    store_head<T, DP>(a.dq.p + at * a.dq.row + head * a.dq.head, a.D,
+                      [&](int d, int j) { return acc[d][j] * f; });
   }
 }
 
 // A tile of keys goes through the queries of its head's G query heads, one head after the other.
-template <typename T, int DP, int KT, int BQ, bool CAUSAL, bool STRICT>
+template <typename T, int DP, int BQ, bool CAUSAL, bool STRICT>
 __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
     AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BQ>;
   constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
-  constexpr int BK = kAttnWaves * KT * 32, STAGE = 2 * L::BYTES + 2 * BQ * 4;
+  constexpr int TILES = DP / 32, NX = BQ / 32;
+  static_assert(NX <= 2, "a step holds one tile's weights while the next one's are formed");
+  constexpr int BK = kAttnWaves * 32, STAGE = 2 * L::BYTES + 2 * BQ * 4;
   static_assert(BQ <= 64, "a wave loads a tile's statistics at once");
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   __shared__ int bad_lds;
@@ -314,24 +380,20 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
     g = __builtin_amdgcn_exp2f(lift - kLift<T>);
   }
 
-  frag k[KT][STEPS], v[KT][STEPS];
-  int row[KT], from[KT];  // the key's place in its sequence; its first query
-#pragma unroll
-  for (int u = 0; u < KT; ++u) {
-    const int j = int(t.at) + (wave * KT + u) * 32 + lane;
-    row[u] = j < Lk ? j : -1;
-    from[u] = CAUSAL && j > Lk - Lq ? j - Lk + Lq : 0;
-    const int64_t at = t.lo + j;
-    load_head<T, DP>(a.k.p + at * a.k.row + place.head * a.k.head, j < Lk, a.D, k[u]);
-    load_head<T, DP>(a.v.p + at * a.v.row + place.head * a.v.head, j < Lk, a.D, v[u]);
-  }
+  // this lane's key: its place in its sequence, its first query
+  const int at = int(t.at) + wave * 32 + lane;
+  const bool live = at < Lk;
+  const int from = a.causal && at > Lk - Lq ? at - Lk + Lq : 0;
+  frag k[STEPS], v[STEPS];
+  load_head<T, DP>(a.k.p + (t.lo + at) * a.k.row + place.head * a.k.head, live, a.D, k);
+  load_head<T, DP>(a.v.p + (t.lo + at) * a.v.row + place.head * a.v.head, live, a.D, v);
   // first queries: of the workgroup's keys, of the wave's, of its last key
   int least = 0, wave_least = 0, wave_most = 0;
-  if (CAUSAL) {
-    const int shift = Lq - Lk, j = int(t.at) + wave * KT * 32;
+  if (a.causal) {
+    const int shift = Lq - Lk, j = int(t.at) + wave * 32;
     least = t.at + shift > 0 ? int(t.at) + shift : 0;
     wave_least = j + shift > 0 ? j + shift : 0;
-    wave_most = j + KT * 32 - 1 + shift > 0 ? j + KT * 32 - 1 + shift : 0;
+    wave_most = j + 31 + shift > 0 ? j + 31 + shift : 0;
   }
   const int begin = least / BQ, last = (Lq + BQ - 1) / BQ;  // tiles of a head
   const int64_t tiles = last > begin ? int64_t(last - begin) * a.G : 0;
@@ -366,17 +428,16 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
 #pragma unroll
     for (int i = 0; i < 4; ++i) lq.clear(lds + (i >> 1) * STAGE + (i & 1) * L::BYTES);
   }
-  floatx16 dk[KT][DP / 32], dv[KT][DP / 32];
+  floatx16 dk[TILES], dv[TILES];
 #pragma unroll
-  for (int u = 0; u < KT; ++u)
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) {
-      zero(dk[u][d]);
-      zero(dv[u][d]);
-    }
-  if (n < end) start(qh, qt, lds);
-  for (int stage = 0; n < end; ++n, stage ^= 1) {
-    char* buf = lds + stage * STAGE;
+  for (int d = 0; d < TILES; ++d) {
+    zero(dk[d]);
+    zero(dv[d]);
+  }
+  // A tile of queries in buffer B.  32 queries' scores and their gradients are formed beside the weights of the
+  // 32 before, and these are multiplied beside the weights of the next.
+  auto step = [&](auto buffer) {
+    char* buf = lds + buffer.value * STAGE;
     loads_in_flight<0>();
     __syncthreads();
     const int query0 = qt * BQ;
@@ -384,90 +445,141 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
       qt = begin;
       ++qh;
     }
-    if (n + 1 < end) start(qh, qt, lds + (stage ^ 1) * STAGE);
-    if (CAUSAL && query0 + BQ <= wave_least) continue;
-    const bool edge = CAUSAL && query0 < wave_most;
+    if (n + 1 < end) start(qh, qt, lds + (1 - buffer.value) * STAGE);
+    // (asked in either case: without these branches the compiler's order of the step takes more registers than
+    // there are, 176 bytes of scratch at 64 values a head and half the speed)
+    if (query0 + BQ <= wave_least) return;
+    const bool edge = query0 < wave_most;
     const float* stats = reinterpret_cast<const float*>(buf + 2 * L::BYTES);
+    floatx16 s[NX], dp[NX];
+    frag p[NX][PS], ds[NX][PS];
+    float4v base[2], minus[2];  // of four weights, and of the next four
+    auto read = [&](int x) {
+      return [=](int i) { return L::read(buf + (i & 1) * L::BYTES, 32 * x, i >> 1); };
+    };
+    auto form = [&](int x, int i, const frag& f) {
+      if (i & 1)
+        Mfma<T>::mma(f, v[i >> 1], dp[x]);
+      else
+        Mfma<T>::mma(f, k[i >> 1], s[x]);
+    };
+    // the weights of 32 queries: what they take, what of them is hidden, and weights lo .. hi - 1
+    auto take = [&](int x, int i) {
+      const int r = 32 * x + acc_row<T>(4 * i);
+      base[i & 1] = *reinterpret_cast<const float4v*>(stats + r);
+      minus[i & 1] = *reinterpret_cast<const float4v*>(stats + BQ + r);
+    };
+    auto prepare = [&](int x) {
+      take(x, 0);
+      if (!edge) return;
 #pragma unroll
-    for (int x = 0; x < BQ / 32; ++x) {
-      floatx16 s[KT], dp[KT];
+      for (int i = 0; i < 16; ++i)
+        if (query0 + 32 * x + acc_row<T>(i) < from) {
+          s[x][i] = -__builtin_inff();
+          dp[x][i] = 0.f;  // (not what a NaN there makes of it)
+        }
+    };
+    auto weigh = [&](int x, int lo, int hi) {
 #pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        zero(s[u]);
-        zero(dp[u]);
+      for (int i = lo; i < hi; ++i) {
+        if ((i & 3) == 0 && i < 12) take(x, (i >> 2) + 1);
+        const float e =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, base[i >> 2 & 1][i & 3]));
+        float d = dp[x][i] + minus[i >> 2 & 1][i & 3];
+        if (kLift<T> != 0.f) d *= g;
+        p[x][i / V][i % V] = T(e);
+        ds[x][i / V][i % V] = T(e * d);
       }
-      auto read = [&](int i) {
-        return Both<T>{L::read(buf, 32 * x, i), L::read(buf + L::BYTES, 32 * x, i)};
+    };
+    auto read_t = [&](int x) {
+      return [=](int i) {
+        return L::read_t(buf + (i & 1 ? 0 : L::BYTES),
+                         32 * x + (i >> 1) / TILES * Mfma<T>::KSTEP, 32 * ((i >> 1) % TILES));
       };
-      Batched<Both<T>, STEPS, 1> f;
-      f.start(read);
-      f.run(read, [&](int i, const Both<T>& qg) {
+    };
+    auto add = [&](int x, int i, const frag& f) {
+      const int d = (i >> 1) % TILES, w = (i >> 1) / TILES;
+      if (i & 1)
+        Mfma<T>::mma(f, ds[x][w], dk[d]);
+      else
+        Mfma<T>::mma(f, p[x][w], dv[d]);
+    };
+    constexpr int FORM = 2 * STEPS, ADD = 2 * PS * TILES;
+    if constexpr (!dkv_beside<T>(DP)) {
 #pragma unroll
-        for (int u = 0; u < KT; ++u) {
-          Mfma<T>::mma(qg.a, k[u][i], s[u]);
-          Mfma<T>::mma(qg.b, v[u][i], dp[u]);
-        }
-      });
-#pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        frag p[PS], ds[PS];
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (query0 + 32 * x + acc_row<T>(i) < from[u]) {
-              s[u][i] = -__builtin_inff();
-              dp[u][i] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int r = 32 * x + acc_row<T>(i);
-          const float4v base = *reinterpret_cast<const float4v*>(stats + r);
-          const float4v minus = *reinterpret_cast<const float4v*>(stats + BQ + r);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + j], c, base[j]));
-            float d = dp[u][i + j] + minus[j];
-            if (kLift<T> != 0.f) d *= g;
-            p[(i + j) / V][(i + j) % V] = T(e);
-            ds[(i + j) / V][(i + j) % V] = T(e * d);
-          }
-        }
+      for (int x = 0; x < NX; ++x) {
+        zero(s[x]);
+        zero(dp[x]);
+        beside<frag, FORM, kAhead>(read(x), [&](int i, const frag& f) { form(x, i, f); });
+        prepare(x);
+        weigh(x, 0, 16);
         if (STRICT && edge) {
-          add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from[u] - query0, BQ, p, dv[u]);
-          add_rows_seen<T, DP, BQ>(buf, 32 * x, from[u] - query0, BQ, ds, dk[u]);
+          add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from - query0, BQ, p[x], dv);
+          add_rows_seen<T, DP, BQ>(buf, 32 * x, from - query0, BQ, ds[x], dk);
         } else {
-          add_rows<T, DP, BQ, kAttnBatch>(buf + L::BYTES, 32 * x, p, dv[u]);
-          add_rows<T, DP, BQ, kAttnBatch>(buf, 32 * x, ds, dk[u]);
+          beside<frag, ADD, kAhead>(read_t(x), [&](int i, const frag& f) { add(x, i, f); });
         }
+      }
+      return;
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      zero(s[x]);
+      zero(dp[x]);
+    }
+    beside<frag, FORM, kAhead>(read(0), [&](int i, const frag& f) { form(0, i, f); });
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      prepare(x);
+      if (x + 1 < NX) {
+        beside<frag, FORM, kAhead>(read(x + 1), [&](int i, const frag& f) {
+          form(x + 1, i, f);
+          weigh(x, 16 * i / FORM, 16 * (i + 1) / FORM);
+        });
+      } else if (x > 0 && !(STRICT && edge)) {
+        beside<frag, ADD, kAhead>(read_t(x - 1), [&](int i, const frag& f) {
+          add(x - 1, i, f);
+          weigh(x, 16 * i / ADD, 16 * (i + 1) / ADD);
+        });
+      } else {
+        weigh(x, 0, 16);
       }
     }
+    if (STRICT && edge) {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from - query0, BQ, p[x], dv);
+        add_rows_seen<T, DP, BQ>(buf, 32 * x, from - query0, BQ, ds[x], dk);
+      }
+    } else {
+      beside<frag, ADD, kAhead>(read_t(NX - 1), [&](int i, const frag& f) { add(NX - 1, i, f); });
+    }
+  };
+  if (n < end) start(qh, qt, lds);
+  while (n < end) {
+    step(std::integral_constant<int, 0>());
+    if (++n == end) break;
+    step(std::integral_constant<int, 1>());
+    ++n;
   }
   bool bad = false;
-  if (CAUSAL && !STRICT) {
-#pragma unroll
-    for (int u = 0; u < KT; ++u) bad |= any_not_finite(dk[u]) || any_not_finite(dv[u]);
-  }
+  if (CAUSAL && !STRICT) bad = any_not_finite(dk) || any_not_finite(dv);
   report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+  if (!live) return;
   const float fk = a.scale * __builtin_amdgcn_exp2f(-lift), fv = __builtin_amdgcn_exp2f(-kLift<T>);
-#pragma unroll
-  for (int u = 0; u < KT; ++u) {
-    if (row[u] < 0) continue;
-    const int64_t r = t.lo + row[u];
-    if (a.shares > 1) {
-      float* to = a.part + (((place.share * 2) * a.ks.rows + r) * a.Hk + place.head) * a.D;
-      store_part<DP, V>(to, a.D, [&](int d, int i) { return dk[u][d][i] * fk; });
-      store_part<DP, V>(to + a.ks.rows * a.Hk * a.D, a.D,
-                        [&](int d, int i) { return dv[u][d][i] * fv; });
-      continue;
-    }
-    if (a.dk.p)
-      store_head<T, DP>(a.dk.p + r * a.dk.row + place.head * a.dk.head, a.D,
-                        [&](int d, int i) { return dk[u][d][i] * fk; });
-    if (a.dv.p)
-      store_head<T, DP>(a.dv.p + r * a.dv.row + place.head * a.dv.head, a.D,
-                        [&](int d, int i) { return dv[u][d][i] * fv; });
+  const int64_t r = t.lo + at;
+  if (a.shares > 1) {
+    float* to = a.part + (((place.share * 2) * a.ks.rows + r) * a.Hk + place.head) * a.D;
+    store_part<DP, V>(to, a.D, [&](int d, int i) { return dk[d][i] * fk; });
+    store_part<DP, V>(to + a.ks.rows * a.Hk * a.D, a.D, [&](int d, int i) { return dv[d][i] * fv; });
+    return;
   }
+  if (a.dk.p)
+    store_head<T, DP>(a.dk.p + r * a.dk.row + place.head * a.dk.head, a.D,
+                      [&](int d, int i) { return dk[d][i] * fk; });
+  if (a.dv.p)
+    store_head<T, DP>(a.dv.p + r * a.dv.row + place.head * a.dv.head, a.D,
+                      [&](int d, int i) { return dv[d][i] * fv; });
 }
 
 // out[r][h] = the sum of the shares' partials, which lie `stride` values apart, in their order.
@@ -492,8 +604,7 @@ __global__ __launch_bounds__(kAttnThreads) void attend_sum(const float* __restri
 }
 
 // ---- host ------------------------------------------------------------------------
-constexpr int kGradTiles = 1;  // tiles of 32 of its own axis a wave
-constexpr int kGradRows = kAttnWaves * kGradTiles * 32;
+constexpr int kGradRows = kAttnWaves * 32;
 
 AttnGradLayout attn_grad_layout(const Seqs& q, const Seqs& k, int H, int Hk, int D,
                                 bool causal) {
@@ -552,13 +663,13 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
     const int64_t groups = attn_groups(slots, a.Hk, a.shares);
     SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
     with_width(a.D, [&](auto w) {
-      constexpr int DP = w.value, N = kGradTiles, B = attn_stage<T>();
+      constexpr int DP = w.value, B = attn_stage<T>();
       const dim3 grid{unsigned(groups)}, block{kAttnThreads};
       if (!a.causal) {
-        attend_dq<T, DP, N, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dq<T, DP, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
       } else {
-        attend_dq<T, DP, N, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
-        attend_dq<T, DP, N, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dq<T, DP, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dq<T, DP, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
       }
       return 0;
     });
@@ -573,13 +684,13 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
     const int64_t groups = attn_groups(slots, a.Hk, a.shares);
     SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
     with_width(a.D, [&](auto w) {
-      constexpr int DP = w.value, N = kGradTiles, B = attn_stage<T>();
+      constexpr int DP = w.value, B = attn_stage<T>();
       const dim3 grid{unsigned(groups)}, block{kAttnThreads};
       if (!a.causal) {
-        attend_dkv<T, DP, N, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dkv<T, DP, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
       } else {
-        attend_dkv<T, DP, N, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
-        attend_dkv<T, DP, N, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dkv<T, DP, B, true, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
+        attend_dkv<T, DP, B, true, true><<<grid, block, 0, s>>>(a, nl, nd, slots);
       }
       return 0;
     });

@@ -34,7 +34,7 @@ struct Moments {
   __device__ __forceinline__ void join(float on, float omean, float om2) {
     const float all = n + on;
     if (on == 0.f) return;
-    const float d = omean - mean, w = on / all;
+    const float d = omean - mean, w = on * __builtin_amdgcn_rcpf(all);  // (one ulp of a weight)
     mean = __builtin_fmaf(d, w, mean);
     m2 += __builtin_fmaf(d * d, n * w, om2);
     n = all;
@@ -92,31 +92,43 @@ __device__ __forceinline__ void row_moments(const T* x, int64_t ldx, int64_t fir
   using vec = NormPiece<T, V>;
 #pragma unroll
   for (int i = 0; i < V; ++i) m[i] = Moments{0.f, 0.f, 0.f};
-  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
-    vec a[kNormRows];
-    int n = 0;
+  // (the next rows are loaded before these are summed)
+  vec a[2][kNormRows];
+  auto load = [&](vec (&to)[kNormRows], int64_t r) {
 #pragma unroll
     for (int j = 0; j < kNormRows; ++j) {
-      a[j] = vec{};
-      if (r + int64_t(j) * per < end) {
-        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
-        n = j + 1;
-      }
+      to[j] = vec{};
+      if (r + int64_t(j) * per < end)
+        to[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
     }
-    const float one = 1.f / float(n);
+  };
+  auto use = [&](const vec (&v)[kNormRows], int64_t r) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kNormRows; ++j) n += r + int64_t(j) * per < end;
+    if (n == 0) return;
+    const float one = __builtin_amdgcn_rcpf(float(n));
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float sum = 0.f, sq = 0.f;
 #pragma unroll
-      for (int j = 0; j < kNormRows; ++j) sum += to_f32(a[j].v[i]);
+      for (int j = 0; j < kNormRows; ++j) sum += to_f32(v[j].v[i]);
       const float mean = sum * one;
 #pragma unroll
       for (int j = 0; j < kNormRows; ++j) {
-        const float d = j < n ? to_f32(a[j].v[i]) - mean : 0.f;
+        const float d = j < n ? to_f32(v[j].v[i]) - mean : 0.f;
         sq = __builtin_fmaf(d, d, sq);
       }
       m[i].join(float(n), mean, sq);
     }
+  };
+  const int64_t step = int64_t(per) * kNormRows;
+  load(a[0], first);
+  for (int64_t r = first; r < end; r += 2 * step) {
+    load(a[1], r + step);
+    use(a[0], r);
+    load(a[0], r + 2 * step);
+    use(a[1], r + step);
   }
 }
 
@@ -203,13 +215,18 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats(NormArgs<T, P> a) {
   const PartChunks k = part_chunks(a.seqs, a.s.chunk, p);
   if (k.len == 0) return;
   Moments m{0.f, 0.f, 0.f};
-  const int64_t n = k.n * a.s.cg;
-  for (int64_t i = threadIdx.x; i < n; i += kNormThreads) {
-    const int64_t j = i / a.s.cg;
-    const int c = g * a.s.cg + int(i - j * a.s.cg);
-    const float2 v = a.part[(k.slot + j) * a.s.C + c];
-    m.join(float(j + 1 < k.n ? a.s.chunk : k.len - j * a.s.chunk), v.x, v.y);
-  }
+  // (neighbouring threads take a chunk's channels)
+  const int wide = a.s.cg < kNormThreads ? a.s.cg : kNormThreads, rows = kNormThreads / wide;
+  const int row = int(threadIdx.x) / wide;
+  if (row < rows)
+    for (int c = int(threadIdx.x) - row * wide; c < a.s.cg; c += wide) {
+      const float2* at = a.part + k.slot * a.s.C + g * a.s.cg + c;
+#pragma unroll 4
+      for (int j = row; j < int(k.n); j += rows) {
+        const float2 v = at[int64_t(j) * a.s.C];
+        m.join(float(j + 1 < k.n ? a.s.chunk : k.len - j * a.s.chunk), v.x, v.y);
+      }
+    }
   m = block_moments(m, lds);
   if (threadIdx.x == 0)
     a.stats[blockIdx.x] = float2{m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps)};
@@ -294,27 +311,39 @@ __device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, i
   constexpr bool FAST = sizeof(T) == 2;
 #pragma unroll
   for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
-    vec a[kNormRows], d[kNormRows];
+  vec a[2][kNormRows], d[2][kNormRows];
+  auto load = [&](int s, int64_t r) {
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j)
+    for (int j = 0; j < kNormRows; ++j) {
+      a[s][j] = d[s][j] = vec{};
       if (r + int64_t(j) * per < end) {
-        a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
-        d[j] = *reinterpret_cast<const vec*>(dy + (r + int64_t(j) * per) * lddy + c);
+        a[s][j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
+        d[s][j] = *reinterpret_cast<const vec*>(dy + (r + int64_t(j) * per) * lddy + c);
       }
+    }
+  };
+  auto use = [&](int s, int64_t r) {
 #pragma unroll
     for (int j = 0; j < kNormRows; ++j) {
       if (r + int64_t(j) * per >= end) break;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float u = (to_f32(a[j].v[i]) - k.mean[i]) * k.inv[i];
+        const float u = (to_f32(a[s][j].v[i]) - k.mean[i]) * k.inv[i];
         float value, slope;
         norm_act<FAST, ACT>(__builtin_fmaf(u, k.w[i], k.b[i]), value, slope);
-        const float dz = to_f32(d[j].v[i]) * slope;
+        const float dz = to_f32(d[s][j].v[i]) * slope;
         s1[i] += dz;
         s2[i] = __builtin_fmaf(dz, u, s2[i]);
       }
     }
+  };
+  const int64_t step = int64_t(per) * kNormRows;
+  load(0, first);
+  for (int64_t r = first; r < end; r += 2 * step) {
+    load(1, r + step);
+    use(0, r);
+    load(0, r + 2 * step);
+    use(1, r + step);
   }
 }
 

@@ -296,6 +296,8 @@ static int launch_linear(const Rows<T>& x, const Rows<T>& w, const LinearOut<T>&
 template <typename T, bool GRAD>
 static int run_linear(const Rows<T>& x, const Rows<T>& w, const LinearOut<T>& o, hipStream_t s) {
   if (!whole(x) || !whole(w)) return launch_linear<T, SmallTile, false, GRAD>(x, w, o, s);
+  if (x.K <= 4 * kStagePieces * Mfma<T>::V && fills<QuickTile>(x.n, cdiv(o.columns, QuickTile::W)))
+    return launch_linear<T, QuickTile, true, GRAD>(x, w, o, s);
   if (o.columns > 128 && fills<LargeTile>(x.n, cdiv(o.columns, LargeTile::W)))
     return launch_linear<T, LargeTile, true, GRAD>(x, w, o, s);
   if (fills<LongTile>(x.n, cdiv(o.columns, LongTile::W)))
