@@ -391,41 +391,48 @@ struct Place {
   int64_t slot;
   int head, share;
 };
-// (an XCD's workgroups are an eighth of the places in a row: those of a key head share its L2)
+// (an XCD's workgroups are an eighth of the places in a row: the tiles of a key head, or of a share of its keys,
+// are neighbours and meet in its L2)
 __device__ __forceinline__ bool find_place(int64_t slots, int heads, int shares, int64_t id,
                                            Place& p) {
   const int64_t total = slots * heads * shares, per = (total + 7) >> 3;
   const int64_t k = (id >> 3) < per ? (id & 7) * per + (id >> 3) : total;
   if (k >= total) return false;
-  const int64_t a = k / shares;
-  p.share = int(k - a * shares);
-  p.head = int(a / slots);
-  p.slot = a - p.head * slots;
+  const int64_t a = k / slots;
+  p.slot = k - a * slots;
+  p.share = int(a / heads);
+  p.head = int(a - int64_t(p.share) * heads);
   return true;
 }
 
 // ---- host ------------------------------------------------------------------------
 constexpr int kAttnMaxDim = 128;
+constexpr int kMostShares = 1024;
 
 // Rows of a tile that passes through LDS.
 template <typename T>
 constexpr int attn_stage() { return sizeof(T) == 4 ? 32 : 64; }
 
-// How many shares the other axis, of `len` rows on average, is cut into where `tiles` tiles do not fill
-// the CUs; a share keeps 256 rows.
-inline int attn_shares(int64_t tiles, int64_t len) {
-  const int64_t want = 768 / (tiles < 1 ? 1 : tiles), most = len / 256;
+// How many shares the other axis, of `len` rows on average, is cut into: where `tiles` tiles leave some of the
+// `groups` workgroups that are resident at a time without work, as many as make one round of them (800
+// rows of 4 heads of 64 over 2 x 30k keys: 864 workgroups for 768 places took 54 us, 768 of them, a share's tiles on
+// one XCD, 38); where the tiles are one round and a part of another, two (12k keys of 4 heads of 128, causal, whole training
+// step 1 113 us with one and 1 058 with two).  A share keeps 256 rows.
+inline int attn_shares(int64_t tiles, int64_t len, int groups) {
+  if (tiles < 1) tiles = 1;
+  const int64_t want = tiles > groups && tiles < 2 * groups ? 2 : groups / tiles, most = len / 256;
   const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : int(n);
+  return n < 1 ? 1 : n < kMostShares ? int(n) : kMostShares;
 }
+
+inline int64_t attn_sequences(const Seqs& s) { return s.off && s.parts > 2 ? s.parts - 2 : 1; }
 
 inline int64_t attn_tiles(const Seqs& s, int mult, int heads, int tile) {
-  return cdiv(s.rows * mult, tile) * heads;
+  const int64_t n = attn_sequences(s);
+  return cdiv(cdiv(s.rows, n) * mult, tile) * n * heads;
 }
 
-inline int64_t attn_length(const Seqs& s) {
-  return s.off && s.parts > 2 ? s.rows / (s.parts - 2) : s.rows;
-}
+inline int64_t attn_length(const Seqs& s) { return s.rows / attn_sequences(s); }
 
 // f(padded head width as a constant)
 template <typename F>
@@ -446,7 +453,7 @@ struct AttnGradLayout {
   int dq_shares, dkv_shares;
 };
 AttnGradLayout attn_grad_layout(const Seqs& q, const Seqs& k, int H, int Hk, int D,
-                                bool causal);
+                                bool causal, int32_t dtype);
 template <typename T>
 int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq, bool need_dkv,
                   hipStream_t s);

@@ -21,7 +21,7 @@ constexpr float kMostWeight = 16384.f;
 // Waves a SIMD.
 template <typename T>
 constexpr int attend_waves(int DP) {
-  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
+  return sizeof(T) == 4 ? (DP <= 32 ? 4 : DP <= 64 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
 }
 
 template <typename T, int DP, int BK, bool CAUSAL, bool STRICT>
@@ -121,8 +121,9 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP)) void attend(Attn
         }
       sum[0] += sum[1];
     };
-    weigh();
-    if (__ballot(sum[0] > kMostWeight || m == -__builtin_inff())) {
+    const bool fresh = __ballot(m == -__builtin_inff()) != 0;
+    if (!fresh) weigh();
+    if (fresh || __ballot(sum[0] > kMostWeight)) {
       float mx = s[0][0];
 #pragma unroll
       for (int x = 0; x < NK; ++x)
@@ -182,7 +183,6 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP)) void attend(Attn
 // The shares' results of a row and head joined, a workgroup each.  Every thread weighs some shares, then adds
 // up four values over some of them (one wave going through all shares by itself took 54 us for one
 // query's 8 heads of 32 in 96 shares, where the pass over 120k keys took 45).
-constexpr int kMostShares = 1024;
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attend_join(AttnArgs<T> a) {
   __shared__ float weight[kMostShares];
@@ -241,6 +241,37 @@ __global__ __launch_bounds__(kAttnThreads) void attend_join(AttnArgs<T> a) {
   }
 }
 
+// The same for few shares, four values a thread.
+constexpr int kFewShares = 16;
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attend_join_few(AttnArgs<T> a) {
+  const int quads = a.D / 4;
+  const int64_t n = a.qs.rows * a.H, i = int64_t(blockIdx.x) * kAttnThreads + threadIdx.x;
+  const int64_t at = i / quads;
+  if (at >= n) return;
+  const int c = int(i - at * quads) * 4;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at;
+  float m = -__builtin_inff();
+  for (int s = 0; s < a.shares; ++s) m = __builtin_fmaxf(m, ml[s * n].x);
+  const float safe = m == -__builtin_inff() ? 0.f : m;
+  float sum = 0.f;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.shares; ++s) {
+    const float2 o = ml[s * n];
+    const float w = __builtin_amdgcn_exp2f(o.x - safe);
+    sum = __builtin_fmaf(w, o.y, sum);
+    v += w * *reinterpret_cast<const float4v*>(a.part + (s * n + at) * a.D + c);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t r = at / a.H, h = at - r * a.H;
+  T* to = a.out.p + r * a.out.row + h * a.out.head + c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) to[j] = from_f32<T>(v[j] * inv);
+  if (a.lse && c == 0)
+    a.lse[h * a.qs.rows + r] = sum == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(sum);
+}
+
 // ---- host ------------------------------------------------------------------------
 constexpr int kForwardRows = kAttnWaves * 32;
 
@@ -262,9 +293,14 @@ static int launch_attend(AttnArgs<T> a, hipStream_t s) {
   });
   SP_LAUNCHED();
   if (a.shares == 1) return SP_OK;
-  const int64_t joins = a.qs.rows * a.H;
+  const bool few = a.shares <= kFewShares;
+  const int64_t rows = a.qs.rows * a.H;
+  const int64_t joins = few ? cdiv(rows * (a.D / 4), kAttnThreads) : rows;
   SP_CHECK_ARG(joins <= kMaxGridX, "attention: too many rows");
-  attend_join<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
+  if (few)
+    attend_join_few<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
+  else
+    attend_join<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
   SP_LAUNCHED();
   return SP_OK;
 }
@@ -336,6 +372,13 @@ static AttnArgs<T> arguments(const sp_attn& c) {
   return a;
 }
 
+// Workgroups that are resident at a time.
+static int forward_groups(int32_t dtype, int dim) {
+  return 256 * with_width(dim, [&](auto w) {
+    return dtype == SP_F32 ? attend_waves<float>(w.value) : attend_waves<__bf16>(w.value);
+  });
+}
+
 struct ForwardLayout {
   size_t part, ml, again, total;
   int shares;
@@ -345,7 +388,8 @@ static ForwardLayout forward_layout(const sp_attn& c) {
   const Seqs q = seqs(c.q_offsets, c.nq, c.sequences), k = seqs(c.k_offsets, c.nk, c.sequences);
   const int G = int(c.heads / c.kv_heads), Hk = int(c.kv_heads);
   ForwardLayout l{};
-  l.shares = attn_shares(attn_tiles(q, G, Hk, kForwardRows), attn_length(k));
+  l.shares = attn_shares(attn_tiles(q, G, Hk, kForwardRows), attn_length(k),
+                         forward_groups(c.dtype, int(c.dim)));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -421,7 +465,7 @@ extern "C" int sp_attention(const sp_attn* c, void* out, int64_t out_row, int64_
 static AttnGradLayout grad_layout(const sp_attn* c) {
   return attn_grad_layout(seqs(c->q_offsets, c->nq, c->sequences),
                           seqs(c->k_offsets, c->nk, c->sequences), int(c->heads),
-                          int(c->kv_heads), int(c->dim), c->causal != 0);
+                          int(c->kv_heads), int(c->dim), c->causal != 0, c->dtype);
 }
 
 extern "C" size_t sp_attention_bwd_workspace(const sp_attn* c) {

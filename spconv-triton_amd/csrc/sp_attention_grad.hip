@@ -20,6 +20,7 @@ constexpr int kGradLoads = 4;  // rows of a group of lanes at a time in attend_g
 constexpr int kTops = 512;  // workgroups of attend_grad_rows at most
 
 constexpr int kAhead = 3;  // operands on their way from LDS
+constexpr int kStats = 64;  // places of a tile's statistics, of each kind
 
 // Whether 32 rows' products are written beside the weights of the 32 rows before, with two tiles' scores in
 // registers.  That pays where a SIMD has one wave in any case (128 values a head, causal, fp16: dQ 451 us
@@ -33,11 +34,11 @@ constexpr bool dkv_beside(int DP) { return DP >= 64 || sizeof(T) == 4; }
 // Waves a SIMD.
 template <typename T>
 constexpr int dq_waves(int DP) {
-  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 1;
+  return sizeof(T) == 4 ? (DP <= 32 ? 4 : DP <= 64 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 1;
 }
 template <typename T>
 constexpr int grad_waves(int DP) {
-  return sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 2 : 1;
+  return sizeof(T) == 4 ? (DP <= 32 ? 3 : 1) : DP <= 32 ? 4 : DP <= 64 ? 2 : 1;
 }
 
 template <typename T>
@@ -357,8 +358,8 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
   constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;
   constexpr int TILES = DP / 32, NX = BQ / 32;
   static_assert(NX <= 2, "a step holds one tile's weights while the next one's are formed");
-  constexpr int BK = kAttnWaves * 32, STAGE = 2 * L::BYTES + 2 * BQ * 4;
-  static_assert(BQ <= 64, "a wave loads a tile's statistics at once");
+  constexpr int BK = kAttnWaves * 32, STAGE = 2 * L::BYTES + 2 * kStats * 4;
+  static_assert(BQ <= kStats, "a wave loads a tile's statistics at once");
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   __shared__ int bad_lds;
   Place place;
@@ -414,13 +415,18 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
     lg.p = g0 + (h0 + head) * a.dout.head;
     lq.start(tile * BQ, to);
     lg.start(tile * BQ, to + L::BYTES);
-    if (wave < 2 && lane64 < BQ) {
+    if (wave < 2) {
+      // (a whole wave, each lane by a selected address: a branch of some lanes here had the compiler save registers
+      // for those lanes only)
       const int r = tile * BQ + lane64;
-      const float* from_ =
-          r < Lq ? (wave ? nd : nl) + (h0 + head) * a.qs.rows + qlo + r : &g_no_row[wave];
+      const char* rows = uniform(reinterpret_cast<const char*>(
+          (wave ? nd : nl) + (h0 + head) * a.qs.rows + qlo));
+      const char* from_ = rows + unsigned(r < Lq ? r : 0) * 4;
+      from_ = r < Lq ? from_ : reinterpret_cast<const char*>(&g_no_row[wave]);
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)from_,
-          (__attribute__((address_space(3))) void*)(to + 2 * L::BYTES + wave * (BQ * 4)), 4, 0, 0);
+          (__attribute__((address_space(3))) void*)(to + 2 * L::BYTES + wave * (kStats * 4)), 4, 0,
+          0);
     }
   };
   const float c = a.scale2;
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
     auto take = [&](int x, int i) {
       const int r = 32 * x + acc_row<T>(4 * i);
       base[i & 1] = *reinterpret_cast<const float4v*>(stats + r);
-      minus[i & 1] = *reinterpret_cast<const float4v*>(stats + BQ + r);
+      minus[i & 1] = *reinterpret_cast<const float4v*>(stats + kStats + r);
     };
     auto prepare = [&](int x) {
       take(x, 0);
@@ -582,35 +588,48 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
                       [&](int d, int i) { return dv[d][i] * fv; });
 }
 
-// out[r][h] = the sum of the shares' partials, which lie `stride` values apart, in their order.
+// out[r][h] = the sum of the shares' partials, which lie `stride` values apart: four values a lane, four runs of
+// the shares summed apart and then in order (one lane for all of 54 shares took 18 us for 20 MB).
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attend_sum(const float* __restrict__ part,
                                                            int64_t stride, int shares,
                                                            int64_t rows, int heads, int D,
                                                            Heads<T> out) {
-  const int quads = D / 4;
-  const int64_t n = rows * heads * quads;
-  for (int64_t i = int64_t(blockIdx.x) * kAttnThreads + threadIdx.x; i < n;
-       i += int64_t(gridDim.x) * kAttnThreads) {
-    const int64_t at = i / quads, r = at / heads;
-    const int c = int(i - at * quads) * 4, h = int(at - r * heads);
-    float4v v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < shares; ++s)
-      v += *reinterpret_cast<const float4v*>(part + s * stride + at * D + c);
-    T* to = out.p + r * out.row + h * out.head + c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = from_f32<T>(v[j]);
+  __shared__ float4v lds[4][64];
+  const int lane = int(threadIdx.x) & 63, run = int(threadIdx.x) >> 6, quads = D / 4;
+  const int64_t i = int64_t(blockIdx.x) * 64 + lane, n = rows * heads * quads;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+  if (i < n) {
+    const int per = (shares + 3) / 4, end = (run + 1) * per < shares ? (run + 1) * per : shares;
+#pragma unroll 8
+    for (int s = run * per; s < end; ++s)
+      v += *reinterpret_cast<const float4v*>(part + s * stride + i * 4);
   }
+  lds[run][lane] = v;
+  __syncthreads();
+  if (run != 0 || i >= n) return;
+  v = ((lds[0][lane] + lds[1][lane]) + lds[2][lane]) + lds[3][lane];
+  const int64_t at = i / quads, r = at / heads;
+  T* to = out.p + r * out.row + (at - r * heads) * out.head + (i - at * quads) * 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) to[j] = from_f32<T>(v[j]);
 }
 
 // ---- host ------------------------------------------------------------------------
 constexpr int kGradRows = kAttnWaves * 32;
 
 AttnGradLayout attn_grad_layout(const Seqs& q, const Seqs& k, int H, int Hk, int D,
-                                bool causal) {
+                                bool causal, int32_t dtype) {
   AttnGradLayout l{};
-  l.dq_shares = attn_shares(attn_tiles(q, H / Hk, Hk, kGradRows), attn_length(k));
-  l.dkv_shares = attn_shares(attn_tiles(k, 1, Hk, kGradRows), attn_length(q) * (H / Hk));
+  with_width(D, [&](auto w) {
+    const bool f32 = dtype == SP_F32;
+    l.dq_shares = attn_shares(attn_tiles(q, H / Hk, Hk, kGradRows), attn_length(k),
+                              256 * (f32 ? dq_waves<float>(w.value) : dq_waves<__bf16>(w.value)));
+    l.dkv_shares =
+        attn_shares(attn_tiles(k, 1, Hk, kGradRows), attn_length(q) * (H / Hk),
+                    256 * (f32 ? grad_waves<float>(w.value) : grad_waves<__bf16>(w.value)));
+    return 0;
+  });
   size_t off = 0;
   auto take = [&](size_t floats) {
     const size_t at = off;
@@ -651,11 +670,13 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
   attend_grad_rows<T><<<unsigned(a.tops), kAttnThreads, 0, s>>>(a, lanes, nl, nd, tops);
   SP_LAUNCHED();
   auto sum = [&](const float* part, int64_t stride, int shares, int64_t n, int heads,
-                 const Heads<T>& out) {
-    if (!out.p) return;
-    const int64_t groups = cdiv(n * heads * (a.D / 4), kAttnThreads);
-    attend_sum<T><<<unsigned(groups < 4096 ? groups : 4096), kAttnThreads, 0, s>>>(
-        part, stride, shares, n, heads, a.D, out);
+                 const Heads<T>& out) -> int {
+    if (!out.p) return SP_OK;
+    const int64_t groups = cdiv(n * heads * (a.D / 4), 64);
+    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
+    attend_sum<T><<<unsigned(groups), kAttnThreads, 0, s>>>(part, stride, shares, n, heads, a.D, out);
+    SP_LAUNCHED();
+    return SP_OK;
   };
   if (need_dq) {
     const int64_t slots = tile_slots(a.qs, a.G, kGradRows);
@@ -675,8 +696,7 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
     });
     SP_LAUNCHED();
     if (a.shares > 1)
-      sum(a.part, a.qs.rows * a.H * a.D, a.shares, a.qs.rows, a.H, a.dq);
-    SP_LAUNCHED();
+      if (int rc = sum(a.part, a.qs.rows * a.H * a.D, a.shares, a.qs.rows, a.H, a.dq)) return rc;
   }
   if (need_dkv) {
     const int64_t slots = tile_slots(a.ks, 1, kGradRows);
@@ -697,10 +717,9 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
     SP_LAUNCHED();
     if (a.shares > 1) {
       const int64_t one = a.ks.rows * a.Hk * a.D;
-      sum(a.part, 2 * one, a.shares, a.ks.rows, a.Hk, a.dk);
-      sum(a.part + one, 2 * one, a.shares, a.ks.rows, a.Hk, a.dv);
+      if (int rc = sum(a.part, 2 * one, a.shares, a.ks.rows, a.Hk, a.dk)) return rc;
+      if (int rc = sum(a.part + one, 2 * one, a.shares, a.ks.rows, a.Hk, a.dv)) return rc;
     }
-    SP_LAUNCHED();
   }
   return SP_OK;
 }
