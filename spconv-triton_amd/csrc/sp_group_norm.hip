@@ -15,11 +15,12 @@
 namespace sp {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormRows = 4;       // rows of a thread at a time
+constexpr int kNormRows = 4;       // rows of a thread at a time; chunks are whole steps of them
 constexpr int kNormChunks = 1024;  // chunks that a call is cut into, about
-// Calls of so many values and parts at most go through one workgroup, in one launch: 60 x 64 fp16 ...
-constexpr int64_t kNormSmall = 16384;
-constexpr int kNormSmallParts = 3;
+// Calls of up to so many values take a workgroup of kSmallThreads a part, in one launch (the gradients of several
+// parts in two), for three of several workgroups.
+constexpr int64_t kNormSmall = 65536;
+constexpr int kSmallThreads = 512;
 
 enum { kActNone = 3 };  // beside the feed-forward block's activations
 
@@ -86,43 +87,43 @@ __device__ __forceinline__ NormLane norm_lane(const NormShape& s, int block) {
 }
 
 // Moments of V channels over rows first, first + per, ... below end.
-template <typename T, int V>
+template <int ROWS, typename T, int V>
 __device__ __forceinline__ void row_moments(const T* x, int64_t ldx, int64_t first, int64_t end,
                                             int per, int c, Moments (&m)[V]) {
   using vec = NormPiece<T, V>;
 #pragma unroll
   for (int i = 0; i < V; ++i) m[i] = Moments{0.f, 0.f, 0.f};
   // (the next rows are loaded before these are summed)
-  vec a[2][kNormRows];
-  auto load = [&](vec (&to)[kNormRows], int64_t r) {
+  vec a[2][ROWS];
+  auto load = [&](vec (&to)[ROWS], int64_t r) {
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       to[j] = vec{};
       if (r + int64_t(j) * per < end)
         to[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
     }
   };
-  auto use = [&](const vec (&v)[kNormRows], int64_t r) {
+  auto use = [&](const vec (&v)[ROWS], int64_t r) {
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) n += r + int64_t(j) * per < end;
+    for (int j = 0; j < ROWS; ++j) n += r + int64_t(j) * per < end;
     if (n == 0) return;
     const float one = __builtin_amdgcn_rcpf(float(n));
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float sum = 0.f, sq = 0.f;
 #pragma unroll
-      for (int j = 0; j < kNormRows; ++j) sum += to_f32(v[j].v[i]);
+      for (int j = 0; j < ROWS; ++j) sum += to_f32(v[j].v[i]);
       const float mean = sum * one;
 #pragma unroll
-      for (int j = 0; j < kNormRows; ++j) {
+      for (int j = 0; j < ROWS; ++j) {
         const float d = j < n ? to_f32(v[j].v[i]) - mean : 0.f;
         sq = __builtin_fmaf(d, d, sq);
       }
       m[i].join(float(n), mean, sq);
     }
   };
-  const int64_t step = int64_t(per) * kNormRows;
+  const int64_t step = int64_t(per) * ROWS;
   load(a[0], first);
   for (int64_t r = first; r < end; r += 2 * step) {
     load(a[1], r + step);
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_moments(NormArgs<T, P> a) {
   const int width = a.s.L * V;
   if (l.on) {
     Moments m[V];
-    row_moments<T, V>(a.x + t.lo * a.ldx, a.ldx, t.at + l.row, end, a.s.per, l.c, m);
+    row_moments<kNormRows, T, V>(a.x + t.lo * a.ldx, a.ldx, t.at + l.row, end, a.s.per, l.c, m);
     const int at = l.c - int(blockIdx.y) * width;
 #pragma unroll
     for (int i = 0; i < V; ++i) lds[l.row * width + at + i] = float2{m[i].mean, m[i].m2};
@@ -251,19 +252,19 @@ struct NormChannels {
 };
 
 // f(pointer offset row) over a thread's rows, kNormRows at a time.
-template <typename T, int V, int ACT>
+template <int ROWS, typename T, int V, int ACT>
 __device__ __forceinline__ void norm_rows(const T* x, int64_t ldx, T* y, int64_t ldy, int64_t first,
                                           int64_t end, int per, int c, const NormChannels<V>& k) {
   using vec = NormPiece<T, V>;
   constexpr bool FAST = sizeof(T) == 2;
-  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
-    vec a[kNormRows];
+  for (int64_t r = first; r < end; r += int64_t(per) * ROWS) {
+    vec a[ROWS];
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (r + int64_t(j) * per < end)
         a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       if (r + int64_t(j) * per >= end) break;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -297,12 +298,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply(NormArgs<T, P> a) {
     return;
   }
   const NormChannels<V> k(a.s, a.stats + int64_t(t.part) * a.s.groups, a.w, a.b, l.c);
-  norm_rows<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, y, a.s.C, t.at + l.row, end, a.s.per, l.c, k);
+  norm_rows<kNormRows, T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, y, a.s.C, t.at + l.row, end, a.s.per, l.c, k);
 }
 
 // ---- gradients ---------------------------------------------------------------------
 // Sums of dz and dz u of V channels over rows first, first + per, ...
-template <typename T, int V, int ACT>
+template <int ROWS, typename T, int V, int ACT>
 __device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, int64_t lddy,
                                          int64_t first, int64_t end, int per, int c,
                                          const NormChannels<V>& k, float (&s1)[V],
@@ -311,10 +312,10 @@ __device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, i
   constexpr bool FAST = sizeof(T) == 2;
 #pragma unroll
   for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-  vec a[2][kNormRows], d[2][kNormRows];
+  vec a[2][ROWS], d[2][ROWS];
   auto load = [&](int s, int64_t r) {
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       a[s][j] = d[s][j] = vec{};
       if (r + int64_t(j) * per < end) {
         a[s][j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
@@ -324,7 +325,7 @@ __device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, i
   };
   auto use = [&](int s, int64_t r) {
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       if (r + int64_t(j) * per >= end) break;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -337,7 +338,7 @@ __device__ __forceinline__ void row_sums(const T* x, int64_t ldx, const T* dy, i
       }
     }
   };
-  const int64_t step = int64_t(per) * kNormRows;
+  const int64_t step = int64_t(per) * ROWS;
   load(0, first);
   for (int64_t r = first; r < end; r += 2 * step) {
     load(1, r + step);
@@ -355,23 +356,23 @@ __device__ __forceinline__ float less(float a, float b, float c) {
   return p - c;
 }
 
-template <typename T, int V, int ACT>
+template <int ROWS, typename T, int V, int ACT>
 __device__ __forceinline__ void grad_rows(const T* x, int64_t ldx, const T* dy, int64_t lddy, T* dx,
                                           int64_t lddx, int64_t first, int64_t end, int per, int c,
                                           const NormChannels<V>& k, const float (&m1)[V],
                                           const float (&m2)[V]) {
   using vec = NormPiece<T, V>;
   constexpr bool FAST = sizeof(T) == 2;
-  for (int64_t r = first; r < end; r += int64_t(per) * kNormRows) {
-    vec a[kNormRows], d[kNormRows];
+  for (int64_t r = first; r < end; r += int64_t(per) * ROWS) {
+    vec a[ROWS], d[ROWS];
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j)
+    for (int j = 0; j < ROWS; ++j)
       if (r + int64_t(j) * per < end) {
         a[j] = *reinterpret_cast<const vec*>(x + (r + int64_t(j) * per) * ldx + c);
         d[j] = *reinterpret_cast<const vec*>(dy + (r + int64_t(j) * per) * lddy + c);
       }
 #pragma unroll
-    for (int j = 0; j < kNormRows; ++j) {
+    for (int j = 0; j < ROWS; ++j) {
       if (r + int64_t(j) * per >= end) break;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -386,8 +387,9 @@ __device__ __forceinline__ void grad_rows(const T* x, int64_t ldx, const T* dy, 
   }
 }
 
+// (two rows a thread and twice as many on their way: with four, 194 registers, a CU holds half as many workgroups)
 template <typename T, typename P, int V, int ACT>
-__global__ __launch_bounds__(kNormThreads) void norm_grad_sums(NormArgs<T, P> a) {
+__global__ __launch_bounds__(kNormThreads, 4) void norm_grad_sums(NormArgs<T, P> a) {
   __shared__ float2 lds[kNormThreads * V];
   const Tile t = find_tile(a.seqs, 1, int(a.s.chunk), blockIdx.x);
   if (t.at >= t.len || a.seqs.outside(t.part)) return;
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_sums(NormArgs<T, P> a)
   if (l.on) {
     const NormChannels<V> k(a.s, a.stats + int64_t(t.part) * a.s.groups, a.w, a.b, l.c);
     float s1[V], s2[V];
-    row_sums<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, t.at + l.row, end,
+    row_sums<2, T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, t.at + l.row, end,
                         a.s.per, l.c, k, s1, s2);
     const int at = l.c - int(blockIdx.y) * width;
 #pragma unroll
@@ -492,136 +494,147 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_apply(NormArgs<T, P> a
     m1[i] = v.x;
     m2[i] = v.y;
   }
-  grad_rows<T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, dx, a.s.C,
+  grad_rows<kNormRows, T, V, ACT>(a.x + t.lo * a.ldx, a.ldx, a.dy + t.lo * a.lddy, a.lddy, dx, a.s.C,
                        t.at + l.row, end, a.s.per, l.c, k, m1, m2);
 }
 
-// ---- small calls: one workgroup, part after part -------------------------------------
+// ---- small calls: a workgroup a part -------------------------------------------------
 template <typename T, typename P, int V, int ACT>
-__global__ __launch_bounds__(kNormThreads) void norm_small(NormArgs<T, P> a) {
-  __shared__ float2 lds[kNormThreads * V];
-  __shared__ float counts[kNormThreads];
+__global__ __launch_bounds__(kSmallThreads) void norm_small(NormArgs<T, P> a) {
+  __shared__ float2 lds[kSmallThreads * V];
+  __shared__ float counts[kSmallThreads];
   const NormLane l = norm_lane<V>(a.s, 0);
-  const int width = a.s.L * V;
-  for (int p = 0; p < a.seqs.parts; ++p) {
-    const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
-    if (len == 0) continue;
-    if (a.seqs.outside(p)) {
-      if (l.on) zero_rows<T, V>(a.y + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c);
-      continue;
-    }
-    if (l.on) {
-      Moments m[V];
-      row_moments<T, V>(a.x + lo * a.ldx, a.ldx, l.row, len, a.s.per, l.c, m);
-#pragma unroll
-      for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{m[i].mean, m[i].m2};
-      if (l.c == 0) counts[l.row] = m[0].n;
-    }
-    __syncthreads();
-    for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
-      const Moments m = column_moments(lds, counts, a.s.per, width, c);
-      lds[c] = float2{m.mean, m.m2};  // (its own column's first place)
-    }
-    __syncthreads();
-    float2* stats = a.stats + int64_t(p) * a.s.groups;
-    for (int g = int(threadIdx.x); g < a.s.groups; g += kNormThreads) {
-      Moments m{0.f, 0.f, 0.f};
-      for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) m.join(float(len), lds[c].x, lds[c].y);
-      stats[g] = float2{m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps)};
-    }
-    __syncthreads();  // (which makes the workgroup's own stores to memory visible to it)
-    if (l.on) {
-      const NormChannels<V> k(a.s, stats, a.w, a.b, l.c);
-      norm_rows<T, V, ACT>(a.x + lo * a.ldx, a.ldx, a.y + lo * a.s.C, a.s.C, l.row, len, a.s.per,
-                           l.c, k);
-    }
+  const int width = a.s.L * V, p = int(blockIdx.x);
+  const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
+  if (len == 0) return;
+  T* y = a.y + lo * a.s.C;
+  if (a.seqs.outside(p)) {
+    if (l.on) zero_rows<T, V>(y, a.s.C, l.row, len, a.s.per, l.c);
+    return;
   }
+  const T* x = a.x + lo * a.ldx;
+  if (l.on) {
+    Moments m[V];
+    row_moments<2, T, V>(x, a.ldx, l.row, len, a.s.per, l.c, m);
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{m[i].mean, m[i].m2};
+    if (l.c == 0) counts[l.row] = m[0].n;
+  }
+  __syncthreads();
+  for (int c = int(threadIdx.x); c < a.s.C; c += kSmallThreads) {
+    const Moments m = column_moments(lds, counts, a.s.per, width, c);
+    lds[c] = float2{m.mean, m.m2};  // (its own column's first place)
+  }
+  __syncthreads();
+  float2* stats = a.stats + int64_t(p) * a.s.groups;
+  for (int g = int(threadIdx.x); g < a.s.groups; g += kSmallThreads) {
+    Moments m{0.f, 0.f, 0.f};
+    for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) m.join(float(len), lds[c].x, lds[c].y);
+    stats[g] = float2{m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps)};
+  }
+  __syncthreads();  // (which makes the workgroup's own stores to memory visible to it)
+  if (!l.on) return;
+  const NormChannels<V> k(a.s, stats, a.w, a.b, l.c);
+  norm_rows<2, T, V, ACT>(x, a.ldx, y, a.s.C, l.row, len, a.s.per, l.c, k);
 }
 
 template <typename T, typename P, int V, int ACT>
-__global__ __launch_bounds__(kNormThreads) void norm_grad_small(NormArgs<T, P> a) {
-  __shared__ float2 lds[kNormThreads * V];
-  __shared__ float2 total[kNormThreads * V];
+__global__ __launch_bounds__(kSmallThreads) void norm_grad_small(NormArgs<T, P> a) {
+  __shared__ float2 lds[kSmallThreads * V];
   const NormLane l = norm_lane<V>(a.s, 0);
-  const int width = a.s.L * V;
-  for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) total[c] = float2{0.f, 0.f};
-  for (int p = 0; p < a.seqs.parts; ++p) {
-    const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
-    if (len == 0) continue;
-    if (a.seqs.outside(p)) {
-      if (l.on && a.dx) zero_rows<T, V>(a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c);
-      continue;
-    }
-    const float2* stats = a.stats + int64_t(p) * a.s.groups;
-    const NormChannels<V> k(a.s, stats, a.w, a.b, l.on ? l.c : 0);
-    const T* x = a.x + lo * a.ldx;
-    const T* dy = a.dy + lo * a.lddy;
-    __syncthreads();
-    if (l.on) {
-      float s1[V], s2[V];
-      row_sums<T, V, ACT>(x, a.ldx, dy, a.lddy, l.row, len, a.s.per, l.c, k, s1, s2);
+  const int width = a.s.L * V, p = int(blockIdx.x);
+  const int64_t lo = a.seqs.bound(p), hi = a.seqs.bound(p + 1), len = hi > lo ? hi - lo : 0;
+  const bool outside = a.seqs.outside(p);
+  if (len == 0 || outside) {
+    if (outside && l.on && a.dx)
+      zero_rows<T, V>(a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c);
+    if (a.seqs.parts > 1)
+      for (int c = int(threadIdx.x); c < a.s.C; c += kSmallThreads)
+        a.sums[int64_t(p) * a.s.C + c] = float2{0.f, 0.f};
+    return;
+  }
+  const NormChannels<V> k(a.s, a.stats + int64_t(p) * a.s.groups, a.w, a.b, l.on ? l.c : 0);
+  const T* x = a.x + lo * a.ldx;
+  const T* dy = a.dy + lo * a.lddy;
+  if (l.on) {
+    float s1[V], s2[V];
+    row_sums<2, T, V, ACT>(x, a.ldx, dy, a.lddy, l.row, len, a.s.per, l.c, k, s1, s2);
 #pragma unroll
-      for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{s1[i], s2[i]};
+    for (int i = 0; i < V; ++i) lds[l.row * width + l.c + i] = float2{s1[i], s2[i]};
+  }
+  __syncthreads();
+  for (int c = int(threadIdx.x); c < a.s.C; c += kSmallThreads) {
+    float2 v{0.f, 0.f};
+    for (int r = 0; r < a.s.per; ++r) {
+      v.x += lds[r * width + c].x;
+      v.y += lds[r * width + c].y;
     }
-    __syncthreads();
-    for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
-      float2 v{0.f, 0.f};
-      for (int r = 0; r < a.s.per; ++r) {
-        v.x += lds[r * width + c].x;
-        v.y += lds[r * width + c].y;
-      }
-      lds[c] = v;
-      total[c].x += v.x;
-      total[c].y += v.y;
-    }
-    __syncthreads();
-    if (l.on && a.dx) {
-      const float count = float(len) * float(a.s.cg);
-      float m1[V], m2[V];
-      int at = -1;
-      float2 all{0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int g = (l.c + i) / a.s.cg;
-        if (g != at) {
-          all = float2{0.f, 0.f};
-          for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) {
-            const float w = a.w ? to_f32(a.w[c]) : 1.f;
-            all.x = __builtin_fmaf(lds[c].x, w, all.x);
-            all.y = __builtin_fmaf(lds[c].y, w, all.y);
-          }
-          at = g;
-        }
-        m1[i] = all.x / count;
-        m2[i] = all.y / count;
-      }
-      grad_rows<T, V, ACT>(x, a.ldx, dy, a.lddy, a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c,
-                           k, m1, m2);
+    lds[c] = v;  // (its own column's first place)
+    if (a.seqs.parts > 1) {
+      a.sums[int64_t(p) * a.s.C + c] = v;
+    } else {
+      if (a.dw) a.dw[c] = from_f32<P>(v.y);
+      if (a.db) a.db[c] = from_f32<P>(v.x);
     }
   }
   __syncthreads();
-  for (int c = int(threadIdx.x); c < a.s.C; c += kNormThreads) {
-    if (a.dw) a.dw[c] = from_f32<P>(total[c].y);
-    if (a.db) a.db[c] = from_f32<P>(total[c].x);
+  if (!l.on || !a.dx) return;
+  const float count = float(len) * float(a.s.cg);
+  float m1[V], m2[V];
+  int at = -1;
+  float2 all{0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int g = (l.c + i) / a.s.cg;
+    if (g != at) {
+      all = float2{0.f, 0.f};
+      for (int c = g * a.s.cg; c < (g + 1) * a.s.cg; ++c) {
+        const float w = a.w ? to_f32(a.w[c]) : 1.f;
+        all.x = __builtin_fmaf(lds[c].x, w, all.x);
+        all.y = __builtin_fmaf(lds[c].y, w, all.y);
+      }
+      at = g;
+    }
+    m1[i] = all.x / count;
+    m2[i] = all.y / count;
   }
+  grad_rows<2, T, V, ACT>(x, a.ldx, dy, a.lddy, a.dx + lo * a.s.C, a.s.C, l.row, len, a.s.per, l.c, k,
+                          m1, m2);
+}
+
+// The parameters' gradients from the parts' sums.
+template <typename T, typename P>
+__global__ __launch_bounds__(kNormThreads) void norm_grad_params(NormArgs<T, P> a) {
+  const int c = int(blockIdx.x) * kNormThreads + int(threadIdx.x);
+  if (c >= a.s.C) return;
+  float2 v{0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < a.seqs.parts; ++p) {
+    const float2 o = a.sums[int64_t(p) * a.s.C + c];
+    v.x += o.x;
+    v.y += o.y;
+  }
+  if (a.dw) a.dw[c] = from_f32<P>(v.y);
+  if (a.db) a.db[c] = from_f32<P>(v.x);
 }
 
 // ---- host ------------------------------------------------------------------------
-static NormShape norm_shape(int64_t rows, int C, int groups, int V) {
+static NormShape norm_shape(int64_t rows, int C, int groups, int V, int threads = kNormThreads) {
   NormShape s{};
   s.C = C;
   s.groups = groups;
   s.cg = C / groups;
-  s.L = C / V < kNormThreads ? C / V : kNormThreads;
-  s.per = kNormThreads / s.L;
+  s.L = C / V < threads ? C / V : threads;
+  s.per = threads / s.L;
   s.blocks = int(cdiv(C, s.L * V));
   const int64_t step = int64_t(s.per) * kNormRows;
   s.chunk = cdiv(cdiv(rows, kNormChunks), step) * step;
   return s;
 }
 
-static bool norm_is_small(int64_t rows, const NormShape& s, const Seqs& q) {
-  return rows * s.C <= kNormSmall && q.parts <= kNormSmallParts && s.blocks == 1;
+// (a row that is wider than a workgroup goes by blocks of its channels)
+static bool norm_is_small(int64_t rows, int64_t C, int V) {
+  return rows * C <= kNormSmall && C <= kSmallThreads * V;
 }
 
 static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
@@ -631,12 +644,12 @@ static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
 // (the sizes do not depend on V, which the tensors' addresses decide)
 static size_t norm_workspace(int64_t rows, int64_t C, int64_t groups, const Seqs& q, int V,
                              bool grad) {
+  const size_t sums = align_up(size_t(q.parts) * C * sizeof(float2), 256);
+  if (norm_is_small(rows, C, V)) return grad && q.parts > 1 ? sums : 0;
   const NormShape s = norm_shape(rows, int(C), int(groups), V);
-  if (norm_is_small(rows, s, q)) return 0;
   size_t n = align_up(size_t(tile_slots(q, 1, int(s.chunk))) * C * sizeof(float2), 256);
   if (grad)
-    n += align_up(size_t(q.parts) * C * sizeof(float2), 256) +
-         align_up(size_t(q.parts) * groups * sizeof(float2), 256);
+    n += sums + align_up(size_t(q.parts) * groups * sizeof(float2), 256);
   return n;
 }
 
@@ -652,15 +665,16 @@ static int norm_act_of(int act, F&& f) {
 
 template <typename T, typename P, int V>
 static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
-  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
-  if (norm_is_small(a.seqs.rows, a.s, a.seqs)) {
+  if (norm_is_small(a.seqs.rows, a.s.C, V)) {
+    a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
     norm_act_of(act, [&](auto k) {
-      norm_small<T, P, V, k.value><<<1, kNormThreads, 0, st>>>(a);
+      norm_small<T, P, V, k.value><<<unsigned(a.seqs.parts), kSmallThreads, 0, st>>>(a);
       return 0;
     });
     SP_LAUNCHED();
     return SP_OK;
   }
+  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
   const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
   const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
   SP_CHECK_ARG(slots <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
@@ -680,15 +694,20 @@ static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
 
 template <typename T, typename P, int V>
 static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
-  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
-  if (norm_is_small(a.seqs.rows, a.s, a.seqs)) {
+  if (norm_is_small(a.seqs.rows, a.s.C, V)) {
+    a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
+    a.sums = reinterpret_cast<float2*>(ws);
     norm_act_of(act, [&](auto k) {
-      norm_grad_small<T, P, V, k.value><<<1, kNormThreads, 0, st>>>(a);
+      norm_grad_small<T, P, V, k.value><<<unsigned(a.seqs.parts), kSmallThreads, 0, st>>>(a);
       return 0;
     });
     SP_LAUNCHED();
+    if (a.seqs.parts == 1 || !(a.dw || a.db)) return SP_OK;
+    norm_grad_params<T, P><<<unsigned(cdiv(a.s.C, kNormThreads)), kNormThreads, 0, st>>>(a);
+    SP_LAUNCHED();
     return SP_OK;
   }
+  a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
   const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
   const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
   const int64_t extra = cdiv(a.s.C, kNormThreads);

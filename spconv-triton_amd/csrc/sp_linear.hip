@@ -170,7 +170,10 @@ struct LinearGram {
   const T *a, *b;
   int64_t lda, ldb;
   int P, Q, tiles_q, tiles, vec_a, vec_b;
-  float *part, *part_b;  // [shares][P][Q], [shares][P]
+  float* part;           // [shares][P][Q], then P sums of rows, `stride` values a share
+  int64_t stride;
+  T *dw, *db;            // each nullable; written by the one share, where there is only one
+  int bias;
 };
 
 template <typename T, int TP, int TQ>
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
   const int p0 = tile / g.tiles_q * TP, q0 = tile % g.tiles_q * TQ;
   const int64_t hi = lo + share < rows ? lo + share : rows;
   const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 64, wq = (wave & 1) * (TQ / 2);
-  const bool sums = g.part_b && q0 == 0 && wq == 0;
+  const bool sums = g.bias && q0 == 0 && wq == 0;
   floatx16 acc[NP][NQ], accb[NP][1];
   clear(acc);
   clear(accb);
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
       }
     });
   }
-  const int64_t at = lo / share;
+  float* part = g.part + lo / share * g.stride;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
 #pragma unroll
   for (int i = 0; i < NP; ++i)
@@ -241,36 +244,54 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
     for (int k = 0; k < 16; ++k) {
       const int p = p0 + wp + 32 * i + (k & 3) + 8 * (k >> 2) + 4 * half;
       if (p >= g.P) continue;
+      const int64_t row = int64_t(p) * g.Q;
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         const int q = q0 + wq + 32 * j + lane;
-        if (q < g.Q) g.part[(at * g.P + p) * g.Q + q] = acc[i][j][k];
+        if (q >= g.Q) continue;
+        if (shares > 1)
+          part[row + q] = acc[i][j][k];
+        else if (g.dw)
+          g.dw[row + q] = from_f32<T>(acc[i][j][k]);
       }
-      if (sums && lane == 0) g.part_b[at * g.P + p] = accb[i][0][k];
+      if (!sums || lane != 0) continue;
+      if (shares > 1)
+        part[int64_t(g.P) * g.Q + p] = accb[i][0][k];
+      else
+        g.db[p] = from_f32<T>(accb[i][0][k]);
     }
 }
 
-// dW and db from their partials, V values a lane, four runs of the shares summed apart and then in order.
+// dW (n values) and db (behind it, m) from their partials, V values a lane, four runs of the shares summed apart and
+// then in order.
 template <typename T, int V>
 __global__ __launch_bounds__(kFfnThreads) void linear_reduce(const float* __restrict__ part,
-                                                             int64_t n, int shares,
-                                                             T* __restrict__ dst) {
+                                                             int64_t stride, int64_t n, int m,
+                                                             int shares, T* __restrict__ dw,
+                                                             T* __restrict__ db) {
   typedef float vec __attribute__((ext_vector_type(V)));
   __shared__ vec lds[4][64];
   const int lane = int(threadIdx.x) & 63, run = int(threadIdx.x) >> 6;
   const int64_t i = (int64_t(blockIdx.x) * 64 + lane) * V;
+  const bool in = i < n ? dw != nullptr : db && i < n + m;  // (V divides n)
   vec v = vec(0.f);
-  if (i < n) {
+  if (in) {
     const int per = (shares + 3) / 4, end = (run + 1) * per < shares ? (run + 1) * per : shares;
 #pragma unroll 8
-    for (int s = run * per; s < end; ++s) v += *reinterpret_cast<const vec*>(part + int64_t(s) * n + i);
+    for (int s = run * per; s < end; ++s)
+      v += *reinterpret_cast<const vec*>(part + int64_t(s) * stride + i);
   }
   lds[run][lane] = v;
   __syncthreads();
-  if (run != 0 || i >= n) return;
+  if (run != 0 || !in) return;
   v = ((lds[0][lane] + lds[1][lane]) + lds[2][lane]) + lds[3][lane];
 #pragma unroll
-  for (int k = 0; k < V; ++k) dst[i + k] = from_f32<T>(v[k]);
+  for (int k = 0; k < V; ++k) {
+    if (i < n)
+      dw[i + k] = from_f32<T>(v[k]);
+    else if (i + k < n + m)
+      db[i - n + k] = from_f32<T>(v[k]);
+  }
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -334,9 +355,9 @@ static int linear_forward(const LinearCall& c) {
 
 // The backward pass's workspace: dz, W transposed, the partials of dW and db.
 struct LinearLayout {
-  size_t dz, wt, part, part_b, total;
+  size_t dz, wt, part, total;
   int Cop;
-  int64_t shares;
+  int64_t shares, stride;  // values of a share's partials
 };
 
 static int64_t linear_gram_tiles(int64_t Co, int64_t C, int t) { return cdiv(Co, t) * cdiv(C, t); }
@@ -359,22 +380,10 @@ static LinearLayout linear_layout(int32_t dtype, int64_t rows, int64_t C, int64_
   };
   if (act != kActNone) l.dz = take(size_t(rows) * l.Cop * z);
   l.wt = take(size_t(C) * l.Cop * z);
-  l.part = take(size_t(l.shares) * Co * C * sizeof(float));
-  l.part_b = take(size_t(l.shares) * Co * sizeof(float));
+  l.stride = cdiv(Co * C + Co, 4) * 4;
+  if (l.shares > 1) l.part = take(size_t(l.shares) * l.stride * sizeof(float));
   l.total = off;
   return l;
-}
-
-template <typename T>
-static int linear_sum(const float* part, int64_t n, int64_t shares, void* dst, hipStream_t s) {
-  if (n % 4 == 0)
-    linear_reduce<T, 4><<<unsigned(cdiv(n, 256)), kFfnThreads, 0, s>>>(part, n, int(shares),
-                                                                       static_cast<T*>(dst));
-  else
-    linear_reduce<T, 1><<<unsigned(cdiv(n, 64)), kFfnThreads, 0, s>>>(part, n, int(shares),
-                                                                      static_cast<T*>(dst));
-  SP_LAUNCHED();
-  return SP_OK;
 }
 
 template <typename T>
@@ -400,8 +409,8 @@ static int linear_backward(const LinearCall& c, const LinearLayout& l) {
   const int t = linear_gram_tile(c.Co, c.C);
   LinearGram<T> g{dz.p, x.p, dz.ld, x.ld, c.Co, c.C, int(cdiv(c.C, t)),
                   int(linear_gram_tiles(c.Co, c.C, t)), dz.vec, x.vec,
-                  reinterpret_cast<float*>(c.ws + l.part),
-                  c.db ? reinterpret_cast<float*>(c.ws + l.part_b) : nullptr};
+                  reinterpret_cast<float*>(c.ws + l.part), l.stride, static_cast<T*>(c.dw),
+                  static_cast<T*>(c.db), c.db != nullptr};
   constexpr int stage = gram_rows<T>();
   const int64_t share = cdiv(cdiv(c.rows, l.shares), stage) * stage, shares = cdiv(c.rows, share);
   const unsigned groups = unsigned(cdiv(shares * g.tiles, 8) * 8);
@@ -410,9 +419,17 @@ static int linear_backward(const LinearCall& c, const LinearLayout& l) {
   else
     linear_gram<T, 128, 128><<<groups, 256, 0, c.stream>>>(g, c.rows, share, int(shares));
   SP_LAUNCHED();
-  if (c.dw)
-    if (int rc = linear_sum<T>(g.part, int64_t(c.Co) * c.C, shares, c.dw, c.stream)) return rc;
-  if (c.db) return linear_sum<T>(g.part_b, c.Co, shares, c.db, c.stream);
+  if (shares == 1) return SP_OK;
+  const int64_t n = int64_t(c.Co) * c.C;
+  auto reduce = [&](auto kernel, int V) {
+    kernel<<<unsigned(cdiv(n + c.Co, 64 * V)), kFfnThreads, 0, c.stream>>>(
+        g.part, l.stride, n, c.Co, int(shares), g.dw, g.db);
+  };
+  if (n % 4 == 0)
+    reduce(linear_reduce<T, 4>, 4);
+  else
+    reduce(linear_reduce<T, 1>, 1);
+  SP_LAUNCHED();
   return SP_OK;
 }
 
