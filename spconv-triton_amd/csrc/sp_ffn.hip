@@ -280,8 +280,8 @@ __global__ __launch_bounds__(2 * TP, 2) void ffn_gram(Gram<T> g0, Gram<T> g1, in
   for (int64_t m = lo; m < hi; m += ROWS, s ^= 1) {
     char* la = lds + s * STAGE;
     char* lb = la + kGramStage * TP;
-    sa.store(la);
-    sb.store(lb);
+    sa.store(la, hi - m);
+    sb.store(lb, hi - m);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) fetch(m + ROWS);
     auto read = [&](int k) {

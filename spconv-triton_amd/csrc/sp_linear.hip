@@ -60,41 +60,80 @@ __device__ __forceinline__ void linear_tile(const Rows<T>& x, const Rows<T>& w,
   int wrow[S::WT];
 #pragma unroll
   for (int i = 0; i < S::WT; ++i) wrow[i] = (wn * S::WT + i) * 32;
-  products<T, S, ASYNC, S::WT>(x, x0, w, nullptr, n0, wrow, xrow, lds, acc);
-#pragma unroll
-  for (int i = 0; i < S::WT; ++i) {
-    const int c0 = n0 + wrow[i];
-    if (o.bias) {
-#pragma unroll
-      for (int p = 0; p < 16 / V; ++p) {
-        const int c = c0 + 2 * V * p + V * half;
-        const frag b = piece_at<T>(o.bias + c, o.n - c, o.vec_b);
-#pragma unroll
-        for (int j = 0; j < S::XT; ++j)
-#pragma unroll
-          for (int k = 0; k < V; ++k) acc[j][i][V * p + k] += to_f32(b[k]);
-      }
-    }
+  // Whole pieces of the bias and of the other input are loaded without a branch of lanes, behind which each load
+  // would wait for the one before it, and in the smaller tiles before the product, which hides them (75k x 256 -> 1024
+  // bf16 with a residual: 134 us, 138 with branches).  What lies past the ends meets outputs that are not written.
+  constexpr bool EARLY = ASYNC && S::XT * S::WT <= 2;
+  const bool whole = (!o.bias || o.vec_b) && (!o.extra || o.vec_e) && o.n % V == 0;
+  frag e[EARLY ? S::WT : 1][S::XT][16 / V];
+  auto load = [&](int i, frag (&to)[S::XT][16 / V]) {
 #pragma unroll
     for (int j = 0; j < S::XT; ++j) {
       const int64_t r = x0 + xrow + 32 * j + lane;
-      frag e[16 / V];
+      const T* row = o.extra + (r < x.n ? r : x.n - 1) * o.lde;
 #pragma unroll
       for (int p = 0; p < 16 / V; ++p) {
-        const int c = c0 + 2 * V * p + V * half;
-        e[p] = frag{};
-        if (o.extra && r < x.n) e[p] = piece_at<T>(o.extra + r * o.lde + c, o.n - c, o.vec_e);
+        const int c = n0 + wrow[i] + 2 * V * p + V * half;
+        to[j][p] = *reinterpret_cast<const frag*>(row + (c < o.n ? c : o.n - V));
       }
-      const floatx16 z = acc[j][i];
-      linear_act16<sizeof(T) == 2>(o.act, z, [&](int k, float value, float slope) {
-        const float v = to_f32(e[k / V][k % V]);
-        acc[j][i][k] = GRAD ? v * slope : value + v;
-      });
-      write_piece_row<T>(o.out, o.ldo, r, x.n, c0, o.columns, o.vec_o, [&](int k, int c) {
-        return GRAD && c >= o.n ? 0.f : acc[j][i][k];
-      });
     }
-  }
+  };
+  if constexpr (EARLY)
+    if (whole && o.extra) {
+#pragma unroll
+      for (int i = 0; i < S::WT; ++i) load(i, e[i]);
+    }
+  products<T, S, ASYNC, S::WT>(x, x0, w, nullptr, n0, wrow, xrow, lds, acc);
+  auto finish = [&](auto fast) {
+    constexpr bool FAST = fast.value;
+#pragma unroll
+    for (int i = 0; i < S::WT; ++i) {
+      const int c0 = n0 + wrow[i];
+      if constexpr (FAST && !EARLY)
+        if (o.extra) load(i, e[0]);
+      if (o.bias) {
+#pragma unroll
+        for (int p = 0; p < 16 / V; ++p) {
+          const int c = c0 + 2 * V * p + V * half;
+          frag b;
+          if constexpr (FAST)
+            b = *reinterpret_cast<const frag*>(o.bias + (c < o.n ? c : o.n - V));
+          else
+            b = piece_at<T>(o.bias + c, o.n - c, o.vec_b);
+#pragma unroll
+          for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[j][i][V * p + k] += to_f32(b[k]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < S::XT; ++j) {
+        const int64_t r = x0 + xrow + 32 * j + lane;
+        frag own[16 / V];
+#pragma unroll
+        for (int p = 0; p < 16 / V; ++p) {
+          const int c = c0 + 2 * V * p + V * half;
+          own[p] = frag{};
+          if constexpr (FAST)
+            own[p] = o.extra ? e[EARLY ? i : 0][j][p] : frag{};
+          else if (o.extra && r < x.n)
+            own[p] = piece_at<T>(o.extra + r * o.lde + c, o.n - c, o.vec_e);
+        }
+        const floatx16 z = acc[j][i];
+        linear_act16<sizeof(T) == 2>(o.act, z, [&](int k, float value, float slope) {
+          const float v = to_f32(own[k / V][k % V]);
+          acc[j][i][k] = GRAD ? v * slope : value + v;
+        });
+        write_piece_row<T>(o.out, o.ldo, r, x.n, c0, o.columns, o.vec_o, [&](int k, int c) {
+          return GRAD && c >= o.n ? 0.f : acc[j][i][k];
+        });
+      }
+    }
+  };
+  if (ASYNC && whole)
+    finish(std::true_type());
+  else
+    finish(std::false_type());
 }
 
 template <typename T, typename S, bool ASYNC, bool GRAD>
@@ -163,8 +202,8 @@ __global__ __launch_bounds__(kFfnThreads) void linear_transpose(const T* __restr
   }
 }
 
-// Partials of dW = dz' x over a share of the rows, TP x TQ a workgroup, and of db: the rows' sums are a
-// product with ones, which the workgroups of the first columns make beside the others.
+// Partials of dW = dz' x over a share of the rows, TP x TQ a workgroup, and of db, which the workgroups of the
+// first columns sum from what they stage.
 template <typename T>
 struct LinearGram {
   const T *a, *b;
@@ -182,7 +221,6 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
   constexpr int THREADS = 2 * TP, ROWS = gram_rows<T>();
   constexpr int NP = 2, NQ = TQ / 64;
   constexpr int STAGE = kGramStage * (TP + TQ);
-  using frag = typename Mfma<T>::frag;
   using SA = GramStage<T, TP, THREADS>;
   using SB = GramStage<T, TQ, THREADS>;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
@@ -193,13 +231,11 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
   const int p0 = tile / g.tiles_q * TP, q0 = tile % g.tiles_q * TQ;
   const int64_t hi = lo + share < rows ? lo + share : rows;
   const int wave = int(threadIdx.x) >> 6, wp = (wave >> 1) * 64, wq = (wave & 1) * (TQ / 2);
-  const bool sums = g.bias && q0 == 0 && wq == 0;
-  floatx16 acc[NP][NQ], accb[NP][1];
+  const bool sums = g.bias && q0 == 0;
+  constexpr int V = Mfma<T>::V;
+  floatx16 acc[NP][NQ];
   clear(acc);
-  clear(accb);
-  frag ones;
-#pragma unroll
-  for (int i = 0; i < Mfma<T>::V; ++i) ones[i] = T(1.f);
+  float db[V] = {};
   SA sa;
   SB sb;
   auto fetch = [&](int64_t m) {
@@ -211,8 +247,9 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
   for (int64_t m = lo; m < hi; m += ROWS, s ^= 1) {
     char* la = lds + s * STAGE;
     char* lb = la + kGramStage * TP;
-    sa.store(la);
-    sb.store(lb);
+    sa.store(la, hi - m);
+    sb.store(lb, hi - m);
+    if (sums) sa.sum(db);
     __syncthreads();  // (the other buffer's readers are past their previous barrier)
     if (m + ROWS < hi) fetch(m + ROWS);
     auto read = [&](int k) {
@@ -230,10 +267,6 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
       for (int i = 0; i < NP; ++i)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) Mfma<T>::mma(f.x[i], f.w[j], acc[i][j]);
-      if (sums) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) Mfma<T>::mma(f.x[i], ones, accb[i][0]);
-      }
     });
   }
   float* part = g.part + lo / share * g.stride;
@@ -254,12 +287,22 @@ __global__ __launch_bounds__(2 * TP, 2) void linear_gram(LinearGram<T> g, int64_
         else if (g.dw)
           g.dw[row + q] = from_f32<T>(acc[i][j][k]);
       }
-      if (!sums || lane != 0) continue;
-      if (shares > 1)
-        part[int64_t(g.P) * g.Q + p] = accb[i][0][k];
-      else
-        g.db[p] = from_f32<T>(accb[i][0][k]);
     }
+  if (!sums) return;
+  __syncthreads();
+  float* all = reinterpret_cast<float*>(lds);  // [THREADS / SA::PER][TP]
+#pragma unroll
+  for (int i = 0; i < V; ++i) all[int(threadIdx.x) * V + i] = db[i];
+  __syncthreads();
+  const int c = int(threadIdx.x);
+  if (c >= TP || p0 + c >= g.P) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < THREADS / SA::PER; ++k) v += all[k * TP + c];
+  if (shares > 1)
+    part[int64_t(g.P) * g.Q + p0 + c] = v;
+  else
+    g.db[p0 + c] = from_f32<T>(v);
 }
 
 // dW (n values) and db (behind it, m) from their partials, V values a lane, four runs of the shares summed apart and
