@@ -10,6 +10,10 @@
 // a chunk.  The statistics of a chunk are each channel's mean and sum of squares about it, formed
 // from a few rows in registers and joined by Chan, Golub and LeVeque's formula, so that a mean far
 // from zero costs no digits; everything is fp32 and joined in a fixed order.
+//
+// 240k x 128 bf16 (61 MB) in five samples: moments 20 us (3.1 TB/s), statistics 9, values 27 (4.6 TB/s), the gradients' sums 31
+// (4.0), their joins 7, dx 35 (5.3).  What the two joins take is latency: a launch of few workgroups and their
+// dependent loads.
 #include "sp_attention.h"  // sequences in packed rows
 
 namespace sp {
@@ -17,9 +21,11 @@ namespace sp {
 constexpr int kNormThreads = 256;
 constexpr int kNormRows = 4;       // rows of a thread at a time; chunks are whole steps of them
 constexpr int kNormChunks = 1024;  // chunks that a call is cut into, about
-// Calls of up to so many values take a workgroup of kSmallThreads a part, in one launch (the gradients of several
-// parts in two), for three of several workgroups.
-constexpr int64_t kNormSmall = 65536;
+// Calls of up to so many values, and samples of up to so many on average, take a workgroup a part, in one launch (the
+// gradients of several parts in two), for three of several workgroups each.  fp16, 64 channels, us in a graph: one part of 256
+// rows 12.3 forward and 9.1 back; of 1 024 rows 19.6 and 16.5, where several workgroups take 14.3 and 11.2; four
+// parts of 256 rows 12.7 and 11.6, for 15.6 and 12.6 of several.
+constexpr int64_t kNormSmall = 65536, kNormSmallPart = 16384;
 constexpr int kSmallThreads = 512;
 
 enum { kActNone = 3 };  // beside the feed-forward block's activations
@@ -633,8 +639,9 @@ static NormShape norm_shape(int64_t rows, int C, int groups, int V, int threads 
 }
 
 // (a row that is wider than a workgroup goes by blocks of its channels)
-static bool norm_is_small(int64_t rows, int64_t C, int V) {
-  return rows * C <= kNormSmall && C <= kSmallThreads * V;
+static bool norm_is_small(int64_t rows, int64_t C, const Seqs& q, int V) {
+  const int64_t samples = q.parts > 2 ? q.parts - 2 : 1, n = rows * C;
+  return n <= kNormSmall && n <= kNormSmallPart * samples && C <= kSmallThreads * V;
 }
 
 static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
@@ -645,7 +652,7 @@ static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
 static size_t norm_workspace(int64_t rows, int64_t C, int64_t groups, const Seqs& q, int V,
                              bool grad) {
   const size_t sums = align_up(size_t(q.parts) * C * sizeof(float2), 256);
-  if (norm_is_small(rows, C, V)) return grad && q.parts > 1 ? sums : 0;
+  if (norm_is_small(rows, C, q, V)) return grad && q.parts > 1 ? sums : 0;
   const NormShape s = norm_shape(rows, int(C), int(groups), V);
   size_t n = align_up(size_t(tile_slots(q, 1, int(s.chunk))) * C * sizeof(float2), 256);
   if (grad)
@@ -665,7 +672,7 @@ static int norm_act_of(int act, F&& f) {
 
 template <typename T, typename P, int V>
 static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
-  if (norm_is_small(a.seqs.rows, a.s.C, V)) {
+  if (norm_is_small(a.seqs.rows, a.s.C, a.seqs, V)) {
     a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
     norm_act_of(act, [&](auto k) {
       norm_small<T, P, V, k.value><<<unsigned(a.seqs.parts), kSmallThreads, 0, st>>>(a);
@@ -694,7 +701,7 @@ static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
 
 template <typename T, typename P, int V>
 static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
-  if (norm_is_small(a.seqs.rows, a.s.C, V)) {
+  if (norm_is_small(a.seqs.rows, a.s.C, a.seqs, V)) {
     a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
     a.sums = reinterpret_cast<float2*>(ws);
     norm_act_of(act, [&](auto k) {
