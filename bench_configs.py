@@ -32,7 +32,10 @@ weights, and prints one JSON object per configuration:
 * ``blocks``: training step of a stem and two ``SparseFFNBlock`` (SubMConv3d
   64 -> 64, norm with residual, gated feed-forward 64 -> 256 -> 64), fp16
   autocast, batch 2 x ~120k voxels in [128, 2048, 2048], the activations of the
-  feed-forward blocks kept as they are and in 8 bits, with the peak memory.
+  feed-forward blocks kept as they are and in 8 bits, with the peak memory;
+* ``attention``: training step of a stem, three strided convolutions to 64 channels and two
+  ``SparseAttentionBlock`` (4 heads of 16, the voxels of each sample attend to each other), fp16
+  autocast, batch 2 x 200k surface voxels in 256^3, rulebooks rebuilt every pass.
 
 Usage: ``python bench_configs.py [--config NAME ...] [--reps R]``.
 """
@@ -495,10 +498,43 @@ def cfg_blocks(reps):
     return {**out, "what": "training step (forward + backward), fp16 autocast, rulebook rebuilt"}
 
 
+def cfg_attention(reps):
+    import spconv_triton.pytorch as spconv
+
+    shape = [256] * 3
+    idx = [surface_cloud(200_000, 256, seed=s) for s in (0, 1)]
+    idx[1][:, 0] = 1
+    it = torch.from_numpy(np.concatenate(idx)).to(DEV)
+    n = it.shape[0]
+    feats = torch.rand(n, 4, device=DEV)
+    torch.manual_seed(0)
+    widths = (16, 32, 64, 64)
+    net = spconv.SparseSequential(
+        spconv.SubMConv3d(4, widths[0], 3, padding=1, indice_key="s"),
+        *(spconv.SparseConv3d(a, b, 3, stride=2, padding=1, indice_key=f"d{i}")
+          for i, (a, b) in enumerate(zip(widths, widths[1:]))),
+        *(spconv.SparseAttentionBlock(widths[-1], 4, indice_key="a") for _ in range(2))).to(DEV)
+
+    def step():
+        x = spconv.SparseConvTensor(feats, it, shape, 2)
+        with torch.autocast("cuda", dtype=torch.float16):
+            y = net(x).features
+            loss = y.float().square().mean()
+        loss.backward()
+        for p in net.parameters():
+            p.grad = None
+        return y.shape[0]
+
+    for _ in range(3):
+        coarse = step()
+    return {"voxels": int(n), "attending": int(coarse), "median_ms": median_ms(step, reps),
+            "what": "training step (forward + backward), fp16 autocast, rulebooks rebuilt"}
+
+
 CONFIGS = {"encoder": cfg_encoder, "resunet": cfg_resunet, "subm4d": cfg_subm4d,
            "wide": cfg_wide, "config1": cfg_config1, "quickstart": cfg_quickstart,
            "lidar_c256": cfg_lidar_c256, "ref_c256": cfg_ref_c256, "wgrad": cfg_wgrad,
-           "blocks": cfg_blocks}
+           "blocks": cfg_blocks, "attention": cfg_attention}
 
 
 def main() -> int:
