@@ -88,7 +88,7 @@ def sample_offsets(indices: torch.Tensor, batch_size: int) -> torch.Tensor:
     """Where the rows of each sample begin and end, int32 ``[batch_size + 1]`` on the indices'
     device: sample b has the rows ``offsets[b] .. offsets[b + 1] - 1``.  The rows have to lie in the
     samples' order, as the rulebooks' outputs and concatenated voxelisations do; others raise a
-    ValueError.  (Reading that from the device blocks the host once.)"""
+    ValueError.  (Reading that from the device blocks the host once, which a captured graph cannot.)"""
     if indices.dim() != 2 or indices.dtype != torch.int32:
         raise ValueError(f"sample_offsets: indices are an int32 [rows, ndim + 1] tensor, got "
                          f"{indices.dtype} {tuple(indices.shape)}")

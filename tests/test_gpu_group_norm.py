@@ -105,7 +105,9 @@ def _run(x, w, b, dy, groups, act=None, offsets=None):
 NAMES = ("y", "dx", "dw", "db")
 SIZES = [([1], 8, 2), ([7], 16, 16), ([300], 64, 8), ([100, 0, 257], 96, 8), ([40, 41], 20, 4),
          ([33], 99, 3), ([1, 2, 3, 4, 5], 64, 32), ([2000, 3000], 128, 32), ([5001], 512, 16),
-         ([600], 640, 5), ([50], 2056, 8), ([900], 300, 1), ([256] * 30, 32, 4)]
+         ([600], 640, 5), ([50], 2056, 8), ([900], 300, 1), ([256] * 30, 32, 4),
+         ([40] * 12, 64, 8), ([3, 0, 2, 1], 1040, 10), ([2, 5], 4100, 4), ([4], 4104, 8),
+         ([1000, 1, 3, 0], 16, 4)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])

@@ -45,7 +45,8 @@ def _run(x, w, b, res, dy, act):
 
 SIZES = [(1, 8, 8), (1, 64, 192), (2, 99, 40), (3, 512, 1024), (4, 20, 33), (5, 16, 16), (33, 64, 96),
          (100, 99, 99), (257, 40, 160), (300, 128, 128), (1000, 256, 768), (777, 320, 130),
-         (64, 33, 700), (513, 24, 20), (129, 1, 1), (20000, 64, 192), (17000, 160, 512)]
+         (64, 33, 700), (513, 24, 20), (129, 1, 1), (20000, 64, 192), (17000, 160, 512),
+         (9001, 264, 520), (70, 136, 264), (6, 8, 8)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
