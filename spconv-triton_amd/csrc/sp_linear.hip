@@ -9,9 +9,9 @@
 // would also hold rows x outputs of memory).  dz is rounded to the rows' type, as an operand of the
 // products that follow; z, the activation and every sum are fp32.
 //
-// 75k x 256 -> 1024 bf16 with gelu and a residual, 3.9e10 operations a product: forward 138 us (346 MB of rows in and out are
-// 70 at a copy's rate; then the activation, whose instructions come after the tile's four stages), dz 146, dx 77
-// (511 TFLOP/s), dW and db 78 (502) and their shares' sums 12 (a library product of these operands: 66 forward,
+// 75k x 256 -> 1024 bf16 with gelu and a residual, 3.9e10 operations a product: forward 128 us (346 MB of rows in and out are
+// 70 at a copy's rate; then the activation, whose instructions come after the tile's four stages), dz 139, dx 74
+// (531 TFLOP/s), dW and db 76 (517) and their shares' sums 12 (a library product of these operands: 66 forward,
 // 53 for dx and 280 for dW).
 #include "sp_tiles.h"
 
@@ -19,13 +19,13 @@ namespace sp {
 
 enum { kActNone = 3 };  // beside the feed-forward block's activations
 
-template <bool FAST, typename F>
-__device__ __forceinline__ void linear_act16(int act, const floatx16& z, F&& f) {
-  if (act == kActNone) {
+template <bool FAST, int ACT, typename F>
+__device__ __forceinline__ void linear_act16(const floatx16& z, F&& f) {
+  if constexpr (ACT == kActNone) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) f(i, z[i], 1.f);
   } else {
-    with_act(act, [&](auto kind) { gate16<FAST, kind.value>(z, f); });
+    gate16<FAST, ACT>(z, f);
   }
 }
 
@@ -66,8 +66,10 @@ __device__ __forceinline__ void linear_tile(const Rows<T>& x, const Rows<T>& w,
 #pragma unroll
   for (int i = 0; i < S::WT; ++i) wrow[i] = (wn * S::WT + i) * 32;
   // Whole pieces of the bias and of the other input are loaded without a branch of lanes, behind which each load
-  // would wait for the one before it, and in the smaller tiles before the product, which hides them (75k x 256 -> 1024
-  // bf16 with a residual: 134 us, 138 with branches).  What lies past the ends meets outputs that are not written.
+  // would wait for the one before it: the bias, which the products are added to, while the first stage is on its way,
+  // the other input in the smaller tiles before it.  What lies past the ends meets outputs that are not written.  The
+  // epilogue is chosen once, not activation by activation within it (75k x 256 -> 1024 bf16, gelu, residual: 128 us,
+  // 138 with branches and the bias added last).
   constexpr bool EARLY = ASYNC && S::XT * S::WT <= 2;
   const bool whole = (!o.bias || o.vec_b) && (!o.extra || o.vec_e) && o.n % V == 0;
   frag e[EARLY ? S::WT : 1][S::XT][16 / V];
@@ -83,34 +85,38 @@ __device__ __forceinline__ void linear_tile(const Rows<T>& x, const Rows<T>& w,
       }
     }
   };
+  auto start = [&](auto get) {
+    frag b[S::WT][16 / V];
+#pragma unroll
+    for (int i = 0; i < S::WT; ++i)
+#pragma unroll
+      for (int p = 0; p < 16 / V; ++p) b[i][p] = get(n0 + wrow[i] + 2 * V * p + V * half);
+#pragma unroll
+    for (int i = 0; i < S::WT; ++i)
+#pragma unroll
+      for (int j = 0; j < S::XT; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[j][i][k] = to_f32(b[i][k / V][k % V]);
+  };
   if constexpr (EARLY)
     if (whole && o.extra) {
 #pragma unroll
       for (int i = 0; i < S::WT; ++i) load(i, e[i]);
     }
-  products<T, S, ASYNC, S::WT>(x, x0, w, nullptr, n0, wrow, xrow, lds, acc);
-  auto finish = [&](auto fast) {
+  products<T, S, ASYNC, S::WT>(x, x0, w, nullptr, n0, wrow, xrow, lds, acc, [&] {
+    if (!o.bias) return;
+    if (whole)
+      start([&](int c) { return *reinterpret_cast<const frag*>(o.bias + (c < o.n ? c : o.n - V)); });
+    else
+      start([&](int c) { return piece_at<T>(o.bias + c, o.n - c, o.vec_b); });
+  });
+  auto finish = [&](auto fast, auto act) {
     constexpr bool FAST = fast.value;
 #pragma unroll
     for (int i = 0; i < S::WT; ++i) {
       const int c0 = n0 + wrow[i];
       if constexpr (FAST && !EARLY)
         if (o.extra) load(i, e[0]);
-      if (o.bias) {
-#pragma unroll
-        for (int p = 0; p < 16 / V; ++p) {
-          const int c = c0 + 2 * V * p + V * half;
-          frag b;
-          if constexpr (FAST)
-            b = *reinterpret_cast<const frag*>(o.bias + (c < o.n ? c : o.n - V));
-          else
-            b = piece_at<T>(o.bias + c, o.n - c, o.vec_b);
-#pragma unroll
-          for (int j = 0; j < S::XT; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[j][i][V * p + k] += to_f32(b[k]);
-        }
-      }
 #pragma unroll
       for (int j = 0; j < S::XT; ++j) {
         const int64_t r = x0 + xrow + 32 * j + lane;
@@ -125,7 +131,7 @@ __device__ __forceinline__ void linear_tile(const Rows<T>& x, const Rows<T>& w,
             own[p] = piece_at<T>(o.extra + r * o.lde + c, o.n - c, o.vec_e);
         }
         const floatx16 z = acc[j][i];
-        linear_act16<sizeof(T) == 2>(o.act, z, [&](int k, float value, float slope) {
+        linear_act16<sizeof(T) == 2, act.value>(z, [&](int k, float value, float slope) {
           const float v = to_f32(own[k / V][k % V]);
           acc[j][i][k] = GRAD ? v * slope : value + v;
         });
@@ -135,10 +141,16 @@ __device__ __forceinline__ void linear_tile(const Rows<T>& x, const Rows<T>& w,
       }
     }
   };
-  if (ASYNC && whole)
-    finish(std::true_type());
+  auto end = [&](auto act) {
+    if (ASYNC && whole)
+      finish(std::true_type(), act);
+    else
+      finish(std::false_type(), act);
+  };
+  if (o.act == kActNone)
+    end(std::integral_constant<int, kActNone>());
   else
-    finish(std::false_type());
+    with_act(o.act, end);
 }
 
 template <typename T, typename S, bool ASYNC, bool GRAD>

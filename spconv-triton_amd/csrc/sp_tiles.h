@@ -129,18 +129,24 @@ struct Operands {
   typename Mfma<T>::frag x[M], w[N];
 };
 
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
+
 // acc[j][i] += the products of x rows xrow + 32 j .. + 31 and weight rows wrow[i] .. + 31 of the stage
-// over all of K.
-template <typename T, typename S, bool ASYNC, int NW>
+// over all of K.  `meanwhile` runs while the first stage is on its way.
+template <typename T, typename S, bool ASYNC, int NW, typename F = Nothing>
 __device__ __forceinline__ void products(const Rows<T>& x, int64_t x0, const Rows<T>& w,
                                          const Rows<T>* w2, int64_t w0, const int (&wrow)[NW],
-                                         int xrow, char* lds, floatx16 (&acc)[S::XT][NW]) {
+                                         int xrow, char* lds, floatx16 (&acc)[S::XT][NW],
+                                         F&& meanwhile = F()) {
   using Stg = Stage<T, S, ASYNC>;
   constexpr int STEP = kStagePieces * Mfma<T>::V;
   const int lane = int(threadIdx.x) & 31, half = (int(threadIdx.x) >> 5) & 1;
   Stg stage(x, x0, w, w2, w0);
   const int steps = (x.K + STEP - 1) / STEP;
   stage.start(x, w, lds, x.K < STEP);
+  meanwhile();
   for (int s = 0; s < steps; ++s) {
     char* buf = lds + (s & 1) * S::BYTES;
     stage.finish(buf);
