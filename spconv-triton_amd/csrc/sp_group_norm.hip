@@ -11,15 +11,16 @@
 // from a few rows in registers and joined by Chan, Golub and LeVeque's formula, so that a mean far
 // from zero costs no digits; everything is fp32 and joined in a fixed order.
 //
-// 240k x 128 bf16 (61 MB) in five samples: moments 20 us (3.1 TB/s), statistics 9, values 27 (4.6 TB/s), the gradients' sums 31
-// (4.0), their joins 7, dx 35 (5.3).  What the two joins take is latency: a launch of few workgroups and their
-// dependent loads.
+// 240k x 128 bf16 (61 MB) in five samples: moments 20 us (3.1 TB/s), statistics 7, values 27 (4.6 TB/s), the gradients' sums 31
+// (4.0), their joins 7, dx 35 (5.3).  What the two joins take is latency: a launch of few workgroups and a
+// batch of loads (one load after the other: 9).
 #include "sp_attention.h"  // sequences in packed rows
 
 namespace sp {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormRows = 4;       // rows of a thread at a time; chunks are whole steps of them
+constexpr int kNormLoads = 8;      // partials that a thread of a join loads at a time
 constexpr int kNormChunks = 1024;  // chunks that a call is cut into, about
 // Calls of up to so many values, and samples of up to so many on average, take a workgroup a part, in one launch (the
 // gradients of several parts in two), for three of several workgroups each.  fp16, 64 channels, us in a graph: one part of 256
@@ -228,10 +229,19 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats(NormArgs<T, P> a) {
   if (row < rows)
     for (int c = int(threadIdx.x) - row * wide; c < a.s.cg; c += wide) {
       const float2* at = a.part + k.slot * a.s.C + g * a.s.cg + c;
-#pragma unroll 4
-      for (int j = row; j < int(k.n); j += rows) {
-        const float2 v = at[int64_t(j) * a.s.C];
-        m.join(float(j + 1 < k.n ? a.s.chunk : k.len - j * a.s.chunk), v.x, v.y);
+      for (int j = row; j < int(k.n); j += kNormLoads * rows) {
+        float2 v[kNormLoads];
+#pragma unroll
+        for (int i = 0; i < kNormLoads; ++i) {
+          const int r = j + i * rows;
+          v[i] = at[int64_t(r < k.n ? r : j) * a.s.C];
+        }
+#pragma unroll
+        for (int i = 0; i < kNormLoads; ++i) {
+          const int r = j + i * rows;
+          if (r < k.n)
+            m.join(float(r + 1 < k.n ? a.s.chunk : k.len - r * a.s.chunk), v[i].x, v[i].y);
+        }
       }
     }
   m = block_moments(m, lds);
@@ -437,10 +447,16 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_join(NormArgs<T, P> a)
   for (int j = wave; j < a.s.cg; j += kNormThreads / 64) {
     const int c = g * a.s.cg + j;
     float2 v{0.f, 0.f};
-    for (int64_t i = lane; i < n; i += 64) {
-      const float2 o = a.part[(k.slot + i) * a.s.C + c];
-      v.x += o.x;
-      v.y += o.y;
+    for (int64_t i = lane; i < n; i += 64 * kNormLoads) {
+      float2 o[kNormLoads];
+#pragma unroll
+      for (int l = 0; l < kNormLoads; ++l)
+        o[l] = a.part[(k.slot + (i + 64 * l < n ? i + 64 * l : i)) * a.s.C + c];
+#pragma unroll
+      for (int l = 0; l < kNormLoads; ++l) {
+        v.x += i + 64 * l < n ? o[l].x : 0.f;
+        v.y += i + 64 * l < n ? o[l].y : 0.f;
+      }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
