@@ -545,8 +545,8 @@ int sp_linear_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int3
  * [nk, kv_heads, dim] of f16, bf16 or f32: *_row elements from row to row, *_head from head to
  * head, all multiples of 16 bytes, as dim (<= 128) is; the values of a head are neighbours.
  * Sequence s has the queries q_offsets[s] .. q_offsets[s + 1] - 1 and the keys of k_offsets likewise
- * (device memory, [sequences + 1], ascending; both null: one sequence of all rows).
- * Offsets are not checked; whatever they hold, no access leaves the rows.  causal: a query sees
+ * (device memory, [sequences + 1], ascending; both null: one sequence of all rows).  nq and nk are
+ * at most 2^31 - 128.  Offsets are not checked; whatever they hold, no access leaves the rows.  causal: a query sees
  * the keys up to its own place counted from the sequence's end (the last query sees all).  A query that sees no key, as
  * those outside all sequences, gets zeros.  Sums and the softmax's statistics are fp32, its
  * weights are rounded to the type between the products. */

@@ -407,6 +407,8 @@ __device__ __forceinline__ bool find_place(int64_t slots, int heads, int shares,
 
 // ---- host ------------------------------------------------------------------------
 constexpr int kAttnMaxDim = 128;
+// (the kernels' 32-bit places go up to a whole tile past the last row)
+constexpr int64_t kAttnMaxRows = (int64_t(1) << 31) - 128;
 constexpr int kMostShares = 1024;
 
 // Rows of a tile that passes through LDS.

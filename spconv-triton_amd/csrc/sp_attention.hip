@@ -337,9 +337,9 @@ static int check_call(const char* what, const sp_attn* a) {
                (long long)a->dim, V);
   if (a->dim > kAttnMaxDim)
     return set_error(SP_ERR_UNSUPPORTED, "%s: heads wider than %d", what, kAttnMaxDim);
-  SP_CHECK_ARG(a->nq >= 0 && a->nk >= 0 && a->nq < (int64_t(1) << 31) &&
-                   a->nk < (int64_t(1) << 31),
-               "%s: bad row counts %lld and %lld", what, (long long)a->nq, (long long)a->nk);
+  SP_CHECK_ARG(a->nq >= 0 && a->nk >= 0 && a->nq <= kAttnMaxRows && a->nk <= kAttnMaxRows,
+               "%s: bad row counts %lld and %lld (at most 2^31 - 128)", what, (long long)a->nq,
+               (long long)a->nk);
   SP_CHECK_ARG((a->q_offsets == nullptr) == (a->k_offsets == nullptr),
                "%s: offsets of queries and keys go together", what);
   SP_CHECK_ARG(!a->q_offsets || (a->sequences >= 0 && a->sequences < (1 << 30)),

@@ -104,3 +104,26 @@ def test_bad_sizes_and_workspaces_are_refused():
         assert backward(c, **kw) == _lib.SP_ERR_INVALID_ARG, kw
     assert L.sp_attention_bwd(ctypes.byref(c), None, p, 1 << 30, None) == _lib.SP_ERR_INVALID_ARG
     assert backward(call(nq=0, nk=0)) == _lib.SP_OK
+
+
+def test_rows_that_32_bit_places_cannot_count_are_refused():
+    """Tiles of 64 and 128 rows are counted in 32 bits: within 127 rows of 2^31 their number wrapped around to
+    a negative one, and the result was zeros.  (Pointers that are not device memory, on the host: a call that was
+    let through would end at its launch, with another status.)"""
+    from spconv_triton.pytorch._impl import _lib
+    from spconv_triton.pytorch._impl.attention import _Call, _Grad
+
+    L = _lib.load_library()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    most = 2 ** 31 - 128
+    for nq, nk, dtype in ((1, most + 1, 0), (most + 1, 1, 2), (1, 2 ** 31 - 64, 1), (2 ** 31 - 1, 1, 0)):
+        c = _Call(p, p, p, 64, 32, 64, 32, 64, 32, nq, nk, 1, 1, 32, 0, None, None, 0.1, 0, dtype)
+        ref = ctypes.byref(c)
+        assert L.sp_attention_workspace(ref) == L.sp_attention_bwd_workspace(ref) == 0
+        assert L.sp_attention(ref, p, 64, 32, None, p, 1 << 62, None) == _lib.SP_ERR_INVALID_ARG
+        g = _Grad(p, p, p, p, p, p, *(64, 32) * 5)
+        assert (L.sp_attention_bwd(ref, ctypes.byref(g), p, 1 << 62, None)
+                == _lib.SP_ERR_INVALID_ARG)
+    c = _Call(p, p, p, 64, 32, 64, 32, 64, 32, most, most, 1, 1, 32, 0, None, None, 0.1, 0, 0)
+    assert L.sp_attention_bwd_workspace(ctypes.byref(c)) > 0
