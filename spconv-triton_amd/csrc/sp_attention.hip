@@ -8,8 +8,10 @@
 // and sum of the softmax; the query heads that share a key head are rows of one tile.
 //
 // Statistics and sums are fp32.  P is rounded to the rows' type between the products, as the matrix
-// instructions take it; relative to a maximum that is at most 2^14 below the
-// largest no weight exceeds 2^14, and what fp16 loses below 2^-14 is less than 2^-25 of the maximum's term.
+// instructions take it.  Weights are relative to a base at or below the largest score, and no weight exceeds 2^15.  fp16
+// rounds weights below 2^-14 to multiples of 2^-24, so its base lies 2^8 below a maximum, and a weight is off by at most
+// 2^-33 of the largest one: over 2^21 keys by half a step of the type.  (With the maximum itself as the base 2^18 keys
+// 25 ln 2 below one other, 2^-7 of the sum, came out as twice as much.)
 //
 // Bound by the vector unit beside the matrix cores: a weight costs an exponential (8 cycles of a SIMD for 64 of them,
 // 4 times an addition), its conversion and its sum, and a matrix instruction keeps the vector unit from
@@ -25,7 +27,11 @@ namespace sp {
 
 // A lane's weights of a tile may sum up to this before they are put relative to a new maximum (fp16 holds
 // weights up to 2^16).
-constexpr float kMostWeight = 16384.f;
+constexpr float kMostWeight = 32768.f;
+
+// The base of the weights below the maximum that sets it, in powers of two.
+template <typename T>
+constexpr float kBelow = std::is_same<T, _Float16>::value ? 8.f : 0.f;
 
 // Waves a SIMD.
 template <typename T>
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP)) void attend(Attn
       for (int x = 0; x < NK; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, s[x][i]);
-      const float now = __builtin_fmaxf(half_max(mx) * c, m);
+      const float now = __builtin_fmaxf(half_max(mx) * c - kBelow<T>, m);
       const float safe = now == -__builtin_inff() ? 0.f : now;
       const float down = __builtin_amdgcn_exp2f(m - safe);
       m = now;
