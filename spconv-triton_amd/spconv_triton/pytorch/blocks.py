@@ -96,29 +96,40 @@ class SparseFFNBlock(SparseModule):
         return mixed.replace_feature(self.ffn(y, total, kept[0] if kept else None))
 
 
+def _edition(t: torch.Tensor) -> int:
+    """Changes with every write to t (tensors of inference mode do not count them)."""
+    return 0 if t.is_inference() else t._version
+
+
 class SampleRows:
     """Where the samples' rows begin and end, as ``indice_dict`` keeps it for a set of voxels."""
 
-    def __init__(self, rows: int, batch_size: int, offsets: torch.Tensor):
-        self.rows, self.batch_size, self.offsets = rows, batch_size, offsets
+    def __init__(self, indices: torch.Tensor, batch_size: int):
+        self.indices, self.edition, self.batch_size = indices, _edition(indices), batch_size
+        self.offsets = ops.sample_offsets(indices, batch_size)
+
+    def of(self, indices: torch.Tensor) -> bool:
+        """Whether these are the voxels that the offsets were formed of, not written to since."""
+        return indices is self.indices and _edition(indices) == self.edition
 
 
 def _samples(x, indice_key: str | None):
     """(offsets of x's samples, the ``indice_dict`` of the result): with a key they are formed once for
-    all layers of these voxels that name it."""
+    all layers of these voxels that name it, and again for other voxels (as many rows may be
+    split between the samples in another way)."""
     if x.batch_size == 1:
         return None, x.indice_dict
     key = None if indice_key is None else f"{indice_key}.samples"
     kept, known = x.find_indice_pair(key), x.indice_dict
-    if kept is None:
-        kept = SampleRows(x.indices.shape[0], x.batch_size,
-                          ops.sample_offsets(x.indices, x.batch_size))
-        if key is not None:
-            known = {**known, key: kept}
-    if kept.rows != x.indices.shape[0] or kept.batch_size != x.batch_size:
-        raise ValueError(f"indice key {indice_key} was given to {kept.rows} voxels of "
+    if kept is not None and (kept.indices.shape[0] != x.indices.shape[0]
+                             or kept.batch_size != x.batch_size):
+        raise ValueError(f"indice key {indice_key} was given to {kept.indices.shape[0]} voxels of "
                          f"{kept.batch_size} samples, here are {x.indices.shape[0]} of "
                          f"{x.batch_size}")
+    if kept is None or not kept.of(x.indices):
+        kept = SampleRows(x.indices, x.batch_size)
+        if key is not None:
+            known = {**known, key: kept}
     return kept.offsets, known
 
 

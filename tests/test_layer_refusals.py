@@ -152,3 +152,40 @@ def test_sample_offsets_on_the_host():
     for bad in ((idx.flip(0), 3), (idx, 2), (idx - 1, 3), (idx.long(), 3), (idx[0], 1), (idx, 0)):
         with pytest.raises(ValueError):
             ops.sample_offsets(*bad)
+
+
+def test_samples_of_a_key_are_those_of_its_voxels():
+    """As many rows of as many samples, split in another way, under the same key: other offsets, and rows out of
+    order are refused as they are without a key.  The voxels that the key was given to keep theirs."""
+    import spconv_triton.pytorch as spconv
+    from spconv_triton.pytorch.blocks import _samples
+
+    def voxels(counts, known=None):
+        batch = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
+        idx = torch.stack([batch, torch.arange(sum(counts))], 1).int()
+        return spconv.SparseConvTensor(torch.zeros(len(idx), 4), idx, [64], len(counts),
+                                       indice_dict=known)
+
+    x = voxels([2, 3])
+    offsets, known = _samples(x, "s")
+    assert offsets.tolist() == [0, 2, 5] and not x.indice_dict
+    same = x.replace_feature(x.features + 1)
+    same.indice_dict = known
+    again, kept = _samples(same, "s")
+    assert again is offsets and kept is known
+    other = voxels([4, 1], known)
+    new, renewed = _samples(other, "s")
+    assert new.tolist() == [0, 4, 5] and known["s.samples"].offsets is offsets
+    assert renewed["s.samples"].offsets is new
+    x.indices[2, 0] = 0  # (written to: no longer what the offsets were formed of)
+    assert _samples(same, "s")[0].tolist() == [0, 3, 5]
+    turned = voxels([2, 3], known)
+    turned.indices = turned.indices.flip(0)
+    with pytest.raises(ValueError, match="order"):
+        _samples(turned, "s")
+    with pytest.raises(ValueError, match="indice key"):
+        _samples(voxels([3, 3], known), "s")
+    with torch.inference_mode():
+        y = voxels([1, 4])
+        offsets, y.indice_dict = _samples(y, "s")
+        assert offsets.tolist() == [0, 1, 5] and _samples(y, "s")[0] is offsets
