@@ -21,6 +21,7 @@ from torch import nn
 
 from spconv_triton.pytorch import functional as Fsp
 from spconv_triton.pytorch import ops
+from spconv_triton.pytorch._impl.attention import MAX_DIM
 from spconv_triton.pytorch.modules import SparseModule
 
 
@@ -201,7 +202,7 @@ class RowLinear(nn.Module):
 class SparseAttentionBlock(SparseModule):
     """``x + out(attention(qkv(norm(x))))`` on a SparseConvTensor: the voxels of each sample attend to each
     other (with ``causal`` to those before them).  ``kv_heads`` heads of keys and values (default:
-    ``heads``) serve ``heads`` heads of queries, each ``channels / heads`` wide.  The voxels have to lie in
+    ``heads``) serve ``heads`` heads of queries, each ``channels / heads`` (up to 128) wide.  The voxels have to lie in
     the samples' order."""
 
     def __init__(self, channels: int, heads: int, kv_heads: int | None = None,
@@ -212,6 +213,9 @@ class SparseAttentionBlock(SparseModule):
         if heads < 1 or kv_heads < 1 or channels % heads or heads % kv_heads:
             raise ValueError(f"SparseAttentionBlock: {channels} channels in {heads} heads of "
                              f"queries and {kv_heads} of keys")
+        if channels // heads > MAX_DIM:
+            raise NotImplementedError(f"SparseAttentionBlock: heads wider than {MAX_DIM} "
+                                      f"({channels} channels in {heads})")
         self.heads, self.kv_heads, self.causal = heads, kv_heads, causal
         self.indice_key = indice_key
         self.norm = SparseGroupNorm(heads if groups is None else groups, channels, eps)

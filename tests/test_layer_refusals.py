@@ -189,3 +189,12 @@ def test_samples_of_a_key_are_those_of_its_voxels():
         y = voxels([1, 4])
         offsets, y.indice_dict = _samples(y, "s")
         assert offsets.tolist() == [0, 1, 5] and _samples(y, "s")[0] is offsets
+
+
+def test_blocks_of_wider_heads_than_attention_takes_are_not_built():
+    import spconv_triton.pytorch as spconv
+
+    for args in ((129, 1), (512, 2), (520, 4, 2)):
+        with pytest.raises(NotImplementedError, match="wider than 128"):
+            spconv.SparseAttentionBlock(*args)
+    assert spconv.SparseAttentionBlock(256, 2).qkv.weight.shape == (768, 256)
