@@ -273,33 +273,45 @@ __device__ __forceinline__ void add_rows(const char* lds, int r0,
 }
 
 // The same where a lane sees the rows lo .. hi - 1 only and the others may hold infinities or NaN, which times
-// the zeros of p would be NaN: one row at a time, added where it is seen.  Slow, and run
-// for tiles whose results came out not finite only.
+// the zeros of p would be NaN: one row at a time on the vector unit, added where it is seen.  Slow (32 rows of 128
+// values are 4096 multiplications a lane for 32 matrix instructions), and run for tiles whose results came out not
+// finite only; what counts is that it needs few registers, so one accumulator at a time goes through the rows.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void add_rows_seen(const char* lds, int r0, int lo, int hi,
-                                           const typename Mfma<T>::frag (&p)[32 / Mfma<T>::KSTEP],
-                                           floatx16 (&acc)[DP / 32]) {
+                                              const typename Mfma<T>::frag (&p)[32 / Mfma<T>::KSTEP],
+                                              floatx16 (&acc)[DP / 32]) {
   using L = HeadTile<T, DP, ROWS>;
   using frag = typename Mfma<T>::frag;
   constexpr int V = Mfma<T>::V, STEPS = 32 / Mfma<T>::KSTEP;
   const int half = (int(threadIdx.x) >> 5) & 1;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) {
 #pragma unroll 1
-  for (int j = 0; j < 32; ++j) {
-    const bool seen = r0 + j >= lo && r0 + j < hi;
+    for (int k = 0; k < 16; ++k) {
+      // weight k of either half is of row 2 V (k / V) + V half + k % V (acc_row); here both halves get both
+      float mine = 0.f;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t) {
-      floatx16 one;
-      zero(one);
+      for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        frag f = L::read_t(lds, r0 + s * Mfma<T>::KSTEP, 32 * t), g = p[s];
+        for (int i = 0; i < V; ++i) mine = s * V + i == k ? to_f32(p[s][i]) : mine;
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine),
+                                                         __float_as_uint(mine), false, false);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (s * Mfma<T>::KSTEP + half * V + i != j) f[i] = g[i] = T(0.f);
-        Mfma<T>::mma(f, g, one);
+      for (int h = 0; h < 2; ++h) {
+        const float w = __uint_as_float(both[h]);
+        const int r = r0 + k / V * 2 * V + V * h + k % V;
+        const bool seen = r >= lo && r < hi;
+#pragma unroll
+        for (int b = 0; b < 16 / V; ++b) {
+          const frag f = *reinterpret_cast<const frag*>(
+              lds + (r * L::PIECES + swizzled<L::PIECES>(r, 32 / V * t + 2 * b + half)) * 16);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float v = to_f32(f[i]) * w;
+            acc[t][V * b + i] += seen ? v : 0.f;
+          }
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][i] += seen ? one[i] : 0.f;
     }
   }
 }

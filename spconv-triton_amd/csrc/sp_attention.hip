@@ -33,15 +33,16 @@ constexpr float kMostWeight = 32768.f;
 template <typename T>
 constexpr float kBelow = std::is_same<T, _Float16>::value ? 8.f : 0.f;
 
-// Waves a SIMD.
+// Waves a SIMD (of a launch that makes results again: as few as leave it all registers).
 template <typename T>
-constexpr int attend_waves(int DP) {
+constexpr int attend_waves(int DP, bool strict = false) {
+  if (strict) return 1;
   return sizeof(T) == 4 ? (DP <= 32 ? 4 : DP <= 64 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
 }
 
 template <typename T, int DP, int BK, bool CAUSAL, bool STRICT>
-__global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP)) void attend(AttnArgs<T> a,
-                                                                            int64_t slots) {
+__global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, STRICT)) void attend(
+    AttnArgs<T> a, int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BK>;
   constexpr int STEPS = DP / Mfma<T>::KSTEP, PS = 32 / Mfma<T>::KSTEP, V = Mfma<T>::V;

@@ -35,13 +35,15 @@ constexpr bool dq_beside(int DP) { return DP > 64 || sizeof(T) == 4; }
 template <typename T>
 constexpr bool dkv_beside(int DP) { return DP >= 64 || sizeof(T) == 4; }
 
-// Waves a SIMD.
+// Waves a SIMD (of a launch that makes results again: as few as leave it all registers).
 template <typename T>
-constexpr int dq_waves(int DP) {
+constexpr int dq_waves(int DP, bool strict = false) {
+  if (strict) return 1;
   return sizeof(T) == 4 ? (DP <= 32 ? 4 : DP <= 64 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 1;
 }
 template <typename T>
-constexpr int grad_waves(int DP) {
+constexpr int grad_waves(int DP, bool strict = false) {
+  if (strict) return 1;
   return sizeof(T) == 4 ? (DP <= 32 ? 3 : 1) : DP <= 32 ? 4 : DP <= 64 ? 2 : 1;
 }
 
@@ -168,7 +170,7 @@ __device__ __forceinline__ float lift_of(float grad_sq, float value_sq) {
 }
 
 template <typename T, int DP, int BK, bool CAUSAL, bool STRICT>
-__global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
+__global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP, STRICT)) void attend_dq(
     AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BK>;
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
       Mfma<T>::mma(f, ds[x][i / TILES], acc[i % TILES]);
     };
     constexpr int FORM = 2 * STEPS, ADD = PS * TILES;
-    if constexpr (!dq_beside<T>(DP)) {
+    if constexpr (STRICT || !dq_beside<T>(DP)) {
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
         zero(s[x]);
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
           form(x + 1, i, f);
           weigh(x, 16 * i / FORM, 16 * (i + 1) / FORM);
         });
-      } else if (x > 0 && !(STRICT && edge)) {
+      } else if (x > 0) {
         beside<frag, ADD, kAhead>(read_t(x - 1), [&](int i, const frag& f) {
           add(x - 1, i, f);
           weigh(x, 16 * i / ADD, 16 * (i + 1) / ADD);
@@ -323,13 +325,7 @@ __global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
         weigh(x, 0, 16);
       }
     }
-    if (STRICT && edge) {
-#pragma unroll
-      for (int x = 0; x < NX; ++x)
-        add_rows_seen<T, DP, BK>(buf, 32 * x, 0, seen - key0, ds[x], acc);
-    } else {
-      beside<frag, ADD, kAhead>(read_t(NX - 1), [&](int i, const frag& f) { add(NX - 1, i, f); });
-    }
+    beside<frag, ADD, kAhead>(read_t(NX - 1), [&](int i, const frag& f) { add(NX - 1, i, f); });
   };
   if (first < end) {
     lk.start(first * BK, lds);
@@ -355,7 +351,7 @@ __global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP)) void attend_dq(
 
 // A tile of keys goes through the queries of its head's G query heads, one head after the other.
 template <typename T, int DP, int BQ, bool CAUSAL, bool STRICT>
-__global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
+__global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP, STRICT)) void attend_dkv(
     AttnArgs<T> a, const float* __restrict__ nl, const float* __restrict__ nd, int64_t slots) {
   using frag = typename Mfma<T>::frag;
   using L = HeadTile<T, DP, BQ>;
@@ -402,14 +398,8 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
   }
   const int begin = least / BQ, last = (Lq + BQ - 1) / BQ;  // tiles of a head
   const int64_t tiles = last > begin ? int64_t(last - begin) * a.G : 0;
-  const int64_t per = (tiles + a.shares - 1) / a.shares;
-  int64_t n = place.share * per;
-  const int64_t end = n + per < tiles ? n + per : tiles;
-  int qh = 0, qt = begin;  // the tile's head and place
-  if (n < end) {
-    qh = int(n / (last - begin));
-    qt = begin + int(n - int64_t(qh) * (last - begin));
-  }
+  const int64_t per = (tiles + a.shares - 1) / a.shares, first = place.share * per;
+  const int64_t end = first + per < tiles ? first + per : tiles;
   const int64_t h0 = int64_t(place.head) * a.G;
   TileLoads<T, DP, BQ> lq(a.q.p + qlo * a.q.row, a.q.row, Lq, a.D);
   TileLoads<T, DP, BQ> lg(a.dout.p + qlo * a.dout.row, a.dout.row, Lq, a.D);
@@ -438,158 +428,174 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP)) void attend_dkv(
 #pragma unroll
     for (int i = 0; i < 4; ++i) lq.clear(lds + (i >> 1) * STAGE + (i & 1) * L::BYTES);
   }
-  floatx16 dk[TILES], dv[TILES];
+  // A pass over the queries, for dk, dv or both.
+  auto pass = [&](auto want_dk, auto want_dv) {
+    constexpr bool DK = want_dk.value, DV = want_dv.value;
+    floatx16 dk[DK ? TILES : 1], dv[DV ? TILES : 1];
 #pragma unroll
-  for (int d = 0; d < TILES; ++d) {
-    zero(dk[d]);
-    zero(dv[d]);
-  }
-  // A tile of queries in buffer B.  32 queries' scores and their gradients are formed beside the weights of the
-  // 32 before, and these are multiplied beside the weights of the next.
-  auto step = [&](auto buffer) {
-    char* buf = lds + buffer.value * STAGE;
-    loads_in_flight<0>();
-    __syncthreads();
-    const int query0 = qt * BQ;
-    if (++qt == last) {
-      qt = begin;
-      ++qh;
+    for (int d = 0; d < TILES; ++d) {
+      if constexpr (DK) zero(dk[d]);
+      if constexpr (DV) zero(dv[d]);
     }
-    if (n + 1 < end) start(qh, qt, lds + (1 - buffer.value) * STAGE);
-    // (asked in either case: without these branches the compiler's order of the step takes more registers than
-    // there are, 176 bytes of scratch at 64 values a head and half the speed)
-    if (query0 + BQ <= wave_least) return;
-    const bool edge = query0 < wave_most;
-    const float* stats = reinterpret_cast<const float*>(buf + 2 * L::BYTES);
-    floatx16 s[NX], dp[NX];
-    frag p[NX][PS], ds[NX][PS];
-    float4v base[2], minus[2];  // of four weights, and of the next four
-    auto read = [&](int x) {
-      return [=](int i) { return L::read(buf + (i & 1) * L::BYTES, 32 * x, i >> 1); };
-    };
-    auto form = [&](int x, int i, const frag& f) {
-      if (i & 1)
-        Mfma<T>::mma(f, v[i >> 1], dp[x]);
-      else
-        Mfma<T>::mma(f, k[i >> 1], s[x]);
-    };
-    // the weights of 32 queries: what they take, what of them is hidden, and weights lo .. hi - 1
-    auto take = [&](int x, int i) {
-      const int r = 32 * x + acc_row<T>(4 * i);
-      base[i & 1] = *reinterpret_cast<const float4v*>(stats + r);
-      minus[i & 1] = *reinterpret_cast<const float4v*>(stats + kStats + r);
-    };
-    auto prepare = [&](int x) {
-      take(x, 0);
-      if (!edge) return;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (query0 + 32 * x + acc_row<T>(i) < from) {
-          s[x][i] = -__builtin_inff();
-          dp[x][i] = 0.f;  // (not what a NaN there makes of it)
-        }
-    };
-    auto weigh = [&](int x, int lo, int hi) {
-#pragma unroll
-      for (int i = lo; i < hi; ++i) {
-        if ((i & 3) == 0 && i < 12) take(x, (i >> 2) + 1);
-        const float e =
-            __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, base[i >> 2 & 1][i & 3]));
-        float d = dp[x][i] + minus[i >> 2 & 1][i & 3];
-        if (kLift<T> != 0.f) d *= g;
-        p[x][i / V][i % V] = T(e);
-        ds[x][i / V][i % V] = T(e * d);
+    int64_t n = first;
+    int qh = 0, qt = begin;  // the tile's head and place
+    if (n < end) {
+      qh = int(n / (last - begin));
+      qt = begin + int(n - int64_t(qh) * (last - begin));
+    }
+    // A tile of queries in buffer B.  32 queries' scores and their gradients are formed beside the weights of the
+    // 32 before, and these are multiplied beside the weights of the next.
+    auto step = [&](auto buffer) {
+      char* buf = lds + buffer.value * STAGE;
+      loads_in_flight<0>();
+      __syncthreads();
+      const int query0 = qt * BQ;
+      if (++qt == last) {
+        qt = begin;
+        ++qh;
       }
-    };
-    auto read_t = [&](int x) {
-      return [=](int i) {
-        return L::read_t(buf + (i & 1 ? 0 : L::BYTES),
-                         32 * x + (i >> 1) / TILES * Mfma<T>::KSTEP, 32 * ((i >> 1) % TILES));
+      if (n + 1 < end) start(qh, qt, lds + (1 - buffer.value) * STAGE);
+      // (asked in either case: without these branches the compiler's order of the step takes more registers than
+      // there are, 176 bytes of scratch at 64 values a head and half the speed)
+      if (query0 + BQ <= wave_least) return;
+      const bool edge = query0 < wave_most;
+      const float* stats = reinterpret_cast<const float*>(buf + 2 * L::BYTES);
+      floatx16 s[NX], dp[NX];
+      frag p[NX][PS], ds[NX][PS];
+      float4v base[2], minus[2];  // of four weights, and of the next four
+      auto read = [&](int x) {
+        return [=](int i) { return L::read(buf + (i & 1) * L::BYTES, 32 * x, i >> 1); };
       };
-    };
-    auto add = [&](int x, int i, const frag& f) {
-      const int d = (i >> 1) % TILES, w = (i >> 1) / TILES;
-      if (i & 1)
-        Mfma<T>::mma(f, ds[x][w], dk[d]);
-      else
-        Mfma<T>::mma(f, p[x][w], dv[d]);
-    };
-    constexpr int FORM = 2 * STEPS, ADD = 2 * PS * TILES;
-    if constexpr (!dkv_beside<T>(DP)) {
+      auto form = [&](int x, int i, const frag& f) {
+        if (i & 1)
+          Mfma<T>::mma(f, v[i >> 1], dp[x]);
+        else
+          Mfma<T>::mma(f, k[i >> 1], s[x]);
+      };
+      // the weights of 32 queries: what they take, what of them is hidden, and weights lo .. hi - 1
+      auto take = [&](int x, int i) {
+        const int r = 32 * x + acc_row<T>(4 * i);
+        base[i & 1] = *reinterpret_cast<const float4v*>(stats + r);
+        minus[i & 1] = *reinterpret_cast<const float4v*>(stats + kStats + r);
+      };
+      auto prepare = [&](int x) {
+        take(x, 0);
+        if (!edge) return;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (query0 + 32 * x + acc_row<T>(i) < from) {
+            s[x][i] = -__builtin_inff();
+            dp[x][i] = 0.f;  // (not what a NaN there makes of it)
+          }
+      };
+      auto weigh = [&](int x, int lo, int hi) {
+#pragma unroll
+        for (int i = lo; i < hi; ++i) {
+          if ((i & 3) == 0 && i < 12) take(x, (i >> 2) + 1);
+          const float e =
+              __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, base[i >> 2 & 1][i & 3]));
+          float d = dp[x][i] + minus[i >> 2 & 1][i & 3];
+          if (kLift<T> != 0.f) d *= g;
+          p[x][i / V][i % V] = T(e);
+          ds[x][i / V][i % V] = T(e * d);
+        }
+      };
+      auto read_t = [&](int x) {
+        return [=](int i) {
+          return L::read_t(buf + (i & 1 ? 0 : L::BYTES),
+                           32 * x + (i >> 1) / TILES * Mfma<T>::KSTEP, 32 * ((i >> 1) % TILES));
+        };
+      };
+      auto add = [&](int x, int i, const frag& f) {
+        const int d = (i >> 1) % TILES, w = (i >> 1) / TILES;
+        if (i & 1) {
+          if constexpr (DK) Mfma<T>::mma(f, ds[x][w], dk[d]);
+        } else {
+          if constexpr (DV) Mfma<T>::mma(f, p[x][w], dv[d]);
+        }
+      };
+      constexpr int FORM = 2 * STEPS, ADD = 2 * PS * TILES;
+      if constexpr (STRICT || !dkv_beside<T>(DP)) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          zero(s[x]);
+          zero(dp[x]);
+          beside<frag, FORM, kAhead>(read(x), [&](int i, const frag& f) { form(x, i, f); });
+          prepare(x);
+          weigh(x, 0, 16);
+          if (STRICT && edge) {
+            if constexpr (DV)
+              add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from - query0, BQ, p[x], dv);
+            if constexpr (DK)
+              add_rows_seen<T, DP, BQ>(buf, 32 * x, from - query0, BQ, ds[x], dk);
+          } else {
+            beside<frag, ADD, kAhead>(read_t(x), [&](int i, const frag& f) { add(x, i, f); });
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
         zero(s[x]);
         zero(dp[x]);
-        beside<frag, FORM, kAhead>(read(x), [&](int i, const frag& f) { form(x, i, f); });
-        prepare(x);
-        weigh(x, 0, 16);
-        if (STRICT && edge) {
-          add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from - query0, BQ, p[x], dv);
-          add_rows_seen<T, DP, BQ>(buf, 32 * x, from - query0, BQ, ds[x], dk);
-        } else {
-          beside<frag, ADD, kAhead>(read_t(x), [&](int i, const frag& f) { add(x, i, f); });
-        }
       }
-      return;
-    }
-#pragma unroll
-    for (int x = 0; x < NX; ++x) {
-      zero(s[x]);
-      zero(dp[x]);
-    }
-    beside<frag, FORM, kAhead>(read(0), [&](int i, const frag& f) { form(0, i, f); });
-#pragma unroll
-    for (int x = 0; x < NX; ++x) {
-      prepare(x);
-      if (x + 1 < NX) {
-        beside<frag, FORM, kAhead>(read(x + 1), [&](int i, const frag& f) {
-          form(x + 1, i, f);
-          weigh(x, 16 * i / FORM, 16 * (i + 1) / FORM);
-        });
-      } else if (x > 0 && !(STRICT && edge)) {
-        beside<frag, ADD, kAhead>(read_t(x - 1), [&](int i, const frag& f) {
-          add(x - 1, i, f);
-          weigh(x, 16 * i / ADD, 16 * (i + 1) / ADD);
-        });
-      } else {
-        weigh(x, 0, 16);
-      }
-    }
-    if (STRICT && edge) {
+      beside<frag, FORM, kAhead>(read(0), [&](int i, const frag& f) { form(0, i, f); });
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
-        add_rows_seen<T, DP, BQ>(buf + L::BYTES, 32 * x, from - query0, BQ, p[x], dv);
-        add_rows_seen<T, DP, BQ>(buf, 32 * x, from - query0, BQ, ds[x], dk);
+        prepare(x);
+        if (x + 1 < NX) {
+          beside<frag, FORM, kAhead>(read(x + 1), [&](int i, const frag& f) {
+            form(x + 1, i, f);
+            weigh(x, 16 * i / FORM, 16 * (i + 1) / FORM);
+          });
+        } else if (x > 0) {
+          beside<frag, ADD, kAhead>(read_t(x - 1), [&](int i, const frag& f) {
+            add(x - 1, i, f);
+            weigh(x, 16 * i / ADD, 16 * (i + 1) / ADD);
+          });
+        } else {
+          weigh(x, 0, 16);
+        }
       }
-    } else {
       beside<frag, ADD, kAhead>(read_t(NX - 1), [&](int i, const frag& f) { add(NX - 1, i, f); });
+    };
+    if (n < end) start(qh, qt, lds);
+    while (n < end) {
+      step(std::integral_constant<int, 0>());
+      if (++n == end) break;
+      step(std::integral_constant<int, 1>());
+      ++n;
     }
+    bool bad = false;
+    if constexpr (CAUSAL && !STRICT) bad = any_not_finite(dk) || any_not_finite(dv);
+    report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
+    if (!live) return;
+    const float fk = a.scale * __builtin_amdgcn_exp2f(-lift), fv = __builtin_amdgcn_exp2f(-kLift<T>);
+    const int64_t r = t.lo + at;
+    if (a.shares > 1) {
+      float* to = a.part + (((place.share * 2) * a.ks.rows + r) * a.Hk + place.head) * a.D;
+      if constexpr (DK) store_part<DP, V>(to, a.D, [&](int d, int i) { return dk[d][i] * fk; });
+      if constexpr (DV)
+        store_part<DP, V>(to + a.ks.rows * a.Hk * a.D, a.D, [&](int d, int i) { return dv[d][i] * fv; });
+      return;
+    }
+    if constexpr (DK)
+      if (a.dk.p)
+        store_head<T, DP>(a.dk.p + r * a.dk.row + place.head * a.dk.head, a.D,
+                          [&](int d, int i) { return dk[d][i] * fk; });
+    if constexpr (DV)
+      if (a.dv.p)
+        store_head<T, DP>(a.dv.p + r * a.dv.row + place.head * a.dv.head, a.D,
+                          [&](int d, int i) { return dv[d][i] * fv; });
   };
-  if (n < end) start(qh, qt, lds);
-  while (n < end) {
-    step(std::integral_constant<int, 0>());
-    if (++n == end) break;
-    step(std::integral_constant<int, 1>());
-    ++n;
+  if constexpr (STRICT) {
+    // (one after the other: both at once take more registers than there are, 1.3 KB of scratch a lane at 128 values)
+    pass(std::true_type(), std::false_type());
+    __syncthreads();  // (the last tile is read by all before the first one is loaded again)
+    pass(std::false_type(), std::true_type());
+  } else {
+    pass(std::true_type(), std::true_type());
   }
-  bool bad = false;
-  if (CAUSAL && !STRICT) bad = any_not_finite(dk) || any_not_finite(dv);
-  report<CAUSAL, STRICT>(a.again, bad, &bad_lds);
-  if (!live) return;
-  const float fk = a.scale * __builtin_amdgcn_exp2f(-lift), fv = __builtin_amdgcn_exp2f(-kLift<T>);
-  const int64_t r = t.lo + at;
-  if (a.shares > 1) {
-    float* to = a.part + (((place.share * 2) * a.ks.rows + r) * a.Hk + place.head) * a.D;
-    store_part<DP, V>(to, a.D, [&](int d, int i) { return dk[d][i] * fk; });
-    store_part<DP, V>(to + a.ks.rows * a.Hk * a.D, a.D, [&](int d, int i) { return dv[d][i] * fv; });
-    return;
-  }
-  if (a.dk.p)
-    store_head<T, DP>(a.dk.p + r * a.dk.row + place.head * a.dk.head, a.D,
-                      [&](int d, int i) { return dk[d][i] * fk; });
-  if (a.dv.p)
-    store_head<T, DP>(a.dv.p + r * a.dv.row + place.head * a.dv.head, a.D,
-                      [&](int d, int i) { return dv[d][i] * fv; });
 }
 
 // out[r][h] = the sum of the shares' partials, which lie `stride` values apart: four values a lane, four runs of

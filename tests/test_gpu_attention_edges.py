@@ -34,3 +34,54 @@ def test_many_small_weights_beside_a_large_one(dtype):
     room = lost + want * (2.01 * UNIT[dtype] + (20 + nk / 64) * STEP)
     off = (out.double() - want).abs().max().item()
     assert off <= room
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("bad", [math.nan, -math.inf])
+@pytest.mark.parametrize("d", [16, 64, 80, 96, 112, 128])
+def test_hidden_rows_in_wide_heads_of_several_sequences(dtype, bad, d):
+    """Causal, a head of keys for two of queries: what does not see a bad row lies within the bounds of a call
+    without it, in its own sequence and in the others."""
+    lens, at = [150, 3, 97], 70
+    n, first = sum(lens), lens[0]
+    args = _inputs(n, n, 4, 2, d, dtype)
+    q, k, v, dout = args
+    off, want = _offsets(lens), _reference(*args, lens, lens, True)
+    k2, v2 = k.clone(), v.clone()
+    k2[at], v2[at + 3] = bad, bad
+    got = _run(q, k2, v2, dout, off, causal=True)
+    assert not got[0][at + 3:first].isfinite().all()
+    _check([t[:at] for t in got[:2]], [[t[:at] for t in w[:2]] for w in want])
+    _check([t[first:] for t in got], [[t[first:] for t in w] for w in want])
+    q2, dout2 = q.clone(), dout.clone()
+    q2[at], dout2[at - 2] = bad, bad
+    got = _run(q2, k, v, dout2, off, causal=True)
+    assert not got[3][:at - 1].isfinite().any() and not got[1][at].isfinite().any()
+    _check([t[at + 1:first] for t in got[2:]], [[t[at + 1:first] for t in w[2:]] for w in want],
+           ("dk", "dv"))
+    _check([t[first:] for t in got], [[t[first:] for t in w] for w in want])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_hidden_rows_where_the_other_axis_is_cut_into_shares(dtype, d):
+    """Shares that are made again overwrite theirs before all are joined."""
+    args = _inputs(200, 1500, 2, 1, d, dtype)
+    q, k, v, dout = args
+    want = _reference(*args, [200], [1500], True)
+    k2, v2 = k.clone(), v.clone()
+    k2[1400], v2[1403] = math.nan, math.inf  # (seen by queries from 100 and 103 on)
+    got = _run(q, k2, v2, dout, causal=True)
+    _check([t[:100] for t in got[:2]], [[t[:100] for t in w[:2]] for w in want])
+    assert not got[0][100:].isfinite().any() and not got[1][100:].isfinite().any()
+    args = _inputs(1500, 200, 2, 1, d, dtype)
+    q, k, v, dout = args
+    want = _reference(*args, [1500], [200], True)
+    q2, dout2 = q.clone(), dout.clone()
+    q2[1400], dout2[1403] = math.inf, math.nan  # (see the keys up to 100 and 103)
+    got = _run(q2, k, v, dout2, causal=True)
+    _check([t[104:] for t in got[2:]], [[t[104:] for t in w[2:]] for w in want], ("dk", "dv"))
+    assert not got[2][:101].isfinite().any() and not got[3][:101].isfinite().any()
+    fine = torch.ones(1500, dtype=torch.bool, device=DEV)
+    fine[1400], fine[1403] = False, False
+    _check([t[fine] for t in got[:2]], [[t[fine] for t in w[:2]] for w in want])
