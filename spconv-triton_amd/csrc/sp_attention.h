@@ -151,9 +151,9 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 }
 
 // Loads of a thread's pieces of tiles of a head's rows.  Whole tiles take an address of the workgroup's and
-// an offset of the lane's for good; the pieces past the head's width are zeroed once and never
-// written.  A tile that passes the last row goes by piece, with zeros past the end (0 times what
-// lies there could be NaN).
+// an offset of the lane's for good.  A tile that passes the last row, or whose head is narrower than DP, goes by
+// piece, with zeros past the ends (0 times what lies there could be NaN).  Every lane loads, at a selected address:
+// behind a branch that some lanes take the compiler once saved registers before the others were back.
 template <typename T, int DP, int ROWS>
 struct TileLoads {
   using L = HeadTile<T, DP, ROWS>;
@@ -174,14 +174,6 @@ struct TileLoads {
     const int m = at_row(j);
     return swizzled<L::PIECES>(m, j * kAttnThreads + int(threadIdx.x) - m * L::PIECES) * L::V;
   }
-  // zeros past the head's width, before the first tile (a barrier follows)
-  __device__ __forceinline__ void clear(char* lds) const {
-#pragma unroll
-    for (int j = 0; j < L::N; ++j)
-      if (at_value(j) >= D)
-        *reinterpret_cast<uint4*>(lds + (j * kAttnThreads + int(threadIdx.x)) * 16) =
-            uint4{0, 0, 0, 0};
-  }
   __device__ __forceinline__ void start(int at, char* lds) const {
     const char* base = uniform(reinterpret_cast<const char*>(p + at * row));
     if (DP == D && at + ROWS <= len) {
@@ -191,10 +183,11 @@ struct TileLoads {
       return;
     }
 #pragma unroll
-    for (int j = 0; j < L::N; ++j)
-      if (at_value(j) < D)
-        copy_piece(at + at_row(j) < len ? static_cast<const void*>(base + off[j]) : &g_zero_piece,
-                   lds + (j * kAttnThreads + wave_of() * 64) * 16);
+    for (int j = 0; j < L::N; ++j) {
+      const bool in = (at_value(j) < D) & (at + at_row(j) < len);
+      copy_piece(in ? static_cast<const void*>(base + off[j]) : &g_zero_piece,
+                 lds + (j * kAttnThreads + wave_of() * 64) * 16);
+    }
   }
 };
 

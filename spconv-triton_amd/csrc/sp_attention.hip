@@ -85,10 +85,6 @@ __global__ __launch_bounds__(kAttnThreads, attend_waves<T>(DP, STRICT)) void att
   const TileLoads<T, DP, BK> lk(a.k.p + klo * a.k.row + place.head * a.k.head, a.k.row, Lk, a.D);
   const TileLoads<T, DP, BK> lv(a.v.p + klo * a.v.row + place.head * a.v.head, a.v.row, Lk, a.D);
   const float c = a.scale2;
-  if (DP != a.D) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
-  }
   floatx16 o[TILES];
   float m = -__builtin_inff(), neg = 0.f, l = 0.f;
 #pragma unroll

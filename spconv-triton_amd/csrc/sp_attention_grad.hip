@@ -231,10 +231,6 @@ __global__ __launch_bounds__(kAttnThreads, dq_waves<T>(DP, STRICT)) void attend_
   const TileLoads<T, DP, BK> lk(a.k.p + klo * a.k.row + place.head * a.k.head, a.k.row, Lk, a.D);
   const TileLoads<T, DP, BK> lv(a.v.p + klo * a.v.row + place.head * a.v.head, a.v.row, Lk, a.D);
   const float c = a.scale2;
-  if (DP != a.D) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lk.clear(lds + i * L::BYTES);
-  }
   floatx16 acc[TILES];
 #pragma unroll
   for (int d = 0; d < TILES; ++d) zero(acc[d]);
@@ -424,10 +420,6 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP, STRICT)) void atten
     }
   };
   const float c = a.scale2;
-  if (DP != a.D) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lq.clear(lds + (i >> 1) * STAGE + (i & 1) * L::BYTES);
-  }
   // A pass over the queries, for dk, dv or both.
   auto pass = [&](auto want_dk, auto want_dv) {
     constexpr bool DK = want_dk.value, DV = want_dv.value;

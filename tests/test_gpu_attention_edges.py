@@ -85,3 +85,19 @@ def test_hidden_rows_where_the_other_axis_is_cut_into_shares(dtype, d):
     fine = torch.ones(1500, dtype=torch.bool, device=DEV)
     fine[1400], fine[1403] = False, False
     _check([t[fine] for t in got[:2]], [[t[fine] for t in w[:2]] for w in want])
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 100), (F32, 108), (F32, 124), (F32, 68), (F16, 104),
+                                     (F16, 120), (BF16, 104), (BF16, 120), (F16, 72), (BF16, 88),
+                                     (F16, 8), (F32, 4), (F32, 36)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_heads_narrower_than_the_kernels(dtype, d, causal):
+    """Tiles whose last pieces are zeros beside the head's values, whole and ragged."""
+    ql, kl = [130, 0, 70, 1], [257, 5, 64, 1]
+    args = _inputs(sum(ql), sum(kl), 4, 2, d, dtype)
+    got = _run(*args, _offsets(ql), _offsets(kl), causal)
+    _check(got, _reference(*args, ql, kl, causal))
+    wide = torch.full((sum(kl), 2, d + 8), math.nan, device=DEV, dtype=dtype)
+    wide[..., :d] = args[2]
+    again = _run(args[0], args[1], wide[..., :d], args[3], _offsets(ql), _offsets(kl), causal)
+    assert all(torch.equal(a, b) for a, b in zip(again, got))
