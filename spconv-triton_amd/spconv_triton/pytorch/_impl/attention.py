@@ -105,18 +105,38 @@ def split_packed(qkv, heads: int, kv_heads: int | None):
     return t[:, :heads], t[:, heads:heads + kv_heads], t[:, heads + kv_heads:]
 
 
-def _heads(t, width: int, vec: int):
-    """(tensor, address, row stride, head stride) as the kernels take them, heads `width` wide."""
+def _as_is(t, width: int, vec: int):
+    """(address, row stride, head stride) where the kernels take t's memory for heads `width` wide,
+    or None."""
     n, h, d = t.shape
     s0, s1, s2 = t.stride()
     p = t.data_ptr()
     if (d == width and (s2 == 1 or d == 1) and (s0 % vec == 0 and s0 < 1 << 23 or n <= 1)
             and ((s1 % vec == 0 and s1 >= d) or h == 1) and p % 16 == 0):
-        return t, p, s0 if n > 1 else 0, s1 if h > 1 else 0
-    t = F.pad(t, (0, width - d)).contiguous() if d < width else t.contiguous()
-    if t.data_ptr() % 16:
-        t = t.clone()
-    return t, t.data_ptr(), h * width, width
+        return p, s0 if n > 1 else 0, s1 if h > 1 else 0
+    return None
+
+
+def _heads(t, width: int, vec: int):
+    """(tensor, address, row stride, head stride) as the kernels take them, heads `width` wide."""
+    own = _as_is(t, width, vec)
+    if own is None:
+        d = t.shape[2]
+        t = F.pad(t, (0, width - d)).contiguous() if d < width else t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        own = t.data_ptr(), t.shape[1] * width, width
+    return t, *own
+
+
+def _room(t, width: int, vec: int):
+    """The same for a result of t's shape: t itself, or memory for a padded copy of it."""
+    own = _as_is(t, width, vec) if t.numel() else (t.data_ptr(), 0, 0)
+    if own is None:
+        n, h, _ = t.shape
+        t = torch.empty((n, h, width), dtype=t.dtype, device=t.device)
+        own = t.data_ptr(), h * width, width
+    return t, *own
 
 
 def _call(q, k, v, offsets, key_offsets, causal, scale):
@@ -190,8 +210,7 @@ def run_attention_backward(dout, q, k, v, out, lse, offsets, key_offsets, causal
             into.append(None)
             args.append((None, 0, 0))
             continue
-        t, p, s0, s1 = _heads(g, width, vec) if g.numel() else (g, g.data_ptr(), 0, 0)
-        # (a copy, where the kernels cannot write the gradient's own memory)
+        t, p, s0, s1 = _room(g, width, vec)
         into.append(t)
         args.append((p, s0, s1))
     (pq, q0, q1), (pk, k0, k1), (pv, v0, v1) = args

@@ -127,3 +127,44 @@ def test_rows_that_32_bit_places_cannot_count_are_refused():
                 == _lib.SP_ERR_INVALID_ARG)
     c = _Call(p, p, p, 64, 32, 64, 32, 64, 32, most, most, 1, 1, 32, 0, None, None, 0.1, 0, 0)
     assert L.sp_attention_bwd_workspace(ctypes.byref(c)) > 0
+
+
+def test_gradients_of_padded_heads_are_not_copied_before_they_hold_anything(no_gpu_needed, monkeypatch):
+    """Heads of 20 fp16 values are padded to 24 for the kernels: the five inputs are copied, and the three gradients
+    get memory of that shape, from which they are copied afterwards."""
+    from spconv_triton.pytorch._impl import _lib
+    from spconv_triton.pytorch._impl import attention as impl
+
+    padded, written = [], []
+
+    def pad(t, by):
+        padded.append(t.data_ptr())
+        return torch.nn.functional.pad(t, by)
+
+    class Library:
+        def sp_attention_bwd_workspace(self, call):
+            return 0
+
+        def sp_attention_bwd(self, call, grad, ws, nbytes, stream):
+            g = ctypes.cast(grad, ctypes.POINTER(impl._Grad)).contents
+            for p, row, head in ((g.dq, g.dq_row, g.dq_head), (g.dk, g.dk_row, g.dk_head),
+                                 (g.dv, g.dv_row, g.dv_head)):
+                written.append((p, row, head))
+                for r in range(3):
+                    for h in range(2):
+                        at = p + 2 * (r * row + h * head)
+                        ctypes.memmove(at, bytes(range(h, h + 48)), 48)
+            return 0
+
+    monkeypatch.setattr(impl, "F", type("F", (), {"pad": staticmethod(pad)}))
+    monkeypatch.setattr(_lib, "lib", Library)
+    monkeypatch.setattr(_lib, "stream_of", lambda device: None)
+    x = [torch.randn(3, 2, 20).half() for _ in range(5)]
+    grads = [torch.empty(3, 2, 20, dtype=torch.float16) for _ in range(3)]
+    impl.run_attention_backward(x[4], *x[:3], x[3], torch.zeros(2, 3), None, None, False, None, grads)
+    assert sorted(padded) == sorted(t.data_ptr() for t in x)
+    assert [w[1:] for w in written] == [(48, 24)] * 3
+    for g in grads:
+        for h in range(2):
+            want = torch.frombuffer(bytearray(range(h, h + 40)), dtype=torch.float16)
+            assert torch.equal(g[:, h].view(torch.int16), want.view(torch.int16).expand(3, 20))
