@@ -28,6 +28,11 @@ constexpr int kNormChunks = 1024;  // chunks that a call is cut into, about
 // parts of 256 rows 12.7 and 11.6, for 15.6 and 12.6 of several.
 constexpr int64_t kNormSmall = 65536, kNormSmallPart = 16384;
 constexpr int kSmallThreads = 512;
+// The parameters' gradients are summed over the parts in slabs of so many rows, slabs over slabs until one is left: four
+// runs of a slab apart and then in order, 64 channels a workgroup.  (A thread a channel going through all parts: a
+// backward pass over 65 536 parts of 4 rows of 64 bf16 channels 17 650 us, 1 915 so; of 196 windows of 1 024 rows 80
+// and 43; and a chain of 70 000 sums was off by 2^-13.)
+constexpr int kNormSlab = 256;
 
 enum { kActNone = 3 };  // beside the feed-forward block's activations
 
@@ -79,6 +84,8 @@ struct NormArgs {
   float2* stats;  // [parts][groups]: mean, inv
   float2* part;   // [slots][C]: a chunk's moments; sums of dz and dz u
   float2* sums;   // [parts][C]: sums of dz and dz u
+  const float2* rows;  // [n_rows][C]: these, or their sums over slabs of them
+  int n_rows;
   float2* back;   // [parts][groups]: mean(w dz), mean(w dz u)
 };
 
@@ -481,20 +488,63 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_join(NormArgs<T, P> a)
   a.back[blockIdx.x] = n ? float2{all.x / count, all.y / count} : float2{0.f, 0.f};
 }
 
-// dx; the workgroups from `slots` on sum the parameters' gradients over the parts.
+// The sum of rows first .. end - 1 at 64 channels from c0 on, a channel a lane of the first wave.
+__device__ __forceinline__ float2 sum_rows(const float2* rows, int64_t first, int64_t end, int C,
+                                           int c0) {
+  static_assert(kNormThreads == 256, "four runs");
+  __shared__ float2 lds[4][64];
+  const int lane = int(threadIdx.x) & 63, run = int(threadIdx.x) >> 6, c = c0 + lane;
+  float2 v{0.f, 0.f};
+  if (c < C) {
+    const int64_t per = (end - first + 3) / 4, lo = first + run * per;
+    const int64_t hi = lo + per < end ? lo + per : end;
+    for (int64_t r = lo; r < hi; r += kNormLoads) {
+      float2 o[kNormLoads];
+#pragma unroll
+      for (int i = 0; i < kNormLoads; ++i) o[i] = rows[(r + i < hi ? r + i : r) * C + c];
+#pragma unroll
+      for (int i = 0; i < kNormLoads; ++i) {
+        v.x += r + i < hi ? o[i].x : 0.f;
+        v.y += r + i < hi ? o[i].y : 0.f;
+      }
+    }
+  }
+  lds[run][lane] = v;
+  __syncthreads();
+#pragma unroll
+  for (int k = 1; k < 4; ++k) {
+    v.x += lds[k][lane].x;
+    v.y += lds[k][lane].y;
+  }
+  return v;  // (of use to the first wave: its own run and the others in order)
+}
+
+// The sums of the slabs of rows [n][C], a row each.
+__global__ __launch_bounds__(kNormThreads) void norm_slabs(const float2* __restrict__ rows, int n,
+                                                           int C, float2* __restrict__ out) {
+  const int blocks = (C + 63) / 64;
+  const int64_t slab = blockIdx.x / blocks, first = slab * kNormSlab;
+  const int c0 = int(blockIdx.x - slab * blocks) * 64;
+  const float2 v = sum_rows(rows, first, first + kNormSlab < n ? first + kNormSlab : n, C, c0);
+  const int c = c0 + int(threadIdx.x);
+  if (threadIdx.x < 64 && c < C) out[slab * C + c] = v;
+}
+
+// The parameters' gradients of 64 channels.
+template <typename T, typename P>
+__device__ __forceinline__ void write_params(const NormArgs<T, P>& a, int c0) {
+  const float2 v = sum_rows(a.rows, 0, a.n_rows, a.s.C, c0);
+  const int c = c0 + int(threadIdx.x);
+  if (threadIdx.x >= 64 || c >= a.s.C) return;
+  if (a.dw) a.dw[c] = from_f32<P>(v.y);
+  if (a.db) a.db[c] = from_f32<P>(v.x);
+}
+
+// dx; the workgroups from `slots` on sum the parameters' gradients.
 template <typename T, typename P, int V, int ACT>
 __global__ __launch_bounds__(kNormThreads) void norm_grad_apply(NormArgs<T, P> a, int64_t slots) {
   if (int64_t(blockIdx.x) >= slots) {
-    const int c = int(blockIdx.x - slots) * kNormThreads + int(threadIdx.x);
-    if (blockIdx.y != 0 || c >= a.s.C) return;
-    float2 v{0.f, 0.f};
-    for (int p = 0; p < a.seqs.parts; ++p) {
-      const float2 o = a.sums[int64_t(p) * a.s.C + c];
-      v.x += o.x;
-      v.y += o.y;
-    }
-    if (a.dw) a.dw[c] = from_f32<P>(v.y);
-    if (a.db) a.db[c] = from_f32<P>(v.x);
+    if (blockIdx.y == 0) write_params(a, int(blockIdx.x - slots) * 64);
     return;
   }
   if (!a.dx) return;
@@ -627,17 +677,7 @@ __global__ __launch_bounds__(kSmallThreads) void norm_grad_small(NormArgs<T, P> 
 // The parameters' gradients from the parts' sums.
 template <typename T, typename P>
 __global__ __launch_bounds__(kNormThreads) void norm_grad_params(NormArgs<T, P> a) {
-  const int c = int(blockIdx.x) * kNormThreads + int(threadIdx.x);
-  if (c >= a.s.C) return;
-  float2 v{0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < a.seqs.parts; ++p) {
-    const float2 o = a.sums[int64_t(p) * a.s.C + c];
-    v.x += o.x;
-    v.y += o.y;
-  }
-  if (a.dw) a.dw[c] = from_f32<P>(v.y);
-  if (a.db) a.db[c] = from_f32<P>(v.x);
+  write_params(a, int(blockIdx.x) * 64);
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -664,10 +704,34 @@ static Seqs norm_seqs(const int32_t* off, int64_t rows, int64_t n) {
   return Seqs{off, rows, off ? int(n) + 2 : 1};
 }
 
+static size_t slabs_bytes(int64_t parts, int64_t C) {
+  return parts > kNormSlab ? align_up(size_t(cdiv(parts, kNormSlab)) * C * sizeof(float2), 256) : 0;
+}
+
+// At most kNormSlab rows that add up to those of the parts: a.rows, between a.sums and the workspace at `slabs`.
+template <typename T, typename P>
+static int join_parts(NormArgs<T, P>& a, char* slabs, hipStream_t st) {
+  float2 *from = a.sums, *to = reinterpret_cast<float2*>(slabs);
+  int64_t n = a.seqs.parts;
+  while (n > kNormSlab && (a.dw || a.db)) {
+    const int64_t next = cdiv(n, kNormSlab), groups = next * cdiv(a.s.C, 64);
+    SP_CHECK_ARG(groups <= kMaxGridX, "group_norm_bwd: too many samples");
+    norm_slabs<<<unsigned(groups), kNormThreads, 0, st>>>(from, int(n), a.s.C, to);
+    SP_LAUNCHED();
+    float2* const read = from;
+    from = to;
+    to = read;
+    n = next;
+  }
+  a.rows = from;
+  a.n_rows = int(n);
+  return SP_OK;
+}
+
 // (the sizes do not depend on V, which the tensors' addresses decide)
 static size_t norm_workspace(int64_t rows, int64_t C, int64_t groups, const Seqs& q, int V,
                              bool grad) {
-  const size_t sums = align_up(size_t(q.parts) * C * sizeof(float2), 256);
+  const size_t sums = align_up(size_t(q.parts) * C * sizeof(float2), 256) + slabs_bytes(q.parts, C);
   if (norm_is_small(rows, C, q, V)) return grad && q.parts > 1 ? sums : 0;
   const NormShape s = norm_shape(rows, int(C), int(groups), V);
   size_t n = align_up(size_t(tile_slots(q, 1, int(s.chunk))) * C * sizeof(float2), 256);
@@ -726,19 +790,23 @@ static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
     });
     SP_LAUNCHED();
     if (a.seqs.parts == 1 || !(a.dw || a.db)) return SP_OK;
-    norm_grad_params<T, P><<<unsigned(cdiv(a.s.C, kNormThreads)), kNormThreads, 0, st>>>(a);
+    ws += align_up(size_t(a.seqs.parts) * a.s.C * sizeof(float2), 256);
+    if (int rc = join_parts(a, ws, st)) return rc;
+    norm_grad_params<T, P><<<unsigned(cdiv(a.s.C, 64)), kNormThreads, 0, st>>>(a);
     SP_LAUNCHED();
     return SP_OK;
   }
   a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
   const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
   const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
-  const int64_t extra = cdiv(a.s.C, kNormThreads);
+  const int64_t extra = a.dw || a.db ? cdiv(a.s.C, 64) : 0;
   SP_CHECK_ARG(slots + extra <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
   a.part = reinterpret_cast<float2*>(ws);
   ws += align_up(size_t(slots) * a.s.C * sizeof(float2), 256);
   a.sums = reinterpret_cast<float2*>(ws);
   ws += align_up(size_t(a.seqs.parts) * a.s.C * sizeof(float2), 256);
+  char* const slabs = ws;
+  ws += slabs_bytes(a.seqs.parts, a.s.C);
   a.back = reinterpret_cast<float2*>(ws);
   const dim3 grid(unsigned(slots), unsigned(a.s.blocks));
   norm_act_of(act, [&](auto k) {
@@ -748,6 +816,7 @@ static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
   SP_LAUNCHED();
   norm_grad_join<T, P><<<unsigned(joins), kNormThreads, 0, st>>>(a);
   SP_LAUNCHED();
+  if (int rc = join_parts(a, slabs, st)) return rc;
   const dim3 last(unsigned(slots + extra), unsigned(a.s.blocks));
   norm_act_of(act, [&](auto k) {
     norm_grad_apply<T, P, V, k.value><<<last, kNormThreads, 0, st>>>(a, slots);
