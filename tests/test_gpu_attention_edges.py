@@ -101,3 +101,15 @@ def test_heads_narrower_than_the_kernels(dtype, d, causal):
     wide[..., :d] = args[2]
     again = _run(args[0], args[1], wide[..., :d], args[3], _offsets(ql), _offsets(kl), causal)
     assert all(torch.equal(a, b) for a, b in zip(again, got))
+
+
+@pytest.mark.parametrize("lengths,h,hk,d,dtype", [
+    ([7, 0, 20] * 22, 2, 1, 32, F16), ([3] * 65, 4, 2, 16, BF16), ([130, 1] * 65, 2, 2, 32, F32),
+    ([0] * 70 + [200] + [0] * 70, 2, 2, 64, F16), ([2, 0, 1, 4] * 1050, 1, 1, 16, F32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_sequences_than_a_wave_looks_at_at_a_time(lengths, h, hk, d, dtype, causal):
+    """Tiles are found 64 ways at a time: 65 to 4200 sequences, empty ones among them, of queries and of keys."""
+    short = [m + (i % 3) for i, m in enumerate(lengths)] if len(lengths) < 200 else lengths
+    args = _inputs(sum(lengths), sum(short), h, hk, d, dtype)
+    got = _run(*args, _offsets(lengths), _offsets(short), causal)
+    _check(got, _reference(*args, lengths, short, causal))
