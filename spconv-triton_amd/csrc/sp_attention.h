@@ -455,6 +455,8 @@ inline int64_t attn_groups(int64_t slots, int heads, int shares) {
   return cdiv(slots * heads * shares, 8) * 8;
 }
 
+constexpr int64_t kAttnMaxGroups = max_groups(kAttnThreads);
+
 struct AttnGradLayout {
   size_t nl, nd, tops, part, again, total;
   int dq_shares, dkv_shares;

@@ -291,7 +291,12 @@ template <typename T>
 static int launch_attend(AttnArgs<T> a, hipStream_t s) {
   const int64_t slots = tile_slots(a.qs, a.G, kForwardRows);
   const int64_t groups = attn_groups(slots, a.Hk, a.shares);
-  SP_CHECK_ARG(groups <= kMaxGridX, "attention: too many rows");
+  const bool few = a.shares <= kFewShares;
+  const int64_t rows = a.qs.rows * a.H;
+  const int64_t joins =
+      a.shares == 1 ? 0 : few ? cdiv(rows * (a.D / 4), kAttnThreads) : rows;
+  SP_CHECK_ARG(groups <= kAttnMaxGroups && joins <= kAttnMaxGroups,
+               "attention: too many rows and sequences for a launch");
   with_width(a.D, [&](auto w) {
     constexpr int DP = w.value, BK = attn_stage<T>();
     const dim3 grid{unsigned(groups)}, block{kAttnThreads};
@@ -305,10 +310,6 @@ static int launch_attend(AttnArgs<T> a, hipStream_t s) {
   });
   SP_LAUNCHED();
   if (a.shares == 1) return SP_OK;
-  const bool few = a.shares <= kFewShares;
-  const int64_t rows = a.qs.rows * a.H;
-  const int64_t joins = few ? cdiv(rows * (a.D / 4), kAttnThreads) : rows;
-  SP_CHECK_ARG(joins <= kMaxGridX, "attention: too many rows");
   if (few)
     attend_join_few<T><<<unsigned(joins), kAttnThreads, 0, s>>>(a);
   else

@@ -664,6 +664,15 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
   a.again = reinterpret_cast<int*>(ws + l.again);
   a.top = tops;
   if (!need_dq && !need_dkv) return SP_OK;
+  const int64_t q_slots = tile_slots(a.qs, a.G, kGradRows), k_slots = tile_slots(a.ks, 1, kGradRows);
+  const int64_t q_groups = attn_groups(q_slots, a.Hk, l.dq_shares);
+  const int64_t k_groups = attn_groups(k_slots, a.Hk, l.dkv_shares);
+  auto sums = [&](int shares, int64_t n) { return shares > 1 ? cdiv(n * (a.D / 4), 64) : 0; };
+  SP_CHECK_ARG((!need_dq || (q_groups <= kAttnMaxGroups &&
+                             sums(l.dq_shares, a.qs.rows * a.H) <= kAttnMaxGroups)) &&
+                   (!need_dkv || (k_groups <= kAttnMaxGroups &&
+                                  sums(l.dkv_shares, a.ks.rows * a.Hk) <= kAttnMaxGroups)),
+               "attention_bwd: too many rows and sequences for a launch");
   int lanes = 0;
   while ((Mfma<T>::V << lanes) < a.D) ++lanes;
   const int64_t most = a.qs.rows * a.H > a.ks.rows * a.Hk ? a.qs.rows * a.H : a.ks.rows * a.Hk;
@@ -674,20 +683,16 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
   auto sum = [&](const float* part, int64_t stride, int shares, int64_t n, int heads,
                  const Heads<T>& out) -> int {
     if (!out.p) return SP_OK;
-    const int64_t groups = cdiv(n * heads * (a.D / 4), 64);
-    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
-    attend_sum<T><<<unsigned(groups), kAttnThreads, 0, s>>>(part, stride, shares, n, heads, a.D, out);
+    attend_sum<T><<<unsigned(cdiv(n * heads * (a.D / 4), 64)), kAttnThreads, 0, s>>>(part, stride, shares, n, heads, a.D, out);
     SP_LAUNCHED();
     return SP_OK;
   };
   if (need_dq) {
-    const int64_t slots = tile_slots(a.qs, a.G, kGradRows);
+    const int64_t slots = q_slots;
     a.shares = l.dq_shares;
-    const int64_t groups = attn_groups(slots, a.Hk, a.shares);
-    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
     with_width(a.D, [&](auto w) {
       constexpr int DP = w.value, B = attn_stage<T>();
-      const dim3 grid{unsigned(groups)}, block{kAttnThreads};
+      const dim3 grid{unsigned(q_groups)}, block{kAttnThreads};
       if (!a.causal) {
         attend_dq<T, DP, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
       } else {
@@ -701,13 +706,11 @@ int attn_backward(AttnArgs<T> a, const AttnGradLayout& l, char* ws, bool need_dq
       if (int rc = sum(a.part, a.qs.rows * a.H * a.D, a.shares, a.qs.rows, a.H, a.dq)) return rc;
   }
   if (need_dkv) {
-    const int64_t slots = tile_slots(a.ks, 1, kGradRows);
+    const int64_t slots = k_slots;
     a.shares = l.dkv_shares;
-    const int64_t groups = attn_groups(slots, a.Hk, a.shares);
-    SP_CHECK_ARG(groups <= kMaxGridX, "attention_bwd: too many rows");
     with_width(a.D, [&](auto w) {
       constexpr int DP = w.value, B = attn_stage<T>();
-      const dim3 grid{unsigned(groups)}, block{kAttnThreads};
+      const dim3 grid{unsigned(k_groups)}, block{kAttnThreads};
       if (!a.causal) {
         attend_dkv<T, DP, B, false, false><<<grid, block, 0, s>>>(a, nl, nd, slots);
       } else {

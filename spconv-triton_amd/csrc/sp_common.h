@@ -44,6 +44,9 @@ inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // of a HIP grid holds at most 2^31-1 workgroups.
 constexpr int64_t kMaxGridX = 0x7fffffffLL;
 
+// Workgroups of a launch at most: a grid has fewer than 2^32 threads.
+constexpr int64_t max_groups(int threads) { return 0xffffffffLL / threads; }
+
 // Bump allocator over a caller-provided workspace (256-byte aligned slices).
 struct WsCursor {
   char* base;

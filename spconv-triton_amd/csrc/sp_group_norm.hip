@@ -708,15 +708,20 @@ static size_t slabs_bytes(int64_t parts, int64_t C) {
   return parts > kNormSlab ? align_up(size_t(cdiv(parts, kNormSlab)) * C * sizeof(float2), 256) : 0;
 }
 
+constexpr int64_t kNormMaxGroups = max_groups(kNormThreads);
+
+static int64_t slab_groups(int64_t parts, int64_t C) {
+  return parts > kNormSlab ? cdiv(parts, kNormSlab) * cdiv(C, 64) : 0;
+}
+
 // At most kNormSlab rows that add up to those of the parts: a.rows, between a.sums and the workspace at `slabs`.
 template <typename T, typename P>
 static int join_parts(NormArgs<T, P>& a, char* slabs, hipStream_t st) {
   float2 *from = a.sums, *to = reinterpret_cast<float2*>(slabs);
   int64_t n = a.seqs.parts;
   while (n > kNormSlab && (a.dw || a.db)) {
-    const int64_t next = cdiv(n, kNormSlab), groups = next * cdiv(a.s.C, 64);
-    SP_CHECK_ARG(groups <= kMaxGridX, "group_norm_bwd: too many samples");
-    norm_slabs<<<unsigned(groups), kNormThreads, 0, st>>>(from, int(n), a.s.C, to);
+    const int64_t next = cdiv(n, kNormSlab);
+    norm_slabs<<<unsigned(slab_groups(n, a.s.C)), kNormThreads, 0, st>>>(from, int(n), a.s.C, to);
     SP_LAUNCHED();
     float2* const read = from;
     from = to;
@@ -753,6 +758,8 @@ static int norm_act_of(int act, F&& f) {
 template <typename T, typename P, int V>
 static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
   if (norm_is_small(a.seqs.rows, a.s.C, a.seqs, V)) {
+    SP_CHECK_ARG(a.seqs.parts <= max_groups(kSmallThreads),
+                 "group_norm: too many samples for a launch");
     a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
     norm_act_of(act, [&](auto k) {
       norm_small<T, P, V, k.value><<<unsigned(a.seqs.parts), kSmallThreads, 0, st>>>(a);
@@ -764,7 +771,8 @@ static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
   a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V);
   const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
   const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
-  SP_CHECK_ARG(slots <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
+  SP_CHECK_ARG(slots * a.s.blocks <= kNormMaxGroups && joins <= kNormMaxGroups,
+               "group_norm: too many samples for a launch");
   a.part = reinterpret_cast<float2*>(ws);
   const dim3 grid(unsigned(slots), unsigned(a.s.blocks));
   norm_moments<T, P, V><<<grid, kNormThreads, 0, st>>>(a);
@@ -782,6 +790,9 @@ static int norm_forward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
 template <typename T, typename P, int V>
 static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
   if (norm_is_small(a.seqs.rows, a.s.C, a.seqs, V)) {
+    SP_CHECK_ARG(a.seqs.parts <= max_groups(kSmallThreads) &&
+                     slab_groups(a.seqs.parts, a.s.C) <= kNormMaxGroups,
+                 "group_norm_bwd: too many samples for a launch");
     a.s = norm_shape(a.seqs.rows, a.s.C, a.s.groups, V, kSmallThreads);
     a.sums = reinterpret_cast<float2*>(ws);
     norm_act_of(act, [&](auto k) {
@@ -800,7 +811,9 @@ static int norm_backward(NormArgs<T, P> a, int act, char* ws, hipStream_t st) {
   const int64_t slots = tile_slots(a.seqs, 1, int(a.s.chunk));
   const int64_t joins = int64_t(a.seqs.parts) * a.s.groups;
   const int64_t extra = a.dw || a.db ? cdiv(a.s.C, 64) : 0;
-  SP_CHECK_ARG(slots + extra <= kMaxGridX && joins <= kMaxGridX, "group_norm: too many samples");
+  SP_CHECK_ARG((slots + extra) * a.s.blocks <= kNormMaxGroups && joins <= kNormMaxGroups &&
+                   slab_groups(a.seqs.parts, a.s.C) <= kNormMaxGroups,
+               "group_norm_bwd: too many samples for a launch");
   a.part = reinterpret_cast<float2*>(ws);
   ws += align_up(size_t(slots) * a.s.C * sizeof(float2), 256);
   a.sums = reinterpret_cast<float2*>(ws);

@@ -368,7 +368,7 @@ template <typename T, typename S, bool ASYNC, bool GRAD>
 static int launch_linear(const Rows<T>& x, const Rows<T>& w, const LinearOut<T>& o,
                          hipStream_t s) {
   const int64_t groups = tile_groups<S>(x.n, cdiv(o.columns, S::W));
-  SP_CHECK_ARG(groups <= kMaxGridX, "linear: too many rows");
+  SP_CHECK_ARG(groups <= max_groups(S::THREADS), "linear: too many rows for a launch");
   linear_rows<T, S, ASYNC, GRAD><<<unsigned(groups), S::THREADS, 0, s>>>(x, w, o);
   SP_LAUNCHED();
   return SP_OK;

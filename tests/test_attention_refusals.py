@@ -168,3 +168,21 @@ def test_gradients_of_padded_heads_are_not_copied_before_they_hold_anything(no_g
         for h in range(2):
             want = torch.frombuffer(bytearray(range(h, h + 40)), dtype=torch.float16)
             assert torch.equal(g[:, h].view(torch.int16), want.view(torch.int16).expand(3, 20))
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    """A grid has fewer than 2^32 threads, and every sequence and key head takes a workgroup.  (On the host: a call
+    that was let through would end at its launch, with another status.)"""
+    from spconv_triton.pytorch._impl import _lib
+    from spconv_triton.pytorch._impl.attention import _Call, _Grad
+
+    L = _lib.load_library()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    for n, heads in ((1 << 24, 1), (1 << 20, 16)):
+        c = _Call(p, p, p, 512, 32, 512, 32, 512, 32, 5000, 5000, heads, heads, 32, n, p, p, 0.1, 0, 0)
+        g = _Grad(p, p, p, p, p, p, *(512, 32) * 5)
+        ref = ctypes.byref(c)
+        assert L.sp_attention(ref, p, 512, 32, None, p, 1 << 62, None) == _lib.SP_ERR_INVALID_ARG
+        assert (L.sp_attention_bwd(ref, ctypes.byref(g), p, 1 << 62, None)
+                == _lib.SP_ERR_INVALID_ARG)

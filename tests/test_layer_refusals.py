@@ -198,3 +198,23 @@ def test_blocks_of_wider_heads_than_attention_takes_are_not_built():
         with pytest.raises(NotImplementedError, match="wider than 128"):
             spconv.SparseAttentionBlock(*args)
     assert spconv.SparseAttentionBlock(256, 2).qkv.weight.shape == (768, 256)
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    """A grid has fewer than 2^32 threads.  (Pointers that are not device memory, on the host: a call that was let
+    through would end at its launch, with another status.)"""
+    from spconv_triton.pytorch._impl import _lib
+
+    L = _lib.load_library()
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 15) // 16 * 16)
+    f16, bad, most = _lib.SP_F16, _lib.SP_ERR_INVALID_ARG, 1 << 62
+    samples = (1 << 24) - 8
+    # (a workgroup a part in calls of few values, of 512 threads; a part and group; a chunk of rows)
+    for rows, c, groups, n in ((1000, 8, 2, 1 << 23), (5000, 64, 8, 1 << 22), (5000, 64, 1, samples)):
+        assert L.sp_group_norm(p, c, f16, rows, c, groups, p, p, f16, 1e-5, 3, p, n, p, p, p, most,
+                               None) == bad
+        assert L.sp_group_norm_bwd(p, c, p, c, f16, rows, c, groups, p, p, f16, 3, p, n, p, p, p, p,
+                                   p, most, None) == bad
+    assert L.sp_linear(p, 8, f16, 1 << 30, 8, p, 8, p, 3, None, 0, p, None) == bad
+    assert L.sp_linear_bwd(p, 8, p, 8, f16, 1 << 30, 8, p, 8, p, 1, p, p, p, p, most, None) == bad
