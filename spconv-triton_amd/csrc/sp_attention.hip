@@ -16,9 +16,9 @@
 // Bound by the vector unit beside the matrix cores: a weight costs an exponential (8 cycles of a SIMD for 64 of them,
 // 4 times an addition), its conversion and its sum, and a matrix instruction keeps the vector unit from
 // issuing for half of its time.  Self-attention of 8 heads of 64 bf16 values, 6.6e11 operations:
-// 815 us, 813 TFLOP/s (a library product of 8192^3 reaches 1 138 on the same card); causal, 128 fp16 values, 1.4e11:
-// 212 us; 4 heads of 16 fp16 values in windows of 1024 rows, where half of the products are padding: 197 us for 8.2e8
-// weights.  One query over 120k keys of 8 heads of 32 fp16 values: 42 us, 2.9 TB/s.
+// 846 us, 783 TFLOP/s (a library product of 8192^3 reaches 1 138 on the same card); causal, 128 fp16 values, 1.4e11:
+// 223 us; 4 heads of 16 fp16 values in windows of 1024 rows, where half of the products are padding: 194 us for 8.2e8
+// weights.  One query over 120k keys of 8 heads of 32 fp16 values: 41 us, 3.0 TB/s.
 // Not faster: two query tiles a wave (945 us for 880 at 64 values), eight waves a workgroup (713 for 625),
 // three key tiles in flight, the next tile's scores beside this tile's weights (892), four waves a SIMD (spills).
 #include "sp_attention.h"

@@ -14,8 +14,8 @@
 // query's own |dO|, for dK, whose sums are over queries, from the largest.
 //
 // Bound by the matrix cores and the vector unit in turn, as the forward pass is: self-attention of 8 heads of 64 bf16
-// values, dQ 1 005 us (9.9e11 operations, 989 TFLOP/s), dK and dV 1 481 (1.33e12, 895); causal, 128 fp16 values, 406 and
-// 485; 5 003 rows of 4 heads of 32 fp32 values 100 and 130 (77 and 79 TFLOP/s, where a product of 8192^3 reaches 154).
+// values, dQ 1 038 us (9.9e11 operations, 958 TFLOP/s), dK and dV 1 480 (1.33e12, 896); causal, 128 fp16 values, 427 and
+// 508; 5 003 rows of 4 heads of 32 fp32 values 100 and 130 (77 and 79 TFLOP/s, where a product of 8192^3 reaches 154).
 #include "sp_attention.h"
 
 namespace sp {

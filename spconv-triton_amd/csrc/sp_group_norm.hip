@@ -11,7 +11,7 @@
 // from a few rows in registers and joined by Chan, Golub and LeVeque's formula, so that a mean far
 // from zero costs no digits; everything is fp32 and joined in a fixed order.
 //
-// 240k x 128 bf16 (61 MB) in two samples: moments 20 us (3.1 TB/s), statistics 7, values 27 (4.6 TB/s), the gradients' sums 31
+// 240k x 128 bf16 (61 MB) in two samples: moments 19 us (3.2 TB/s), statistics 7, values 27 (4.6 TB/s), the gradients' sums 31
 // (4.0), their joins 7, dx 35 (5.3).  What the two joins take is latency: a launch of few workgroups and a
 // batch of loads (one load after the other: 9).
 #include "sp_attention.h"  // sequences in packed rows

@@ -9,9 +9,9 @@
 // would also hold rows x outputs of memory).  dz is rounded to the rows' type, as an operand of the
 // products that follow; z, the activation and every sum are fp32.
 //
-// 75k x 256 -> 1024 bf16 with gelu and a residual, 3.9e10 operations a product: forward 128 us (346 MB of rows in and out are
-// 70 at a copy's rate; then the activation, whose instructions come after the tile's four stages), dz 139, dx 74
-// (531 TFLOP/s), dW and db 76 (517) and their shares' sums 12 (a library product of these operands: 66 forward,
+// 75k x 256 -> 1024 bf16 with gelu and a residual, 3.9e10 operations a product: forward 132 us (346 MB of rows in and out are
+// 70 at a copy's rate; then the activation, whose instructions come after the tile's four stages), dz 137, dx 74
+// (531 TFLOP/s), dW and db 77 (510) and their shares' sums 12 (a library product of these operands: 66 forward,
 // 53 for dx and 280 for dW).
 #include "sp_tiles.h"
 
