@@ -408,11 +408,12 @@ __global__ __launch_bounds__(kAttnThreads, grad_waves<T>(DP, STRICT)) void atten
     if (wave < 2) {
       // (a whole wave, each lane by a selected address: a branch of some lanes here had the compiler save registers
       // for those lanes only)
-      const int r = tile * BQ + lane64;
+      // (the lane's part of the address is of this tile: a row's own times 4 would pass 32 bits)
+      const int first_row = tile * BQ;
       const char* rows = uniform(reinterpret_cast<const char*>(
-          (wave ? nd : nl) + (h0 + head) * a.qs.rows + qlo));
-      const char* from_ = rows + unsigned(r < Lq ? r : 0) * 4;
-      from_ = r < Lq ? from_ : reinterpret_cast<const char*>(&g_no_row[wave]);
+          (wave ? nd : nl) + (h0 + head) * a.qs.rows + qlo + first_row));
+      const char* from_ = first_row + lane64 < Lq ? rows + unsigned(lane64) * 4
+                                                  : reinterpret_cast<const char*>(&g_no_row[wave]);
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)from_,
           (__attribute__((address_space(3))) void*)(to + 2 * L::BYTES + wave * (kStats * 4)), 4, 0,
